@@ -31,15 +31,30 @@ from .multiply_base4 import butterfly_multiply_base4  # noqa: E402
 from .butterfly import Butterfly, ButterflyBmm, ButterflyUnitary  # noqa: E402
 from .butterfly_base4 import ButterflyBase4  # noqa: E402
 from .graphed import GraphedStep  # noqa: E402
-from . import combine, complex_utils, diagonal, kops, legacy, legacy_permutation, multiply, multiply_base4, permutation, special  # noqa: E402,F401
+from .loss import LinearCrossEntropy, linear_cross_entropy  # noqa: E402
+from .recurrence import gated_recurrence, gated_recurrence_step  # noqa: E402
+from .rowwise import (DropoutAdd, DropoutAddLayerNorm, LayerNorm, dropout_add, dropout_add_layer_norm,  # noqa: E402
+                      layer_norm, rng_next)
+from . import combine, complex_utils, diagonal, kops, legacy, legacy_permutation, loss, multiply, multiply_base4, permutation, recurrence, rowwise, sequence_model, special  # noqa: E402,F401
 
 __all__ = [
     "Butterfly",
     "ButterflyBase4",
     "ButterflyBmm",
     "ButterflyUnitary",
+    "DropoutAdd",
+    "DropoutAddLayerNorm",
     "GraphedStep",
+    "LayerNorm",
+    "LinearCrossEntropy",
     "butterfly_multiply",
     "butterfly_multiply_base4",
+    "dropout_add",
+    "dropout_add_layer_norm",
+    "gated_recurrence",
+    "gated_recurrence_step",
+    "layer_norm",
+    "linear_cross_entropy",
+    "rng_next",
     "__version__",
 ]

@@ -11,7 +11,7 @@ import torch
 _PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_PKG_DIR, "libbutterfly_hip.so")
 
-BF_F32, BF_C64 = 0, 1
+BF_F32, BF_C64, BF_BF16 = 0, 1, 2
 BF_ERR_INVALID, BF_ERR_UNSUPPORTED, BF_ERR_HIP, BF_ERR_WORKSPACE = -1, -2, -3, -4
 
 SYMBOLS = [
@@ -31,6 +31,9 @@ SYMBOLS = [
     "bf_butterfly_multiply_base4_saved_bytes", "bf_butterfly_multiply_base4_fw_saving",
     "bf_butterfly_multiply_base4_bw_saved_workspace_bytes", "bf_butterfly_multiply_base4_bw_saved",
     "bf_layer_takes_real", "bf_layer_kept_bytes", "bf_layer_fw_workspace_bytes", "bf_layer_fw", "bf_layer_bw_workspace_bytes", "bf_layer_bw",
+    "bf_rng_next", "bf_rowwise_fw", "bf_rowwise_bw_workspace_bytes", "bf_rowwise_bw",
+    "bf_recurrence_workspace_bytes", "bf_recurrence_fw", "bf_recurrence_bw", "bf_recurrence_step",
+    "bf_linear_xent_fw_workspace_bytes", "bf_linear_xent_bw_workspace_bytes", "bf_linear_xent_fw", "bf_linear_xent_bw",
 ]
 
 NOALLOC_SCRATCH_BYTES = 48 << 20
@@ -66,6 +69,24 @@ class Layer(ctypes.Structure):
         ("in_perm", ctypes.c_void_p),
         ("out_index", ctypes.c_void_p),
     ]
+
+
+class Rowwise(ctypes.Structure):
+    _fields_ = [("dtype", ctypes.c_int32), ("param_dtype", ctypes.c_int32), ("rows", ctypes.c_int64), ("cols", ctypes.c_int64),
+                ("x_stride", ctypes.c_int64), ("residual_stride", ctypes.c_int64), ("grad_y_stride", ctypes.c_int64),
+                ("grad_sum_stride", ctypes.c_int64), ("drop_probability", ctypes.c_double), ("eps", ctypes.c_double)]
+
+
+class Recurrence(ctypes.Structure):
+    _fields_ = [("dtype", ctypes.c_int32), ("sigmoid", ctypes.c_int32), ("batch", ctypes.c_int64), ("steps", ctypes.c_int64),
+                ("channels", ctypes.c_int64), ("gate_stride", ctypes.c_int64 * 2), ("x_stride", ctypes.c_int64 * 2),
+                ("grad_stride", ctypes.c_int64 * 2), ("reset_stride", ctypes.c_int64 * 2)]
+
+
+class LinearXent(ctypes.Structure):
+    _fields_ = [("dtype", ctypes.c_int32), ("reduction", ctypes.c_int32), ("rows", ctypes.c_int64), ("features", ctypes.c_int64),
+                ("vocab", ctypes.c_int64), ("hidden_stride", ctypes.c_int64), ("weight_stride", ctypes.c_int64),
+                ("ignore_index", ctypes.c_int64)]
 
 
 _lib = None
@@ -130,6 +151,22 @@ def lib():
         L.bf_layer_bw_workspace_bytes.argtypes = [pl, ctypes.c_int, sz]
         L.bf_layer_bw_workspace_bytes.restype = sz
         L.bf_layer_bw.argtypes = [pl, vp, vp, vp, sz, vp, vp, vp, vp, vp, sz, vp]
+        pr, pc, px = ctypes.POINTER(Rowwise), ctypes.POINTER(Recurrence), ctypes.POINTER(LinearXent)
+        L.bf_rng_next.argtypes = [vp, vp, vp]
+        L.bf_rowwise_fw.argtypes = [pr] + [vp] * 9
+        L.bf_rowwise_bw_workspace_bytes.argtypes = [pr]
+        L.bf_rowwise_bw_workspace_bytes.restype = sz
+        L.bf_rowwise_bw.argtypes = [pr] + [vp] * 11 + [sz, vp]
+        L.bf_recurrence_workspace_bytes.argtypes = [pc]
+        L.bf_recurrence_workspace_bytes.restype = sz
+        L.bf_recurrence_fw.argtypes = [pc] + [vp] * 7 + [sz, vp]
+        L.bf_recurrence_bw.argtypes = [pc] + [vp] * 11 + [sz, vp]
+        L.bf_recurrence_step.argtypes = [pc] + [vp] * 5
+        for name in ("bf_linear_xent_fw_workspace_bytes", "bf_linear_xent_bw_workspace_bytes"):
+            getattr(L, name).argtypes = [px]
+            getattr(L, name).restype = sz
+        L.bf_linear_xent_fw.argtypes = [px] + [vp] * 6 + [sz, vp]
+        L.bf_linear_xent_bw.argtypes = [px] + [vp] * 8 + [sz, vp]
         _lib = L
     return _lib
 

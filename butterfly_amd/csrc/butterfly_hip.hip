@@ -16,6 +16,7 @@
 #include <utility>
 
 #include "common.hpp"
+#include "error.hpp"
 #include "generic.hpp"
 #include "scale.hpp"
 #include "launch.hpp"
@@ -25,11 +26,11 @@
 
 namespace {
 
-using namespace bf;
-
 thread_local std::string g_last_error;
 
-int fail(int code, const char *fmt, ...)
+}  // namespace
+
+int bf::fail(int code, const char *fmt, ...)
 {
     char buf[512];
     va_list ap;
@@ -40,12 +41,9 @@ int fail(int code, const char *fmt, ...)
     return code;
 }
 
-#define BF_HIP_CHECK(expr)                                                              \
-    do {                                                                                \
-        hipError_t e_ = (expr);                                                         \
-        if (e_ != hipSuccess)                                                           \
-            return fail(BF_ERR_HIP, "%s failed: %s", #expr, hipGetErrorString(e_));     \
-    } while (0)
+namespace {
+
+using namespace bf;
 
 // (gfx950 has 160 KiB of LDS per compute unit)
 constexpr size_t kGenericFwLds = 128 * 1024;    // most a generic forward workgroup stages

@@ -1,0 +1,347 @@
+// Entry points of the linear layer with softmax cross entropy (xent.hpp): argument checks, workspace, launches.
+
+#include "../../include/butterfly_hip.h"
+
+#include <algorithm>
+
+#include "error.hpp"
+#include "xent.hpp"
+
+namespace {
+
+using namespace bf;
+
+int check_xent(const bf_linear_xent *p)
+{
+    if (!p) return fail(BF_ERR_INVALID, "loss descriptor is NULL");
+    if (p->dtype != BF_F32 && p->dtype != BF_BF16) return fail(BF_ERR_INVALID, "dtype must be BF_F32 or BF_BF16");
+    if (p->reduction != BF_XENT_NONE && p->reduction != BF_XENT_MEAN && p->reduction != BF_XENT_SUM)
+        return fail(BF_ERR_INVALID, "reduction must be BF_XENT_NONE, BF_XENT_MEAN or BF_XENT_SUM");
+    if (p->rows < 0 || p->features < 1 || p->vocab < 1) return fail(BF_ERR_INVALID, "rows must be >= 0, features and vocab >= 1");
+    if (p->rows > (1 << 24) || p->features > (1 << 16) || p->vocab > (1 << 24))
+        return fail(BF_ERR_UNSUPPORTED, "rows and vocab up to 2^24, features up to 2^16 are supported");
+    if (p->hidden_stride < 0 || p->weight_stride < 0) return fail(BF_ERR_INVALID, "strides must be non-negative");
+    return BF_OK;
+}
+
+size_t up256(size_t v) { return (v + 255) & ~(size_t)255; }
+int64_t up_to(int64_t v, int64_t m) { return (v + m - 1) / m * m; }
+
+// bfloat16 weights are read where they lie if 16-byte units divide their rows; others are laid out anew.
+bool weight_in_place(const bf_linear_xent *p)
+{
+    return p->dtype == BF_BF16 && p->features % 8 == 0 && p->weight_stride % 8 == 0 && p->weight_stride >= p->features &&
+           p->weight_stride <= (1 << 20);
+}
+
+// Tiles of 256 x 256 where there are enough of them for three quarters of the compute units, of 128 x 128 otherwise.
+bool large_tiles(int64_t m, int64_t n) { return ((m + 255) / 256) * ((n + 255) / 256) >= 192; }
+
+struct Product {
+    bool large = false;
+    int tiles_m = 0, tiles_n = 0, splits = 1;
+};
+
+// k steps are cut where the tiles alone leave compute units idle, down to 16 steps a part.
+Product product(int64_t m, int64_t n, int64_t steps, bool may_split)
+{
+    Product r;
+    r.large = large_tiles(m, n);
+    const int64_t t = r.large ? 256 : 128;
+    r.tiles_m = (int)((m + t - 1) / t);
+    r.tiles_n = (int)((n + t - 1) / t);
+    const int64_t tiles = (int64_t)r.tiles_m * r.tiles_n;
+    if (may_split && !r.large)
+        r.splits = (int)std::max<int64_t>(1, std::min<int64_t>({512 / std::max<int64_t>(tiles, 1), steps / 16, 32}));
+    return r;
+}
+
+constexpr size_t kPieceBytes = (size_t)256 << 20;   // d_l of a piece of the vocabulary
+
+struct XentPlan {
+    int64_t features_up = 0, rows_up = 0;       // padded to k steps, to tiles
+    size_t hidden_plane = 0, weight_plane = 0;  // bytes
+    int planes = 1;
+    Product logits;
+    // backward
+    int64_t piece = 0;                          // vocabulary entries of a piece, whole tiles
+    Product to_hidden, to_weight;
+    // offsets into the workspace
+    size_t scalars = 0, index = 0, position = 0, label = 0, picked = 0, losses = 0, partial = 0, hidden = 0, weight = 0;
+    size_t share = 0, lse_at = 0, d_l = 0, d_l_plane = 0, sums_hidden = 0, sums_weight = 0;
+    size_t total = 0;
+};
+
+XentPlan plan(const bf_linear_xent *p, bool backward)
+{
+    XentPlan r;
+    r.planes = p->dtype == BF_F32 ? 2 : 1;
+    r.features_up = up_to(p->features, kMatK);
+    r.rows_up = up_to(std::max<int64_t>(p->rows, 1), 256);
+    r.hidden_plane = up256((size_t)r.rows_up * r.features_up * 2);
+    r.weight_plane = up256((size_t)p->vocab * r.features_up * 2);
+    size_t at = 0;
+    auto take = [&](size_t bytes) {
+        const size_t here = at;
+        at += up256(bytes);
+        return here;
+    };
+    const size_t rows = (size_t)std::max<int64_t>(p->rows, 1);
+    r.scalars = take(sizeof(XentScalars));
+    r.index = take(rows * 4);
+    r.position = take(rows * 4);
+    r.label = take(rows * 4);
+    r.hidden = take(r.hidden_plane * r.planes);
+    if (!weight_in_place(p)) r.weight = take(r.weight_plane * r.planes);
+    if (!backward) {
+        r.logits = product(p->vocab, p->rows, 0, false);
+        r.picked = take(rows * 4);
+        r.losses = take(rows * 4);
+        r.partial = take((size_t)2 * r.logits.tiles_m * rows * sizeof(float2));
+    } else {
+        const int64_t most = (int64_t)(kPieceBytes / ((size_t)r.rows_up * 2 * r.planes)) / 256 * 256;
+        r.piece = std::min<int64_t>(up_to(p->vocab, 256), std::max<int64_t>(most, 2048));
+        const int64_t pieces = (p->vocab + r.piece - 1) / r.piece;
+        r.piece = std::min<int64_t>(up_to((p->vocab + pieces - 1) / pieces, 256), r.piece);
+        r.logits = product(r.piece, p->rows, 0, false);
+        r.to_hidden = product(p->features, p->rows, r.piece / kMatK, true);
+        r.to_weight = product(p->features, r.piece, (p->rows + kMatK - 1) / kMatK, true);
+        r.share = take(rows * 4);
+        r.lse_at = take(rows * 4);
+        r.d_l_plane = up256((size_t)r.rows_up * r.piece * 2);
+        r.d_l = take(r.d_l_plane * r.planes);
+        r.sums_hidden = take((size_t)r.to_hidden.splits * rows * p->features * sizeof(float));
+        if (r.to_weight.splits > 1) r.sums_weight = take((size_t)r.to_weight.splits * r.piece * p->features * sizeof(float));
+    }
+    r.total = at;
+    return r;
+}
+
+int check_memory(const XentPlan &r, const void *weight, const void *workspace, size_t bytes)
+{
+    if (reinterpret_cast<uintptr_t>(weight) & 15) return fail(BF_ERR_INVALID, "weight must be 16-byte aligned");
+    if (!workspace || bytes < r.total)
+        return fail(BF_ERR_WORKSPACE, "workspace of %zu bytes needed, %zu given", r.total, workspace ? bytes : 0);
+    if (reinterpret_cast<uintptr_t>(workspace) & 255) return fail(BF_ERR_WORKSPACE, "workspace must be 256-byte aligned");
+    return BF_OK;
+}
+
+template <typename T>
+T *part(void *workspace, size_t offset)
+{
+    return reinterpret_cast<T *>(static_cast<char *>(workspace) + offset);
+}
+
+void pack(const bf_linear_xent *p, const void *x, char *out, int64_t out_rows, int64_t rows, int64_t x_stride, int64_t stride,
+          size_t plane, const int *index, XentScalars *scalars, int which, hipStream_t s)
+{
+    if (p->dtype == BF_F32 && rows > 0) {
+        unsigned *largest = which ? &scalars->weight_max : &scalars->hidden_max;
+        xent_largest_kernel<<<dim3((unsigned)std::min<int64_t>(rows, 2048)), dim3(256), 0, s>>>(
+            static_cast<const float *>(x), rows, p->features, x_stride, index, scalars, largest);
+    }
+    const XentPackArgs a = {x, out, out_rows, p->features, x_stride, stride, (int64_t)plane, index, scalars, which};
+    const int64_t units = out_rows * (stride / 16);
+    const dim3 grid((unsigned)std::min<int64_t>((units + 255) / 256, 8192));
+    if (p->dtype == BF_F32) xent_pack_kernel<float><<<grid, dim3(256), 0, s>>>(a);
+    else xent_pack_kernel<bf16><<<grid, dim3(256), 0, s>>>(a);
+}
+
+// What both directions start with: the counted rows, hidden and weight as operands.
+void prepare(const bf_linear_xent *p, const XentPlan &r, const void *hidden, const void *weight, const int64_t *target, void *ws,
+             float *picked, MatOperand &h, MatOperand &w, hipStream_t s)
+{
+    XentScalars *scalars = part<XentScalars>(ws, r.scalars);
+    const XentRowsArgs rows = {target, p->rows, p->vocab, p->ignore_index, scalars, part<int>(ws, r.index),
+                               part<int>(ws, r.position), part<int>(ws, r.label), picked};
+    xent_rows_kernel<<<dim3(1), dim3(kXentThreads), 0, s>>>(rows);
+    char *hp = part<char>(ws, r.hidden), *wp = part<char>(ws, r.weight);
+    const int64_t stride = r.features_up * 2;
+    pack(p, hidden, hp, r.rows_up, p->rows, p->hidden_stride, stride, r.hidden_plane, part<int>(ws, r.index), scalars, 0, s);
+    h = {hp, (int64_t)r.hidden_plane, stride, r.rows_up * stride};
+    if (weight_in_place(p)) {
+        w = {static_cast<const char *>(weight), 0, p->weight_stride * 2, ((p->vocab - 1) * p->weight_stride + p->features) * 2};
+    } else {
+        pack(p, weight, wp, p->vocab, p->vocab, p->weight_stride, stride, r.weight_plane, nullptr, scalars, 1, s);
+        w = {wp, (int64_t)r.weight_plane, stride, p->vocab * stride};
+    }
+}
+
+template <bool F16, bool BACKWARD>
+void launch_logits(const Product &r, const XentTileArgs &a, hipStream_t s)
+{
+    const dim3 grid((unsigned)(r.tiles_m * r.tiles_n)), threads(kMatThreads);
+    if (r.large) xent_logits_kernel<F16, 256, 256, BACKWARD><<<grid, threads, 0, s>>>(a);
+    else xent_logits_kernel<F16, 128, 128, BACKWARD><<<grid, threads, 0, s>>>(a);
+}
+
+template <MatLayout LB>
+void launch_grad(const bf_linear_xent *p, const Product &r, const XentGradArgs &a, hipStream_t s)
+{
+    const dim3 grid((unsigned)(r.tiles_m * r.tiles_n * r.splits)), threads(kMatThreads);
+    if (p->dtype == BF_F32) {
+        if (r.large) xent_grad_kernel<float, LB, 256, 256><<<grid, threads, 0, s>>>(a);
+        else xent_grad_kernel<float, LB, 128, 128><<<grid, threads, 0, s>>>(a);
+    } else {
+        if (r.large) xent_grad_kernel<bf16, LB, 256, 256><<<grid, threads, 0, s>>>(a);
+        else xent_grad_kernel<bf16, LB, 128, 128><<<grid, threads, 0, s>>>(a);
+    }
+}
+
+void gather(const bf_linear_xent *p, const XentGatherArgs &a, hipStream_t s)
+{
+    const dim3 grid((unsigned)std::min<int64_t>(a.rows, 8192));
+    if (p->dtype == BF_F32) xent_gather_kernel<float><<<grid, dim3(256), 0, s>>>(a);
+    else xent_gather_kernel<bf16><<<grid, dim3(256), 0, s>>>(a);
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t bf_linear_xent_fw_workspace_bytes(const bf_linear_xent *p)
+{
+    return check_xent(p) ? BF_SIZE_INVALID : plan(p, false).total;
+}
+
+size_t bf_linear_xent_bw_workspace_bytes(const bf_linear_xent *p)
+{
+    return check_xent(p) ? BF_SIZE_INVALID : plan(p, true).total;
+}
+
+int bf_linear_xent_fw(const bf_linear_xent *p, const void *hidden, const void *weight, const int64_t *target, float *loss,
+                      float *lse, void *workspace, size_t workspace_bytes, void *stream)
+{
+    int rc = check_xent(p);
+    if (rc) return rc;
+    if (p->rows > 0 && (!hidden || !target || !lse)) return fail(BF_ERR_INVALID, "hidden, target or lse is NULL");
+    if (!weight || (!loss && (p->rows > 0 || p->reduction != BF_XENT_NONE))) return fail(BF_ERR_INVALID, "weight or loss is NULL");
+    if (p->rows == 0 && p->reduction == BF_XENT_NONE) return BF_OK;
+    const XentPlan r = plan(p, false);
+    if ((rc = check_memory(r, weight, workspace, workspace_bytes))) return rc;
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    MatOperand h, w;
+    float *picked = part<float>(workspace, r.picked);
+    prepare(p, r, hidden, weight, target, workspace, picked, h, w, s);
+    XentScalars *scalars = part<XentScalars>(workspace, r.scalars);
+    float *losses = p->reduction == BF_XENT_NONE ? loss : part<float>(workspace, r.losses);
+    if (p->rows > 0) {
+        XentTileArgs a = {};
+        a.weight = w;
+        a.hidden = h;
+        a.scalars = scalars;
+        a.label = part<int>(workspace, r.label);
+        a.rows = p->rows;
+        a.vocab = p->vocab;
+        a.features_steps = (int)(r.features_up / kMatK);
+        a.tiles_m = r.logits.tiles_m;
+        a.tiles_n = r.logits.tiles_n;
+        a.partial = part<float2>(workspace, r.partial);
+        a.picked = picked;
+        if (p->dtype == BF_F32) launch_logits<true, false>(r.logits, a, s);
+        else launch_logits<false, false>(r.logits, a, s);
+        const XentJoinArgs j = {a.partial, picked, part<int>(workspace, r.position), p->rows, 2 * r.logits.tiles_m, lse, losses};
+        xent_join_kernel<<<dim3((unsigned)((p->rows + 15) / 16)), dim3(256), 0, s>>>(j);
+    }
+    if (p->reduction != BF_XENT_NONE)
+        xent_total_kernel<<<dim3(1), dim3(kXentThreads), 0, s>>>(losses, p->rows, scalars, p->reduction == BF_XENT_MEAN, loss);
+    BF_HIP_CHECK(hipGetLastError());
+    return BF_OK;
+}
+
+int bf_linear_xent_bw(const bf_linear_xent *p, const void *hidden, const void *weight, const int64_t *target, const float *lse,
+                      const float *grad, void *d_hidden, void *d_weight, void *workspace, size_t workspace_bytes, void *stream)
+{
+    int rc = check_xent(p);
+    if (rc) return rc;
+    if (p->rows > 0 && (!hidden || !target || !lse)) return fail(BF_ERR_INVALID, "hidden, target or lse is NULL");
+    if (!weight || (!grad && (p->rows > 0 || p->reduction != BF_XENT_NONE))) return fail(BF_ERR_INVALID, "weight or grad is NULL");
+    if (!d_hidden && !d_weight) return BF_OK;
+    const XentPlan r = plan(p, true);
+    if ((rc = check_memory(r, weight, workspace, workspace_bytes))) return rc;
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    MatOperand h, w;
+    prepare(p, r, hidden, weight, target, workspace, nullptr, h, w, s);
+    XentScalars *scalars = part<XentScalars>(workspace, r.scalars);
+    if (grad) {
+        const XentShareArgs g = {grad, lse, part<int>(workspace, r.index), part<int>(workspace, r.label), scalars,
+                                 p->reduction == BF_XENT_NONE, p->reduction == BF_XENT_MEAN,
+                                 part<float>(workspace, r.share), part<float>(workspace, r.lse_at)};
+        xent_share_kernel<<<dim3(1), dim3(kXentThreads), 0, s>>>(g);
+    }
+    const size_t elem = p->dtype == BF_F32 ? 4 : 2;
+    char *d_l = part<char>(workspace, r.d_l);
+    const int64_t d_l_stride = r.piece * 2;
+    const MatOperand d_l_operand = {d_l, (int64_t)r.d_l_plane, d_l_stride, r.rows_up * d_l_stride};
+    for (int64_t first = 0; first < p->vocab; first += r.piece) {
+        const int64_t entries = std::min<int64_t>(r.piece, p->vocab - first);
+        MatOperand wp = w;
+        wp.base += first * w.stride;
+        wp.bytes -= first * w.stride;
+        XentTileArgs a = {};
+        a.weight = wp;
+        a.hidden = h;
+        a.scalars = scalars;
+        a.label = part<int>(workspace, r.label);
+        a.rows = p->rows;
+        a.vocab = entries;
+        a.first = first;
+        a.features_steps = (int)(r.features_up / kMatK);
+        Product logits = r.logits;   // (a shorter last piece: fewer tiles of the same size)
+        const int64_t side = logits.large ? 256 : 128;
+        logits.tiles_m = (int)((entries + side - 1) / side);
+        a.tiles_m = logits.tiles_m;
+        a.tiles_n = logits.tiles_n;
+        a.lse = part<float>(workspace, r.lse_at);
+        a.share = part<float>(workspace, r.share);
+        a.d_l = d_l;
+        a.stride = d_l_stride;
+        a.plane = (int64_t)r.d_l_plane;
+        if (p->rows > 0) {
+            if (p->dtype == BF_F32) launch_logits<true, true>(logits, a, s);
+            else launch_logits<false, true>(logits, a, s);
+        }
+        if (d_hidden && p->rows > 0) {
+            XentGradArgs g = {};
+            g.a = wp;
+            g.b = d_l_operand;
+            g.scalars = scalars;
+            g.m = p->features;
+            g.n = p->rows;
+            g.tiles_m = r.to_hidden.tiles_m;
+            g.tiles_n = r.to_hidden.tiles_n;
+            g.steps = (int)((entries + kMatK - 1) / kMatK);
+            g.splits = r.to_hidden.splits;
+            g.add = first > 0;
+            g.partial = part<float>(workspace, r.sums_hidden);
+            launch_grad<kRows>(p, r.to_hidden, g, s);
+        }
+        if (d_weight) {
+            XentGradArgs g = {};
+            Product to_weight = r.to_weight;
+            const int64_t t = to_weight.large ? 256 : 128;
+            to_weight.tiles_n = (int)((entries + t - 1) / t);
+            g.a = h;
+            g.b = d_l_operand;
+            g.scalars = scalars;
+            g.m = p->features;
+            g.n = entries;
+            g.tiles_m = to_weight.tiles_m;
+            g.tiles_n = to_weight.tiles_n;
+            g.splits = to_weight.splits;
+            char *out = static_cast<char *>(d_weight) + (size_t)first * p->features * elem;
+            if (g.splits > 1) g.partial = part<float>(workspace, r.sums_weight);
+            else g.out = out;
+            launch_grad<kCols>(p, to_weight, g, s);
+            if (g.splits > 1)
+                gather(p, {g.partial, nullptr, scalars, out, entries, entries, p->features, g.splits, 1}, s);
+        }
+    }
+    if (d_hidden && p->rows > 0)
+        gather(p, {part<float>(workspace, r.sums_hidden), part<int>(workspace, r.position), scalars, d_hidden, p->rows, p->rows,
+                   p->features, r.to_hidden.splits, 0}, s);
+    BF_HIP_CHECK(hipGetLastError());
+    return BF_OK;
+}
+
+}  // extern "C"

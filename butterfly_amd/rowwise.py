@@ -1,0 +1,146 @@
+"""What stands between two layers of a block: dropout, residual addition and layer norm, each row read once.
+
+``layer_norm``, ``dropout_add`` and ``dropout_add_layer_norm`` (one kernel each way) with their modules.
+Dropout is counter-based: ``rng`` is a tensor of two int64, a seed and the number of the call, and the mask is a
+function of those, the row and the column (see ``dropout_mask``), made again in the backward pass instead
+of stored.  Rows are float32 or bfloat16, of any width and row stride; ``weight`` and ``bias`` float32 or the
+rows' dtype; statistics are formed in float32.  Host tensors run as tensor operations.
+
+No counterpart in the reference, whose users take these from PyTorch."""
+import torch
+from torch import nn
+
+ops = torch.ops.torch_butterfly
+
+
+def layer_norm(x, weight=None, bias=None, eps=1e-5):
+    """``(x - mean) / sqrt(var + eps) * weight + bias`` over the last dimension."""
+    if x.is_cuda:
+        return ops.layer_norm(x, weight, bias, eps)
+    return _host_norm(x, weight, bias, eps)
+
+
+def dropout_add(x, rng, p, residual=None):
+    """``residual + dropout(x)``: elements dropped with probability ``p`` (in steps of 1/65536), the others scaled by
+    the inverse of the probability to stay.  A dropped element contributes zero whatever it is."""
+    if x.is_cuda:
+        return ops.dropout_add(x, rng, p, residual)
+    return _host_total(x, rng, p, residual)
+
+
+def dropout_add_layer_norm(x, rng, p, residual=None, weight=None, bias=None, eps=1e-5):
+    """``(y, sum)`` with ``sum = residual + dropout(x)`` and ``y = layer_norm(sum)``."""
+    if x.is_cuda:
+        return ops.dropout_add_layer_norm(x, rng, p, residual, weight, bias, eps)
+    total = _host_total(x, rng, p, residual)
+    return _host_norm(total, weight, bias, eps), total
+
+
+def rng_next(rng):
+    """A copy of ``rng``, whose call number then goes up by one (on the device, in stream order: recorded in a HIP
+    graph, every replay takes the next number)."""
+    if rng.is_cuda:
+        return ops.rng_next(rng)
+    taken = rng.clone()
+    rng[1] += 1
+    return taken
+
+
+def dropout_mask(rng, rows, cols, p):
+    """The elements that ``dropout_add`` keeps of (rows, cols), as bool, in plain tensor operations: Philox4x32-10 with
+    key ``rng[0]`` and counter (column // 8, row, low and high half of ``rng[1]``) gives four 32-bit words for
+    eight columns; column c takes the low (c even) or high 16 bits of word (c % 8) // 2 and is kept where they are
+    at least ``round(65536 p)``."""
+    groups, low = -(-cols // 8), 0xFFFFFFFF
+    device = rng.device
+    shape = (rows, groups)
+    c = [torch.arange(groups, device=device).expand(shape), torch.arange(rows, device=device).unsqueeze(1).expand(shape),
+         (rng[1] & low).expand(shape), (rng[1] >> 32 & low).expand(shape)]
+    k = [rng[0] & low, rng[0] >> 32 & low]
+
+    def product(a, m):   # (high, low) words of a * m, through halves of a
+        mid = (a >> 16) * m + ((a & 0xFFFF) * m >> 16)
+        return mid >> 16, a * (m & 0xFFFF) + ((a * (m >> 16) & 0xFFFF) << 16) & low
+
+    for _ in range(10):
+        (high0, low0), (high2, low2) = product(c[0], 0xD2511F53), product(c[2], 0xCD9E8D57)
+        c = [high2 ^ c[1] ^ k[0], low2, high0 ^ c[3] ^ k[1], low0]
+        k = [k[0] + 0x9E3779B9 & low, k[1] + 0xBB67AE85 & low]
+    words = torch.stack(c, -1)
+    return torch.stack((words & 0xFFFF, words >> 16), -1).reshape(rows, groups * 8)[:, :cols] >= round(65536 * p)
+
+
+def _host_total(x, rng, p, residual):
+    if not 0 <= p <= 1:
+        raise ValueError(f"p must be between 0 and 1, got {p}")
+    threshold = round(65536 * p)
+    total = x
+    if threshold > 0:
+        keep = dropout_mask(rng, x.numel() // max(1, x.shape[-1]), x.shape[-1], p).reshape(x.shape)
+        scale = 65536 / (65536 - threshold) if threshold < 65536 else 0.0
+        total = torch.where(keep, x * scale, torch.zeros((), dtype=x.dtype))
+    return total if residual is None else residual + total
+
+
+def _host_norm(x, weight, bias, eps):
+    wide = x if x.dtype == torch.float64 else x.float()
+    centred = wide - wide.mean(-1, keepdim=True)
+    y = centred * torch.rsqrt(centred.square().mean(-1, keepdim=True) + eps)
+    if weight is not None:
+        y = y * weight
+    if bias is not None:
+        y = y + bias
+    return y.to(x.dtype)
+
+
+class LayerNorm(nn.Module):
+    """``layer_norm`` over ``size`` features, with ``weight`` and ``bias`` (``elementwise_affine``) as ``nn.LayerNorm``
+    names them."""
+
+    def __init__(self, size, eps=1e-5, elementwise_affine=True, bias=True):
+        super().__init__()
+        self.size, self.eps = size, eps
+        self.weight = nn.Parameter(torch.ones(size)) if elementwise_affine else None
+        self.bias = nn.Parameter(torch.zeros(size)) if elementwise_affine and bias else None
+
+    def forward(self, x):
+        return layer_norm(x, self.weight, self.bias, self.eps)
+
+
+class _Dropping(nn.Module):
+    """Holds ``p`` and the generator's (seed, call), part of the state dict: a resumed run goes on where it stopped."""
+
+    def __init__(self, p):
+        super().__init__()
+        if not 0 <= p <= 1:
+            raise ValueError(f"p must be between 0 and 1, got {p}")
+        self.p = p
+        self.register_buffer("rng", torch.stack((torch.randint(1 << 62, ()), torch.zeros((), dtype=torch.int64))))
+
+    def _draw(self):
+        """(rng of this call, p): nothing is dropped outside of training."""
+        if not self.training or self.p == 0:
+            return None, 0.0
+        return rng_next(self.rng), self.p
+
+
+class DropoutAdd(_Dropping):
+    """``residual + dropout(x)``, another mask at every call."""
+
+    def forward(self, x, residual=None):
+        rng, p = self._draw()
+        return x if p == 0 and residual is None else dropout_add(x, rng, p, residual)
+
+
+class DropoutAddLayerNorm(_Dropping):
+    """``(layer_norm(sum), sum)`` with ``sum = residual + dropout(x)``: the end of one block and the norm of the next."""
+
+    def __init__(self, size, p=0.1, eps=1e-5):
+        super().__init__(p)
+        self.size, self.eps = size, eps
+        self.weight = nn.Parameter(torch.ones(size))
+        self.bias = nn.Parameter(torch.zeros(size))
+
+    def forward(self, x, residual=None):
+        rng, p = self._draw()
+        return dropout_add_layer_norm(x, rng, p, residual, self.weight, self.bias, self.eps)

@@ -25,6 +25,7 @@ extern "C" {
 
 #define BF_F32 0
 #define BF_C64 1
+#define BF_BF16 2 /* the operators beside the multiply only (bf_rowwise_*, bf_recurrence_*, bf_linear_xent_*) */
 
 #define BF_OK 0
 #define BF_ERR_INVALID (-1)     /* bad shape / stride / argument                      */
@@ -302,6 +303,111 @@ int bf_layer_bw(const bf_layer *l, const void *input, const void *grad, const vo
 int bf_butterfly_multiply_bw_noalloc(const bf_problem *p, const void *twiddle, const void *input,
                                      const void *grad, void *d_twiddle, void *d_input,
                                      void *stream);
+
+/* ---- beside the multiply: operators of a block built from butterfly layers ------------------- */
+/* No counterpart in the reference's operator set: what its users take from PyTorch there.        */
+
+/* Rows of a dropout, residual addition and layer norm, each part optional:
+ *   sum = residual + (keep ? x * scale : 0),  y = (sum - mean) / sqrt(var + eps) * weight + bias
+ * Columns are adjacent, rows `*_stride` elements apart (0: one row for all); sum, y and every
+ * gradient are dense (rows, cols).  Statistics and sums are formed in float.                    */
+typedef struct bf_rowwise {
+    int32_t dtype;       /* BF_F32 or BF_BF16: x, residual, sum, y and their gradients            */
+    int32_t param_dtype; /* BF_F32 or dtype: weight, bias and their gradients                     */
+    int64_t rows, cols;
+    int64_t x_stride;    /* of x; bw: of sum                                                      */
+    int64_t residual_stride, grad_y_stride, grad_sum_stride;
+    double drop_probability; /* p in [0, 1], in steps of 1/65536: t = round(65536 p)              */
+    double eps;
+} bf_rowwise;
+
+/* The generator of dropped elements is Philox4x32-10: key = the 64 bits of rng[0] (a seed), counter =
+ * (column / 8, row, low and high half of rng[1] (the number of the call)); column c of a row takes
+ * bits 16 (c % 2) .. + 15 of word (c % 8) / 2 and is kept where they are >= t, scaled by
+ * 65536 / (65536 - t).  No mask is stored: forward and backward make the same one from rng, two
+ * device integers.
+ * bf_rng_next: taken = state, then state[1] += 1, in stream order: what a module draws per call
+ * (also from a recorded graph, whose every replay then drops other elements).                   */
+int bf_rng_next(int64_t *state, int64_t *taken, void *stream);
+
+/* residual, rng (when drop_probability is 0), weight (ones), bias (zeros) may be NULL; sum or y may be NULL
+ * (not wanted; without y there is no norm and no weight, bias or stats).  stats: (rows, 2) floats,
+ * the mean and 1 / sqrt(var + eps) of each row, for the backward call; may be NULL.              */
+int bf_rowwise_fw(const bf_rowwise *p, const void *x, const void *residual, const int64_t *rng,
+                  const void *weight, const void *bias, void *sum, void *y, float *stats, void *stream);
+
+/* Backward of a call with a norm (without one it is bf_rowwise_fw on the gradient).  sum: what the forward
+ * call normalised (x itself where nothing was dropped or added).  grad_sum, weight and every
+ * result may be NULL.  d_residual is also the gradient of sum; d_x = d_residual through the mask.
+ * d_weight and d_bias are summed in a fixed order (bitwise reproducible) through the workspace. */
+size_t bf_rowwise_bw_workspace_bytes(const bf_rowwise *p);
+int bf_rowwise_bw(const bf_rowwise *p, const void *sum, const void *grad_y, const void *grad_sum,
+                  const int64_t *rng, const void *weight, const float *stats, void *d_x,
+                  void *d_residual, void *d_weight, void *d_bias, void *workspace,
+                  size_t workspace_bytes, void *stream);
+
+/* Gated linear recurrence over sequences, channel by channel: h_t = a_t h_{t-1} + b_t from h_{-1} = state, with
+ * a = 1 / (1 + exp(-gate)), b = (1 - a) x (sigmoid) or a = gate, b = x (linear).  Rows are (batch, steps,
+ * channels) with adjacent channels and the given strides of batch and steps; h and the gradients are dense.
+ * States (state, last and their gradients) are dense (batch, channels) in float, or complex64 for
+ * BF_C64.  reset (bytes, may be NULL): where set, h_{t-1} counts as zero whatever it is (a
+ * packed document starts).                                                                      */
+typedef struct bf_recurrence {
+    int32_t dtype;   /* BF_F32, BF_BF16 or (linear) BF_C64 */
+    int32_t sigmoid; /* 0: linear                          */
+    int64_t batch, steps, channels;
+    int64_t gate_stride[2], x_stride[2], grad_stride[2], reset_stride[2]; /* (batch, steps) */
+} bf_recurrence;
+
+/* Of either call: 0 where the sequences stay whole. */
+size_t bf_recurrence_workspace_bytes(const bf_recurrence *p);
+/* state (zeros), reset and last (not wanted) may be NULL. */
+int bf_recurrence_fw(const bf_recurrence *p, const void *gate, const void *x, const void *state,
+                     const uint8_t *reset, void *h, void *last, void *workspace,
+                     size_t workspace_bytes, void *stream);
+/* h: what the forward call wrote.  grad, grad_last (zeros) and d_state (not wanted) may be NULL, x too for
+ * linear gates.                                                                                 */
+int bf_recurrence_bw(const bf_recurrence *p, const void *gate, const void *x, const void *state,
+                     const uint8_t *reset, const void *h, const void *grad, const void *grad_last,
+                     void *d_gate, void *d_x, void *d_state, void *workspace,
+                     size_t workspace_bytes, void *stream);
+/* One step of every sequence, for serving: gate, x, h (batch, channels), the state updated in place.
+ * steps and the strides of steps are not read.                                                  */
+int bf_recurrence_step(const bf_recurrence *p, const void *gate, const void *x, void *state,
+                       void *h, void *stream);
+
+/* Softmax cross entropy of logits = hidden weight^T (rows, vocab), which are never held as a whole:
+ *   loss_i = log sum_v exp(l_iv) - l_i,target(i);  a row whose target is ignore_index counts for
+ *   nothing (loss 0, gradient 0); a target that is no entry of the vocabulary makes loss and
+ *   gradients NaN.  Mean: over the rows that count (NaN if there is none).
+ * hidden (rows, features), weight (vocab, features), features adjacent, rows `*_stride` elements
+ * apart, weight 16-byte aligned.  BF_BF16: products of bfloat16 with sums in float, the logits' gradient in bfloat16.
+ * BF_F32: every factor as two float16 numbers of together 22 bits, sums in float.
+ * Gradients are dense, summed in a fixed order.                                                 */
+#define BF_XENT_NONE 0
+#define BF_XENT_MEAN 1
+#define BF_XENT_SUM 2
+typedef struct bf_linear_xent {
+    int32_t dtype;     /* BF_F32 or BF_BF16: hidden, weight and their gradients */
+    int32_t reduction; /* BF_XENT_*                                             */
+    int64_t rows, features, vocab;
+    int64_t hidden_stride, weight_stride;
+    int64_t ignore_index;
+} bf_linear_xent;
+
+/* The workspace (256-byte aligned) holds hidden and, where it cannot be read as it lies (float, rows that
+ * 16 bytes do not divide), weight in the products' form, and backward the logits' gradient over a
+ * piece of the vocabulary, up to some 256 MiB.                                                   */
+size_t bf_linear_xent_fw_workspace_bytes(const bf_linear_xent *p);
+size_t bf_linear_xent_bw_workspace_bytes(const bf_linear_xent *p);
+/* loss: one float, or (rows) with BF_XENT_NONE.  lse: (rows), for the backward call. */
+int bf_linear_xent_fw(const bf_linear_xent *p, const void *hidden, const void *weight,
+                      const int64_t *target, float *loss, float *lse, void *workspace,
+                      size_t workspace_bytes, void *stream);
+/* grad: the loss's gradient, one float or (rows).  d_hidden or d_weight may be NULL. */
+int bf_linear_xent_bw(const bf_linear_xent *p, const void *hidden, const void *weight,
+                      const int64_t *target, const float *lse, const float *grad, void *d_hidden,
+                      void *d_weight, void *workspace, size_t workspace_bytes, void *stream);
 
 #ifdef __cplusplus
 }
