@@ -43,32 +43,35 @@ struct MatOperand {
     int64_t bytes;         // of a plane from base on that may be read: loads beyond are zero
 };
 
+// lds_addr: where the wavefront's 64 units go (wave-uniform); offsets from the descriptor's base, within 2^31.
+// (m0 is not saved: nothing else in these kernels uses it, and the compiler is told; its warning is that it
+// will not keep it for anybody either)
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
 __device__ __forceinline__ void load_unit_to_lds(MatDesc desc, unsigned lds_addr, int voff, int soff)
 {
-    int keep_m0;
-    asm volatile("s_mov_b32 %0, m0\n\t"
-                 "s_mov_b32 m0, %1\n\t"
+    asm volatile("s_mov_b32 m0, %0\n\t"
                  "s_nop 0\n\t"
-                 "buffer_load_dwordx4 %2, %3, %4 offen lds\n\t"
-                 "s_mov_b32 m0, %0"
-                 : "=&s"(keep_m0)
-                 : "s"(__builtin_amdgcn_readfirstlane(lds_addr)), "v"(voff), "s"(desc), "s"(soff)
-                 : "memory");
+                 "buffer_load_dwordx4 %1, %2, %3 offen lds"
+                 :
+                 : "s"(lds_addr), "v"(voff), "s"(desc), "s"(soff)
+                 : "memory", "m0");
 }
+#pragma clang diagnostic pop
 
-// One operand's way into LDS: SIZE rows or columns of it, k step by k step.
+// One operand's way into LDS: SIZE rows or columns of it, k step by k step.  From step to step only the lanes' offsets
+// move (a wavefront that is alone on its SIMD has few instructions to spare between MFMAs); the
+// descriptor's base moves every kSteps() steps, before they pass 2^30.
 template <MatLayout LAYOUT, int SIZE, bool SPREAD>
 struct MatFeed {
     static constexpr int kLoads = SIZE / 32;                 // of a wavefront a step
     static constexpr int kUnits = SIZE / 8;                  // kCols: 16-byte units of a k row
     static constexpr int kPerLoad = LAYOUT == kRows ? 8 : 64 / kUnits;   // rows that a load covers
     static constexpr int kVariants = LAYOUT == kRows ? 1 : 4;
-    const char *at;
-    int64_t left;
-    int stride, wave;
-    int voff[kVariants];
+    int stride, wave, first_voff[kVariants], voff[kVariants], soff[kLoads];
+    MatDesc desc;
 
-    __device__ __forceinline__ void init(const MatOperand &o, int first)
+    __device__ __forceinline__ void init(const MatOperand &o)
     {
         const int lane = threadIdx.x & 63;
         wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -77,14 +80,21 @@ struct MatFeed {
             // SPREAD: LDS row 16 t + i holds row 64 (t / 4) + 16 (i / 4) + 4 (t % 4) + i % 4, so that the
             // four rows a lane gets of each of four tiles' results are sixteen neighbours
             const int row = SPREAD ? (lane >> 5) * 16 + ((lane >> 3) & 3) : lane >> 3;
-            voff[0] = row * stride + ((lane & 7) ^ (lane >> 3)) * 16;
+            first_voff[0] = row * stride + ((lane & 7) ^ (lane >> 3)) * 16;
         } else {
             const int row = lane / kUnits, unit = lane % kUnits;
 #pragma unroll
-            for (int v = 0; v < 4; ++v) voff[v] = row * stride + ((unit ^ (place(v, row) << 1)) * 16);
+            for (int v = 0; v < 4; ++v) first_voff[v] = row * stride + ((unit ^ (place(v, row) << 1)) * 16);
         }
-        start(o, first, 0);
+#pragma unroll
+        for (int j = 0; j < kLoads; ++j) {
+            const int jj = wave * kLoads + j;
+            soff[j] = (LAYOUT == kRows && SPREAD ? (jj >> 3) * 64 + (jj & 1) * 32 + ((jj >> 1) & 3) * 4 : jj * kPerLoad) * stride;
+        }
     }
+
+    // steps that one base serves
+    __device__ __forceinline__ int steps() const { return LAYOUT == kRows ? 1 << 20 : max(1, (1 << 30) / (kMatK * stride) - 1); }
 
     // s(r) of the rows that load number j of a wavefront covers, as far as it depends on j (v) and the lane's row
     static __device__ __forceinline__ int place(int v, int row)
@@ -96,31 +106,27 @@ struct MatFeed {
         return LAYOUT == kRows ? 0 : kPerLoad == 2 ? (j & 1) | (j >> 2 & 1) << 1 : j >> 1 & 1;
     }
 
-    // to k step `step`, SIZE rows or columns from `first` on
-    __device__ __forceinline__ void start(const MatOperand &o, int first, int64_t step, int plane = 0)
+    // to k step `step`, SIZE rows or columns from `first` on; nothing: loads of zeros from there on
+    __device__ __forceinline__ void start(const MatOperand &o, int first, int64_t step, int plane, bool nothing)
     {
         const int64_t skip = LAYOUT == kRows ? first * o.stride + step * (kMatK * 2) : step * kMatK * o.stride + (int64_t)first * 2;
-        at = o.base + plane * o.plane + skip;
-        left = o.bytes - skip;
-    }
-
-    __device__ __forceinline__ void issue(unsigned lds)
-    {
-        const unsigned long long a = (unsigned long long)at;
-        MatDesc d;
-        d.x = __builtin_amdgcn_readfirstlane((int)(unsigned)a);
-        d.y = __builtin_amdgcn_readfirstlane((int)((a >> 32) & 0xffff));
-        d.z = __builtin_amdgcn_readfirstlane((int)(left < 0 ? 0 : left < 0x7fffff00 ? left : 0x7fffff00));
-        d.w = 0x00020000;
+        const unsigned long long a = (unsigned long long)(o.base + plane * o.plane + skip);
+        const int64_t left = nothing ? 0 : o.bytes - skip;
+        desc.x = __builtin_amdgcn_readfirstlane((int)(unsigned)a);
+        desc.y = __builtin_amdgcn_readfirstlane((int)((a >> 32) & 0xffff));
+        desc.z = __builtin_amdgcn_readfirstlane((int)(left < 0 ? 0 : left < 0x7fffff00 ? left : 0x7fffff00));
+        desc.w = 0x00020000;
 #pragma unroll
-        for (int j = 0; j < kLoads; ++j) {
-            const int jj = wave * kLoads + j;
-            const int row = LAYOUT == kRows && SPREAD ? (jj >> 3) * 64 + (jj & 1) * 32 + ((jj >> 1) & 3) * 4 : jj * kPerLoad;
-            load_unit_to_lds(d, lds + jj * 1024, voff[variant(j)], row * stride);
-        }
-        const int64_t step = LAYOUT == kRows ? kMatK * 2 : (int64_t)kMatK * stride;
-        at += step;
-        left -= step;
+        for (int v = 0; v < kVariants; ++v) voff[v] = first_voff[v];
+    }
+    __device__ __forceinline__ void load(unsigned lds, int j) const
+    {
+        load_unit_to_lds(desc, lds + (wave * kLoads + j) * 1024, voff[variant(j)], soff[j]);
+    }
+    __device__ __forceinline__ void advance()
+    {
+#pragma unroll
+        for (int v = 0; v < kVariants; ++v) voff[v] += LAYOUT == kRows ? kMatK * 2 : kMatK * stride;
     }
 };
 
@@ -147,42 +153,57 @@ struct MatReader {
     }
 
     template <int HALF>
-    __device__ __forceinline__ void read(LdsByte *buffer, Frag (&f)[kTiles]) const
+    __device__ __forceinline__ Frag read(LdsByte *buffer, int t) const
     {
-#pragma unroll
-        for (int t = 0; t < kTiles; ++t) {
-            if constexpr (LAYOUT == kRows) {
-                f[t] = *(__attribute__((address_space(3))) const Frag *)(buffer + addr[HALF] + t * 2048);
-            } else {
-                typedef short Quad16 __attribute__((ext_vector_type(4)));
-                typedef __attribute__((address_space(3))) Quad16 LdsQuad;
-                LdsByte *a = buffer + addr[t] + HALF * 32 * SIZE * 2;
-                const Quad16 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsQuad *)a);
-                const Quad16 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsQuad *)(a + 4 * SIZE * 2));
-                typedef short Oct16 __attribute__((ext_vector_type(8)));
-                f[t] = __builtin_bit_cast(Frag, (Oct16)__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
-            }
+        if constexpr (LAYOUT == kRows) {
+            return *(__attribute__((address_space(3))) const Frag *)(buffer + addr[HALF] + t * 2048);
+        } else {
+            typedef short Quad16 __attribute__((ext_vector_type(4)));
+            typedef short Oct16 __attribute__((ext_vector_type(8)));
+            typedef __attribute__((address_space(3))) Quad16 LdsQuad;
+            LdsByte *a = buffer + addr[t] + HALF * 32 * SIZE * 2;
+            const Quad16 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsQuad *)a);
+            const Quad16 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsQuad *)(a + 4 * SIZE * 2));
+            return __builtin_bit_cast(Frag, (Oct16)__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
         }
     }
 };
 
+// c += a b, the sums in accumulation registers: as builtins the compiler moves every one of 256 of them
+// to ordinary registers and back once a step.  What it then no longer sees: two wait states between a vector
+// instruction that writes an operand and the MFMA that reads it (mfma_operand, behind which an operand is where
+// its MFMAs read it), and those between the last MFMA and the first read of its sums (mfma_settle; a sum's next
+// MFMA is kMT kNT of them away).
 template <bool F16>
-__device__ __forceinline__ Acc4 mfma(Frag a, Frag b, Acc4 c)
+__device__ __forceinline__ void mfma(Frag a, Frag b, Acc4 &c)
 {
-    if constexpr (F16)
-        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
-    else
-        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    if constexpr (F16) asm("v_mfma_f32_16x16x32_f16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
+    else asm("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
 }
 
-// The tile at (m0, n0) over k steps first .. first + count - 1 (count may be zero).  acc[mt][nt][r] is element
-// (m, n) with n = n0 + BN / 2 * (wave & 1) + 16 nt + lane % 16 and m = m0 + BM / 2 * (wave >> 1) + what
-// tile_row() says.  F16: both operands in two planes.
+__device__ __forceinline__ void mfma_operand(Frag &f) { asm volatile("s_nop 1" : "+v"(f)); }
+
+template <int MT, int NT>
+__device__ __forceinline__ void mfma_settle(Acc4 (&acc)[MT][NT])
+{
+    asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");
+    // (every sum passes through here: none is read in front of it)
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < NT; ++j) asm volatile("" : "+a"(acc[i][j]));
+}
+
+// Tiles of BM x BN, one after another, as one stream of k steps: while a step is computed the one after the next is
+// asked for, across the boundary between two tiles too, so the next tile's first steps arrive while the
+// sums of the one before are dealt with.  acc[mt][nt][r] is element (m, n) with n = n0 + BN / 2 * (wave & 1) + 16 nt +
+// lane % 16 and m = m0 + BM / 2 * (wave >> 1) + what tile_row() says.  F16: both operands in two planes.
 template <MatLayout LA, MatLayout LB, bool F16, int BM, int BN, bool SPREAD>
-struct MatTile {
-    static constexpr int kMT = BM / 32, kNT = BN / 32;
+struct MatTiles {
+    static constexpr int kMT = BM / 32, kNT = BN / 32, kPasses = F16 ? 3 : 1;
     static constexpr int kBytesA = BM * kMatK * 2, kBytesB = BN * kMatK * 2, kBuffer = kBytesA + kBytesB;
     static constexpr int kLds = 2 * kBuffer;
+    static_assert(kMT == kNT, "reads and loads are dealt out to rows of MFMAs");
 
     // m of result r of tile mt, from the wavefront's first
     static __device__ __forceinline__ int tile_row(int mt)
@@ -191,73 +212,143 @@ struct MatTile {
         return SPREAD ? (mt >> 2) * 64 + g * 16 + (mt & 3) * 4 : mt * 16 + g * 4;
     }
 
-    static __device__ __forceinline__ void run(const MatOperand &a, const MatOperand &b, int m0, int n0, int64_t first,
-                                               int count, char *lds_bytes, Acc4 (&acc)[kMT][kNT])
+    const MatOperand &a, &b;
+    LdsByte *near;
+    unsigned lds, buffer = 0;
+    MatFeed<LA, BM, SPREAD> feed_a;
+    MatFeed<LB, BN, false> feed_b;
+    MatReader<LA, BM> read_a;
+    MatReader<LB, BN> read_b;
+    Frag fa[2][kMT], fb[2][kNT];
+    // the tile that is asked for: its place, its first k step, their number; how far it is asked for
+    int m0 = 0, n0 = 0, first = 0, count = 0, pass = kPasses - 1, fed = 0, until = 0;
+
+    __device__ __forceinline__ MatTiles(const MatOperand &a_, const MatOperand &b_, char *lds_bytes)
+        : a(a_), b(b_), near((LdsByte *)lds_bytes), lds((unsigned)(unsigned long long)(LdsByte *)lds_bytes)
     {
-        LdsByte *near = (LdsByte *)lds_bytes;
-        const unsigned lds = (unsigned)(unsigned long long)near;
         const int wave = threadIdx.x >> 6;
+        feed_a.init(a);
+        feed_b.init(b);
+        read_a.init(0, wave >> 1);
+        read_b.init(kBytesA, wave & 1);
+    }
+
+    // next(m0, n0, first, count): the next tile (count >= 1), or false when there is none
+    template <typename Next>
+    __device__ __forceinline__ void feed_begin(Next &next)
+    {
+        if (fed == until) {
+            if (fed == count) {
+                fed = 0;
+                if (++pass == kPasses) {
+                    pass = 0;
+                    if (!next(m0, n0, first, count)) count = 0x7fffffff;
+                }
+            }
+            // (the small products first; behind the last tile loads of nothing)
+            const bool nothing = count == 0x7fffffff;
+            feed_a.start(a, m0, first + (nothing ? 0 : fed), F16 && pass == 1, nothing);
+            feed_b.start(b, n0, first + (nothing ? 0 : fed), F16 && pass == 0, nothing);
+            until = min(count - fed, min(feed_a.steps(), feed_b.steps())) + fed;
+        }
+        ++fed;
+    }
+    __device__ __forceinline__ void feed_end()
+    {
+        feed_a.advance();
+        feed_b.advance();
+    }
+
+    template <typename Next>
+    __device__ __forceinline__ void feed(unsigned to, Next &next)
+    {
+        feed_begin(next);
+#pragma unroll
+        for (int i = 0; i < kMT; ++i) {
+            feed_a.load(lds + to, i);
+            feed_b.load(lds + to + kBytesA, i);
+        }
+        feed_end();
+    }
+
+    static __device__ __forceinline__ void barrier()
+    {
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+    }
+
+    // Before the first step.
+    template <typename Next>
+    __device__ __forceinline__ void begin(Next &next)
+    {
+        feed(0, next);
+        feed(kBuffer, next);
+        // (the second step's loads may still be on their way)
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kMT + kNT) : "memory");
+        barrier();
+#pragma unroll
+        for (int i = 0; i < kMT; ++i) {
+            fa[0][i] = read_a.template read<0>(near, i);
+            fb[0][i] = read_b.template read<0>(near, i);
+        }
+    }
+
+    // Behind the last step: no load may write LDS that is another workgroup's.
+    static __device__ __forceinline__ void end() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory"); }
+
+    // One k step.  Reads and loads are spread between the MFMAs, which take 16 clocks each and wait for nothing
+    // but their operands: in front of each row of kNT of them two reads and two loads.
+    template <typename Next>
+    __device__ __forceinline__ void step(Next &next, Acc4 (&acc)[kMT][kNT])
+    {
+#pragma unroll
+        for (int i = 0; i < kMT; ++i) {
+            fa[1][i] = read_a.template read<1>(near + buffer, i);
+            fb[1][i] = read_b.template read<1>(near + buffer, i);
+            if (i == 0) {
+#pragma unroll
+                for (int j = 0; j < kNT; ++j) mfma_operand(fb[0][j]);
+            }
+            mfma_operand(fa[0][i]);
+#pragma unroll
+            for (int j = 0; j < kNT; ++j) mfma<F16>(fa[0][i], fb[0][j], acc[i][j]);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        // this buffer is read, the other one's loads have landed, for all four wavefronts
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        barrier();
+        feed_begin(next);
+        const unsigned other = kBuffer - buffer;
+#pragma unroll
+        for (int i = 0; i < kMT; ++i) {
+            feed_a.load(lds + buffer, i);
+            feed_b.load(lds + buffer + kBytesA, i);
+            fa[0][i] = read_a.template read<0>(near + other, i);
+            fb[0][i] = read_b.template read<0>(near + other, i);
+            if (i == 0) {
+#pragma unroll
+                for (int j = 0; j < kNT; ++j) mfma_operand(fb[1][j]);
+            }
+            mfma_operand(fa[1][i]);
+#pragma unroll
+            for (int j = 0; j < kNT; ++j) mfma<F16>(fa[1][i], fb[1][j], acc[i][j]);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        feed_end();
+        buffer = other;
+    }
+
+    // A tile's sums, over `steps` steps.
+    template <typename Next>
+    __device__ __forceinline__ void run(int steps, Next &next, Acc4 (&acc)[kMT][kNT])
+    {
 #pragma unroll
         for (int i = 0; i < kMT; ++i)
 #pragma unroll
             for (int j = 0; j < kNT; ++j) acc[i][j] = Acc4{0.0f, 0.0f, 0.0f, 0.0f};
-        const int steps = count * (F16 ? 3 : 1);
-        if (steps <= 0) return;
-        MatFeed<LA, BM, SPREAD> feed_a;
-        MatFeed<LB, BN, false> feed_b;
-        feed_a.init(a, m0);
-        feed_b.init(b, n0);
-        MatReader<LA, BM> read_a;
-        MatReader<LB, BN> read_b;
-        read_a.init(0, wave >> 1);
-        read_b.init(kBytesA, wave & 1);
-        int pass = 0, fed = 0;
-        auto feed = [&](unsigned buffer) {
-            if (fed == 0) {
-                // (the small products first)
-                feed_a.start(a, m0, first, F16 && pass == 1);
-                feed_b.start(b, n0, first, F16 && pass == 0);
-            }
-            feed_a.issue(lds + buffer);
-            feed_b.issue(lds + buffer + kBytesA);
-            if (++fed == count) {
-                fed = 0;
-                ++pass;
-            }
-        };
-        auto arrive = [&] {
-            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-            __builtin_amdgcn_s_barrier();
-            asm volatile("" ::: "memory");
-        };
-        Frag fa[2][kMT], fb[2][kNT];
-        feed(0);
-        arrive();
-        if (steps > 1) feed(kBuffer);
-        read_a.template read<0>(near, fa[0]);
-        read_b.template read<0>(near, fb[0]);
-        for (int step = 0; step < steps; ++step) {
-            const unsigned buffer = (unsigned)(step & 1) * kBuffer;
-            read_a.template read<1>(near + buffer, fa[1]);
-            read_b.template read<1>(near + buffer, fb[1]);
-#pragma unroll
-            for (int i = 0; i < kMT; ++i)
-#pragma unroll
-                for (int j = 0; j < kNT; ++j) acc[i][j] = mfma<F16>(fa[0][i], fb[0][j], acc[i][j]);
-            // this buffer is read, the other one's loads have landed, for all four wavefronts
-            __builtin_amdgcn_sched_barrier(0);
-            arrive();
-            if (step + 2 < steps) feed(buffer);
-            if (step + 1 < steps) {
-                read_a.template read<0>(near + kBuffer - buffer, fa[0]);
-                read_b.template read<0>(near + kBuffer - buffer, fb[0]);
-            }
-#pragma unroll
-            for (int i = 0; i < kMT; ++i)
-#pragma unroll
-                for (int j = 0; j < kNT; ++j) acc[i][j] = mfma<F16>(fa[1][i], fb[1][j], acc[i][j]);
-            __builtin_amdgcn_sched_barrier(0);
-        }
+        mfma_settle(acc);
+        for (int s = 0; s < steps * kPasses; ++s) step(next, acc);
+        mfma_settle(acc);
     }
 };
 

@@ -34,26 +34,30 @@ bool weight_in_place(const bf_linear_xent *p)
            p->weight_stride <= (1 << 20);
 }
 
-// Tiles of 256 x 256 where there are enough of them for three quarters of the compute units, of 128 x 128 otherwise.
-bool large_tiles(int64_t m, int64_t n) { return ((m + 255) / 256) * ((n + 255) / 256) >= 192; }
-
 struct Product {
     bool large = false;
     int tiles_m = 0, tiles_n = 0, splits = 1;
 };
 
-// k steps are cut where the tiles alone leave compute units idle, down to 16 steps a part.
+// Tiles of 256 x 256 where there are enough of them, with the k steps cut into parts of at least 16 if they may be,
+// for three quarters of the compute units; of 128 x 128 otherwise, cut for two workgroups a compute unit.
 Product product(int64_t m, int64_t n, int64_t steps, bool may_split)
 {
+    auto tiles = [&](int64_t side) { return ((m + side - 1) / side) * ((n + side - 1) / side); };
+    const int64_t parts = may_split ? std::min<int64_t>(std::max<int64_t>(steps / 16, 1), 32) : 1;
     Product r;
-    r.large = large_tiles(m, n);
-    const int64_t t = r.large ? 256 : 128;
+    r.large = tiles(256) * parts >= 192;
+    const int64_t t = r.large ? 256 : 128, here = std::max<int64_t>(tiles(t), 1);
     r.tiles_m = (int)((m + t - 1) / t);
     r.tiles_n = (int)((n + t - 1) / t);
-    const int64_t tiles = (int64_t)r.tiles_m * r.tiles_n;
-    if (may_split && !r.large)
-        r.splits = (int)std::max<int64_t>(1, std::min<int64_t>({512 / std::max<int64_t>(tiles, 1), steps / 16, 32}));
+    r.splits = (int)std::max<int64_t>(1, std::min<int64_t>(parts, (r.large ? 256 : 512) / here));
     return r;
+}
+
+// As many as are at work at a time: one a compute unit for large tiles (128 KiB of LDS), two for small ones.
+unsigned workgroups(const Product &r)
+{
+    return (unsigned)std::min<int64_t>((int64_t)r.tiles_m * r.tiles_n * r.splits, r.large ? 256 : 512);
 }
 
 constexpr size_t kPieceBytes = (size_t)256 << 20;   // d_l of a piece of the vocabulary
@@ -137,7 +141,7 @@ void pack(const bf_linear_xent *p, const void *x, char *out, int64_t out_rows, i
 {
     if (p->dtype == BF_F32 && rows > 0) {
         unsigned *largest = which ? &scalars->weight_max : &scalars->hidden_max;
-        xent_largest_kernel<<<dim3((unsigned)std::min<int64_t>(rows, 2048)), dim3(256), 0, s>>>(
+        xent_largest_kernel<<<dim3((unsigned)std::min<int64_t>((rows + 3) / 4, 1024)), dim3(256), 0, s>>>(
             static_cast<const float *>(x), rows, p->features, x_stride, index, scalars, largest);
     }
     const XentPackArgs a = {x, out, out_rows, p->features, x_stride, stride, (int64_t)plane, index, scalars, which};
@@ -170,7 +174,7 @@ void prepare(const bf_linear_xent *p, const XentPlan &r, const void *hidden, con
 template <bool F16, bool BACKWARD>
 void launch_logits(const Product &r, const XentTileArgs &a, hipStream_t s)
 {
-    const dim3 grid((unsigned)(r.tiles_m * r.tiles_n)), threads(kMatThreads);
+    const dim3 grid(workgroups(r)), threads(kMatThreads);
     if (r.large) xent_logits_kernel<F16, 256, 256, BACKWARD><<<grid, threads, 0, s>>>(a);
     else xent_logits_kernel<F16, 128, 128, BACKWARD><<<grid, threads, 0, s>>>(a);
 }
@@ -178,7 +182,7 @@ void launch_logits(const Product &r, const XentTileArgs &a, hipStream_t s)
 template <MatLayout LB>
 void launch_grad(const bf_linear_xent *p, const Product &r, const XentGradArgs &a, hipStream_t s)
 {
-    const dim3 grid((unsigned)(r.tiles_m * r.tiles_n * r.splits)), threads(kMatThreads);
+    const dim3 grid(workgroups(r)), threads(kMatThreads);
     if (p->dtype == BF_F32) {
         if (r.large) xent_grad_kernel<float, LB, 256, 256><<<grid, threads, 0, s>>>(a);
         else xent_grad_kernel<float, LB, 128, 128><<<grid, threads, 0, s>>>(a);

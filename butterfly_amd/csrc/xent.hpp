@@ -90,13 +90,19 @@ __global__ __launch_bounds__(kXentThreads) void xent_rows_kernel(XentRowsArgs a)
 __global__ __launch_bounds__(256) void xent_largest_kernel(const float *x, int64_t rows, int64_t cols, int64_t stride,
                                                            const int *index, const XentScalars *scalars, unsigned *largest)
 {
+    __shared__ unsigned lds[4];
     const int64_t n = index ? scalars->counted : rows;
     unsigned m = 0;
-    for (int64_t r = blockIdx.x; r < n; r += gridDim.x) {
+    for (int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); r < n; r += (int64_t)gridDim.x * 4) {
         const float *row = x + (index ? index[r] : r) * stride;
-        for (int64_t c = threadIdx.x; c < cols; c += 256) {
-            const unsigned v = __float_as_uint(row[c]) & 0x7fffffffu;
-            m = v > m ? v : m;
+        for (int c = (threadIdx.x & 63) * 8; c < (int)cols; c += 512) {
+            float v[8];
+            load8(row, c, (int)cols, 0.0f, v);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const unsigned b = __float_as_uint(v[i]) & 0x7fffffffu;
+                m = b > m ? b : m;
+            }
         }
     }
 #pragma unroll
@@ -104,7 +110,12 @@ __global__ __launch_bounds__(256) void xent_largest_kernel(const float *x, int64
         const unsigned v = (unsigned)__shfl_xor((int)m, d, 64);
         m = v > m ? v : m;
     }
-    if ((threadIdx.x & 63) == 0 && m > 0) atomicMax(largest, m);
+    // (one atomic a workgroup: all of them go to one address, one after another)
+    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = m;
+    __syncthreads();
+    if (threadIdx.x != 0) return;
+    for (int w = 1; w < 4; ++w) m = lds[w] > m ? lds[w] : m;
+    if (m > 0) atomicMax(largest, m);
 }
 
 // 2^e that brings the number to 2^14 .. 2^15 (infinite, NaN or zero: 1)
@@ -116,13 +127,18 @@ __device__ __forceinline__ float scale_of(unsigned bits)
     return __uint_as_float((unsigned)((up > 100 ? 100 : up) + 127) << 23);
 }
 
-__device__ __forceinline__ uint32_t pack_f16(float a, float b)
+// Two numbers' upper and lower float16 halves.  The numbers are hidden from the compiler: rounded from the
+// product that made one of them, not from the number itself, an upper half could be another one than
+// the lower half is the rest to.
+__device__ __forceinline__ void split_f16(float a, float b, uint32_t &high, uint32_t &low)
 {
     typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
-    const f16x2 v = {(_Float16)a, (_Float16)b};
-    return __builtin_bit_cast(uint32_t, v);
+    asm("" : "+v"(a), "+v"(b));
+    const f16x2 h = {(_Float16)a, (_Float16)b};
+    const f16x2 l = {(_Float16)(a - (float)h[0]), (_Float16)(b - (float)h[1])};
+    high = __builtin_bit_cast(uint32_t, h);
+    low = __builtin_bit_cast(uint32_t, l);
 }
-__device__ __forceinline__ float rest_f16(float v) { return v - (float)(_Float16)v; }
 
 struct XentPackArgs {
     const void *x;
@@ -156,8 +172,7 @@ __global__ __launch_bounds__(256) void xent_pack_kernel(XentPackArgs a)
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
             if constexpr (F16) {
-                w[k] = pack_f16(v[2 * k] * scale, v[2 * k + 1] * scale);
-                low[k] = pack_f16(rest_f16(v[2 * k] * scale), rest_f16(v[2 * k + 1] * scale));
+                split_f16(v[2 * k] * scale, v[2 * k + 1] * scale, w[k], low[k]);
             } else {
                 w[k] = pack_bf16(v[2 * k], v[2 * k + 1]);
             }
@@ -205,76 +220,140 @@ __device__ __forceinline__ void tile_at(int id, int tiles_m, int tiles_n, int ba
     tn = in / height;
 }
 
+constexpr float kLog2e = 1.44269504088896340736f;
+
+// exp(l - v) is formed as exp2(l log2(e) + from), from = -v log2(e) rounded; the factor that undoes the rounding.
+__device__ __forceinline__ float rounded_off(float v, float from) { return __builtin_amdgcn_exp2f(-fmaf(v, kLog2e, from)); }
+
+// Workgroups stay for tile after tile (grid: as many as the chip holds at a time), so that a tile's exponentials and
+// stores run while the next one's operands arrive.
 template <bool F16, int BM, int BN, bool BACKWARD>
 __global__ __launch_bounds__(kMatThreads, 1) void xent_logits_kernel(XentTileArgs a)
 {
-    using Tile = MatTile<kRows, kRows, F16, BM, BN, true>;
+    using Tile = MatTiles<kRows, kRows, F16, BM, BN, true>;
     __shared__ __attribute__((aligned(1024))) char lds[Tile::kLds];
     const int counted = a.scalars->counted;
-    int tm, tn;
-    tile_at(xcd_order(blockIdx.x, a.tiles_m * a.tiles_n), a.tiles_m, a.tiles_n, 8, tm, tn);
-    const int m0 = tm * BM, n0 = tn * BN;
-    if (n0 >= counted) return;
-    Acc4 acc[Tile::kMT][Tile::kNT];
-    Tile::run(a.weight, a.hidden, m0, n0, 0, a.features_steps, lds, acc);
+    const int tiles_n = (counted + BN - 1) / BN, total = a.tiles_m * tiles_n;
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, part = wave >> 1;
     // (powers of two, each within the range of float)
     const float scale_h = F16 ? 1.0f / a.scalars->hidden_scale : 1.0f, scale_w = F16 ? 1.0f / a.scalars->weight_scale : 1.0f;
-    const int mw = m0 + part * (BM / 2);
+    if ((int)blockIdx.x >= total) return;
+    Tile tiles(a.weight, a.hidden, lds);
+    int ahead = blockIdx.x;
+    auto next = [&](int &m, int &n, int &first, int &count) {
+        if (ahead >= total) return false;
+        int tm, tn;
+        tile_at(xcd_order(ahead, total), a.tiles_m, tiles_n, 8, tm, tn);
+        m = tm * BM;
+        n = tn * BN;
+        first = 0;
+        count = a.features_steps;
+        ahead += gridDim.x;
+        return true;
+    };
+    tiles.begin(next);
+    for (int id = blockIdx.x; id < total; id += gridDim.x) {
+        Acc4 acc[Tile::kMT][Tile::kNT];
+        tiles.run(a.features_steps, next, acc);
+        int tm, tn;
+        tile_at(xcd_order(id, total), a.tiles_m, tiles_n, 8, tm, tn);
+        const int n0 = tn * BN, mw = tm * BM + part * (BM / 2), of = 2 * tm + part;
+        const bool whole = mw + BM / 2 <= a.vocab;   // no entry past the vocabulary's end
 #pragma unroll
-    for (int j = 0; j < Tile::kNT; ++j) {
-        const int row = n0 + (wave & 1) * (BN / 2) + j * 16 + (lane & 15);
-        const bool there = row < counted;
-        const int label = there ? a.label[row] - (int)a.first : -1;
-        if constexpr (!BACKWARD) {
-            float top = -INFINITY;
+        for (int j = 0; j < Tile::kNT; ++j) {
+            const int row = n0 + (wave & 1) * (BN / 2) + j * 16 + (lane & 15);
+            const bool there = row < counted;
+            // the label's place among the wavefront's entries, if it is one of them
+            const int label = there ? a.label[row] - (int)a.first - mw : -1;
+            const bool labelled = __any(label >= 0 && label < BM / 2);
+            if constexpr (F16) {
 #pragma unroll
-            for (int i = 0; i < Tile::kMT; ++i)
+                for (int i = 0; i < Tile::kMT; ++i) acc[i][j] = acc[i][j] * scale_h * scale_w;
+            }
+            if constexpr (!BACKWARD) {
+                if (labelled) {
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int v = mw + Tile::tile_row(i) + r;
-                    if constexpr (F16) acc[i][j][r] = acc[i][j][r] * scale_h * scale_w;
-                    if (v == label && there) a.picked[row] = acc[i][j][r];
-                    if (v < a.vocab) top = fmaxf(top, acc[i][j][r]);
+                    for (int i = 0; i < Tile::kMT; ++i)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r)
+                            if (Tile::tile_row(i) + r == label) a.picked[row] = acc[i][j][r];
                 }
-            top = fmaxf(top, __shfl_xor(top, 16, 64));
-            top = fmaxf(top, __shfl_xor(top, 32, 64));
-            // (NaN is no maximum, and an infinite one would make NaN of its own term: both show in the sum)
-            const float from = top == -INFINITY ? 0.0f : top;
-            float sum = 0.0f;
+                if (!whole) {
 #pragma unroll
-            for (int i = 0; i < Tile::kMT; ++i)
+                    for (int i = 0; i < Tile::kMT; ++i)
 #pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    if (mw + Tile::tile_row(i) + r < a.vocab) sum += __expf(acc[i][j][r] - from);
-            sum += __shfl_xor(sum, 16, 64);
-            sum += __shfl_xor(sum, 32, 64);
-            if (lane < 16 && there) a.partial[(int64_t)(2 * tm + part) * a.rows + row] = make_float2(top, sum);
-        } else {
-            const float lse = there ? a.lse[row] : 0.0f, share = there ? a.share[row] : 0.0f;
-#pragma unroll
-            for (int i = 0; i < Tile::kMT; ++i) {
-                const int v0 = mw + Tile::tile_row(i);
-                float p[4];
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const float l = (F16 ? acc[i][j][r] * scale_h * scale_w : acc[i][j][r]) - lse;
-                    p[r] = F16 ? expf(l) : __expf(l);
-                    if (v0 + r == label) p[r] -= 1.0f;
-                    p[r] = v0 + r < a.vocab && share != 0.0f ? p[r] * share : 0.0f;
-                    if constexpr (F16) p[r] *= 32768.0f;
+                        for (int r = 0; r < 4; ++r)
+                            if (mw + Tile::tile_row(i) + r >= a.vocab) acc[i][j][r] = -INFINITY;
                 }
-                char *out = a.d_l + (int64_t)row * a.stride + v0 * 2;
-                if constexpr (F16) {
-                    *reinterpret_cast<uint2 *>(out) = make_uint2(pack_f16(p[0], p[1]), pack_f16(p[2], p[3]));
-                    *reinterpret_cast<uint2 *>(out + a.plane) =
-                        make_uint2(pack_f16(rest_f16(p[0]), rest_f16(p[1])), pack_f16(rest_f16(p[2]), rest_f16(p[3])));
-                } else {
-                    *reinterpret_cast<uint2 *>(out) = make_uint2(pack_bf16(p[0], p[1]), pack_bf16(p[2], p[3]));
+                float top = -INFINITY;
+#pragma unroll
+                for (int i = 0; i < Tile::kMT; ++i)
+                    top = fmaxf(fmaxf(fmaxf(top, acc[i][j][0]), fmaxf(acc[i][j][1], acc[i][j][2])), acc[i][j][3]);
+                top = fmaxf(top, __shfl_xor(top, 16, 64));
+                top = fmaxf(top, __shfl_xor(top, 32, 64));
+                // (NaN is no maximum, and an infinite one would make NaN of its own term: both show in the sum)
+                const float at = top == -INFINITY ? 0.0f : top, from = -at * kLog2e;
+                float sum = 0.0f;
+#pragma unroll
+                for (int i = 0; i < Tile::kMT; ++i)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) sum += __builtin_amdgcn_exp2f(fmaf(acc[i][j][r], kLog2e, from));
+                sum += __shfl_xor(sum, 16, 64);
+                sum += __shfl_xor(sum, 32, 64);
+                if (lane < 16 && there) a.partial[(int64_t)of * a.rows + row] = make_float2(top, sum * rounded_off(at, from));
+            } else {
+                const float share = there ? a.share[row] : 0.0f;
+                // (no share: the exponentials of minus infinity, zeros)
+                const float lse = share != 0.0f ? a.lse[row] : INFINITY, from = -lse * kLog2e;
+                const float exact = share != 0.0f ? rounded_off(lse, from) : 1.0f;
+#pragma unroll
+                for (int i = 0; i < Tile::kMT; ++i)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) acc[i][j][r] = __builtin_amdgcn_exp2f(fmaf(acc[i][j][r], kLog2e, from));
+                if (labelled) {
+#pragma unroll
+                    for (int i = 0; i < Tile::kMT; ++i)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r)
+                            if (Tile::tile_row(i) + r == label && share != 0.0f) acc[i][j][r] -= 1.0f / exact;
+                }
+                if (!whole) {
+#pragma unroll
+                    for (int i = 0; i < Tile::kMT; ++i)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r)
+                            if (mw + Tile::tile_row(i) + r >= a.vocab) acc[i][j][r] = 0.0f;
+                }
+                const float factor = share * exact * (F16 ? 32768.0f : 1.0f);
+                char *out = a.d_l + (int64_t)row * a.stride + (mw + Tile::tile_row(0)) * 2;
+                // sixteen neighbouring entries from four tiles
+#pragma unroll
+                for (int i = 0; i < Tile::kMT; i += 4) {
+                    uint32_t w[8], low[8];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const Acc4 p = acc[i + k][j] * factor;
+                        if constexpr (F16) {
+                            split_f16(p[0], p[1], w[2 * k], low[2 * k]);
+                            split_f16(p[2], p[3], w[2 * k + 1], low[2 * k + 1]);
+                        } else {
+                            w[2 * k] = pack_bf16(p[0], p[1]);
+                            w[2 * k + 1] = pack_bf16(p[2], p[3]);
+                        }
+                    }
+                    uint4 *to = reinterpret_cast<uint4 *>(out + i / 4 * 128);
+                    to[0] = make_uint4(w[0], w[1], w[2], w[3]);
+                    to[1] = make_uint4(w[4], w[5], w[6], w[7]);
+                    if constexpr (F16) {
+                        uint4 *below = reinterpret_cast<uint4 *>(out + a.plane + i / 4 * 128);
+                        below[0] = make_uint4(low[0], low[1], low[2], low[3]);
+                        below[1] = make_uint4(low[4], low[5], low[6], low[7]);
+                    }
                 }
             }
         }
     }
+    Tile::end();
 }
 
 // ---- a row's log-sum-exp and loss ------------------------------------------------------------------------------
@@ -382,58 +461,89 @@ struct XentGradArgs {
     void *out;                  // (n, m) dense in T
 };
 
+// Parts of at least one step.
+__device__ __forceinline__ int xent_splits(int splits, int steps) { return splits < steps ? splits : steps > 1 ? steps : 1; }
+
 // d_hidden: n are rows, k the vocabulary (d_l row by row); d_weight: n the vocabulary, k the counted rows
 template <typename T, MatLayout LB, int BM, int BN>
 __global__ __launch_bounds__(kMatThreads, 1) void xent_grad_kernel(XentGradArgs a)
 {
     constexpr bool F16 = sizeof(T) == 4, OF_WEIGHT = LB == kCols;
-    using Tile = MatTile<kCols, LB, F16, BM, BN, false>;
+    using Tile = MatTiles<kCols, LB, F16, BM, BN, false>;
     __shared__ __attribute__((aligned(1024))) char lds[Tile::kLds];
     const int counted = a.scalars->counted;
-    const int tiles = a.tiles_m * a.tiles_n, split = blockIdx.x / tiles;
-    int tm, tn;
-    tile_at(xcd_order(blockIdx.x % tiles, tiles), a.tiles_m, a.tiles_n, 8, tm, tn);
-    const int m0 = tm * BM, n0 = tn * BN;
-    if (!OF_WEIGHT && n0 >= counted) return;
+    const int tiles_n = OF_WEIGHT ? a.tiles_n : (counted + BN - 1) / BN, tiles = a.tiles_m * tiles_n;
     const int steps = OF_WEIGHT ? (counted + kMatK - 1) / kMatK : a.steps;
-    const int per = (steps + a.splits - 1) / a.splits, first = split * per;
-    const int count = steps - first < per ? steps - first : per;
-    Acc4 acc[Tile::kMT][Tile::kNT];
-    Tile::run(a.a, a.b, m0, n0, first, count, lds, acc);
+    const int splits = xent_splits(a.splits, steps), total = tiles * splits;
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     float scale = a.scalars->grad_scale;
     if constexpr (F16) scale *= 1.0f / 32768.0f / (OF_WEIGHT ? a.scalars->hidden_scale : a.scalars->weight_scale);
+    if ((int)blockIdx.x >= total) return;
+    Tile tile(a.a, a.b, lds);
+    auto place = [&](int id, int &tm, int &tn, int &split, int &first, int &count) {
+        const int at = xcd_order(id, total);
+        split = at / tiles;
+        tile_at(at - split * tiles, a.tiles_m, tiles_n, 8, tm, tn);
+        first = (int)((int64_t)steps * split / splits);
+        count = (int)((int64_t)steps * (split + 1) / splits) - first;
+    };
+    int ahead = blockIdx.x;
+    auto next = [&](int &m, int &n, int &first, int &count) {
+        if (ahead >= total || steps == 0) return false;
+        int tm, tn, split;
+        place(ahead, tm, tn, split, first, count);
+        m = tm * BM;
+        n = tn * BN;
+        ahead += gridDim.x;
+        return true;
+    };
+    tile.begin(next);
+    for (int id = blockIdx.x; id < total; id += gridDim.x) {
+        int tm, tn, split, first, count;
+        place(id, tm, tn, split, first, count);
+        Acc4 acc[Tile::kMT][Tile::kNT];
+        tile.run(count, next, acc);
+        const int m0 = tm * BM, n0 = tn * BN;
+        float *partial = a.partial + (int64_t)split * a.n * a.m;
 #pragma unroll
-    for (int j = 0; j < Tile::kNT; ++j) {
-        const int64_t row = n0 + (wave & 1) * (BN / 2) + j * 16 + (lane & 15);
-        if (row >= (OF_WEIGHT ? a.n : (int64_t)counted)) continue;
+        for (int j = 0; j < Tile::kNT; ++j) {
+            const int64_t row = n0 + (wave & 1) * (BN / 2) + j * 16 + (lane & 15);
+            if (row >= (OF_WEIGHT ? a.n : (int64_t)counted)) continue;
 #pragma unroll
-        for (int i = 0; i < Tile::kMT; ++i) {
-            const int64_t m = m0 + (wave >> 1) * (BM / 2) + Tile::tile_row(i);
-            if (m >= a.m) continue;
-            if (a.out) {
-                T *out = reinterpret_cast<T *>(a.out) + row * a.m + m;
-                const Acc4 v = acc[i][j] * scale;
-                if (m + 4 <= a.m) {
-                    if constexpr (F16) {
-                        *reinterpret_cast<quad_at_4 *>(out) = quad_at_4{v[0], v[1], v[2], v[3]};
+            for (int i = 0; i < Tile::kMT; ++i) {
+                const int64_t m = m0 + (wave >> 1) * (BM / 2) + Tile::tile_row(i);
+                if (m >= a.m) continue;
+                if (a.out) {
+                    T *out = reinterpret_cast<T *>(a.out) + row * a.m + m;
+                    const Acc4 v = acc[i][j] * scale;
+                    if (m + 4 <= a.m) {
+                        if constexpr (F16) {
+                            *reinterpret_cast<quad_at_4 *>(out) = quad_at_4{v[0], v[1], v[2], v[3]};
+                        } else {
+                            typedef uint32_t pair_at_2 __attribute__((ext_vector_type(2), aligned(2)));
+                            *reinterpret_cast<pair_at_2 *>(out) = pair_at_2{pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3])};
+                        }
                     } else {
-                        typedef uint32_t pair_at_2 __attribute__((ext_vector_type(2), aligned(2)));
-                        *reinterpret_cast<pair_at_2 *>(out) = pair_at_2{pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3])};
+#pragma unroll
+                        for (int r = 0; r < 4; ++r)
+                            if (m + r < a.m) out[r] = (T)v[r];
                     }
                 } else {
+                    float *out = partial + row * a.m + m;
+                    if (m + 4 <= a.m) {
+                        quad_at_4 v = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
+                        if (a.add) v += *reinterpret_cast<quad_at_4 *>(out);
+                        *reinterpret_cast<quad_at_4 *>(out) = v;
+                    } else {
 #pragma unroll
-                    for (int r = 0; r < 4; ++r)
-                        if (m + r < a.m) out[r] = (T)v[r];
+                        for (int r = 0; r < 4; ++r)
+                            if (m + r < a.m) out[r] = (a.add ? out[r] : 0.0f) + acc[i][j][r];
+                    }
                 }
-            } else {
-                float *out = a.partial + ((int64_t)split * a.n + row) * a.m + m;
-#pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    if (m + r < a.m) out[r] = (a.add ? out[r] : 0.0f) + acc[i][j][r];
             }
         }
     }
+    Tile::end();
 }
 
 struct XentGatherArgs {
@@ -452,13 +562,14 @@ __global__ __launch_bounds__(256) void xent_gather_kernel(XentGatherArgs a)
     constexpr bool F16 = sizeof(T) == 4;
     float scale = a.scalars->grad_scale;
     if constexpr (F16) scale *= 1.0f / 32768.0f / (a.of_weight ? a.scalars->hidden_scale : a.scalars->weight_scale);
+    const int splits = a.of_weight ? xent_splits(a.splits, (a.scalars->counted + kMatK - 1) / kMatK) : a.splits;
     for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
         const int64_t at = a.position ? a.position[row] : row;
         T *out = reinterpret_cast<T *>(a.out) + row * a.m;
         for (int64_t m = threadIdx.x; m < a.m; m += 256) {
             float s = 0.0f;
             if (at >= 0) {
-                for (int p = 0; p < a.splits; ++p) s += a.partial[((int64_t)p * a.n + at) * a.m + m];
+                for (int p = 0; p < splits; ++p) s += a.partial[((int64_t)p * a.n + at) * a.m + m];
                 s *= scale;
             }
             out[m] = (T)s;
