@@ -31,7 +31,11 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef __attribute__((address_space(3))) char LdsByte;
 
 constexpr int kMatK = 64;          // k's of a step
-constexpr int kMatThreads = 256;
+
+// Wavefronts of a workgroup, two along m: those of a large tile are two on each SIMD, so that one of them computes while the
+// other one's loads and reads are taken; small tiles leave room for two workgroups a compute unit instead.
+constexpr int mat_waves(int bm, int bn) { return bm * bn >= 256 * 256 ? 8 : 4; }
+constexpr int mat_threads(int bm, int bn) { return 64 * mat_waves(bm, bn); }
 
 enum MatLayout { kRows, kCols };
 
@@ -62,12 +66,12 @@ __device__ __forceinline__ void load_unit_to_lds(MatDesc desc, unsigned lds_addr
 // One operand's way into LDS: SIZE rows or columns of it, k step by k step.  From step to step only the lanes' offsets
 // move (a wavefront that is alone on its SIMD has few instructions to spare between MFMAs); the
 // descriptor's base moves every kSteps() steps, before they pass 2^30.
-template <MatLayout LAYOUT, int SIZE, bool SPREAD>
+template <MatLayout LAYOUT, int SIZE, bool SPREAD, int WAVES>
 struct MatFeed {
-    static constexpr int kLoads = SIZE / 32;                 // of a wavefront a step
+    static constexpr int kLoads = SIZE / 8 / WAVES;          // of a wavefront a step
     static constexpr int kUnits = SIZE / 8;                  // kCols: 16-byte units of a k row
     static constexpr int kPerLoad = LAYOUT == kRows ? 8 : 64 / kUnits;   // rows that a load covers
-    static constexpr int kVariants = LAYOUT == kRows ? 1 : 4;
+    static constexpr int kVariants = LAYOUT == kRows ? 1 : kLoads;
     int stride, wave, first_voff[kVariants], voff[kVariants], soff[kLoads];
     MatDesc desc;
 
@@ -84,7 +88,10 @@ struct MatFeed {
         } else {
             const int row = lane / kUnits, unit = lane % kUnits;
 #pragma unroll
-            for (int v = 0; v < 4; ++v) first_voff[v] = row * stride + ((unit ^ (place(v, row) << 1)) * 16);
+            for (int j = 0; j < kLoads; ++j) {
+                const int r = (wave * kLoads + j) * kPerLoad + row, s = (r & 3) | ((r >> 3) & 1) << 2;
+                first_voff[j] = row * stride + (unit ^ s << 1) * 16;
+            }
         }
 #pragma unroll
         for (int j = 0; j < kLoads; ++j) {
@@ -95,16 +102,6 @@ struct MatFeed {
 
     // steps that one base serves
     __device__ __forceinline__ int steps() const { return LAYOUT == kRows ? 1 << 20 : max(1, (1 << 30) / (kMatK * stride) - 1); }
-
-    // s(r) of the rows that load number j of a wavefront covers, as far as it depends on j (v) and the lane's row
-    static __device__ __forceinline__ int place(int v, int row)
-    {
-        return kPerLoad == 2 ? ((v & 1) * 2 + row) | (v >> 1) << 2 : row | (v & 1) << 2;
-    }
-    static constexpr int variant(int j)
-    {
-        return LAYOUT == kRows ? 0 : kPerLoad == 2 ? (j & 1) | (j >> 2 & 1) << 1 : j >> 1 & 1;
-    }
 
     // to k step `step`, SIZE rows or columns from `first` on; nothing: loads of zeros from there on
     __device__ __forceinline__ void start(const MatOperand &o, int first, int64_t step, int plane, bool nothing)
@@ -121,7 +118,7 @@ struct MatFeed {
     }
     __device__ __forceinline__ void load(unsigned lds, int j) const
     {
-        load_unit_to_lds(desc, lds + (wave * kLoads + j) * 1024, voff[variant(j)], soff[j]);
+        load_unit_to_lds(desc, lds + (wave * kLoads + j) * 1024, voff[LAYOUT == kRows ? 0 : j], soff[j]);
     }
     __device__ __forceinline__ void advance()
     {
@@ -131,9 +128,9 @@ struct MatFeed {
 };
 
 // One operand's way out of LDS: the wavefront's 16-wide tiles of a half step (32 k's).
-template <MatLayout LAYOUT, int SIZE>
+template <MatLayout LAYOUT, int SIZE, int PARTS>
 struct MatReader {
-    static constexpr int kTiles = SIZE / 32;
+    static constexpr int kTiles = SIZE / 16 / PARTS;
     unsigned addr[LAYOUT == kRows ? 2 : kTiles];
 
     // offset: of the operand in a buffer
@@ -196,14 +193,17 @@ __device__ __forceinline__ void mfma_settle(Acc4 (&acc)[MT][NT])
 
 // Tiles of BM x BN, one after another, as one stream of k steps: while a step is computed the one after the next is
 // asked for, across the boundary between two tiles too, so the next tile's first steps arrive while the
-// sums of the one before are dealt with.  acc[mt][nt][r] is element (m, n) with n = n0 + BN / 2 * (wave & 1) + 16 nt +
-// lane % 16 and m = m0 + BM / 2 * (wave >> 1) + what tile_row() says.  F16: both operands in two planes.
+// sums of the one before are dealt with.  acc[mt][nt][r] is element (m, n) with n = n0 + kPartN wave_n() + 16 nt +
+// lane % 16 and m = m0 + kPartM wave_m() + what tile_row() says.  F16: both operands in two planes.
 template <MatLayout LA, MatLayout LB, bool F16, int BM, int BN, bool SPREAD>
 struct MatTiles {
-    static constexpr int kMT = BM / 32, kNT = BN / 32, kPasses = F16 ? 3 : 1;
+    static constexpr int kWaves = mat_waves(BM, BN), kWavesM = 2, kWavesN = kWaves / kWavesM;
+    static constexpr int kPartM = BM / kWavesM, kPartN = BN / kWavesN;     // a wavefront's part
+    static constexpr int kMT = kPartM / 16, kNT = kPartN / 16, kPasses = F16 ? 3 : 1;
     static constexpr int kBytesA = BM * kMatK * 2, kBytesB = BN * kMatK * 2, kBuffer = kBytesA + kBytesB;
     static constexpr int kLds = 2 * kBuffer;
-    static_assert(kMT == kNT, "reads and loads are dealt out to rows of MFMAs");
+    static constexpr int kLoadsA = BM / 8 / kWaves, kLoads = (BM + BN) / 8 / kWaves;
+    static_assert(kMT >= kNT && kLoads % kMT == 0, "reads and loads are dealt out to rows of MFMAs");
 
     // m of result r of tile mt, from the wavefront's first
     static __device__ __forceinline__ int tile_row(int mt)
@@ -212,13 +212,17 @@ struct MatTiles {
         return SPREAD ? (mt >> 2) * 64 + g * 16 + (mt & 3) * 4 : mt * 16 + g * 4;
     }
 
+    // The wavefront's part of a tile.
+    static __device__ __forceinline__ int wave_m() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) / kWavesN; }
+    static __device__ __forceinline__ int wave_n() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) % kWavesN; }
+
     const MatOperand &a, &b;
     LdsByte *near;
     unsigned lds, buffer = 0;
-    MatFeed<LA, BM, SPREAD> feed_a;
-    MatFeed<LB, BN, false> feed_b;
-    MatReader<LA, BM> read_a;
-    MatReader<LB, BN> read_b;
+    MatFeed<LA, BM, SPREAD, kWaves> feed_a;
+    MatFeed<LB, BN, false, kWaves> feed_b;
+    MatReader<LA, BM, kWavesM> read_a;
+    MatReader<LB, BN, kWavesN> read_b;
     Frag fa[2][kMT], fb[2][kNT];
     // the tile that is asked for: its place, its first k step, their number; how far it is asked for
     int m0 = 0, n0 = 0, first = 0, count = 0, pass = kPasses - 1, fed = 0, until = 0;
@@ -226,11 +230,10 @@ struct MatTiles {
     __device__ __forceinline__ MatTiles(const MatOperand &a_, const MatOperand &b_, char *lds_bytes)
         : a(a_), b(b_), near((LdsByte *)lds_bytes), lds((unsigned)(unsigned long long)(LdsByte *)lds_bytes)
     {
-        const int wave = threadIdx.x >> 6;
         feed_a.init(a);
         feed_b.init(b);
-        read_a.init(0, wave >> 1);
-        read_b.init(kBytesA, wave & 1);
+        read_a.init(0, wave_m());
+        read_b.init(kBytesA, wave_n());
     }
 
     // next(m0, n0, first, count): the next tile (count >= 1), or false when there is none
@@ -253,6 +256,11 @@ struct MatTiles {
         }
         ++fed;
     }
+    __device__ __forceinline__ void feed_load(unsigned to, int i)
+    {
+        if (i < kLoadsA) feed_a.load(lds + to, i);
+        else feed_b.load(lds + to + kBytesA, i - kLoadsA);
+    }
     __device__ __forceinline__ void feed_end()
     {
         feed_a.advance();
@@ -264,10 +272,7 @@ struct MatTiles {
     {
         feed_begin(next);
 #pragma unroll
-        for (int i = 0; i < kMT; ++i) {
-            feed_a.load(lds + to, i);
-            feed_b.load(lds + to + kBytesA, i);
-        }
+        for (int i = 0; i < kLoads; ++i) feed_load(to, i);
         feed_end();
     }
 
@@ -284,12 +289,12 @@ struct MatTiles {
         feed(0, next);
         feed(kBuffer, next);
         // (the second step's loads may still be on their way)
-        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kMT + kNT) : "memory");
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kLoads) : "memory");
         barrier();
 #pragma unroll
         for (int i = 0; i < kMT; ++i) {
             fa[0][i] = read_a.template read<0>(near, i);
-            fb[0][i] = read_b.template read<0>(near, i);
+            if (i < kNT) fb[0][i] = read_b.template read<0>(near, i);
         }
     }
 
@@ -304,7 +309,7 @@ struct MatTiles {
 #pragma unroll
         for (int i = 0; i < kMT; ++i) {
             fa[1][i] = read_a.template read<1>(near + buffer, i);
-            fb[1][i] = read_b.template read<1>(near + buffer, i);
+            if (i < kNT) fb[1][i] = read_b.template read<1>(near + buffer, i);
             if (i == 0) {
 #pragma unroll
                 for (int j = 0; j < kNT; ++j) mfma_operand(fb[0][j]);
@@ -321,10 +326,10 @@ struct MatTiles {
         const unsigned other = kBuffer - buffer;
 #pragma unroll
         for (int i = 0; i < kMT; ++i) {
-            feed_a.load(lds + buffer, i);
-            feed_b.load(lds + buffer + kBytesA, i);
+#pragma unroll
+            for (int k = 0; k < kLoads / kMT; ++k) feed_load(buffer, i * (kLoads / kMT) + k);
             fa[0][i] = read_a.template read<0>(near + other, i);
-            fb[0][i] = read_b.template read<0>(near + other, i);
+            if (i < kNT) fb[0][i] = read_b.template read<0>(near + other, i);
             if (i == 0) {
 #pragma unroll
                 for (int j = 0; j < kNT; ++j) mfma_operand(fb[1][j]);

@@ -174,7 +174,7 @@ void prepare(const bf_linear_xent *p, const XentPlan &r, const void *hidden, con
 template <bool F16, bool BACKWARD>
 void launch_logits(const Product &r, const XentTileArgs &a, hipStream_t s)
 {
-    const dim3 grid(workgroups(r)), threads(kMatThreads);
+    const dim3 grid(workgroups(r)), threads(r.large ? mat_threads(256, 256) : mat_threads(128, 128));
     if (r.large) xent_logits_kernel<F16, 256, 256, BACKWARD><<<grid, threads, 0, s>>>(a);
     else xent_logits_kernel<F16, 128, 128, BACKWARD><<<grid, threads, 0, s>>>(a);
 }
@@ -182,7 +182,7 @@ void launch_logits(const Product &r, const XentTileArgs &a, hipStream_t s)
 template <MatLayout LB>
 void launch_grad(const bf_linear_xent *p, const Product &r, const XentGradArgs &a, hipStream_t s)
 {
-    const dim3 grid(workgroups(r)), threads(kMatThreads);
+    const dim3 grid(workgroups(r)), threads(r.large ? mat_threads(256, 256) : mat_threads(128, 128));
     if (p->dtype == BF_F32) {
         if (r.large) xent_grad_kernel<float, LB, 256, 256><<<grid, threads, 0, s>>>(a);
         else xent_grad_kernel<float, LB, 128, 128><<<grid, threads, 0, s>>>(a);

@@ -228,13 +228,13 @@ __device__ __forceinline__ float rounded_off(float v, float from) { return __bui
 // Workgroups stay for tile after tile (grid: as many as the chip holds at a time), so that a tile's exponentials and
 // stores run while the next one's operands arrive.
 template <bool F16, int BM, int BN, bool BACKWARD>
-__global__ __launch_bounds__(kMatThreads, 1) void xent_logits_kernel(XentTileArgs a)
+__global__ __launch_bounds__(mat_threads(BM, BN), 1) void xent_logits_kernel(XentTileArgs a)
 {
     using Tile = MatTiles<kRows, kRows, F16, BM, BN, true>;
     __shared__ __attribute__((aligned(1024))) char lds[Tile::kLds];
     const int counted = a.scalars->counted;
     const int tiles_n = (counted + BN - 1) / BN, total = a.tiles_m * tiles_n;
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, part = wave >> 1;
+    const int lane = threadIdx.x & 63, part = Tile::wave_m();
     // (powers of two, each within the range of float)
     const float scale_h = F16 ? 1.0f / a.scalars->hidden_scale : 1.0f, scale_w = F16 ? 1.0f / a.scalars->weight_scale : 1.0f;
     if ((int)blockIdx.x >= total) return;
@@ -257,15 +257,15 @@ __global__ __launch_bounds__(kMatThreads, 1) void xent_logits_kernel(XentTileArg
         tiles.run(a.features_steps, next, acc);
         int tm, tn;
         tile_at(xcd_order(id, total), a.tiles_m, tiles_n, 8, tm, tn);
-        const int n0 = tn * BN, mw = tm * BM + part * (BM / 2), of = 2 * tm + part;
-        const bool whole = mw + BM / 2 <= a.vocab;   // no entry past the vocabulary's end
+        const int n0 = tn * BN, mw = tm * BM + part * Tile::kPartM, of = Tile::kWavesM * tm + part;
+        const bool whole = mw + Tile::kPartM <= a.vocab;   // no entry past the vocabulary's end
 #pragma unroll
         for (int j = 0; j < Tile::kNT; ++j) {
-            const int row = n0 + (wave & 1) * (BN / 2) + j * 16 + (lane & 15);
+            const int row = n0 + Tile::wave_n() * Tile::kPartN + j * 16 + (lane & 15);
             const bool there = row < counted;
             // the label's place among the wavefront's entries, if it is one of them
             const int label = there ? a.label[row] - (int)a.first - mw : -1;
-            const bool labelled = __any(label >= 0 && label < BM / 2);
+            const bool labelled = __any(label >= 0 && label < Tile::kPartM);
             if constexpr (F16) {
 #pragma unroll
                 for (int i = 0; i < Tile::kMT; ++i) acc[i][j] = acc[i][j] * scale_h * scale_w;
@@ -466,7 +466,7 @@ __device__ __forceinline__ int xent_splits(int splits, int steps) { return split
 
 // d_hidden: n are rows, k the vocabulary (d_l row by row); d_weight: n the vocabulary, k the counted rows
 template <typename T, MatLayout LB, int BM, int BN>
-__global__ __launch_bounds__(kMatThreads, 1) void xent_grad_kernel(XentGradArgs a)
+__global__ __launch_bounds__(mat_threads(BM, BN), 1) void xent_grad_kernel(XentGradArgs a)
 {
     constexpr bool F16 = sizeof(T) == 4, OF_WEIGHT = LB == kCols;
     using Tile = MatTiles<kCols, LB, F16, BM, BN, false>;
@@ -475,7 +475,7 @@ __global__ __launch_bounds__(kMatThreads, 1) void xent_grad_kernel(XentGradArgs 
     const int tiles_n = OF_WEIGHT ? a.tiles_n : (counted + BN - 1) / BN, tiles = a.tiles_m * tiles_n;
     const int steps = OF_WEIGHT ? (counted + kMatK - 1) / kMatK : a.steps;
     const int splits = xent_splits(a.splits, steps), total = tiles * splits;
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const int lane = threadIdx.x & 63;
     float scale = a.scalars->grad_scale;
     if constexpr (F16) scale *= 1.0f / 32768.0f / (OF_WEIGHT ? a.scalars->hidden_scale : a.scalars->weight_scale);
     if ((int)blockIdx.x >= total) return;
@@ -507,11 +507,11 @@ __global__ __launch_bounds__(kMatThreads, 1) void xent_grad_kernel(XentGradArgs 
         float *partial = a.partial + (int64_t)split * a.n * a.m;
 #pragma unroll
         for (int j = 0; j < Tile::kNT; ++j) {
-            const int64_t row = n0 + (wave & 1) * (BN / 2) + j * 16 + (lane & 15);
+            const int64_t row = n0 + Tile::wave_n() * Tile::kPartN + j * 16 + (lane & 15);
             if (row >= (OF_WEIGHT ? a.n : (int64_t)counted)) continue;
 #pragma unroll
             for (int i = 0; i < Tile::kMT; ++i) {
-                const int64_t m = m0 + (wave >> 1) * (BM / 2) + Tile::tile_row(i);
+                const int64_t m = m0 + Tile::wave_m() * Tile::kPartM + Tile::tile_row(i);
                 if (m >= a.m) continue;
                 if (a.out) {
                     T *out = reinterpret_cast<T *>(a.out) + row * a.m + m;
