@@ -30,7 +30,7 @@ bool nothing(const bf_recurrence *p) { return p->batch == 0 || p->channels == 0;
 
 struct RecurrencePlan {
     int64_t groups = 1, chunk = 0, chunks = 1;
-    int waves = 1;
+    int waves = 1, waves_bw = 1;
     size_t state_bytes = 0, a_bytes = 0, workspace = 0;   // a_bytes: of one of chunk_a, chunk_b
 };
 
@@ -40,7 +40,7 @@ struct RecurrencePlan {
 RecurrencePlan plan(const bf_recurrence *p)
 {
     RecurrencePlan r;
-    const int v = p->dtype == BF_BF16 ? RecBF16::V : 1, s = p->dtype == BF_C64 ? RecC64::S : RecF32::S;
+    const int v = p->dtype == BF_BF16 && p->channels > 1 ? RecBF16::V : 1, s = p->dtype == BF_C64 ? RecC64::S : RecF32::S;
     r.groups = (p->channels + 64 * v - 1) / (64 * v);
     const int64_t whole = r.groups * p->batch, tile = (int64_t)kRecWaves * s;
     r.chunk = std::max<int64_t>(p->steps, 1);
@@ -50,6 +50,8 @@ RecurrencePlan plan(const bf_recurrence *p)
         r.chunks = (p->steps + r.chunk - 1) / r.chunk;
     }
     r.waves = (int)std::min<int64_t>((r.chunk + s - 1) / s, kRecWaves);
+    const int sb = p->dtype == BF_BF16 && p->channels > 1 ? RecBF16::SB : s;
+    r.waves_bw = (int)std::min<int64_t>((r.chunk + sb - 1) / sb, kRecWaves);
     r.state_bytes = (size_t)p->batch * (size_t)p->channels * (p->dtype == BF_C64 ? 8 : 4);
     if (r.chunks > 1) {
         r.a_bytes = ((size_t)r.chunks * r.state_bytes + 255) / 256 * 256;
@@ -101,6 +103,8 @@ template <typename F>
 void with_kind(const bf_recurrence *p, F &&f)
 {
     if (p->dtype == BF_C64) f(RecC64(), std::false_type());
+    else if (p->dtype == BF_BF16 && p->channels == 1 && p->sigmoid) f(RecBF16One(), std::true_type());
+    else if (p->dtype == BF_BF16 && p->channels == 1) f(RecBF16One(), std::false_type());
     else if (p->dtype == BF_BF16 && p->sigmoid) f(RecBF16(), std::true_type());
     else if (p->dtype == BF_BF16) f(RecBF16(), std::false_type());
     else if (p->sigmoid) f(RecF32(), std::true_type());
@@ -191,8 +195,8 @@ int bf_recurrence_bw(const bf_recurrence *p, const void *gate, const void *x, co
         constexpr bool SIG = decltype(sigmoid)::value;
         const unsigned x_blocks = (unsigned)(r.groups * p->batch);
         if (r.chunks > 1)
-            recurrence_bw_kernel<Tr, SIG, true><<<dim3(x_blocks, (unsigned)r.chunks), dim3(64 * r.waves), 0, s>>>(a);
-        recurrence_bw_kernel<Tr, SIG, false><<<dim3(x_blocks, (unsigned)r.chunks), dim3(64 * r.waves), 0, s>>>(a);
+            recurrence_bw_kernel<Tr, SIG, true><<<dim3(x_blocks, (unsigned)r.chunks), dim3(64 * r.waves_bw), 0, s>>>(a);
+        recurrence_bw_kernel<Tr, SIG, false><<<dim3(x_blocks, (unsigned)r.chunks), dim3(64 * r.waves_bw), 0, s>>>(a);
     });
     BF_HIP_CHECK(hipGetLastError());
     return BF_OK;

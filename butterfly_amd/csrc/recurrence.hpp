@@ -22,6 +22,8 @@
 // or decays close to one would lose it.
 #pragma once
 
+#include <type_traits>
+
 #include "common.hpp"
 #include "vec8.hpp"
 
@@ -45,21 +47,21 @@ struct RecurrenceArgs {
     int *chunk_cut;                     // (chunks, batch): a reset inside
 };
 
-// V channels a lane, in registers as V accumulators.
+// V channels a lane, in registers as V accumulators; S steps a wavefront forward, SB backward.
 struct RecF32 {
     using Elem = float;
     using Acc = float;
-    static constexpr int V = 1, S = 8;
+    static constexpr int V = 1, S = 8, SB = 8;
 };
 struct RecBF16 {
     using Elem = bf16;
     using Acc = float;
-    static constexpr int V = 2, S = 8;
+    static constexpr int V = 2, S = 8, SB = 4;   // (eight steps of four tensors of two channels do not fit 128 registers)
 };
 struct RecC64 {
     using Elem = float2;
     using Acc = float2;
-    static constexpr int V = 1, S = 4;
+    static constexpr int V = 1, S = 4, SB = 4;
 };
 
 __device__ __forceinline__ float one_of(float) { return 1.0f; }
@@ -67,23 +69,46 @@ __device__ __forceinline__ float2 one_of(float2) { return make_float2(1.0f, 0.0f
 __device__ __forceinline__ bool is_zero(float v) { return v == 0.0f; }
 __device__ __forceinline__ bool is_zero(float2 v) { return v.x == 0.0f && v.y == 0.0f; }
 
-// What a lane loads of one row: Raw is what is in flight, widened when it is used.  Columns past the end
-// repeat the row's last ones (every address is valid); nothing of theirs is stored.
-__device__ __forceinline__ float raw_load(const float *row, int c, int n) { return row[c < n ? c : n - 1]; }
-__device__ __forceinline__ float2 raw_load(const float2 *row, int c, int n) { return row[c < n ? c : n - 1]; }
-__device__ __forceinline__ uint32_t raw_load(const bf16 *row, int c, int n)
+// A single channel of bfloat16: no neighbour to load with it.
+struct RecBF16One {
+    using Elem = bf16;
+    using Acc = float;
+    static constexpr int V = 1, S = 8, SB = 8;
+};
+
+// What a lane loads of one row, on its way until widen() looks at it.  Columns past the end repeat the row's last ones (every
+// address is valid); nothing of theirs is stored.  A pair that the row's end cuts is loaded from one column
+// before, and its first half is the upper one.
+template <typename Tr>
+struct RecLoad {
+    static constexpr int V = Tr::V;
+    using E = typename Tr::Elem;
+    using Raw = std::conditional_t<V == 2, uint32_t, E>;
+    int at;
+    bool cut;
+
+    __device__ __forceinline__ RecLoad(int c, int n) : at(c + V <= n ? c : n - V), cut(V == 2 && c == n - 1) {}
+    __device__ __forceinline__ Raw load(const E *row) const
+    {
+        typedef uint32_t word_at_2 __attribute__((aligned(2)));
+        if constexpr (V == 2) return *reinterpret_cast<const word_at_2 *>(row + at);
+        else return row[at];
+    }
+    __device__ __forceinline__ void widen(Raw raw, typename Tr::Acc (&v)[V]) const
+    {
+        if constexpr (V == 2) {
+            v[0] = __builtin_bit_cast(float, cut ? raw & 0xffff0000u : raw << 16);
+            v[1] = __builtin_bit_cast(float, raw & 0xffff0000u);
+        } else if constexpr (sizeof(E) == 2) {
+            v[0] = (float)raw;
+        } else {
+            v[0] = raw;
+        }
+    }
+};
+__device__ __forceinline__ void put(bf16 *row, int c, int n, const float (&v)[1])
 {
-    typedef uint32_t word_at_2 __attribute__((aligned(2)));
-    if (n == 1) return *reinterpret_cast<const uint16_t *>(row);
-    const uint32_t v = *reinterpret_cast<const word_at_2 *>(row + (c < n - 1 ? c : n - 2));
-    return c == n - 1 ? v >> 16 : v;
-}
-__device__ __forceinline__ void widen(float raw, float (&v)[1]) { v[0] = raw; }
-__device__ __forceinline__ void widen(float2 raw, float2 (&v)[1]) { v[0] = raw; }
-__device__ __forceinline__ void widen(uint32_t raw, float (&v)[2])
-{
-    v[0] = __builtin_bit_cast(float, raw << 16);
-    v[1] = __builtin_bit_cast(float, raw & 0xffff0000u);
+    if (c < n) row[c] = (bf16)v[0];
 }
 __device__ __forceinline__ void put(float *row, int c, int n, const float (&v)[1])
 {
@@ -139,6 +164,20 @@ template <typename A>
 __device__ __forceinline__ A chunk_of(bool cut, A a, A h, A b)
 {
     return cut || is_zero(h) ? b : mac(b, a, h);
+}
+
+// carry behind chunk j (columns past the end repeat the last one)
+template <int V, typename A>
+__device__ __forceinline__ void compose(const RecurrenceArgs &p, int j, int64_t b, int c, int n, A (&carry)[V])
+{
+    const int64_t at = (j * p.batch + b) * n;
+    const bool cut = p.chunk_cut[j * p.batch + b];
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+        const int col = c + v < n ? c + v : n - 1;
+        const A ca = reinterpret_cast<const A *>(p.chunk_a)[at + col], cb = reinterpret_cast<const A *>(p.chunk_b)[at + col];
+        carry[v] = chunk_of(cut, ca, carry[v], cb);
+    }
 }
 
 // The runs of a tile's wavefronts, and what enters each.  Two buffers that alternate: one barrier a tile.
@@ -198,7 +237,8 @@ __global__ __launch_bounds__(64 * kRecWaves) void recurrence_fw_kernel(Recurrenc
     const int64_t end = begin + p.chunk < p.steps ? begin + p.chunk : p.steps;
     const E *gate = reinterpret_cast<const E *>(p.gate) + b * p.gate_b;
     const E *x = reinterpret_cast<const E *>(p.x) + b * p.x_b;
-    using Raw = decltype(raw_load(gate, 0, 0));
+    using Raw = typename RecLoad<Tr>::Raw;
+    const RecLoad<Tr> in(c, n);
 
     A carry[V], whole[V];
     bool any_cut = false;
@@ -207,15 +247,8 @@ __global__ __launch_bounds__(64 * kRecWaves) void recurrence_fw_kernel(Recurrenc
         for (int v = 0; v < V; ++v) { carry[v] = zero_of(A()); whole[v] = one_of(A()); }
     } else {
         get_state<V>(p.state ? reinterpret_cast<const A *>(p.state) + b * n : nullptr, c, n, carry);
-        for (int j = 0; j < (int)blockIdx.y; ++j) {
-            const int64_t at = (j * p.batch + b) * n;
-            A ca[V], cb[V];
-            get_state<V>(reinterpret_cast<const A *>(p.chunk_a) + at, c, n, ca);
-            get_state<V>(reinterpret_cast<const A *>(p.chunk_b) + at, c, n, cb);
-            const bool cut = p.chunk_cut[j * p.batch + b];
-#pragma unroll
-            for (int v = 0; v < V; ++v) carry[v] = chunk_of(cut, ca[v], carry[v], cb[v]);
-        }
+#pragma unroll 4
+        for (int j = 0; j < (int)blockIdx.y; ++j) compose(p, j, b, c, n, carry);
     }
 
     Raw next_z[S], next_x[S];
@@ -225,8 +258,8 @@ __global__ __launch_bounds__(64 * kRecWaves) void recurrence_fw_kernel(Recurrenc
 #pragma unroll
         for (int s = 0; s < S; ++s) {
             const int64_t at = t + s < end ? t + s : end - 1;
-            next_z[s] = raw_load(gate + at * p.gate_t, c, n);
-            next_x[s] = raw_load(x + at * p.x_t, c, n);
+            next_z[s] = in.load(gate + at * p.gate_t);
+            next_x[s] = in.load(x + at * p.x_t);
         }
         next_cut = reset_bits(p, b, t, end, S, lane);
     };
@@ -239,8 +272,8 @@ __global__ __launch_bounds__(64 * kRecWaves) void recurrence_fw_kernel(Recurrenc
         A za[S][V], zb[S][V];
 #pragma unroll
         for (int s = 0; s < S; ++s) {
-            widen(next_z[s], za[s]);
-            widen(next_x[s], zb[s]);
+            in.widen(next_z[s], za[s]);
+            in.widen(next_x[s], zb[s]);
         }
         if (t0 + waves * S < end) fetch(t0 + waves * S);
         A ra[V], rb[V];
@@ -248,14 +281,14 @@ __global__ __launch_bounds__(64 * kRecWaves) void recurrence_fw_kernel(Recurrenc
         for (int v = 0; v < V; ++v) { ra[v] = one_of(A()); rb[v] = zero_of(A()); }
 #pragma unroll
         for (int s = 0; s < S; ++s) {
-            const bool cut = (cuts >> s) & 1, in = s < count;
+            const bool cut = (cuts >> s) & 1;
 #pragma unroll
             for (int v = 0; v < V; ++v) {
                 A a, rest;
                 gate_of<SIG>(za[s][v], a, rest);
                 if constexpr (SIG) zb[s][v] = mul(rest, zb[s][v]);
                 za[s][v] = a;
-                if (!in) continue;   // steps past the end change nothing
+                if (s >= count) continue;   // steps past the end change nothing
                 rb[v] = step_of(cut, a, rb[v], zb[s][v]);
                 ra[v] = cut ? zero_of(A()) : mul(ra[v], a);
             }
@@ -308,7 +341,7 @@ __global__ __launch_bounds__(64 * kRecWaves) void recurrence_bw_kernel(Recurrenc
 {
     using A = typename Tr::Acc;
     using E = typename Tr::Elem;
-    constexpr int V = Tr::V, S = Tr::S;
+    constexpr int V = Tr::V, S = Tr::SB;
     __shared__ Runs<Tr> runs;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
     const int64_t b = blockIdx.x / (unsigned)p.groups;
@@ -319,7 +352,8 @@ __global__ __launch_bounds__(64 * kRecWaves) void recurrence_bw_kernel(Recurrenc
     const E *x = reinterpret_cast<const E *>(p.x) + b * p.x_b;
     const E *grad = p.grad ? reinterpret_cast<const E *>(p.grad) + b * p.grad_b : nullptr;
     const E *h = reinterpret_cast<const E *>(p.h) + b * p.steps * n;
-    using Raw = decltype(raw_load(gate, 0, 0));
+    using Raw = typename RecLoad<Tr>::Raw;
+    const RecLoad<Tr> in(c, n);
 
     A carry[V], whole[V];
     bool any_cut = false;
@@ -328,15 +362,8 @@ __global__ __launch_bounds__(64 * kRecWaves) void recurrence_bw_kernel(Recurrenc
         for (int v = 0; v < V; ++v) { carry[v] = zero_of(A()); whole[v] = one_of(A()); }
     } else {
         get_state<V>(p.grad_last ? reinterpret_cast<const A *>(p.grad_last) + b * n : nullptr, c, n, carry);
-        for (int j = (int)gridDim.y - 1; j > (int)blockIdx.y; --j) {
-            const int64_t at = (j * p.batch + b) * n;
-            A ca[V], cb[V];
-            get_state<V>(reinterpret_cast<const A *>(p.chunk_a) + at, c, n, ca);
-            get_state<V>(reinterpret_cast<const A *>(p.chunk_b) + at, c, n, cb);
-            const bool cut = p.chunk_cut[j * p.batch + b];
-#pragma unroll
-            for (int v = 0; v < V; ++v) carry[v] = chunk_of(cut, ca[v], carry[v], cb[v]);
-        }
+#pragma unroll 4
+        for (int j = (int)gridDim.y - 1; j > (int)blockIdx.y; --j) compose(p, j, b, c, n, carry);
     }
 
     Raw next_z[S], next_g[S], next_x[S], next_p[S];
@@ -346,11 +373,11 @@ __global__ __launch_bounds__(64 * kRecWaves) void recurrence_bw_kernel(Recurrenc
 #pragma unroll
         for (int s = 0; s < S; ++s) {
             const int64_t at = t + s < end ? t + s : end - 1;
-            next_z[s] = raw_load(gate + at * p.gate_t, c, n);
-            next_g[s] = grad ? raw_load(grad + at * p.grad_t, c, n) : Raw();
+            next_z[s] = in.load(gate + at * p.gate_t);
+            next_g[s] = grad ? in.load(grad + at * p.grad_t) : Raw();
             if constexpr (!AGGREGATE) {
-                if constexpr (SIG) next_x[s] = raw_load(x + at * p.x_t, c, n);
-                next_p[s] = raw_load(h + (at > 0 ? at - 1 : 0) * n, c, n);
+                if constexpr (SIG) next_x[s] = in.load(x + at * p.x_t);
+                next_p[s] = in.load(h + (at > 0 ? at - 1 : 0) * n);
             }
         }
         next_cut = reset_bits(p, b, t, end, S, lane);
@@ -366,11 +393,11 @@ __global__ __launch_bounds__(64 * kRecWaves) void recurrence_bw_kernel(Recurrenc
         A za[S][V], zg[S][V], zr[S][V], zp[S][V];
 #pragma unroll
         for (int s = 0; s < S; ++s) {
-            widen(next_z[s], za[s]);
-            widen(next_g[s], zg[s]);
+            in.widen(next_z[s], za[s]);
+            in.widen(next_g[s], zg[s]);
             if constexpr (!AGGREGATE) {
-                widen(next_p[s], zp[s]);
-                if constexpr (SIG) widen(next_x[s], zr[s]);
+                in.widen(next_p[s], zp[s]);
+                if constexpr (SIG) in.widen(next_x[s], zr[s]);
             }
         }
         if constexpr (!AGGREGATE) {
@@ -387,7 +414,7 @@ __global__ __launch_bounds__(64 * kRecWaves) void recurrence_bw_kernel(Recurrenc
         for (int v = 0; v < V; ++v) { ra[v] = one_of(A()); rb[v] = zero_of(A()); }
 #pragma unroll
         for (int s = S - 1; s >= 0; --s) {
-            const bool cut = (cuts >> s) & 1, in = s < count;
+            const bool cut = (cuts >> s) & 1;
 #pragma unroll
             for (int v = 0; v < V; ++v) {
                 A a, rest;
@@ -400,7 +427,7 @@ __global__ __launch_bounds__(64 * kRecWaves) void recurrence_bw_kernel(Recurrenc
                     }
                 }
                 za[s][v] = conj_of(a);
-                if (!in) continue;
+                if (s >= count) continue;
                 rb[v] = cut ? zero_of(A()) : mul(za[s][v], add(zg[s][v], rb[v]));
                 ra[v] = cut ? zero_of(A()) : mul(ra[v], za[s][v]);
             }
@@ -466,10 +493,11 @@ __global__ __launch_bounds__(256) void recurrence_step_kernel(RecurrenceArgs p)
     constexpr int V = Tr::V;
     const int c = (blockIdx.x * 256 + threadIdx.x) * V, n = p.channels;
     if (c >= n) return;
+    const RecLoad<Tr> in(c, n);
     for (int64_t b = blockIdx.y; b < p.batch; b += gridDim.y) {
         A z[V], x[V], h[V];
-        widen(raw_load(reinterpret_cast<const E *>(p.gate) + b * p.gate_b, c, n), z);
-        widen(raw_load(reinterpret_cast<const E *>(p.x) + b * p.x_b, c, n), x);
+        in.widen(in.load(reinterpret_cast<const E *>(p.gate) + b * p.gate_b), z);
+        in.widen(in.load(reinterpret_cast<const E *>(p.x) + b * p.x_b), x);
         A *state = reinterpret_cast<A *>(p.last) + b * n;
         get_state<V>(state, c, n, h);
 #pragma unroll
