@@ -31,12 +31,12 @@ bool nothing(const bf_recurrence *p) { return p->batch == 0 || p->channels == 0;
 struct RecurrencePlan {
     int64_t groups = 1, chunk = 0, chunks = 1;
     int waves = 1, waves_bw = 1;
-    size_t state_bytes = 0, a_bytes = 0, workspace = 0;   // a_bytes: of one of chunk_a, chunk_b
+    size_t state_bytes = 0, chunk_bytes = 0, run_bytes = 0, workspace = 0;   // of one of chunk_a, chunk_b; run_a, run_b
 };
 
 // Channels times batch make `groups * batch` workgroups.  From 192 of them on (three quarters of the compute units)
 // the sequence stays whole and is read once; below, it is cut until some 512 are at work, in
-// chunks of whole tiles (16 wavefronts of S steps), at the price of a second read of the gates and inputs.
+// chunks of 16 runs of whole blocks of S steps, at the price of a second read of the gates and inputs.
 RecurrencePlan plan(const bf_recurrence *p)
 {
     RecurrencePlan r;
@@ -54,8 +54,9 @@ RecurrencePlan plan(const bf_recurrence *p)
     r.waves_bw = (int)std::min<int64_t>((r.chunk + sb - 1) / sb, kRecWaves);
     r.state_bytes = (size_t)p->batch * (size_t)p->channels * (p->dtype == BF_C64 ? 8 : 4);
     if (r.chunks > 1) {
-        r.a_bytes = ((size_t)r.chunks * r.state_bytes + 255) / 256 * 256;
-        r.workspace = 2 * r.a_bytes + (size_t)r.chunks * (size_t)p->batch * sizeof(int);
+        r.chunk_bytes = ((size_t)r.chunks * r.state_bytes + 255) / 256 * 256;
+        r.run_bytes = ((size_t)r.chunks * kRecWaves * r.state_bytes + 255) / 256 * 256;
+        r.workspace = 2 * (r.chunk_bytes + r.run_bytes) + (size_t)r.chunks * (1 + kRecWaves) * (size_t)p->batch * sizeof(int);
     }
     return r;
 }
@@ -77,9 +78,12 @@ void fill(RecurrenceArgs &a, const bf_recurrence *p, const RecurrencePlan &r, vo
     a.chunk = r.chunk;
     if (r.chunks > 1) {
         char *w = static_cast<char *>(workspace);
-        a.chunk_a = w;
-        a.chunk_b = w + r.a_bytes;
-        a.chunk_cut = reinterpret_cast<int *>(w + 2 * r.a_bytes);
+        a.run_a = w;
+        a.run_b = w + r.run_bytes;
+        a.chunk_a = w + 2 * r.run_bytes;
+        a.chunk_b = w + 2 * r.run_bytes + r.chunk_bytes;
+        a.chunk_cut = reinterpret_cast<int *>(w + 2 * (r.run_bytes + r.chunk_bytes));
+        a.run_cut = a.chunk_cut + r.chunks * p->batch;
     }
 }
 
@@ -157,10 +161,13 @@ int bf_recurrence_fw(const bf_recurrence *p, const void *gate, const void *x, co
         using Tr = decltype(kind);
         constexpr bool SIG = decltype(sigmoid)::value;
         const unsigned x_blocks = (unsigned)(r.groups * p->batch);
-        // (the last chunk's composition enters nothing)
-        if (r.chunks > 1)
-            recurrence_fw_kernel<Tr, SIG, true><<<dim3(x_blocks, (unsigned)r.chunks - 1), dim3(64 * r.waves), 0, s>>>(a);
-        recurrence_fw_kernel<Tr, SIG, false><<<dim3(x_blocks, (unsigned)r.chunks), dim3(64 * r.waves), 0, s>>>(a);
+        if (r.chunks > 1) {
+            const dim3 grid(x_blocks, (unsigned)r.chunks), threads(64 * kRecWaves);
+            recurrence_runs_kernel<Tr, SIG, false><<<grid, threads, 0, s>>>(a);
+            recurrence_chunk_fw_kernel<Tr, SIG><<<grid, threads, 0, s>>>(a);
+        } else {
+            recurrence_fw_kernel<Tr, SIG><<<dim3(x_blocks), dim3(64 * r.waves), 0, s>>>(a);
+        }
     });
     BF_HIP_CHECK(hipGetLastError());
     return BF_OK;
@@ -194,9 +201,13 @@ int bf_recurrence_bw(const bf_recurrence *p, const void *gate, const void *x, co
         using Tr = decltype(kind);
         constexpr bool SIG = decltype(sigmoid)::value;
         const unsigned x_blocks = (unsigned)(r.groups * p->batch);
-        if (r.chunks > 1)
-            recurrence_bw_kernel<Tr, SIG, true><<<dim3(x_blocks, (unsigned)r.chunks), dim3(64 * r.waves_bw), 0, s>>>(a);
-        recurrence_bw_kernel<Tr, SIG, false><<<dim3(x_blocks, (unsigned)r.chunks), dim3(64 * r.waves_bw), 0, s>>>(a);
+        if (r.chunks > 1) {
+            const dim3 grid(x_blocks, (unsigned)r.chunks), threads(64 * kRecWaves);
+            recurrence_runs_kernel<Tr, SIG, true><<<grid, threads, 0, s>>>(a);
+            recurrence_chunk_bw_kernel<Tr, SIG><<<grid, threads, 0, s>>>(a);
+        } else {
+            recurrence_bw_kernel<Tr, SIG><<<dim3(x_blocks), dim3(64 * r.waves_bw), 0, s>>>(a);
+        }
     });
     BF_HIP_CHECK(hipGetLastError());
     return BF_OK;

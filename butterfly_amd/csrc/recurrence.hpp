@@ -14,9 +14,9 @@
 // side by side in time: each holds S steps in registers, works out its (A, B), the wavefronts
 // exchange those through LDS (one barrier a tile of 16 S steps), and each then runs its steps again from its own h, the
 // next tile's elements on their way meanwhile.  Everything is read and written once.
-// Where channels times batch are too few workgroups to fill the chip the sequence is cut into chunks: one
-// launch forms the chunks' (A, B), the next one starts each chunk from their composition in
-// ascending order (the same sums at every call).
+// Where channels times batch are too few workgroups to fill the chip the sequence is cut into chunks of 16 runs, a
+// wavefront each: one launch forms the runs' and chunks' (A, B), the next one starts each run from their
+// composition in a fixed order (the same sums at every call).
 //
 // h is kept in float (complex64: two) whatever the rows' type; 1 - a is s(-gate), not a difference,
 // or decays close to one would lose it.
@@ -43,8 +43,9 @@ struct RecurrenceArgs {
     int64_t steps, chunk;               // chunk: steps of a chunk (the last one may be shorter)
     int64_t batch;
     int channels, groups;               // groups: workgroups across the channels
-    void *chunk_a, *chunk_b;            // (chunks, batch, channels)
-    int *chunk_cut;                     // (chunks, batch): a reset inside
+    void *chunk_a, *chunk_b;            // (chunks, batch, channels): what a chunk does
+    void *run_a, *run_b;                // (chunks, kRecWaves, batch, channels): what stands in front of a run in its chunk
+    int *chunk_cut, *run_cut;           // the same by sequence: a reset inside
 };
 
 // V channels a lane, in registers as V accumulators; S steps a wavefront forward, SB backward.
@@ -52,16 +53,19 @@ struct RecF32 {
     using Elem = float;
     using Acc = float;
     static constexpr int V = 1, S = 8, SB = 8;
+    static constexpr bool kExact = true;
 };
 struct RecBF16 {
     using Elem = bf16;
     using Acc = float;
     static constexpr int V = 2, S = 8, SB = 4;   // (eight steps of four tensors of two channels do not fit 128 registers)
+    static constexpr bool kExact = false;   // (the gates have eight bits)
 };
 struct RecC64 {
     using Elem = float2;
     using Acc = float2;
     static constexpr int V = 1, S = 4, SB = 4;
+    static constexpr bool kExact = true;
 };
 
 __device__ __forceinline__ float one_of(float) { return 1.0f; }
@@ -74,6 +78,7 @@ struct RecBF16One {
     using Elem = bf16;
     using Acc = float;
     static constexpr int V = 1, S = 8, SB = 8;
+    static constexpr bool kExact = false;
 };
 
 // What a lane loads of one row, on its way until widen() looks at it.  Columns past the end repeat the row's last ones (every
@@ -84,15 +89,15 @@ struct RecLoad {
     static constexpr int V = Tr::V;
     using E = typename Tr::Elem;
     using Raw = std::conditional_t<V == 2, uint32_t, E>;
-    int at;
+    uint32_t at;   // bytes: with a row's address in scalar registers a load needs no address arithmetic
     bool cut;
 
-    __device__ __forceinline__ RecLoad(int c, int n) : at(c + V <= n ? c : n - V), cut(V == 2 && c == n - 1) {}
+    __device__ __forceinline__ RecLoad(int c, int n) : at((uint32_t)(c + V <= n ? c : n - V) * (uint32_t)sizeof(E)), cut(V == 2 && c == n - 1) {}
     __device__ __forceinline__ Raw load(const E *row) const
     {
         typedef uint32_t word_at_2 __attribute__((aligned(2)));
-        if constexpr (V == 2) return *reinterpret_cast<const word_at_2 *>(row + at);
-        else return row[at];
+        if constexpr (V == 2) return *reinterpret_cast<const word_at_2 *>(reinterpret_cast<const char *>(row) + at);
+        else return *reinterpret_cast<const E *>(reinterpret_cast<const char *>(row) + at);
     }
     __device__ __forceinline__ void widen(Raw raw, typename Tr::Acc (&v)[V]) const
     {
@@ -138,18 +143,28 @@ __device__ __forceinline__ void put_state(A *row, int c, int n, const A (&v)[V])
         if (c + i < n) row[c + i] = v[i];
 }
 
-// s(z) and s(-z) from one exponential of a number that is not positive: neither overflows or cancels
+// s(z) and s(-z) from one exponential, e = exp(-z): 1 / (1 + e) and e / (1 + e), neither a difference.  e stops at 2^126,
+// where the first is as good as zero and the second still one.  EXACT: the exponent's rounding (2^-24 of it, so some 2^-21 of
+// e at the ends) is put back.
+template <bool EXACT>
 __device__ __forceinline__ void sigmoids(float z, float &a, float &rest)
 {
-    const float e = expf(-fabsf(z)), r = __builtin_amdgcn_rcpf(1.0f + e);
-    a = z >= 0.0f ? r : e * r;
-    rest = z >= 0.0f ? e * r : r;
+    constexpr float kLog2e = 1.44269504088896340736f;
+    float t = -z * kLog2e;
+    t = t > 126.0f ? 126.0f : t;   // (NaN stays NaN)
+    float e = __builtin_amdgcn_exp2f(t);
+    if constexpr (EXACT) {
+        const float off = fmaf(-z, kLog2e, -t);
+        e = fabsf(off) < 1.0f ? fmaf(e, off * 0.69314718f, e) : e;   // (not where t was cut or z is infinite)
+    }
+    a = __builtin_amdgcn_rcpf(1.0f + e);
+    rest = e * a;
 }
 
-template <bool SIG, typename A>
+template <bool SIG, bool EXACT, typename A>
 __device__ __forceinline__ void gate_of(A z, A &a, A &rest)
 {
-    if constexpr (SIG) sigmoids(z, a, rest);
+    if constexpr (SIG) sigmoids<EXACT>(z, a, rest);
     else { a = z; rest = one_of(z); }
 }
 
@@ -166,16 +181,15 @@ __device__ __forceinline__ A chunk_of(bool cut, A a, A h, A b)
     return cut || is_zero(h) ? b : mac(b, a, h);
 }
 
-// carry behind chunk j (columns past the end repeat the last one)
+// carry behind the composition in a slot (columns past the end repeat the last one)
 template <int V, typename A>
-__device__ __forceinline__ void compose(const RecurrenceArgs &p, int j, int64_t b, int c, int n, A (&carry)[V])
+__device__ __forceinline__ void compose(const void *from_a, const void *from_b, const int *from_cut, int64_t slot, int c, int n, A (&carry)[V])
 {
-    const int64_t at = (j * p.batch + b) * n;
-    const bool cut = p.chunk_cut[j * p.batch + b];
+    const bool cut = from_cut[slot];
 #pragma unroll
     for (int v = 0; v < V; ++v) {
         const int col = c + v < n ? c + v : n - 1;
-        const A ca = reinterpret_cast<const A *>(p.chunk_a)[at + col], cb = reinterpret_cast<const A *>(p.chunk_b)[at + col];
+        const A ca = reinterpret_cast<const A *>(from_a)[slot * n + col], cb = reinterpret_cast<const A *>(from_b)[slot * n + col];
         carry[v] = chunk_of(cut, ca, carry[v], cb);
     }
 }
@@ -213,7 +227,7 @@ __device__ __forceinline__ void exchange(Runs<Tr> &runs, int turn, int wave, int
     }
 }
 
-// The resets of a wavefront's S steps as bits, steps past `end` unset.
+// The resets of `steps` steps from t on as bits, steps past `end` unset.
 __device__ __forceinline__ uint64_t reset_bits(const RecurrenceArgs &a, int64_t b, int64_t t, int64_t end, int steps, int lane)
 {
     if (!a.reset) return 0;
@@ -222,51 +236,87 @@ __device__ __forceinline__ uint64_t reset_bits(const RecurrenceArgs &a, int64_t 
     return __ballot(r != 0);
 }
 
-// grid (batch x groups, chunks); 64 x waves threads.  AGGREGATE: forms the chunks' (A, B) and writes nothing else.
-template <typename Tr, bool SIG, bool AGGREGATE>
+// What a wavefront works on: 64 V channels of a sequence.
+template <typename Tr>
+struct RecPlace {
+    using E = typename Tr::Elem;
+    using A = typename Tr::Acc;
+    int lane, wave, waves, c, n;
+    int64_t b, begin, end;     // the workgroup's steps
+
+    __device__ __forceinline__ explicit RecPlace(const RecurrenceArgs &p)
+        : lane(threadIdx.x & 63), wave(__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)), waves(blockDim.x >> 6),
+          c(((int)(blockIdx.x % (unsigned)p.groups) * 64 + lane) * Tr::V), n(p.channels), b(blockIdx.x / (unsigned)p.groups),
+          begin((int64_t)blockIdx.y * p.chunk), end(begin + p.chunk < p.steps ? begin + p.chunk : p.steps)
+    {
+    }
+    __device__ __forceinline__ const E *rows(const void *p, int64_t stride) const { return reinterpret_cast<const E *>(p) + b * stride; }
+    __device__ __forceinline__ const A *state(const void *p) const { return p ? reinterpret_cast<const A *>(p) + b * n : nullptr; }
+    __device__ __forceinline__ A *state(void *p) const { return reinterpret_cast<A *>(p) + b * n; }
+};
+
+// S rows of one tensor from step t on (those past `end` repeat the last one).
+template <int S, typename Tr>
+__device__ __forceinline__ void load_steps(typename RecLoad<Tr>::Raw (&raw)[S], const RecLoad<Tr> &in, const typename Tr::Elem *rows,
+                                           int64_t stride, int64_t t, int64_t end)
+{
+    const typename Tr::Elem *row = rows + (t < end ? t : end - 1) * stride;
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+        raw[s] = in.load(row);
+        if (t + s + 1 < end) row += stride;
+    }
+}
+// The h in front of each of S steps from t on (t = 0: the first step's own, to be replaced by the state).
+template <int S, typename Tr>
+__device__ __forceinline__ void load_before(typename RecLoad<Tr>::Raw (&raw)[S], const RecLoad<Tr> &in, const typename Tr::Elem *rows,
+                                            int64_t stride, int64_t t, int64_t end)
+{
+    const int64_t first = (t < end ? t : end - 1) - 1;
+    const typename Tr::Elem *row = rows + (first < 0 ? 0 : first) * stride;
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+        raw[s] = in.load(row);
+        if (first + s >= 0 && t + s + 1 < end) row += stride;
+    }
+}
+
+// f(std::true_type) where none of S steps is a reset and all of them exist, the rule; f(std::false_type) otherwise.
+template <typename F>
+__device__ __forceinline__ void by_kind(bool plain, F &&f)
+{
+    if (plain) f(std::true_type());
+    else f(std::false_type());
+}
+
+// ---- sequences that stay whole ---------------------------------------------------------------------------
+// grid (batch x groups); 64 x waves threads.
+template <typename Tr, bool SIG>
 __global__ __launch_bounds__(64 * kRecWaves) void recurrence_fw_kernel(RecurrenceArgs p)
 {
     using A = typename Tr::Acc;
     using E = typename Tr::Elem;
     constexpr int V = Tr::V, S = Tr::S;
     __shared__ Runs<Tr> runs;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
-    const int64_t b = blockIdx.x / (unsigned)p.groups;
-    const int c = ((int)(blockIdx.x % (unsigned)p.groups) * 64 + lane) * V, n = p.channels;
-    const int64_t begin = (int64_t)blockIdx.y * p.chunk;
-    const int64_t end = begin + p.chunk < p.steps ? begin + p.chunk : p.steps;
-    const E *gate = reinterpret_cast<const E *>(p.gate) + b * p.gate_b;
-    const E *x = reinterpret_cast<const E *>(p.x) + b * p.x_b;
-    using Raw = typename RecLoad<Tr>::Raw;
+    const RecPlace<Tr> at(p);
+    const int c = at.c, n = at.n;
+    const int64_t end = at.end;
     const RecLoad<Tr> in(c, n);
-
-    A carry[V], whole[V];
-    bool any_cut = false;
-    if constexpr (AGGREGATE) {
-#pragma unroll
-        for (int v = 0; v < V; ++v) { carry[v] = zero_of(A()); whole[v] = one_of(A()); }
-    } else {
-        get_state<V>(p.state ? reinterpret_cast<const A *>(p.state) + b * n : nullptr, c, n, carry);
-#pragma unroll 4
-        for (int j = 0; j < (int)blockIdx.y; ++j) compose(p, j, b, c, n, carry);
-    }
-
-    Raw next_z[S], next_x[S];
+    const E *gate = at.rows(p.gate, p.gate_b), *x = at.rows(p.x, p.x_b);
+    A carry[V];
+    get_state<V>(at.state(p.state), c, n, carry);
+    typename RecLoad<Tr>::Raw next_z[S], next_x[S];
     uint64_t next_cut = 0;
-    auto fetch = [&](int64_t t0) {
-        const int64_t t = t0 + wave * S;
-#pragma unroll
-        for (int s = 0; s < S; ++s) {
-            const int64_t at = t + s < end ? t + s : end - 1;
-            next_z[s] = in.load(gate + at * p.gate_t);
-            next_x[s] = in.load(x + at * p.x_t);
-        }
-        next_cut = reset_bits(p, b, t, end, S, lane);
+    auto fetch = [&](int64_t t) {
+        load_steps<S, Tr>(next_z, in, gate, p.gate_t, t, end);
+        load_steps<S, Tr>(next_x, in, x, p.x_t, t, end);
+        next_cut = reset_bits(p, at.b, t, end, S, at.lane);
     };
-    fetch(begin);
+    fetch(at.wave * S);
+    const int tile = at.waves * S;
     int turn = 0;
-    for (int64_t t0 = begin; t0 < end; t0 += waves * S, turn ^= 1) {
-        const int64_t t = t0 + wave * S;
+    for (int64_t t0 = 0; t0 < end; t0 += tile, turn ^= 1) {
+        const int64_t t = t0 + at.wave * S;
         const int count = (int)(end - t < 0 ? 0 : end - t < S ? end - t : S);
         const uint64_t cuts = next_cut;
         A za[S][V], zb[S][V];
@@ -275,213 +325,369 @@ __global__ __launch_bounds__(64 * kRecWaves) void recurrence_fw_kernel(Recurrenc
             in.widen(next_z[s], za[s]);
             in.widen(next_x[s], zb[s]);
         }
-        if (t0 + waves * S < end) fetch(t0 + waves * S);
-        A ra[V], rb[V];
+        if (t0 + tile < end) fetch(t + tile);
+        A ra[V], rb[V], mine[V];
 #pragma unroll
         for (int v = 0; v < V; ++v) { ra[v] = one_of(A()); rb[v] = zero_of(A()); }
-#pragma unroll
-        for (int s = 0; s < S; ++s) {
-            const bool cut = (cuts >> s) & 1;
-#pragma unroll
-            for (int v = 0; v < V; ++v) {
-                A a, rest;
-                gate_of<SIG>(za[s][v], a, rest);
-                if constexpr (SIG) zb[s][v] = mul(rest, zb[s][v]);
-                za[s][v] = a;
-                if (s >= count) continue;   // steps past the end change nothing
-                rb[v] = step_of(cut, a, rb[v], zb[s][v]);
-                ra[v] = cut ? zero_of(A()) : mul(ra[v], a);
-            }
-        }
-        A mine[V];
-        if constexpr (AGGREGATE) {
-#pragma unroll
-            for (int v = 0; v < V; ++v) {
-                runs.a[turn][wave][v][lane] = ra[v];
-                runs.b[turn][wave][v][lane] = rb[v];
-            }
-            if (lane == 0) runs.cut[turn][wave] = cuts != 0;
-            __syncthreads();
-            for (int w = 0; w < waves; ++w) {
-                const bool cut = runs.cut[turn][w];
-                any_cut |= cut;
-#pragma unroll
-                for (int v = 0; v < V; ++v) {
-                    const A ca = runs.a[turn][w][v][lane];
-                    carry[v] = step_of(cut, ca, carry[v], runs.b[turn][w][v][lane]);
-                    whole[v] = mul(whole[v], ca);
-                }
-            }
-        } else {
-            exchange<Tr, false>(runs, turn, wave, waves, lane, cuts != 0, ra, rb, carry, mine);
-            E *out = reinterpret_cast<E *>(p.h) + (b * p.steps + t) * n;
+        by_kind(cuts == 0 && count == S, [&](auto plain) {
 #pragma unroll
             for (int s = 0; s < S; ++s) {
-                const bool cut = (cuts >> s) & 1;
-#pragma unroll
-                for (int v = 0; v < V; ++v) mine[v] = step_of(cut, za[s][v], mine[v], zb[s][v]);
-                if (s < count) put(out + (int64_t)s * n, c, n, mine);
-            }
-        }
-    }
-    if (wave != 0) return;
-    if constexpr (AGGREGATE) {
-        const int64_t at = (blockIdx.y * p.batch + b) * n;
-        put_state<V>(reinterpret_cast<A *>(p.chunk_a) + at, c, n, whole);
-        put_state<V>(reinterpret_cast<A *>(p.chunk_b) + at, c, n, carry);
-        if (lane == 0 && c == 0) p.chunk_cut[blockIdx.y * p.batch + b] = any_cut;
-    } else if (p.last && blockIdx.y == gridDim.y - 1) {
-        put_state<V>(reinterpret_cast<A *>(p.last) + b * n, c, n, carry);
-    }
-}
-
-// The same from the last step back, on c: c -> conj(a) (grad + c).
-template <typename Tr, bool SIG, bool AGGREGATE>
-__global__ __launch_bounds__(64 * kRecWaves) void recurrence_bw_kernel(RecurrenceArgs p)
-{
-    using A = typename Tr::Acc;
-    using E = typename Tr::Elem;
-    constexpr int V = Tr::V, S = Tr::SB;
-    __shared__ Runs<Tr> runs;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
-    const int64_t b = blockIdx.x / (unsigned)p.groups;
-    const int c = ((int)(blockIdx.x % (unsigned)p.groups) * 64 + lane) * V, n = p.channels;
-    const int64_t begin = (int64_t)blockIdx.y * p.chunk;
-    const int64_t end = begin + p.chunk < p.steps ? begin + p.chunk : p.steps;
-    const E *gate = reinterpret_cast<const E *>(p.gate) + b * p.gate_b;
-    const E *x = reinterpret_cast<const E *>(p.x) + b * p.x_b;
-    const E *grad = p.grad ? reinterpret_cast<const E *>(p.grad) + b * p.grad_b : nullptr;
-    const E *h = reinterpret_cast<const E *>(p.h) + b * p.steps * n;
-    using Raw = typename RecLoad<Tr>::Raw;
-    const RecLoad<Tr> in(c, n);
-
-    A carry[V], whole[V];
-    bool any_cut = false;
-    if constexpr (AGGREGATE) {
-#pragma unroll
-        for (int v = 0; v < V; ++v) { carry[v] = zero_of(A()); whole[v] = one_of(A()); }
-    } else {
-        get_state<V>(p.grad_last ? reinterpret_cast<const A *>(p.grad_last) + b * n : nullptr, c, n, carry);
-#pragma unroll 4
-        for (int j = (int)gridDim.y - 1; j > (int)blockIdx.y; --j) compose(p, j, b, c, n, carry);
-    }
-
-    Raw next_z[S], next_g[S], next_x[S], next_p[S];
-    uint64_t next_cut = 0;
-    auto fetch = [&](int64_t t0) {
-        const int64_t t = t0 + wave * S;
-#pragma unroll
-        for (int s = 0; s < S; ++s) {
-            const int64_t at = t + s < end ? t + s : end - 1;
-            next_z[s] = in.load(gate + at * p.gate_t);
-            next_g[s] = grad ? in.load(grad + at * p.grad_t) : Raw();
-            if constexpr (!AGGREGATE) {
-                if constexpr (SIG) next_x[s] = in.load(x + at * p.x_t);
-                next_p[s] = in.load(h + (at > 0 ? at - 1 : 0) * n);
-            }
-        }
-        next_cut = reset_bits(p, b, t, end, S, lane);
-    };
-    const int tile = waves * S;
-    const int64_t first = begin + (end - 1 - begin) / tile * tile;   // the chunk's last tile
-    fetch(first);
-    int turn = 0;
-    for (int64_t t0 = first; t0 >= begin; t0 -= tile, turn ^= 1) {
-        const int64_t t = t0 + wave * S;
-        const int count = (int)(end - t < 0 ? 0 : end - t < S ? end - t : S);
-        const uint64_t cuts = next_cut;
-        A za[S][V], zg[S][V], zr[S][V], zp[S][V];
-#pragma unroll
-        for (int s = 0; s < S; ++s) {
-            in.widen(next_z[s], za[s]);
-            in.widen(next_g[s], zg[s]);
-            if constexpr (!AGGREGATE) {
-                in.widen(next_p[s], zp[s]);
-                if constexpr (SIG) in.widen(next_x[s], zr[s]);
-            }
-        }
-        if constexpr (!AGGREGATE) {
-            if (t == 0) {
-                A first_state[V];
-                get_state<V>(p.state ? reinterpret_cast<const A *>(p.state) + b * n : nullptr, c, n, first_state);
-#pragma unroll
-                for (int v = 0; v < V; ++v) zp[0][v] = first_state[v];
-            }
-        }
-        if (t0 - tile >= begin) fetch(t0 - tile);
-        A ra[V], rb[V];
-#pragma unroll
-        for (int v = 0; v < V; ++v) { ra[v] = one_of(A()); rb[v] = zero_of(A()); }
-#pragma unroll
-        for (int s = S - 1; s >= 0; --s) {
-            const bool cut = (cuts >> s) & 1;
-#pragma unroll
-            for (int v = 0; v < V; ++v) {
-                A a, rest;
-                gate_of<SIG>(za[s][v], a, rest);
-                if constexpr (!AGGREGATE) {
-                    if (cut) zp[s][v] = zero_of(A());
-                    if constexpr (SIG) {
-                        zp[s][v] = (zp[s][v] - zr[s][v]) * (a * rest);
-                        zr[s][v] = rest;
-                    }
-                }
-                za[s][v] = conj_of(a);
-                if (s >= count) continue;
-                rb[v] = cut ? zero_of(A()) : mul(za[s][v], add(zg[s][v], rb[v]));
-                ra[v] = cut ? zero_of(A()) : mul(ra[v], za[s][v]);
-            }
-        }
-        if constexpr (AGGREGATE) {
-#pragma unroll
-            for (int v = 0; v < V; ++v) {
-                runs.a[turn][wave][v][lane] = ra[v];
-                runs.b[turn][wave][v][lane] = rb[v];
-            }
-            if (lane == 0) runs.cut[turn][wave] = cuts != 0;
-            __syncthreads();
-            for (int w = waves - 1; w >= 0; --w) {
-                const bool cut = runs.cut[turn][w];
-                any_cut |= cut;
+                const bool cut = !plain.value && (cuts >> s & 1);
 #pragma unroll
                 for (int v = 0; v < V; ++v) {
-                    const A ca = runs.a[turn][w][v][lane];
-                    carry[v] = step_of(cut, ca, carry[v], runs.b[turn][w][v][lane]);
-                    whole[v] = mul(whole[v], ca);
+                    A a, rest;
+                    gate_of<SIG, Tr::kExact>(za[s][v], a, rest);
+                    if constexpr (SIG) zb[s][v] = mul(rest, zb[s][v]);
+                    za[s][v] = a;
+                    if (!plain.value && s >= count) continue;   // steps past the end change nothing
+                    rb[v] = step_of(cut, a, rb[v], zb[s][v]);
+                    ra[v] = cut ? zero_of(A()) : mul(ra[v], a);
                 }
             }
-        } else {
-            A mine[V];
-            exchange<Tr, true>(runs, turn, wave, waves, lane, cuts != 0, ra, rb, carry, mine);
-            E *dz = reinterpret_cast<E *>(p.d_gate) + (b * p.steps + t) * n;
-            E *dx = reinterpret_cast<E *>(p.d_x) + (b * p.steps + t) * n;
+        });
+        exchange<Tr, false>(runs, turn, at.wave, at.waves, at.lane, cuts != 0, ra, rb, carry, mine);
+        E *out = reinterpret_cast<E *>(p.h) + (at.b * p.steps + t) * n;
+        by_kind(cuts == 0 && count == S, [&](auto plain) {
 #pragma unroll
-            for (int s = S - 1; s >= 0; --s) {
-                const bool cut = (cuts >> s) & 1;
-                if (s >= count) continue;
+            for (int s = 0; s < S; ++s) {
+                const bool cut = !plain.value && (cuts >> s & 1);
+#pragma unroll
+                for (int v = 0; v < V; ++v) mine[v] = step_of(cut, za[s][v], mine[v], zb[s][v]);
+                if (plain.value || s < count) put(out, c, n, mine);
+                out += n;
+            }
+        });
+    }
+    if (at.wave == 0 && p.last) put_state<V>(at.state(p.last), c, n, carry);
+}
+
+// Operands of S steps backward, in registers: a, grad, (p - x) a (1 - a) or p, 1 - a.
+template <typename Tr, bool SIG>
+struct RecBack {
+    static constexpr int V = Tr::V, S = Tr::SB;
+    using A = typename Tr::Acc;
+    using E = typename Tr::Elem;
+    typename RecLoad<Tr>::Raw next_z[S], next_g[S], next_x[S], next_p[S];
+    uint64_t next_cut = 0;
+    A a[S][V], g[S][V], u[S][V], r[S][V];
+
+    __device__ __forceinline__ void fetch(const RecurrenceArgs &p, const RecPlace<Tr> &at, const RecLoad<Tr> &in, int64_t t, int64_t end)
+    {
+        load_steps<S, Tr>(next_z, in, at.rows(p.gate, p.gate_b), p.gate_t, t, end);
+        // (without a gradient of h: something that is there, and not looked at)
+        if (p.grad) load_steps<S, Tr>(next_g, in, at.rows(p.grad, p.grad_b), p.grad_t, t, end);
+        if constexpr (SIG) load_steps<S, Tr>(next_x, in, at.rows(p.x, p.x_b), p.x_t, t, end);
+        load_before<S, Tr>(next_p, in, at.rows(p.h, p.steps * at.n), at.n, t, end);
+        next_cut = reset_bits(p, at.b, t, end, S, at.lane);
+    }
+    __device__ __forceinline__ void take(const RecurrenceArgs &p, const RecPlace<Tr> &at, const RecLoad<Tr> &in, int64_t t)
+    {
+#pragma unroll
+        for (int s = 0; s < S; ++s) {
+            in.widen(next_z[s], a[s]);
+            in.widen(next_p[s], u[s]);
+            if constexpr (SIG) in.widen(next_x[s], r[s]);
+        }
+        if (p.grad) {
+#pragma unroll
+            for (int s = 0; s < S; ++s) in.widen(next_g[s], g[s]);
+        } else {
+#pragma unroll
+            for (int s = 0; s < S; ++s)
+#pragma unroll
+                for (int v = 0; v < V; ++v) g[s][v] = zero_of(A());
+        }
+        if (t == 0) get_state<V>(at.state(p.state), at.c, at.n, u[0]);
+    }
+    template <bool PLAIN>
+    __device__ __forceinline__ void gates(uint64_t cuts)
+    {
+#pragma unroll
+        for (int s = 0; s < S; ++s)
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                A gate, rest;
+                gate_of<SIG, Tr::kExact>(a[s][v], gate, rest);
+                if (!PLAIN && (cuts >> s & 1)) u[s][v] = zero_of(A());
+                if constexpr (SIG) {
+                    u[s][v] = (u[s][v] - r[s][v]) * (gate * rest);
+                    r[s][v] = rest;
+                }
+                a[s][v] = conj_of(gate);
+            }
+    }
+    // The steps from the last one back, c going through them; rows of the results from step t on.
+    template <bool PLAIN>
+    __device__ __forceinline__ void steps(const RecurrenceArgs &p, const RecPlace<Tr> &at, int64_t t, int count, uint64_t cuts, A (&c)[V])
+    {
+        const int64_t row = (at.b * p.steps + t + S - 1) * at.n;
+        E *dz = reinterpret_cast<E *>(p.d_gate) + row, *dx = reinterpret_cast<E *>(p.d_x) + row;
+#pragma unroll
+        for (int s = S - 1; s >= 0; --s) {
+            if (PLAIN || s < count) {
+                const bool cut = !PLAIN && (cuts >> s & 1);
                 A out_z[V], out_x[V];
 #pragma unroll
                 for (int v = 0; v < V; ++v) {
-                    const A e = add(zg[s][v], mine[v]);
-                    out_z[v] = mul(e, conj_of(zp[s][v]));
-                    if constexpr (SIG) out_x[v] = mul(e, zr[s][v]);
+                    const A e = add(g[s][v], c[v]);
+                    out_z[v] = mul(e, conj_of(u[s][v]));
+                    if constexpr (SIG) out_x[v] = mul(e, r[s][v]);
                     else out_x[v] = e;
-                    mine[v] = cut ? zero_of(A()) : mul(za[s][v], e);
+                    c[v] = cut ? zero_of(A()) : mul(a[s][v], e);
                 }
-                put(dz + (int64_t)s * n, c, n, out_z);
-                put(dx + (int64_t)s * n, c, n, out_x);
+                put(dz, at.c, at.n, out_z);
+                put(dx, at.c, at.n, out_x);
             }
+            dz -= at.n;
+            dx -= at.n;
         }
     }
-    if (wave != 0) return;
-    if constexpr (AGGREGATE) {
-        const int64_t at = (blockIdx.y * p.batch + b) * n;
-        put_state<V>(reinterpret_cast<A *>(p.chunk_a) + at, c, n, whole);
-        put_state<V>(reinterpret_cast<A *>(p.chunk_b) + at, c, n, carry);
-        if (lane == 0 && c == 0) p.chunk_cut[blockIdx.y * p.batch + b] = any_cut;
-    } else if (p.d_state && blockIdx.y == 0) {
-        put_state<V>(reinterpret_cast<A *>(p.d_state) + b * n, c, n, carry);
+};
+
+// The same from the last step back, on c: c -> conj(a) (grad + c).
+template <typename Tr, bool SIG>
+__global__ __launch_bounds__(64 * kRecWaves) void recurrence_bw_kernel(RecurrenceArgs p)
+{
+    using A = typename Tr::Acc;
+    constexpr int V = Tr::V, S = Tr::SB;
+    __shared__ Runs<Tr> runs;
+    const RecPlace<Tr> at(p);
+    const int64_t end = at.end;
+    const RecLoad<Tr> in(at.c, at.n);
+    A carry[V];
+    get_state<V>(at.state(p.grad_last), at.c, at.n, carry);
+    RecBack<Tr, SIG> back;
+    const int tile = at.waves * S;
+    const int64_t first = (end - 1) / tile * tile;   // the last tile
+    back.fetch(p, at, in, first + at.wave * S, end);
+    int turn = 0;
+    for (int64_t t0 = first; t0 >= 0; t0 -= tile, turn ^= 1) {
+        const int64_t t = t0 + at.wave * S;
+        const int count = (int)(end - t < 0 ? 0 : end - t < S ? end - t : S);
+        const uint64_t cuts = back.next_cut;
+        back.take(p, at, in, t);
+        if (t0 - tile >= 0) back.fetch(p, at, in, t - tile, end);
+        A ra[V], rb[V], mine[V];
+#pragma unroll
+        for (int v = 0; v < V; ++v) { ra[v] = one_of(A()); rb[v] = zero_of(A()); }
+        by_kind(cuts == 0 && count == S, [&](auto plain) {
+            back.template gates<plain.value>(cuts);
+#pragma unroll
+            for (int s = S - 1; s >= 0; --s) {
+                const bool cut = !plain.value && (cuts >> s & 1);
+                if (!plain.value && s >= count) continue;
+#pragma unroll
+                for (int v = 0; v < V; ++v) {
+                    rb[v] = cut ? zero_of(A()) : mul(back.a[s][v], add(back.g[s][v], rb[v]));
+                    ra[v] = cut ? zero_of(A()) : mul(ra[v], back.a[s][v]);
+                }
+            }
+        });
+        exchange<Tr, true>(runs, turn, at.wave, at.waves, at.lane, cuts != 0, ra, rb, carry, mine);
+        by_kind(cuts == 0 && count == S, [&](auto plain) { back.template steps<plain.value>(p, at, t, count, cuts, mine); });
     }
+    if (at.wave == 0 && p.d_state) put_state<V>(at.state(p.d_state), at.c, at.n, carry);
+}
+
+// ---- sequences cut into chunks ------------------------------------------------------------------------------
+// grid (batch x groups, chunks), kRecWaves wavefronts, each with a run of its own: len = chunk / kRecWaves steps.  The first
+// launch forms every run's (A, B) as composed from the chunk's start (backward: end) up to the run, and the chunks';
+// the second one starts each run from there, and the wavefronts need nothing of each other.
+
+template <typename Tr, bool SIG, bool BACKWARD>
+__global__ __launch_bounds__(64 * kRecWaves) void recurrence_runs_kernel(RecurrenceArgs p)
+{
+    using A = typename Tr::Acc;
+    constexpr int V = Tr::V, S = Tr::S;
+    __shared__ Runs<Tr> runs;
+    const RecPlace<Tr> at(p);
+    const RecLoad<Tr> in(at.c, at.n);
+    const int64_t len = p.chunk / kRecWaves, begin = at.begin + at.wave * len;
+    const int64_t end = begin + len < at.end ? begin + len : at.end;
+    // forward (gates, inputs), backward (gates, gradients)
+    const void *second = BACKWARD ? p.grad : p.x;
+    const int64_t second_b = BACKWARD ? p.grad_b : p.x_b, second_t = BACKWARD ? p.grad_t : p.x_t;
+    A ra[V], rb[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) { ra[v] = one_of(A()); rb[v] = zero_of(A()); }
+    bool any_cut = false;
+    if (begin < end) {
+        typename RecLoad<Tr>::Raw next_z[S], next_x[S];
+        uint64_t next_cut = 0;
+        auto fetch = [&](int64_t t) {
+            load_steps<S, Tr>(next_z, in, at.rows(p.gate, p.gate_b), p.gate_t, t, end);
+            if (second) load_steps<S, Tr>(next_x, in, at.rows(second, second_b), second_t, t, end);
+            next_cut = reset_bits(p, at.b, t, end, S, at.lane);
+        };
+        const int64_t blocks = (end - begin + S - 1) / S;
+        fetch(BACKWARD ? begin + (blocks - 1) * S : begin);
+        for (int64_t k = 0; k < blocks; ++k) {
+            const int64_t t = begin + (BACKWARD ? blocks - 1 - k : k) * S;
+            const int count = (int)(end - t < S ? end - t : S);
+            const uint64_t cuts = next_cut;
+            A za[S][V], zb[S][V];
+#pragma unroll
+            for (int s = 0; s < S; ++s) in.widen(next_z[s], za[s]);
+            if (second) {
+#pragma unroll
+                for (int s = 0; s < S; ++s) in.widen(next_x[s], zb[s]);
+            } else {
+#pragma unroll
+                for (int s = 0; s < S; ++s)
+#pragma unroll
+                    for (int v = 0; v < V; ++v) zb[s][v] = zero_of(A());
+            }
+            if (k + 1 < blocks) fetch(BACKWARD ? t - S : t + S);
+            any_cut |= cuts != 0;
+            by_kind(cuts == 0 && count == S, [&](auto plain) {
+#pragma unroll
+                for (int i = 0; i < S; ++i) {
+                    const int s = BACKWARD ? S - 1 - i : i;
+                    const bool cut = !plain.value && (cuts >> s & 1);
+                    if (!plain.value && s >= count) continue;
+#pragma unroll
+                    for (int v = 0; v < V; ++v) {
+                        A a, rest;
+                        gate_of<SIG, Tr::kExact>(za[s][v], a, rest);
+                        if constexpr (BACKWARD) {
+                            a = conj_of(a);
+                            rb[v] = cut ? zero_of(A()) : mul(a, add(zb[s][v], rb[v]));
+                        } else {
+                            rb[v] = step_of(cut, a, rb[v], SIG ? mul(rest, zb[s][v]) : zb[s][v]);
+                        }
+                        ra[v] = cut ? zero_of(A()) : mul(ra[v], a);
+                    }
+                }
+            });
+        }
+    }
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+        runs.a[0][at.wave][v][at.lane] = ra[v];
+        runs.b[0][at.wave][v][at.lane] = rb[v];
+    }
+    if (at.lane == 0) runs.cut[0][at.wave] = any_cut;
+    __syncthreads();
+    // what stands in front of this wavefront's run, and (the last one's own wavefront) behind all of them
+    const int turn = BACKWARD ? kRecWaves - 1 - at.wave : at.wave, last = turn == kRecWaves - 1;
+    A pa[V], pb[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) { pa[v] = one_of(A()); pb[v] = zero_of(A()); }
+    bool cut = false;
+    auto write = [&](void *to_a, void *to_b, int *to_cut, int64_t slot) {
+        put_state<V>(reinterpret_cast<A *>(to_a) + (slot * p.batch + at.b) * at.n, at.c, at.n, pa);
+        put_state<V>(reinterpret_cast<A *>(to_b) + (slot * p.batch + at.b) * at.n, at.c, at.n, pb);
+        if (at.lane == 0 && at.c == 0) to_cut[slot * p.batch + at.b] = cut;
+    };
+    auto add_run = [&](int i) {
+        const int w = BACKWARD ? kRecWaves - 1 - i : i;
+        const bool cut_w = runs.cut[0][w];
+        cut |= cut_w;
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            const A ca = runs.a[0][w][v][at.lane], cb = runs.b[0][w][v][at.lane];
+            pb[v] = step_of(cut_w, ca, pb[v], cb);
+            pa[v] = cut_w ? zero_of(A()) : mul(pa[v], ca);
+        }
+    };
+    for (int i = 0; i < turn; ++i) add_run(i);
+    write(p.run_a, p.run_b, p.run_cut, (int64_t)blockIdx.y * kRecWaves + at.wave);
+    if (last) {
+        add_run(turn);
+        write(p.chunk_a, p.chunk_b, p.chunk_cut, blockIdx.y);
+    }
+}
+
+// What enters a wavefront's run: the state through the chunks in front of its own, then through the runs.
+template <typename Tr, bool BACKWARD>
+__device__ __forceinline__ void enter_run(const RecurrenceArgs &p, const RecPlace<Tr> &at, const void *state, typename Tr::Acc (&carry)[Tr::V])
+{
+    get_state<Tr::V>(at.state(state), at.c, at.n, carry);
+    const int chunks = BACKWARD ? (int)gridDim.y - 1 - (int)blockIdx.y : (int)blockIdx.y;
+#pragma unroll 8
+    for (int i = 0; i < chunks; ++i)
+        compose<Tr::V>(p.chunk_a, p.chunk_b, p.chunk_cut, (BACKWARD ? (int)gridDim.y - 1 - i : i) * p.batch + at.b, at.c, at.n, carry);
+    compose<Tr::V>(p.run_a, p.run_b, p.run_cut, ((int64_t)blockIdx.y * kRecWaves + at.wave) * p.batch + at.b, at.c, at.n, carry);
+}
+
+template <typename Tr, bool SIG>
+__global__ __launch_bounds__(64 * kRecWaves) void recurrence_chunk_fw_kernel(RecurrenceArgs p)
+{
+    using A = typename Tr::Acc;
+    using E = typename Tr::Elem;
+    constexpr int V = Tr::V, S = Tr::S;
+    const RecPlace<Tr> at(p);
+    const int c = at.c, n = at.n;
+    const RecLoad<Tr> in(c, n);
+    const int64_t len = p.chunk / kRecWaves, begin = at.begin + at.wave * len;
+    const int64_t end = begin + len < at.end ? begin + len : at.end;
+    if (begin >= end) return;
+    typename RecLoad<Tr>::Raw next_z[S], next_x[S];
+    uint64_t next_cut = 0;
+    auto fetch = [&](int64_t t) {
+        load_steps<S, Tr>(next_z, in, at.rows(p.gate, p.gate_b), p.gate_t, t, end);
+        load_steps<S, Tr>(next_x, in, at.rows(p.x, p.x_b), p.x_t, t, end);
+        next_cut = reset_bits(p, at.b, t, end, S, at.lane);
+    };
+    fetch(begin);
+    A h[V];
+    enter_run<Tr, false>(p, at, p.state, h);
+    E *out = reinterpret_cast<E *>(p.h) + (at.b * p.steps + begin) * n;
+    for (int64_t t = begin; t < end; t += S) {
+        const int count = (int)(end - t < S ? end - t : S);
+        const uint64_t cuts = next_cut;
+        A za[S][V], zb[S][V];
+#pragma unroll
+        for (int s = 0; s < S; ++s) {
+            in.widen(next_z[s], za[s]);
+            in.widen(next_x[s], zb[s]);
+        }
+        if (t + S < end) fetch(t + S);
+        by_kind(cuts == 0 && count == S, [&](auto plain) {
+#pragma unroll
+            for (int s = 0; s < S; ++s) {
+                const bool cut = !plain.value && (cuts >> s & 1);
+                if (!plain.value && s >= count) continue;
+#pragma unroll
+                for (int v = 0; v < V; ++v) {
+                    A a, rest;
+                    gate_of<SIG, Tr::kExact>(za[s][v], a, rest);
+                    h[v] = step_of(cut, a, h[v], SIG ? mul(rest, zb[s][v]) : zb[s][v]);
+                }
+                put(out, c, n, h);
+                out += n;
+            }
+        });
+    }
+    if (end == p.steps && p.last) put_state<V>(at.state(p.last), c, n, h);
+}
+
+template <typename Tr, bool SIG>
+__global__ __launch_bounds__(64 * kRecWaves) void recurrence_chunk_bw_kernel(RecurrenceArgs p)
+{
+    using A = typename Tr::Acc;
+    constexpr int V = Tr::V, S = Tr::SB;
+    const RecPlace<Tr> at(p);
+    const RecLoad<Tr> in(at.c, at.n);
+    const int64_t len = p.chunk / kRecWaves, begin = at.begin + at.wave * len;
+    const int64_t end = begin + len < at.end ? begin + len : at.end;
+    if (begin >= end) return;
+    RecBack<Tr, SIG> back;
+    const int64_t first = begin + (end - begin - 1) / S * S;
+    back.fetch(p, at, in, first, end);
+    A carry[V];
+    enter_run<Tr, true>(p, at, p.grad_last, carry);
+    for (int64_t t = first; t >= begin; t -= S) {
+        const int count = (int)(end - t < S ? end - t : S);
+        const uint64_t cuts = back.next_cut;
+        back.take(p, at, in, t);
+        if (t > begin) back.fetch(p, at, in, t - S, end);
+        by_kind(cuts == 0 && count == S, [&](auto plain) {
+            back.template gates<plain.value>(cuts);
+            back.template steps<plain.value>(p, at, t, count, cuts, carry);
+        });
+    }
+    if (begin == 0 && p.d_state) put_state<V>(at.state(p.d_state), at.c, at.n, carry);
 }
 
 // One step of every sequence, the state updated in place.  grid (channels / 256 rounded up, batch).
@@ -503,7 +709,7 @@ __global__ __launch_bounds__(256) void recurrence_step_kernel(RecurrenceArgs p)
 #pragma unroll
         for (int v = 0; v < V; ++v) {
             A a, rest;
-            gate_of<SIG>(z[v], a, rest);
+            gate_of<SIG, Tr::kExact>(z[v], a, rest);
             h[v] = mac(SIG ? mul(rest, x[v]) : x[v], a, h[v]);
         }
         put_state<V>(state, c, n, h);
