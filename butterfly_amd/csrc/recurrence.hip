@@ -40,17 +40,18 @@ struct RecurrencePlan {
 RecurrencePlan plan(const bf_recurrence *p)
 {
     RecurrencePlan r;
-    const int v = p->dtype == BF_BF16 && p->channels > 1 ? RecBF16::V : 1, s = p->dtype == BF_C64 ? RecC64::S : RecF32::S;
+    const bool pairs = p->dtype == BF_BF16 && p->channels > 1;
+    const int v = pairs ? RecBF16::V : 1, s = p->dtype == BF_C64 ? RecC64::S : pairs ? RecBF16::S : RecF32::S;
     r.groups = (p->channels + 64 * v - 1) / (64 * v);
     const int64_t whole = r.groups * p->batch, tile = (int64_t)kRecWaves * s;
     r.chunk = std::max<int64_t>(p->steps, 1);
     if (whole < 192 && p->steps > tile) {
         const int64_t wanted = std::min<int64_t>((512 + whole - 1) / whole, (p->steps + tile - 1) / tile);
-        r.chunk = ((p->steps + wanted - 1) / wanted + tile - 1) / tile * tile;
+        r.chunk = std::max<int64_t>((p->steps / wanted + tile / 2) / tile, 1) * tile;
         r.chunks = (p->steps + r.chunk - 1) / r.chunk;
     }
     r.waves = (int)std::min<int64_t>((r.chunk + s - 1) / s, kRecWaves);
-    const int sb = p->dtype == BF_BF16 && p->channels > 1 ? RecBF16::SB : s;
+    const int sb = p->dtype == BF_C64 ? RecC64::SB : pairs ? RecBF16::SB : RecF32::SB;
     r.waves_bw = (int)std::min<int64_t>((r.chunk + sb - 1) / sb, kRecWaves);
     r.state_bytes = (size_t)p->batch * (size_t)p->channels * (p->dtype == BF_C64 ? 8 : 4);
     if (r.chunks > 1) {
@@ -76,6 +77,7 @@ void fill(RecurrenceArgs &a, const bf_recurrence *p, const RecurrencePlan &r, vo
     a.channels = (int)p->channels;
     a.groups = (int)r.groups;
     a.chunk = r.chunk;
+    a.chunks = (int)r.chunks;
     if (r.chunks > 1) {
         char *w = static_cast<char *>(workspace);
         a.run_a = w;
@@ -162,7 +164,7 @@ int bf_recurrence_fw(const bf_recurrence *p, const void *gate, const void *x, co
         constexpr bool SIG = decltype(sigmoid)::value;
         const unsigned x_blocks = (unsigned)(r.groups * p->batch);
         if (r.chunks > 1) {
-            const dim3 grid(x_blocks, (unsigned)r.chunks), threads(64 * kRecWaves);
+            const dim3 grid(x_blocks, ((unsigned)r.chunks + 7) / 8 * 8), threads(64 * kRecWaves);
             recurrence_runs_kernel<Tr, SIG, false><<<grid, threads, 0, s>>>(a);
             recurrence_chunk_fw_kernel<Tr, SIG><<<grid, threads, 0, s>>>(a);
         } else {
@@ -202,7 +204,7 @@ int bf_recurrence_bw(const bf_recurrence *p, const void *gate, const void *x, co
         constexpr bool SIG = decltype(sigmoid)::value;
         const unsigned x_blocks = (unsigned)(r.groups * p->batch);
         if (r.chunks > 1) {
-            const dim3 grid(x_blocks, (unsigned)r.chunks), threads(64 * kRecWaves);
+            const dim3 grid(x_blocks, ((unsigned)r.chunks + 7) / 8 * 8), threads(64 * kRecWaves);
             recurrence_runs_kernel<Tr, SIG, true><<<grid, threads, 0, s>>>(a);
             recurrence_chunk_bw_kernel<Tr, SIG><<<grid, threads, 0, s>>>(a);
         } else {

@@ -42,7 +42,7 @@ struct RecurrenceArgs {
     int64_t gate_b, gate_t, x_b, x_t, grad_b, grad_t, reset_b, reset_t;
     int64_t steps, chunk;               // chunk: steps of a chunk (the last one may be shorter)
     int64_t batch;
-    int channels, groups;               // groups: workgroups across the channels
+    int channels, groups, chunks;       // groups: workgroups across the channels
     void *chunk_a, *chunk_b;            // (chunks, batch, channels): what a chunk does
     void *run_a, *run_b;                // (chunks, kRecWaves, batch, channels): what stands in front of a run in its chunk
     int *chunk_cut, *run_cut;           // the same by sequence: a reset inside
@@ -241,14 +241,29 @@ template <typename Tr>
 struct RecPlace {
     using E = typename Tr::Elem;
     using A = typename Tr::Acc;
-    int lane, wave, waves, c, n;
+    int lane, wave, waves, chunk, c, n;
     int64_t b, begin, end;     // the workgroup's steps
 
+    // Workgroups go to the eight XCDs in turn.  Rows seldom begin at a cache line, so the groups of channels of one
+    // chunk belong on one XCD, behind each other, where a line that two of them share is in one L2: chunk k is XCD k % 8's
+    // (grid: chunks up to a multiple of 8), and whole sequences are runs of neighbours for each XCD.
     __device__ __forceinline__ explicit RecPlace(const RecurrenceArgs &p)
-        : lane(threadIdx.x & 63), wave(__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)), waves(blockDim.x >> 6),
-          c(((int)(blockIdx.x % (unsigned)p.groups) * 64 + lane) * Tr::V), n(p.channels), b(blockIdx.x / (unsigned)p.groups),
-          begin((int64_t)blockIdx.y * p.chunk), end(begin + p.chunk < p.steps ? begin + p.chunk : p.steps)
+        : lane(threadIdx.x & 63), wave(__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)), waves(blockDim.x >> 6), n(p.channels)
     {
+        const uint64_t id = (uint64_t)blockIdx.y * gridDim.x + blockIdx.x, xcd = id % 8;
+        unsigned x;
+        if (p.chunks > 1) {
+            chunk = (int)(id / 8 / gridDim.x * 8 + xcd);
+            x = (unsigned)(id / 8 % gridDim.x);
+        } else {
+            const unsigned per = gridDim.x / 8, over = gridDim.x % 8;
+            chunk = 0;
+            x = (unsigned)(xcd * per + (xcd < over ? xcd : over) + id / 8);
+        }
+        b = x / (unsigned)p.groups;
+        c = ((int)(x % (unsigned)p.groups) * 64 + lane) * Tr::V;
+        begin = (int64_t)chunk * p.chunk;
+        end = begin + p.chunk < p.steps ? begin + p.chunk : p.steps;
     }
     __device__ __forceinline__ const E *rows(const void *p, int64_t stride) const { return reinterpret_cast<const E *>(p) + b * stride; }
     __device__ __forceinline__ const A *state(const void *p) const { return p ? reinterpret_cast<const A *>(p) + b * n : nullptr; }
@@ -501,6 +516,7 @@ __global__ __launch_bounds__(64 * kRecWaves) void recurrence_runs_kernel(Recurre
     constexpr int V = Tr::V, S = Tr::S;
     __shared__ Runs<Tr> runs;
     const RecPlace<Tr> at(p);
+    if (at.chunk >= p.chunks) return;
     const RecLoad<Tr> in(at.c, at.n);
     const int64_t len = p.chunk / kRecWaves, begin = at.begin + at.wave * len;
     const int64_t end = begin + len < at.end ? begin + len : at.end;
@@ -591,10 +607,10 @@ __global__ __launch_bounds__(64 * kRecWaves) void recurrence_runs_kernel(Recurre
         }
     };
     for (int i = 0; i < turn; ++i) add_run(i);
-    write(p.run_a, p.run_b, p.run_cut, (int64_t)blockIdx.y * kRecWaves + at.wave);
+    write(p.run_a, p.run_b, p.run_cut, (int64_t)at.chunk * kRecWaves + at.wave);
     if (last) {
         add_run(turn);
-        write(p.chunk_a, p.chunk_b, p.chunk_cut, blockIdx.y);
+        write(p.chunk_a, p.chunk_b, p.chunk_cut, at.chunk);
     }
 }
 
@@ -603,11 +619,11 @@ template <typename Tr, bool BACKWARD>
 __device__ __forceinline__ void enter_run(const RecurrenceArgs &p, const RecPlace<Tr> &at, const void *state, typename Tr::Acc (&carry)[Tr::V])
 {
     get_state<Tr::V>(at.state(state), at.c, at.n, carry);
-    const int chunks = BACKWARD ? (int)gridDim.y - 1 - (int)blockIdx.y : (int)blockIdx.y;
+    const int chunks = BACKWARD ? p.chunks - 1 - at.chunk : at.chunk;
 #pragma unroll 8
     for (int i = 0; i < chunks; ++i)
-        compose<Tr::V>(p.chunk_a, p.chunk_b, p.chunk_cut, (BACKWARD ? (int)gridDim.y - 1 - i : i) * p.batch + at.b, at.c, at.n, carry);
-    compose<Tr::V>(p.run_a, p.run_b, p.run_cut, ((int64_t)blockIdx.y * kRecWaves + at.wave) * p.batch + at.b, at.c, at.n, carry);
+        compose<Tr::V>(p.chunk_a, p.chunk_b, p.chunk_cut, (BACKWARD ? p.chunks - 1 - i : i) * p.batch + at.b, at.c, at.n, carry);
+    compose<Tr::V>(p.run_a, p.run_b, p.run_cut, ((int64_t)at.chunk * kRecWaves + at.wave) * p.batch + at.b, at.c, at.n, carry);
 }
 
 template <typename Tr, bool SIG>
@@ -617,6 +633,7 @@ __global__ __launch_bounds__(64 * kRecWaves) void recurrence_chunk_fw_kernel(Rec
     using E = typename Tr::Elem;
     constexpr int V = Tr::V, S = Tr::S;
     const RecPlace<Tr> at(p);
+    if (at.chunk >= p.chunks) return;
     const int c = at.c, n = at.n;
     const RecLoad<Tr> in(c, n);
     const int64_t len = p.chunk / kRecWaves, begin = at.begin + at.wave * len;
@@ -668,6 +685,7 @@ __global__ __launch_bounds__(64 * kRecWaves) void recurrence_chunk_bw_kernel(Rec
     using A = typename Tr::Acc;
     constexpr int V = Tr::V, S = Tr::SB;
     const RecPlace<Tr> at(p);
+    if (at.chunk >= p.chunks) return;
     const RecLoad<Tr> in(at.c, at.n);
     const int64_t len = p.chunk / kRecWaves, begin = at.begin + at.wave * len;
     const int64_t end = begin + len < at.end ? begin + len : at.end;
