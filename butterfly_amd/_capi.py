@@ -33,7 +33,8 @@ SYMBOLS = [
     "bf_layer_takes_real", "bf_layer_kept_bytes", "bf_layer_fw_workspace_bytes", "bf_layer_fw", "bf_layer_bw_workspace_bytes", "bf_layer_bw",
     "bf_rng_next", "bf_rowwise_fw", "bf_rowwise_bw_workspace_bytes", "bf_rowwise_bw",
     "bf_recurrence_workspace_bytes", "bf_recurrence_fw", "bf_recurrence_bw", "bf_recurrence_step",
-    "bf_linear_xent_fw_workspace_bytes", "bf_linear_xent_bw_workspace_bytes", "bf_linear_xent_fw", "bf_linear_xent_bw",
+    "bf_linear_xent_kept_bytes", "bf_linear_xent_fw_workspace_bytes", "bf_linear_xent_bw_workspace_bytes", "bf_linear_xent_fw",
+    "bf_linear_xent_bw",
 ]
 
 NOALLOC_SCRATCH_BYTES = 48 << 20
@@ -162,11 +163,11 @@ def lib():
         L.bf_recurrence_fw.argtypes = [pc] + [vp] * 7 + [sz, vp]
         L.bf_recurrence_bw.argtypes = [pc] + [vp] * 11 + [sz, vp]
         L.bf_recurrence_step.argtypes = [pc] + [vp] * 5
-        for name in ("bf_linear_xent_fw_workspace_bytes", "bf_linear_xent_bw_workspace_bytes"):
+        for name in ("bf_linear_xent_kept_bytes", "bf_linear_xent_fw_workspace_bytes", "bf_linear_xent_bw_workspace_bytes"):
             getattr(L, name).argtypes = [px]
             getattr(L, name).restype = sz
-        L.bf_linear_xent_fw.argtypes = [px] + [vp] * 6 + [sz, vp]
-        L.bf_linear_xent_bw.argtypes = [px] + [vp] * 8 + [sz, vp]
+        L.bf_linear_xent_fw.argtypes = [px] + [vp] * 5 + [sz, vp, sz, vp]
+        L.bf_linear_xent_bw.argtypes = [px] + [vp] * 3 + [sz, vp, vp, vp, sz, vp]
         _lib = L
     return _lib
 

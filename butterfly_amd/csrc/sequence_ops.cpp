@@ -574,6 +574,7 @@ bf_linear_xent describe(const Xent &o, const Tensor &hidden, const Tensor &weigh
     return d;
 }
 
+// (loss, kept operands)
 std::tuple<Tensor, Tensor> xent_fw(const Xent &o)
 {
     const Guard guard(o.hidden.device());
@@ -581,18 +582,19 @@ std::tuple<Tensor, Tensor> xent_fw(const Xent &o)
     const bf_linear_xent d = describe(o, hidden, weight);
     const auto options = hidden.options().dtype(at::kFloat);
     Tensor loss = o.reduction == BF_XENT_NONE ? at::empty(o.target.sizes(), options) : at::empty({}, options);
-    Tensor lse = at::empty({d.rows}, options);
     const size_t bytes = valid_size(bf_linear_xent_fw_workspace_bytes(&d));
-    const Tensor ws = workspace_like(hidden, bytes);
+    const size_t kept_bytes = valid_size(bf_linear_xent_kept_bytes(&d));
+    const Tensor ws = workspace_like(hidden, bytes), kept = workspace_like(hidden, kept_bytes);
     check_rc(bf_linear_xent_fw(&d, hidden.data_ptr(), weight.data_ptr(), target.data_ptr<int64_t>(), loss.data_ptr<float>(),
-                               lse.data_ptr<float>(), ptr(ws), bytes, current_stream()),
+                               ptr(kept), kept_bytes, ptr(ws), bytes, current_stream()),
              o.who);
-    return {loss, lse};
+    return {loss, kept};
 }
 
 struct XentNode : public torch::autograd::Node {
-    SavedSlot hidden, weight, target, lse;
-    int64_t ignore_index = -100, reduction = BF_XENT_MEAN;
+    SavedSlot weight, kept;
+    c10::SmallVector<int64_t, 6> hidden_shape;
+    bf_linear_xent desc = {};
 
     // edges: hidden, weight
     variable_list apply(variable_list &&grads) override
@@ -601,32 +603,27 @@ struct XentNode : public torch::autograd::Node {
         if (!grads[0].defined()) return out;
         std::lock_guard<std::mutex> lock(mutex_);
         const auto self = getptr();
-        Xent o;
-        o.hidden = hidden.get(self);
-        o.weight = weight.get(self);
-        o.target = target.get(self);
-        o.ignore_index = ignore_index;
-        o.reduction = reduction;
-        const Tensor sums = lse.get(self);
+        const Tensor saved = weight.get(self), operands = kept.get(self);
         const bool want_hidden = task_should_compute_output(0), want_weight = task_should_compute_output(1);
         at::AutoDispatchBelowADInplaceOrView below;
-        const Guard guard(o.hidden.device());
-        const Tensor h = rows_of(o.hidden), w = aligned_rows_of(o.weight), t = o.target.contiguous(), g = grads[0].contiguous();
-        const bf_linear_xent d = describe(o, h, w);
-        if (want_hidden) out[0] = at::empty(o.hidden.sizes(), h.options());
-        if (want_weight) out[1] = at::empty(o.weight.sizes(), w.options());
+        const Guard guard(saved.device());
+        const Tensor w = aligned_rows_of(saved), g = grads[0].contiguous();
+        bf_linear_xent d = desc;
+        d.weight_stride = row_stride(w);
+        if (want_hidden) out[0] = at::empty(hidden_shape, w.options());
+        if (want_weight) out[1] = at::empty(saved.sizes(), w.options());
         const size_t bytes = valid_size(bf_linear_xent_bw_workspace_bytes(&d));
-        const Tensor ws = workspace_like(h, bytes);
-        check_rc(bf_linear_xent_bw(&d, h.data_ptr(), w.data_ptr(), t.data_ptr<int64_t>(), sums.data_ptr<float>(),
-                                   g.data_ptr<float>(), ptr(out[0]), ptr(out[1]), ptr(ws), bytes, current_stream()),
-                 o.who);
+        const Tensor ws = workspace_like(w, bytes);
+        check_rc(bf_linear_xent_bw(&d, w.data_ptr(), g.data_ptr<float>(), operands.data_ptr(),
+                                   (size_t)operands.numel(), ptr(out[0]), ptr(out[1]), ptr(ws), bytes, current_stream()),
+                 "linear_cross_entropy");
         return out;
     }
 
     void release_variables() override
     {
         std::lock_guard<std::mutex> lock(mutex_);
-        for (SavedSlot *s : {&hidden, &weight, &target, &lse}) s->drop();
+        for (SavedSlot *s : {&weight, &kept}) s->drop();
     }
 
     std::string name() const override { return "LinearCrossEntropyBackward"; }
@@ -660,17 +657,15 @@ Tensor linear_cross_entropy(Tensor hidden, Tensor weight, Tensor target, int64_t
     }
     std::shared_ptr<XentNode> node(new XentNode(), torch::autograd::deleteNode);
     node->set_next_edges(torch::autograd::collect_next_edges(hidden, weight));
-    Tensor loss, lse;
+    Tensor loss, kept;
     {
         at::AutoDispatchBelowADInplaceOrView below;
-        std::tie(loss, lse) = xent_fw(o);
+        std::tie(loss, kept) = xent_fw(o);
+        node->desc = describe(o, rows_of(hidden), rows_of(weight));
     }
-    node->hidden.set(hidden);
+    node->hidden_shape = hidden.sizes();
     node->weight.set(weight);
-    node->target.set(target);
-    node->lse.set(lse);
-    node->ignore_index = ignore_index;
-    node->reduction = reduction;
+    node->kept.set(kept);
     torch::autograd::set_history(loss, node);
     return loss;
 }

@@ -70,9 +70,10 @@ struct XentPlan {
     // backward
     int64_t piece = 0;                          // vocabulary entries of a piece, whole tiles
     Product to_hidden, to_weight;
-    // offsets into the workspace
-    size_t scalars = 0, index = 0, position = 0, label = 0, picked = 0, losses = 0, partial = 0, hidden = 0, weight = 0;
-    size_t share = 0, lse_at = 0, d_l = 0, d_l_plane = 0, sums_hidden = 0, sums_weight = 0;
+    // offsets into what the forward call leaves for the backward one, and into the workspaces
+    size_t scalars = 0, index = 0, position = 0, label = 0, lse = 0, hidden = 0, weight = 0, kept = 0;
+    size_t picked = 0, losses = 0, partial = 0;
+    size_t share = 0, d_l = 0, d_l_plane = 0, sums_hidden = 0, sums_weight = 0;
     size_t total = 0;
 };
 
@@ -95,8 +96,11 @@ XentPlan plan(const bf_linear_xent *p, bool backward)
     r.index = take(rows * 4);
     r.position = take(rows * 4);
     r.label = take(rows * 4);
+    r.lse = take(rows * 4);
     r.hidden = take(r.hidden_plane * r.planes);
     if (!weight_in_place(p)) r.weight = take(r.weight_plane * r.planes);
+    r.kept = at;
+    at = 0;
     if (!backward) {
         r.logits = product(p->vocab, p->rows, 0, false);
         r.picked = take(rows * 4);
@@ -111,7 +115,6 @@ XentPlan plan(const bf_linear_xent *p, bool backward)
         r.to_hidden = product(p->features, p->rows, r.piece / kMatK, true);
         r.to_weight = product(p->features, r.piece, (p->rows + kMatK - 1) / kMatK, true);
         r.share = take(rows * 4);
-        r.lse_at = take(rows * 4);
         r.d_l_plane = up256((size_t)r.rows_up * r.piece * 2);
         r.d_l = take(r.d_l_plane * r.planes);
         r.sums_hidden = take((size_t)r.to_hidden.splits * rows * p->features * sizeof(float));
@@ -121,8 +124,11 @@ XentPlan plan(const bf_linear_xent *p, bool backward)
     return r;
 }
 
-int check_memory(const XentPlan &r, const void *weight, const void *workspace, size_t bytes)
+int check_memory(const XentPlan &r, const void *weight, const void *kept, size_t kept_bytes, const void *workspace, size_t bytes)
 {
+    if (!kept || kept_bytes < r.kept)
+        return fail(BF_ERR_WORKSPACE, "room for %zu bytes of kept operands needed, %zu given", r.kept, kept ? kept_bytes : 0);
+    if (reinterpret_cast<uintptr_t>(kept) & 255) return fail(BF_ERR_WORKSPACE, "the kept operands must be 256-byte aligned");
     if (reinterpret_cast<uintptr_t>(weight) & 15) return fail(BF_ERR_INVALID, "weight must be 16-byte aligned");
     if (!workspace || bytes < r.total)
         return fail(BF_ERR_WORKSPACE, "workspace of %zu bytes needed, %zu given", r.total, workspace ? bytes : 0);
@@ -151,24 +157,31 @@ void pack(const bf_linear_xent *p, const void *x, char *out, int64_t out_rows, i
     else xent_pack_kernel<bf16><<<grid, dim3(256), 0, s>>>(a);
 }
 
-// What both directions start with: the counted rows, hidden and weight as operands.
-void prepare(const bf_linear_xent *p, const XentPlan &r, const void *hidden, const void *weight, const int64_t *target, void *ws,
-             float *picked, MatOperand &h, MatOperand &w, hipStream_t s)
+// Hidden and weight as the products read them: what prepare() made of them, or weight itself.
+void operands(const bf_linear_xent *p, const XentPlan &r, const void *weight, void *kept, MatOperand &h, MatOperand &w)
 {
-    XentScalars *scalars = part<XentScalars>(ws, r.scalars);
-    const XentRowsArgs rows = {target, p->rows, p->vocab, p->ignore_index, scalars, part<int>(ws, r.index),
-                               part<int>(ws, r.position), part<int>(ws, r.label), picked};
-    xent_rows_kernel<<<dim3(1), dim3(kXentThreads), 0, s>>>(rows);
-    char *hp = part<char>(ws, r.hidden), *wp = part<char>(ws, r.weight);
+    char *hp = part<char>(kept, r.hidden), *wp = part<char>(kept, r.weight);
     const int64_t stride = r.features_up * 2;
-    pack(p, hidden, hp, r.rows_up, p->rows, p->hidden_stride, stride, r.hidden_plane, part<int>(ws, r.index), scalars, 0, s);
     h = {hp, (int64_t)r.hidden_plane, stride, r.rows_up * stride};
-    if (weight_in_place(p)) {
+    if (weight_in_place(p))
         w = {static_cast<const char *>(weight), 0, p->weight_stride * 2, ((p->vocab - 1) * p->weight_stride + p->features) * 2};
-    } else {
-        pack(p, weight, wp, p->vocab, p->vocab, p->weight_stride, stride, r.weight_plane, nullptr, scalars, 1, s);
+    else
         w = {wp, (int64_t)r.weight_plane, stride, p->vocab * stride};
-    }
+}
+
+// The counted rows, and both operands in that form, for both directions.
+void prepare(const bf_linear_xent *p, const XentPlan &r, const void *hidden, const void *weight, const int64_t *target, void *kept,
+             float *picked, hipStream_t s)
+{
+    XentScalars *scalars = part<XentScalars>(kept, r.scalars);
+    const XentRowsArgs rows = {target, p->rows, p->vocab, p->ignore_index, scalars, part<int>(kept, r.index),
+                               part<int>(kept, r.position), part<int>(kept, r.label), picked};
+    xent_rows_kernel<<<dim3(1), dim3(kXentThreads), 0, s>>>(rows);
+    const int64_t stride = r.features_up * 2;
+    pack(p, hidden, part<char>(kept, r.hidden), r.rows_up, p->rows, p->hidden_stride, stride, r.hidden_plane,
+         part<int>(kept, r.index), scalars, 0, s);
+    if (!weight_in_place(p))
+        pack(p, weight, part<char>(kept, r.weight), p->vocab, p->vocab, p->weight_stride, stride, r.weight_plane, nullptr, scalars, 1, s);
 }
 
 template <bool F16, bool BACKWARD>
@@ -194,7 +207,8 @@ void launch_grad(const bf_linear_xent *p, const Product &r, const XentGradArgs &
 
 void gather(const bf_linear_xent *p, const XentGatherArgs &a, hipStream_t s)
 {
-    const dim3 grid((unsigned)std::min<int64_t>(a.rows, 8192));
+    const int64_t units = a.rows * ((a.m + 7) / 8);
+    const dim3 grid((unsigned)std::min<int64_t>((units + 255) / 256, 8192));
     if (p->dtype == BF_F32) xent_gather_kernel<float><<<grid, dim3(256), 0, s>>>(a);
     else xent_gather_kernel<bf16><<<grid, dim3(256), 0, s>>>(a);
 }
@@ -202,6 +216,11 @@ void gather(const bf_linear_xent *p, const XentGatherArgs &a, hipStream_t s)
 }  // namespace
 
 extern "C" {
+
+size_t bf_linear_xent_kept_bytes(const bf_linear_xent *p)
+{
+    return check_xent(p) ? BF_SIZE_INVALID : plan(p, false).kept;
+}
 
 size_t bf_linear_xent_fw_workspace_bytes(const bf_linear_xent *p)
 {
@@ -214,27 +233,28 @@ size_t bf_linear_xent_bw_workspace_bytes(const bf_linear_xent *p)
 }
 
 int bf_linear_xent_fw(const bf_linear_xent *p, const void *hidden, const void *weight, const int64_t *target, float *loss,
-                      float *lse, void *workspace, size_t workspace_bytes, void *stream)
+                      void *kept, size_t kept_bytes, void *workspace, size_t workspace_bytes, void *stream)
 {
     int rc = check_xent(p);
     if (rc) return rc;
-    if (p->rows > 0 && (!hidden || !target || !lse)) return fail(BF_ERR_INVALID, "hidden, target or lse is NULL");
+    if (p->rows > 0 && (!hidden || !target)) return fail(BF_ERR_INVALID, "hidden or target is NULL");
     if (!weight || (!loss && (p->rows > 0 || p->reduction != BF_XENT_NONE))) return fail(BF_ERR_INVALID, "weight or loss is NULL");
     if (p->rows == 0 && p->reduction == BF_XENT_NONE) return BF_OK;
     const XentPlan r = plan(p, false);
-    if ((rc = check_memory(r, weight, workspace, workspace_bytes))) return rc;
+    if ((rc = check_memory(r, weight, kept, kept_bytes, workspace, workspace_bytes))) return rc;
     hipStream_t s = static_cast<hipStream_t>(stream);
     MatOperand h, w;
     float *picked = part<float>(workspace, r.picked);
-    prepare(p, r, hidden, weight, target, workspace, picked, h, w, s);
-    XentScalars *scalars = part<XentScalars>(workspace, r.scalars);
+    prepare(p, r, hidden, weight, target, kept, picked, s);
+    operands(p, r, weight, kept, h, w);
+    XentScalars *scalars = part<XentScalars>(kept, r.scalars);
     float *losses = p->reduction == BF_XENT_NONE ? loss : part<float>(workspace, r.losses);
     if (p->rows > 0) {
         XentTileArgs a = {};
         a.weight = w;
         a.hidden = h;
         a.scalars = scalars;
-        a.label = part<int>(workspace, r.label);
+        a.label = part<int>(kept, r.label);
         a.rows = p->rows;
         a.vocab = p->vocab;
         a.features_steps = (int)(r.features_up / kMatK);
@@ -244,8 +264,9 @@ int bf_linear_xent_fw(const bf_linear_xent *p, const void *hidden, const void *w
         a.picked = picked;
         if (p->dtype == BF_F32) launch_logits<true, false>(r.logits, a, s);
         else launch_logits<false, false>(r.logits, a, s);
-        const XentJoinArgs j = {a.partial, picked, part<int>(workspace, r.position), p->rows, 2 * r.logits.tiles_m, lse, losses};
-        xent_join_kernel<<<dim3((unsigned)((p->rows + 15) / 16)), dim3(256), 0, s>>>(j);
+        const XentJoinArgs j = {a.partial, picked, part<int>(kept, r.position), part<int>(kept, r.label), p->rows, 2 * r.logits.tiles_m,
+                                part<float>(kept, r.lse), losses};
+        xent_join_kernel<<<dim3((unsigned)((p->rows + 31) / 32)), dim3(512), 0, s>>>(j);
     }
     if (p->reduction != BF_XENT_NONE)
         xent_total_kernel<<<dim3(1), dim3(kXentThreads), 0, s>>>(losses, p->rows, scalars, p->reduction == BF_XENT_MEAN, loss);
@@ -253,26 +274,22 @@ int bf_linear_xent_fw(const bf_linear_xent *p, const void *hidden, const void *w
     return BF_OK;
 }
 
-int bf_linear_xent_bw(const bf_linear_xent *p, const void *hidden, const void *weight, const int64_t *target, const float *lse,
-                      const float *grad, void *d_hidden, void *d_weight, void *workspace, size_t workspace_bytes, void *stream)
+int bf_linear_xent_bw(const bf_linear_xent *p, const void *weight, const float *grad, void *kept, size_t kept_bytes, void *d_hidden, void *d_weight, void *workspace, size_t workspace_bytes, void *stream)
 {
     int rc = check_xent(p);
     if (rc) return rc;
-    if (p->rows > 0 && (!hidden || !target || !lse)) return fail(BF_ERR_INVALID, "hidden, target or lse is NULL");
     if (!weight || (!grad && (p->rows > 0 || p->reduction != BF_XENT_NONE))) return fail(BF_ERR_INVALID, "weight or grad is NULL");
     if (!d_hidden && !d_weight) return BF_OK;
     const XentPlan r = plan(p, true);
-    if ((rc = check_memory(r, weight, workspace, workspace_bytes))) return rc;
+    if ((rc = check_memory(r, weight, kept, kept_bytes, workspace, workspace_bytes))) return rc;
     hipStream_t s = static_cast<hipStream_t>(stream);
     MatOperand h, w;
-    prepare(p, r, hidden, weight, target, workspace, nullptr, h, w, s);
-    XentScalars *scalars = part<XentScalars>(workspace, r.scalars);
-    if (grad) {
-        const XentShareArgs g = {grad, lse, part<int>(workspace, r.index), part<int>(workspace, r.label), scalars,
-                                 p->reduction == BF_XENT_NONE, p->reduction == BF_XENT_MEAN,
-                                 part<float>(workspace, r.share), part<float>(workspace, r.lse_at)};
-        xent_share_kernel<<<dim3(1), dim3(kXentThreads), 0, s>>>(g);
-    }
+    operands(p, r, weight, kept, h, w);
+    XentScalars *scalars = part<XentScalars>(kept, r.scalars);
+    const XentGrad gradient = {grad, p->reduction == BF_XENT_NONE, p->reduction == BF_XENT_MEAN};
+    if (gradient.each && p->rows > 0)
+        xent_share_kernel<<<dim3(1), dim3(kXentThreads), 0, s>>>(gradient, part<int>(kept, r.index), scalars,
+                                                                 part<float>(workspace, r.share));
     const size_t elem = p->dtype == BF_F32 ? 4 : 2;
     char *d_l = part<char>(workspace, r.d_l);
     const int64_t d_l_stride = r.piece * 2;
@@ -286,7 +303,7 @@ int bf_linear_xent_bw(const bf_linear_xent *p, const void *hidden, const void *w
         a.weight = wp;
         a.hidden = h;
         a.scalars = scalars;
-        a.label = part<int>(workspace, r.label);
+        a.label = part<int>(kept, r.label);
         a.rows = p->rows;
         a.vocab = entries;
         a.first = first;
@@ -296,8 +313,8 @@ int bf_linear_xent_bw(const bf_linear_xent *p, const void *hidden, const void *w
         logits.tiles_m = (int)((entries + side - 1) / side);
         a.tiles_m = logits.tiles_m;
         a.tiles_n = logits.tiles_n;
-        a.lse = part<float>(workspace, r.lse_at);
-        a.share = part<float>(workspace, r.share);
+        a.lse = part<float>(kept, r.lse);
+        a.share = gradient.each ? part<float>(workspace, r.share) : nullptr;
         a.d_l = d_l;
         a.stride = d_l_stride;
         a.plane = (int64_t)r.d_l_plane;
@@ -310,6 +327,7 @@ int bf_linear_xent_bw(const bf_linear_xent *p, const void *hidden, const void *w
             g.a = wp;
             g.b = d_l_operand;
             g.scalars = scalars;
+            g.grad = gradient;
             g.m = p->features;
             g.n = p->rows;
             g.tiles_m = r.to_hidden.tiles_m;
@@ -328,6 +346,7 @@ int bf_linear_xent_bw(const bf_linear_xent *p, const void *hidden, const void *w
             g.a = h;
             g.b = d_l_operand;
             g.scalars = scalars;
+            g.grad = gradient;
             g.m = p->features;
             g.n = entries;
             g.tiles_m = to_weight.tiles_m;
@@ -338,11 +357,11 @@ int bf_linear_xent_bw(const bf_linear_xent *p, const void *hidden, const void *w
             else g.out = out;
             launch_grad<kCols>(p, to_weight, g, s);
             if (g.splits > 1)
-                gather(p, {g.partial, nullptr, scalars, out, entries, entries, p->features, g.splits, 1}, s);
+                gather(p, {g.partial, nullptr, scalars, gradient, out, entries, entries, p->features, g.splits, 1}, s);
         }
     }
     if (d_hidden && p->rows > 0)
-        gather(p, {part<float>(workspace, r.sums_hidden), part<int>(workspace, r.position), scalars, d_hidden, p->rows, p->rows,
+        gather(p, {part<float>(workspace, r.sums_hidden), part<int>(kept, r.position), scalars, gradient, d_hidden, p->rows, p->rows,
                    p->features, r.to_hidden.splits, 0}, s);
     BF_HIP_CHECK(hipGetLastError());
     return BF_OK;

@@ -29,7 +29,7 @@ constexpr int kXentThreads = 1024;   // of the single-workgroup kernels
 
 struct XentScalars {
     float hidden_scale, weight_scale;   // the powers of two
-    float grad_scale;                   // largest |g_i| (d_l is kept over it)
+    float grad_scale;                   // one gradient a row: the largest |g_i| (d_l is kept over it)
     unsigned hidden_max, weight_max;    // bits of the largest magnitudes
     int counted;                        // rows whose target is not ignored
 };
@@ -43,42 +43,53 @@ struct XentRowsArgs {
     int *index;          // (rows) the counted rows in ascending order
     int *position;       // (rows) a row's place among them, -1: ignored
     int *label;          // (rows) by place: the target, -1 where it is no entry of the vocabulary
-    float *picked;       // (rows) by place: NaN, for the target's logit; NULL: not wanted
+    float *picked;       // (rows) by place: NaN, for the target's logit
 };
 
+// 8192 rows a round, eight times 64 neighbours a wavefront.
 __global__ __launch_bounds__(kXentThreads) void xent_rows_kernel(XentRowsArgs a)
 {
-    __shared__ int sums[kXentThreads / 64];
-    const int64_t per = (a.rows + kXentThreads - 1) / kXentThreads, begin = threadIdx.x * per;
-    const int64_t end = begin + per < a.rows ? begin + per : a.rows;
-    int n = 0;
-    for (int64_t i = begin; i < end; ++i) n += a.target[i] != a.ignore;
-    int at = n;   // inclusive sum over the wavefront
+    constexpr int kEach = 8, kWaves = kXentThreads / 64;
+    __shared__ int sums[2][kWaves];
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    int done = 0, turn = 0;
+    for (int64_t from = 0; from < a.rows; from += kXentThreads * kEach, turn ^= 1) {
+        const int64_t begin = from + wave * (64 * kEach) + lane;
+        int64_t t[kEach];
 #pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-        const int v = __shfl_up(at, d, 64);
-        if ((int)(threadIdx.x & 63) >= d) at += v;
-    }
-    if ((threadIdx.x & 63) == 63) sums[threadIdx.x >> 6] = at;
-    __syncthreads();
-    int before = 0, total = 0;
-    for (int w = 0; w < kXentThreads / 64; ++w) {
-        if (w < (int)(threadIdx.x >> 6)) before += sums[w];
-        total += sums[w];
-    }
-    at += before - n;
-    for (int64_t i = begin; i < end; ++i) {
-        const int64_t t = a.target[i];
-        const bool in = t != a.ignore;
-        a.position[i] = in ? at : -1;
-        if (!in) continue;
-        a.index[at] = (int)i;
-        a.label[at] = t >= 0 && t < a.vocab ? (int)t : -1;
-        if (a.picked) a.picked[at] = __builtin_nanf("");
-        ++at;
+        for (int k = 0; k < kEach; ++k) t[k] = begin + 64 * k < a.rows ? a.target[begin + 64 * k] : a.ignore;
+        uint64_t counts[kEach];
+        int n = 0;
+#pragma unroll
+        for (int k = 0; k < kEach; ++k) {
+            counts[k] = __ballot(t[k] != a.ignore);
+            n += __popcll(counts[k]);
+        }
+        if (lane == 0) sums[turn][wave] = n;
+        __syncthreads();
+        int at = done;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) {
+            const int v = sums[turn][w];
+            if (w < wave) at += v;
+            done += v;
+        }
+#pragma unroll
+        for (int k = 0; k < kEach; ++k) {
+            const int64_t row = begin + 64 * k;
+            const bool in = counts[k] >> lane & 1;
+            const int place = at + __popcll(counts[k] & ((1ull << lane) - 1));
+            if (row < a.rows) a.position[row] = in ? place : -1;
+            if (in) {
+                a.index[place] = (int)row;
+                a.label[place] = t[k] >= 0 && t[k] < a.vocab ? (int)t[k] : -1;
+                a.picked[place] = __builtin_nanf("");
+            }
+            at += __popcll(counts[k]);
+        }
     }
     if (threadIdx.x == 0) {
-        a.scalars->counted = total;
+        a.scalars->counted = done;
         a.scalars->hidden_max = a.scalars->weight_max = 0;
         a.scalars->hidden_scale = a.scalars->weight_scale = a.scalars->grad_scale = 1.0f;
     }
@@ -185,6 +196,17 @@ __global__ __launch_bounds__(256) void xent_pack_kernel(XentPackArgs a)
 
 // ---- the logits' tiles --------------------------------------------------------------------------------------
 
+struct XentGrad {
+    const float *grad;      // one number, or one a row (each)
+    int each, mean;
+
+    __device__ __forceinline__ float scale(const XentScalars *s) const
+    {
+        if (each) return s->grad_scale;
+        return s->counted == 0 ? 0.0f : mean ? *grad / (float)s->counted : *grad;
+    }
+};
+
 struct XentTileArgs {
     MatOperand weight, hidden;
     const XentScalars *scalars;
@@ -198,7 +220,7 @@ struct XentTileArgs {
     float2 *partial;            // (2 tiles_m, rows): maximum, sum
     float *picked;
     // backward
-    const float *lse, *share;   // by place; share: g_i over the largest
+    const float *lse, *share;   // by place; share NULL: ones
     char *d_l;                  // (rows, stride bytes), in F16 two planes
     int64_t stride, plane;
 };
@@ -302,7 +324,7 @@ __global__ __launch_bounds__(mat_threads(BM, BN), 1) void xent_logits_kernel(Xen
                 sum += __shfl_xor(sum, 32, 64);
                 if (lane < 16 && there) a.partial[(int64_t)of * a.rows + row] = make_float2(top, sum * rounded_off(at, from));
             } else {
-                const float share = there ? a.share[row] : 0.0f;
+                const float share = there ? a.share ? a.share[row] : 1.0f : 0.0f;
                 // (no share: the exponentials of minus infinity, zeros)
                 const float lse = share != 0.0f ? a.lse[row] : INFINITY, from = -lse * kLog2e;
                 const float exact = share != 0.0f ? rounded_off(lse, from) : 1.0f;
@@ -361,18 +383,19 @@ __global__ __launch_bounds__(mat_threads(BM, BN), 1) void xent_logits_kernel(Xen
 struct XentJoinArgs {
     const float2 *partial;
     const float *picked;
-    const int *position;
+    const int *position, *label;
     int64_t rows;
     int parts;
-    float *lse, *losses;    // (rows), as the caller numbers them; zero where ignored
+    float *lse;             // (rows) by place; NaN where the target is no entry of the vocabulary, so all that follows is
+    float *losses;          // (rows), as the caller numbers them; zero where ignored
 };
 
-// 16 rows and 16 runs of partials a workgroup
-__global__ __launch_bounds__(256) void xent_join_kernel(XentJoinArgs a)
+// 32 rows and 16 runs of partials a workgroup
+__global__ __launch_bounds__(512) void xent_join_kernel(XentJoinArgs a)
 {
-    __shared__ float2 lds[16][17];
-    const int64_t row = (int64_t)blockIdx.x * 16 + (threadIdx.x & 15);
-    const int run = threadIdx.x >> 4, at = row < a.rows ? a.position[row] : -1;
+    __shared__ float2 lds[16][33];
+    const int64_t row = (int64_t)blockIdx.x * 32 + (threadIdx.x & 31);
+    const int run = threadIdx.x >> 5, at = row < a.rows ? a.position[row] : -1;
     const int per = (a.parts + 15) / 16, end = (run + 1) * per < a.parts ? (run + 1) * per : a.parts;
     float top = -INFINITY, sum = 0.0f;
     auto join = [&](float2 p) {
@@ -384,16 +407,18 @@ __global__ __launch_bounds__(256) void xent_join_kernel(XentJoinArgs a)
             sum += p.x == top || p.x == -INFINITY ? p.y : p.y * __expf(p.x - top);
         }
     };
-    if (at >= 0)
+    if (at >= 0) {
+#pragma unroll 8
         for (int p = run * per; p < end; ++p) join(a.partial[(int64_t)p * a.rows + at]);
-    lds[run][threadIdx.x & 15] = make_float2(top, sum);
+    }
+    lds[run][threadIdx.x & 31] = make_float2(top, sum);
     __syncthreads();
     if (run != 0 || row >= a.rows) return;
     top = -INFINITY;
     sum = 0.0f;
     for (int i = 0; i < 16; ++i) join(lds[i][threadIdx.x]);
     const float lse = (top == -INFINITY ? 0.0f : top) + logf(sum);
-    a.lse[row] = at >= 0 ? lse : 0.0f;
+    if (at >= 0) a.lse[at] = a.label[at] < 0 ? __builtin_nanf("") : lse;
     a.losses[row] = at >= 0 ? lse - a.picked[at] : 0.0f;
 }
 
@@ -403,6 +428,7 @@ __global__ __launch_bounds__(kXentThreads) void xent_total_kernel(const float *l
 {
     __shared__ float sums[kXentThreads / 64];
     float s = 0.0f;
+#pragma unroll 8
     for (int64_t i = threadIdx.x; i < rows; i += kXentThreads) s += losses[i];
     s = lanes_sum<64>(s);
     if ((threadIdx.x & 63) == 0) sums[threadIdx.x >> 6] = s;
@@ -413,39 +439,22 @@ __global__ __launch_bounds__(kXentThreads) void xent_total_kernel(const float *l
     *loss = mean ? s / (float)scalars->counted : s;
 }
 
-// ---- backward: what each row's d_l is multiplied by ---------------------------------------------------------------
-
-struct XentShareArgs {
-    const float *grad;      // one number, or one a row (each)
-    const float *lse;       // (rows), as the caller numbers them
-    const int *index, *label;
-    XentScalars *scalars;
-    int each, mean;
-    float *share, *lse_at;  // by place
-};
-
-__global__ __launch_bounds__(kXentThreads) void xent_share_kernel(XentShareArgs a)
+// ---- backward: what the rows' d_l are multiplied by ---------------------------------------------------------------
+// g_i = scale share_i.  One gradient for all: shares of one.  One a row: scale is the largest |g_i|.
+__global__ __launch_bounds__(kXentThreads) void xent_share_kernel(XentGrad g, const int *index, XentScalars *scalars, float *share)
 {
     __shared__ float sums[kXentThreads / 64];
-    const int n = a.scalars->counted;
+    const int n = scalars->counted;
     float most = 0.0f;
-    if (a.each) {
-        for (int i = threadIdx.x; i < n; i += kXentThreads) most = fmaxf(most, fabsf(a.grad[a.index[i]]));
+    for (int i = threadIdx.x; i < n; i += kXentThreads) most = fmaxf(most, fabsf(g.grad[index[i]]));
 #pragma unroll
-        for (int d = 1; d < 64; d *= 2) most = fmaxf(most, __shfl_xor(most, d, 64));
-        if ((threadIdx.x & 63) == 0) sums[threadIdx.x >> 6] = most;
-        __syncthreads();
-        for (int w = 0; w < kXentThreads / 64; ++w) most = fmaxf(most, sums[w]);
-    } else {
-        most = n == 0 ? 0.0f : a.mean ? *a.grad / (float)n : *a.grad;
-    }
-    if (threadIdx.x == 0) a.scalars->grad_scale = most;
-    for (int i = threadIdx.x; i < n; i += kXentThreads) {
-        float s = 1.0f;
-        if (a.each) s = most == 0.0f ? a.grad[a.index[i]] : a.grad[a.index[i]] / most;   // (zeros and NaN only)
-        a.share[i] = a.label[i] < 0 ? __builtin_nanf("") : s;
-        a.lse_at[i] = a.lse[a.index[i]];
-    }
+    for (int d = 1; d < 64; d *= 2) most = fmaxf(most, __shfl_xor(most, d, 64));
+    if ((threadIdx.x & 63) == 0) sums[threadIdx.x >> 6] = most;
+    __syncthreads();
+    for (int w = 0; w < kXentThreads / 64; ++w) most = fmaxf(most, sums[w]);
+    if (threadIdx.x == 0) scalars->grad_scale = most;
+    // (all zero: the numbers themselves, zeros and NaN)
+    for (int i = threadIdx.x; i < n; i += kXentThreads) share[i] = most == 0.0f ? g.grad[index[i]] : g.grad[index[i]] / most;
 }
 
 // ---- backward: the gradients' products -----------------------------------------------------------------------------
@@ -453,6 +462,7 @@ __global__ __launch_bounds__(kXentThreads) void xent_share_kernel(XentShareArgs 
 struct XentGradArgs {
     MatOperand a, b;            // a: what is multiplied with d_l, along m; b: d_l
     const XentScalars *scalars;
+    XentGrad grad;
     int64_t m, n;               // sizes of the result (n rows of m)
     int tiles_m, tiles_n;
     int steps, splits;          // k steps in all (d_weight: an upper bound), parts they are cut into
@@ -476,7 +486,7 @@ __global__ __launch_bounds__(mat_threads(BM, BN), 1) void xent_grad_kernel(XentG
     const int steps = OF_WEIGHT ? (counted + kMatK - 1) / kMatK : a.steps;
     const int splits = xent_splits(a.splits, steps), total = tiles * splits;
     const int lane = threadIdx.x & 63;
-    float scale = a.scalars->grad_scale;
+    float scale = a.grad.scale(a.scalars);
     if constexpr (F16) scale *= 1.0f / 32768.0f / (OF_WEIGHT ? a.scalars->hidden_scale : a.scalars->weight_scale);
     if ((int)blockIdx.x >= total) return;
     Tile tile(a.a, a.b, lds);
@@ -550,30 +560,37 @@ struct XentGatherArgs {
     const float *partial;       // (splits, n, m)
     const int *position;        // rows of the result come from these places (-1: zeros); NULL: as they are
     const XentScalars *scalars;
+    XentGrad grad;
     void *out;
     int64_t rows, n, m;         // rows of the result, of a split
     int splits, of_weight;
 };
 
-// The splits' sums in ascending order, scaled and rounded once.
+// The splits' sums in ascending order, scaled and rounded once: eight neighbours a thread.
 template <typename T>
 __global__ __launch_bounds__(256) void xent_gather_kernel(XentGatherArgs a)
 {
     constexpr bool F16 = sizeof(T) == 4;
-    float scale = a.scalars->grad_scale;
+    float scale = a.grad.scale(a.scalars);
     if constexpr (F16) scale *= 1.0f / 32768.0f / (a.of_weight ? a.scalars->hidden_scale : a.scalars->weight_scale);
     const int splits = a.of_weight ? xent_splits(a.splits, (a.scalars->counted + kMatK - 1) / kMatK) : a.splits;
-    for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
-        const int64_t at = a.position ? a.position[row] : row;
-        T *out = reinterpret_cast<T *>(a.out) + row * a.m;
-        for (int64_t m = threadIdx.x; m < a.m; m += 256) {
-            float s = 0.0f;
-            if (at >= 0) {
-                for (int p = 0; p < splits; ++p) s += a.partial[((int64_t)p * a.n + at) * a.m + m];
-                s *= scale;
+    const int m = (int)a.m, units = (m + 7) / 8;
+    const int64_t total = a.rows * units;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+        const int64_t row = i / units, at = a.position ? a.position[row] : row;
+        const int col = (int)(i - row * units) * 8;
+        float s[8] = {};
+        if (at >= 0) {
+            for (int p = 0; p < splits; ++p) {
+                float v[8];
+                load8(a.partial + ((int64_t)p * a.n + at) * m, col, m, 0.0f, v);
+#pragma unroll
+                for (int k = 0; k < 8; ++k) s[k] += v[k];
             }
-            out[m] = (T)s;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) s[k] *= scale;
         }
+        store8(reinterpret_cast<T *>(a.out) + row * m, col, m, s);
     }
 }
 

@@ -395,19 +395,23 @@ typedef struct bf_linear_xent {
     int64_t ignore_index;
 } bf_linear_xent;
 
-/* The workspace (256-byte aligned) holds hidden and, where it cannot be read as it lies (float, rows that
- * 16 bytes do not divide), weight in the products' form, and backward the logits' gradient over a
- * piece of the vocabulary, up to some 256 MiB.                                                   */
+/* kept (256-byte aligned): what the forward call leaves for the backward one, which rows count and the operands in the
+ * products' form (and their log-sum-exps): hidden's counted rows and, where it cannot be read as it lies (float, rows that 16
+ * bytes do not divide), weight.  A call without a backward one gives it the same room.
+ * The workspaces (256-byte aligned) hold 16 bytes for each row and 256 (128) entries forward, and backward the
+ * logits' gradient over a piece of the vocabulary, up to some 256 MiB, and the sums of d_hidden's and d_weight's
+ * parts.                                                                                         */
+size_t bf_linear_xent_kept_bytes(const bf_linear_xent *p);
 size_t bf_linear_xent_fw_workspace_bytes(const bf_linear_xent *p);
 size_t bf_linear_xent_bw_workspace_bytes(const bf_linear_xent *p);
-/* loss: one float, or (rows) with BF_XENT_NONE.  lse: (rows), for the backward call. */
+/* loss: one float, or (rows) with BF_XENT_NONE. */
 int bf_linear_xent_fw(const bf_linear_xent *p, const void *hidden, const void *weight,
-                      const int64_t *target, float *loss, float *lse, void *workspace,
+                      const int64_t *target, float *loss, void *kept, size_t kept_bytes, void *workspace, size_t workspace_bytes, void *stream);
+/* weight, kept: of the forward call.  grad: the loss's gradient, one float or (rows).  d_hidden or
+ * d_weight may be NULL.                                                                          */
+int bf_linear_xent_bw(const bf_linear_xent *p, const void *weight, const float *grad, void *kept,
+                      size_t kept_bytes, void *d_hidden, void *d_weight, void *workspace,
                       size_t workspace_bytes, void *stream);
-/* grad: the loss's gradient, one float or (rows).  d_hidden or d_weight may be NULL. */
-int bf_linear_xent_bw(const bf_linear_xent *p, const void *hidden, const void *weight,
-                      const int64_t *target, const float *lse, const float *grad, void *d_hidden,
-                      void *d_weight, void *workspace, size_t workspace_bytes, void *stream);
 
 #ifdef __cplusplus
 }

@@ -160,14 +160,20 @@ def test_c_abi_refuses_bad_descriptors():
     refused(-1, lambda: L.bf_recurrence_step(ctypes.byref(c), one, one, one, one, null), b"sizes")
 
     x = _capi.LinearXent(dtype=0, reduction=1, rows=8, features=16, vocab=100, hidden_stride=16, weight_stride=16, ignore_index=-100)
-    need = L.bf_linear_xent_fw_workspace_bytes(ctypes.byref(x))
-    assert 0 < need < _capi.SIZE_INVALID
-    call = lambda ws, size: lambda: L.bf_linear_xent_fw(ctypes.byref(x), one, one, one, one, one, ws, size, null)  # noqa: E731
+    need, kept = L.bf_linear_xent_fw_workspace_bytes(ctypes.byref(x)), L.bf_linear_xent_kept_bytes(ctypes.byref(x))
+    assert 0 < need < _capi.SIZE_INVALID and 0 < kept < _capi.SIZE_INVALID
+
+    def call(ws, size, weight=one, keep=one, keep_bytes=1 << 40):
+        return lambda: L.bf_linear_xent_fw(ctypes.byref(x), one, weight, one, one, keep, keep_bytes, ws, size, null)
+
     refused(-4, call(one, need - 1), b"workspace")
     refused(-4, call(ctypes.c_void_p(264), need), b"aligned")
-    refused(-4, lambda: L.bf_linear_xent_bw(ctypes.byref(x), one, one, one, one, one, one, one, null, 0, null), b"workspace")
-    refused(-1, lambda: L.bf_linear_xent_fw(ctypes.byref(x), one, ctypes.c_void_p(264), one, one, one, one, need, null), b"aligned")
-    refused(-1, lambda: L.bf_linear_xent_fw(ctypes.byref(x), one, null, one, one, one, one, need, null), b"NULL")
+    refused(-4, call(one, need, keep_bytes=kept - 1), b"kept")
+    refused(-4, call(one, need, keep=null), b"kept")
+    refused(-4, call(one, need, keep=ctypes.c_void_p(264)), b"aligned")
+    refused(-4, lambda: L.bf_linear_xent_bw(ctypes.byref(x), one, one, one, kept, one, one, null, 0, null), b"workspace")
+    refused(-1, call(one, need, weight=ctypes.c_void_p(264)), b"aligned")
+    refused(-1, call(one, need, weight=null), b"NULL")
     for field, value, code, text in (("dtype", 1, -1, b"dtype"), ("reduction", 3, -1, b"reduction"), ("vocab", 0, -1, b"vocab"),
                                      ("hidden_stride", -1, -1, b"strides"), ("features", 1 << 20, -2, b"2^16")):
         keep = getattr(x, field)
@@ -181,10 +187,11 @@ def test_workspace_of_a_loss_stays_bounded():
     from butterfly_amd import _capi
     L = _capi.lib()
     x = _capi.LinearXent(dtype=2, reduction=1, rows=16384, features=1024, vocab=1 << 20, hidden_stride=1024, weight_stride=1024)
-    # hidden, the logits' gradient over a piece (256 MiB) and d_hidden's sums; the logits would be 32 GiB
-    assert L.bf_linear_xent_bw_workspace_bytes(ctypes.byref(x)) < (32 << 20) + (256 << 20) + (64 << 20) + (1 << 20)
-    # hidden, and 16 bytes for each row and 256 entries
-    assert L.bf_linear_xent_fw_workspace_bytes(ctypes.byref(x)) < (32 << 20) + (1 << 30) + (1 << 20)
-    # weights that 16 bytes do not divide have room for a copy
+    # the logits' gradient over a piece (256 MiB), d_hidden's sums, two parts of d_weight's piece; the logits would be 32 GiB
+    assert L.bf_linear_xent_bw_workspace_bytes(ctypes.byref(x)) < (256 << 20) + (64 << 20) + (64 << 20) + (1 << 20)
+    # 16 bytes for each row and 256 entries
+    assert L.bf_linear_xent_fw_workspace_bytes(ctypes.byref(x)) < (1 << 30) + (1 << 20)
+    # hidden; weights that 16 bytes do not divide have room for a copy too
+    assert L.bf_linear_xent_kept_bytes(ctypes.byref(x)) < (32 << 20) + (1 << 20)
     x.features = x.weight_stride = 1023
-    assert L.bf_linear_xent_fw_workspace_bytes(ctypes.byref(x)) > (2 << 30)
+    assert L.bf_linear_xent_kept_bytes(ctypes.byref(x)) > (2 << 30)
