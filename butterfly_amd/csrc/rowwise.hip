@@ -119,6 +119,14 @@ void launch_bw(const RowArgs &a, int64_t blocks, hipStream_t stream)
     }
 }
 
+template <typename P>
+void launch_sums(const ColumnSumArgs &c, hipStream_t s)
+{
+    const int entries = 2 * c.slice;
+    if (entries >= 4096) column_sums_kernel<P, 16><<<dim3((unsigned)((entries + 63) / 64)), dim3(1024), 0, s>>>(c);
+    else column_sums_kernel<P, 4><<<dim3((unsigned)((entries + 15) / 16)), dim3(1024), 0, s>>>(c);
+}
+
 __global__ void rng_next_kernel(int64_t *state, int64_t *taken)
 {
     const int64_t seed = state[0], call = state[1];
@@ -209,9 +217,8 @@ int bf_rowwise_bw(const bf_rowwise *p, const void *sum, const void *grad_y, cons
     }
     if (params) {
         const ColumnSumArgs c = {a.partial, d_weight, d_bias, (int)blocks, a.slice, a.cols};
-        const dim3 grid((unsigned)((2 * a.slice + 63) / 64));
-        if (p->param_dtype == BF_F32) column_sums_kernel<float><<<grid, dim3(1024), 0, s>>>(c);
-        else column_sums_kernel<bf16><<<grid, dim3(1024), 0, s>>>(c);
+        if (p->param_dtype == BF_F32) launch_sums<float>(c, s);
+        else launch_sums<bf16>(c, s);
         BF_HIP_CHECK(hipGetLastError());
     }
     return BF_OK;

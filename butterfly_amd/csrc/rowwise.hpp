@@ -488,32 +488,48 @@ __global__ __launch_bounds__(256) void norm_param_partial_kernel(RowArgs a)
     }
 }
 
-// out[c] = sum of the slices' entry c, for d_weight and d_bias side by side: 64 entries and 16 runs of
-// slices a workgroup, each run ascending, the runs in ascending order (in double: a sum over many rows
-// that nearly cancels keeps what the slices hold).
+// out[c] = sum of the slices' entry c, for d_weight and d_bias side by side: Q times four neighbouring entries and
+// 1024 / Q runs of slices a workgroup, each run ascending, the runs joined pairwise (in double: a sum over many rows
+// that nearly cancels keeps what the slices hold).  Q = 16 reads 256 bytes of a slice at a time, 4 makes four times as
+// many workgroups for narrow rows.
 struct ColumnSumArgs {
     const float *partial;     // (parts, 2, slice)
     void *d_weight, *d_bias;  // NULL: not wanted
     int parts, slice, cols;
 };
 
-template <typename P>
+template <typename P, int Q>
 __global__ __launch_bounds__(1024) void column_sums_kernel(ColumnSumArgs a)
 {
-    __shared__ double lds[16][64];
-    const int at = blockIdx.x * 64 + (threadIdx.x & 63), run = threadIdx.x >> 6;
-    double s = 0.0;
-    if (at < 2 * a.slice)
-        for (int p = run; p < a.parts; p += 16) s += a.partial[(int64_t)p * 2 * a.slice + at];
-    lds[run][threadIdx.x & 63] = s;
-    __syncthreads();
-    if (run != 0 || at >= 2 * a.slice) return;
-    s = 0.0;
+    constexpr int kRuns = 1024 / Q;
+    __shared__ double lds[kRuns][4 * Q];
+    const int at = (blockIdx.x * Q + threadIdx.x % Q) * 4, run = threadIdx.x / Q;
+    double s[4] = {};
+    if (at < 2 * a.slice) {
+#pragma unroll 4
+        for (int p = run; p < a.parts; p += kRuns) {
+            const quad_at_4 v = *reinterpret_cast<const quad_at_4 *>(a.partial + (int64_t)p * 2 * a.slice + at);
 #pragma unroll
-    for (int i = 0; i < 16; ++i) s += lds[i][threadIdx.x];
-    const int col = at < a.slice ? at : at - a.slice;
-    void *out = at < a.slice ? a.d_weight : a.d_bias;
-    if (out && col < a.cols) reinterpret_cast<P *>(out)[col] = (P)(float)s;
+            for (int i = 0; i < 4; ++i) s[i] += v[i];
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) lds[run][threadIdx.x % Q * 4 + i] = s[i];
+    __syncthreads();
+#pragma unroll
+    for (int half = kRuns / 2; half >= 1; half /= 2) {
+        if (run < half) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) lds[run][threadIdx.x % Q * 4 + i] += lds[run + half][threadIdx.x % Q * 4 + i];
+        }
+        __syncthreads();
+    }
+    if (threadIdx.x >= 4 * Q) return;
+    const int entry = blockIdx.x * Q * 4 + threadIdx.x;
+    if (entry >= 2 * a.slice) return;
+    const int col = entry < a.slice ? entry : entry - a.slice;
+    void *out = entry < a.slice ? a.d_weight : a.d_bias;
+    if (out && col < a.cols) reinterpret_cast<P *>(out)[col] = (P)(float)lds[0][threadIdx.x];
 }
 
 }  // namespace bf
