@@ -163,9 +163,11 @@ int bf_recurrence_fw(const bf_recurrence *p, const void *gate, const void *x, co
         using Tr = decltype(kind);
         constexpr bool SIG = decltype(sigmoid)::value;
         const unsigned x_blocks = (unsigned)(r.groups * p->batch);
+        const dim3 enter((unsigned)((p->batch * p->channels + 63) / 64));
         if (r.chunks > 1) {
             const dim3 grid(x_blocks, ((unsigned)r.chunks + 7) / 8 * 8), threads(64 * kRecWaves);
             recurrence_runs_kernel<Tr, SIG, false><<<grid, threads, 0, s>>>(a);
+            recurrence_enter_kernel<Tr, false><<<enter, dim3(64), 0, s>>>(a);
             recurrence_chunk_fw_kernel<Tr, SIG><<<grid, threads, 0, s>>>(a);
         } else {
             recurrence_fw_kernel<Tr, SIG><<<dim3(x_blocks), dim3(64 * r.waves), 0, s>>>(a);
@@ -203,9 +205,11 @@ int bf_recurrence_bw(const bf_recurrence *p, const void *gate, const void *x, co
         using Tr = decltype(kind);
         constexpr bool SIG = decltype(sigmoid)::value;
         const unsigned x_blocks = (unsigned)(r.groups * p->batch);
+        const dim3 enter((unsigned)((p->batch * p->channels + 63) / 64));
         if (r.chunks > 1) {
             const dim3 grid(x_blocks, ((unsigned)r.chunks + 7) / 8 * 8), threads(64 * kRecWaves);
             recurrence_runs_kernel<Tr, SIG, true><<<grid, threads, 0, s>>>(a);
+            recurrence_enter_kernel<Tr, true><<<enter, dim3(64), 0, s>>>(a);
             recurrence_chunk_bw_kernel<Tr, SIG><<<grid, threads, 0, s>>>(a);
         } else {
             recurrence_bw_kernel<Tr, SIG><<<dim3(x_blocks), dim3(64 * r.waves_bw), 0, s>>>(a);

@@ -15,8 +15,8 @@
 // exchange those through LDS (one barrier a tile of 16 S steps), and each then runs its steps again from its own h, the
 // next tile's elements on their way meanwhile.  Everything is read and written once.
 // Where channels times batch are too few workgroups to fill the chip the sequence is cut into chunks of 16 runs, a
-// wavefront each: one launch forms the runs' and chunks' (A, B), the next one starts each run from their
-// composition in a fixed order (the same sums at every call).
+// wavefront each: one launch forms the runs' and chunks' (A, B), the next one walks the chunks, the third one
+// starts each run from there (a fixed order: the same sums at every call).
 //
 // h is kept in float (complex64: two) whatever the rows' type; 1 - a is s(-gate), not a difference,
 // or decays close to one would lose it.
@@ -507,7 +507,8 @@ __global__ __launch_bounds__(64 * kRecWaves) void recurrence_bw_kernel(Recurrenc
 // ---- sequences cut into chunks ------------------------------------------------------------------------------
 // grid (batch x groups, chunks), kRecWaves wavefronts, each with a run of its own: len = chunk / kRecWaves steps.  The first
 // launch forms every run's (A, B) as composed from the chunk's start (backward: end) up to the run, and the chunks';
-// the second one starts each run from there, and the wavefronts need nothing of each other.
+// the second one walks those from chunk to chunk; the third one starts each run from there, and the wavefronts need
+// nothing of each other.
 
 template <typename Tr, bool SIG, bool BACKWARD>
 __global__ __launch_bounds__(64 * kRecWaves) void recurrence_runs_kernel(RecurrenceArgs p)
@@ -614,15 +615,45 @@ __global__ __launch_bounds__(64 * kRecWaves) void recurrence_runs_kernel(Recurre
     }
 }
 
-// What enters a wavefront's run: the state through the chunks in front of its own, then through the runs.
+// What enters each chunk, in the place of its A: the state through the chunks in front of it, one after another.
 template <typename Tr, bool BACKWARD>
-__device__ __forceinline__ void enter_run(const RecurrenceArgs &p, const RecPlace<Tr> &at, const void *state, typename Tr::Acc (&carry)[Tr::V])
+__global__ __launch_bounds__(64) void recurrence_enter_kernel(RecurrenceArgs p)
 {
-    get_state<Tr::V>(at.state(state), at.c, at.n, carry);
-    const int chunks = BACKWARD ? p.chunks - 1 - at.chunk : at.chunk;
-#pragma unroll 8
-    for (int i = 0; i < chunks; ++i)
-        compose<Tr::V>(p.chunk_a, p.chunk_b, p.chunk_cut, (BACKWARD ? p.chunks - 1 - i : i) * p.batch + at.b, at.c, at.n, carry);
+    using A = typename Tr::Acc;
+    const int64_t states = p.batch * p.channels, at = (int64_t)blockIdx.x * 64 + threadIdx.x;
+    if (at >= states) return;
+    const int64_t b = at / p.channels;
+    const A *state = reinterpret_cast<const A *>(BACKWARD ? p.grad_last : p.state);
+    A *a = reinterpret_cast<A *>(p.chunk_a) + at, carry = state ? state[at] : zero_of(A());
+    const A *add_b = reinterpret_cast<const A *>(p.chunk_b) + at;
+    constexpr int kAhead = 32;   // loads on their way at a time: the walk itself is short
+    for (int from = 0; from < p.chunks; from += kAhead) {
+        A ca[kAhead], cb[kAhead];
+        bool cut[kAhead];
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+            const int k = from + i < p.chunks ? from + i : p.chunks - 1;
+            const int64_t slot = BACKWARD ? p.chunks - 1 - k : k;
+            ca[i] = a[slot * states];
+            cb[i] = add_b[slot * states];
+            cut[i] = p.chunk_cut[slot * p.batch + b] != 0;
+        }
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+            if (from + i < p.chunks) {
+                a[(int64_t)(BACKWARD ? p.chunks - 1 - from - i : from + i) * states] = carry;
+                carry = chunk_of(cut[i], ca[i], carry, cb[i]);
+            }
+        }
+    }
+}
+
+// What enters a wavefront's run.
+template <typename Tr>
+__device__ __forceinline__ void enter_run(const RecurrenceArgs &p, const RecPlace<Tr> &at, typename Tr::Acc (&carry)[Tr::V])
+{
+    using A = typename Tr::Acc;
+    get_state<Tr::V>(reinterpret_cast<const A *>(p.chunk_a) + (at.chunk * p.batch + at.b) * at.n, at.c, at.n, carry);
     compose<Tr::V>(p.run_a, p.run_b, p.run_cut, ((int64_t)at.chunk * kRecWaves + at.wave) * p.batch + at.b, at.c, at.n, carry);
 }
 
@@ -648,7 +679,7 @@ __global__ __launch_bounds__(64 * kRecWaves) void recurrence_chunk_fw_kernel(Rec
     };
     fetch(begin);
     A h[V];
-    enter_run<Tr, false>(p, at, p.state, h);
+    enter_run(p, at, h);
     E *out = reinterpret_cast<E *>(p.h) + (at.b * p.steps + begin) * n;
     for (int64_t t = begin; t < end; t += S) {
         const int count = (int)(end - t < S ? end - t : S);
@@ -694,7 +725,7 @@ __global__ __launch_bounds__(64 * kRecWaves) void recurrence_chunk_bw_kernel(Rec
     const int64_t first = begin + (end - begin - 1) / S * S;
     back.fetch(p, at, in, first, end);
     A carry[V];
-    enter_run<Tr, true>(p, at, p.grad_last, carry);
+    enter_run(p, at, carry);
     for (int64_t t = first; t >= begin; t -= S) {
         const int count = (int)(end - t < S ? end - t : S);
         const uint64_t cuts = back.next_cut;
