@@ -1,4 +1,5 @@
-// Entry points of the linear layer with softmax cross entropy (xent.hpp): argument checks, workspace, launches.
+// Entry points of the linear layer with softmax cross entropy (xent.hpp, of few rows xent_few.hpp): argument checks,
+// workspace, launches.
 
 #include "../../include/butterfly_hip.h"
 
@@ -6,6 +7,7 @@
 
 #include "error.hpp"
 #include "xent.hpp"
+#include "xent_few.hpp"
 
 namespace {
 
@@ -124,7 +126,71 @@ XentPlan plan(const bf_linear_xent *p, bool backward)
     return r;
 }
 
-int check_memory(const XentPlan &r, const void *weight, const void *kept, size_t kept_bytes, const void *workspace, size_t bytes)
+// ---- few rows ----
+
+// (the logits, which stay in memory, take no more room than float weights)
+bool few_rows(const bf_linear_xent *p) { return p->rows > 0 && p->rows <= kFewRows && p->rows <= p->features; }
+
+struct XentFewPlan {
+    int tiles = 1, entry_tiles = 1, parts = 1;              // of 16 rows; of 16 entries a workgroup; partial maxima and sums
+    int64_t stride = 0, steps = 0;                          // of the logits' rows; of 32 entries
+    int columns = 1, splits_hidden = 1, splits_weight = 1;  // parts of the columns, of the vocabulary
+    size_t scalars = 0, index = 0, position = 0, label = 0, lse = 0, by_feature = 0, by_row = 0, logits = 0, kept = 0;
+    size_t losses = 0, partial = 0, d_by_entry = 0, d_by_row = 0, sums = 0;
+    size_t total = 0;
+};
+
+XentFewPlan few_plan(const bf_linear_xent *p, bool backward)
+{
+    const bool wide = p->dtype == BF_F32;
+    const int64_t planes = wide ? 3 : 1, each = wide ? 4 : 8, chunk = wide ? 32 : 64, chunk_frags = wide ? 3 : 2;
+    XentFewPlan r;
+    r.tiles = p->rows <= 16 ? 1 : p->rows <= 32 ? 2 : 4;
+    r.entry_tiles = p->vocab >= 64 * 512 ? 4 : 1;
+    r.parts = (int)((p->vocab + 16 * r.entry_tiles - 1) / (16 * r.entry_tiles));
+    r.stride = up_to(p->vocab, 64);
+    r.steps = (p->vocab + 31) / 32;
+    r.columns = (int)((p->features + 16 * each - 1) / (16 * each));
+    // wavefronts for all compute units, of four steps or tiles and more
+    r.splits_hidden = (int)std::max<int64_t>(1, std::min<int64_t>(2048 / r.columns, r.steps / 4));
+    r.splits_weight = (int)std::max<int64_t>(1, std::min<int64_t>(4096 / r.columns, r.steps / 2));
+    size_t at = 0;
+    auto take = [&](size_t bytes) {
+        const size_t here = at;
+        at += up256(bytes);
+        return here;
+    };
+    const size_t rows = (size_t)p->rows, row_steps = (size_t)(r.tiles + 1) / 2;
+    r.scalars = take(sizeof(XentScalars));
+    r.index = take(rows * 4);
+    r.position = take(rows * 4);
+    r.label = take(rows * 4);
+    r.lse = take(rows * 4);
+    r.by_feature = take((size_t)((p->features + chunk - 1) / chunk) * chunk_frags * r.tiles * 1024);
+    r.by_row = take((size_t)r.columns * row_steps * planes * each * 1024);
+    r.logits = take(rows * r.stride * 4);
+    r.kept = at;
+    at = 0;
+    if (!backward) {
+        r.losses = take(rows * 4);
+        r.partial = take(rows * r.parts * sizeof(float2));
+    } else {
+        r.d_by_entry = take((size_t)r.steps * planes * r.tiles * 1024);
+        r.d_by_row = take((size_t)r.steps * 2 * row_steps * planes * 1024);
+        r.sums = take((size_t)r.splits_hidden * rows * p->features * 4);
+    }
+    r.total = at;
+    return r;
+}
+
+size_t kept_bytes_of(const bf_linear_xent *p) { return few_rows(p) ? few_plan(p, false).kept : plan(p, false).kept; }
+size_t workspace_bytes_of(const bf_linear_xent *p, bool backward)
+{
+    return few_rows(p) ? few_plan(p, backward).total : plan(p, backward).total;
+}
+
+template <typename Plan>
+int check_memory(const Plan &r, const void *weight, const void *kept, size_t kept_bytes, const void *workspace, size_t bytes)
 {
     if (!kept || kept_bytes < r.kept)
         return fail(BF_ERR_WORKSPACE, "room for %zu bytes of kept operands needed, %zu given", r.kept, kept ? kept_bytes : 0);
@@ -213,23 +279,93 @@ void gather(const bf_linear_xent *p, const XentGatherArgs &a, hipStream_t s)
     else xent_gather_kernel<bf16><<<grid, dim3(256), 0, s>>>(a);
 }
 
+template <typename T, int NT>
+void few_fw(const bf_linear_xent *p, const XentFewPlan &r, const void *hidden, const void *weight, const int64_t *target, float *loss,
+            void *kept, void *workspace, hipStream_t s)
+{
+    XentScalars *scalars = part<XentScalars>(kept, r.scalars);
+    int *index = part<int>(kept, r.index), *position = part<int>(kept, r.position), *label = part<int>(kept, r.label);
+    const XentFewPackArgs pack = {hidden, target, p->hidden_stride, (int)p->rows, r.tiles, (int)p->features, p->vocab, p->ignore_index,
+                                  scalars, index, position, label, part<char>(kept, r.by_feature), part<char>(kept, r.by_row)};
+    const size_t slots = (r.logits - r.by_feature) / 16;   // (an upper bound of the threads with work)
+    xent_few_pack_kernel<T><<<dim3((unsigned)std::min<size_t>((slots + kFewThreads - 1) / kFewThreads, 1024)), dim3(kFewThreads), 0, s>>>(pack);
+    float *logits = part<float>(kept, r.logits);
+    float2 *partial = part<float2>(workspace, r.partial);
+    const XentFewLogitsArgs l = {weight, p->weight_stride, p->vocab, (int)p->features, r.parts, scalars, part<char>(kept, r.by_feature),
+                                 logits, r.stride, partial};
+    if (r.entry_tiles == 4) xent_few_logits_kernel<T, NT, 4><<<dim3((unsigned)r.parts), dim3(kFewThreads), 0, s>>>(l);
+    else xent_few_logits_kernel<T, NT, 1><<<dim3((unsigned)r.parts), dim3(kFewThreads), 0, s>>>(l);
+    float *losses = p->reduction == BF_XENT_NONE ? loss : part<float>(workspace, r.losses);
+    const XentFewJoinArgs j = {partial, logits, r.stride, index, position, label, scalars, r.parts, part<float>(kept, r.lse), losses};
+    xent_few_join_kernel<<<dim3((unsigned)p->rows), dim3(kFewThreads), 0, s>>>(j);
+    if (p->reduction != BF_XENT_NONE)
+        xent_total_kernel<<<dim3(1), dim3(kXentThreads), 0, s>>>(losses, p->rows, scalars, p->reduction == BF_XENT_MEAN, loss);
+}
+
+template <typename T, int NT>
+void few_bw(const bf_linear_xent *p, const XentFewPlan &r, const void *weight, const float *grad, void *kept, void *d_hidden,
+            void *d_weight, void *workspace, hipStream_t s)
+{
+    const XentScalars *scalars = part<XentScalars>(kept, r.scalars);
+    const XentGrad gradient = {grad, p->reduction == BF_XENT_NONE, p->reduction == BF_XENT_MEAN};
+    char *by_entry = d_hidden ? part<char>(workspace, r.d_by_entry) : nullptr, *by_row = d_weight ? part<char>(workspace, r.d_by_row) : nullptr;
+    const XentFewDlArgs d = {part<float>(kept, r.logits), r.stride, p->vocab, part<float>(kept, r.lse), part<int>(kept, r.index),
+                             part<int>(kept, r.label), scalars, gradient, by_entry, by_row};
+    xent_few_dl_kernel<T, NT><<<dim3((unsigned)r.steps), dim3(64 * NT), 0, s>>>(d);
+    XentFewGradArgs g = {};
+    g.weight = weight;
+    g.weight_stride = p->weight_stride;
+    g.vocab = p->vocab;
+    g.features = (int)p->features;
+    g.rows = (int)p->rows;
+    g.scalars = scalars;
+    g.grad = gradient;
+    g.by_entry = by_entry;
+    g.by_row = by_row;
+    g.hidden = part<char>(kept, r.by_row);
+    g.parts = r.columns;
+    g.splits_hidden = r.splits_hidden;
+    g.splits_weight = r.splits_weight;
+    g.blocks_hidden = d_hidden ? (r.columns * r.splits_hidden + 3) / 4 : 0;
+    g.partial = part<float>(workspace, r.sums);
+    g.d_weight = d_weight;
+    const int blocks_weight = d_weight ? (r.columns * r.splits_weight + 3) / 4 : 0;
+    xent_few_grad_kernel<T, NT><<<dim3((unsigned)(g.blocks_hidden + blocks_weight)), dim3(kFewThreads), 0, s>>>(g);
+    if (!d_hidden) return;
+    const XentFewGatherArgs a = {g.partial, part<int>(kept, r.position), scalars, gradient, d_hidden, (int)p->rows, (int)p->features, r.splits_hidden};
+    xent_few_gather_kernel<T><<<dim3((unsigned)((p->features + 127) / 128), (unsigned)p->rows), dim3(1024), 0, s>>>(a);
+}
+
+// f(the type, tiles of rows) of a call
+template <typename Call>
+void few_dispatch(const bf_linear_xent *p, const XentFewPlan &r, Call &&call)
+{
+    auto typed = [&](auto type) {
+        if (r.tiles == 1) call(type, std::integral_constant<int, 1>());
+        else if (r.tiles == 2) call(type, std::integral_constant<int, 2>());
+        else call(type, std::integral_constant<int, 4>());
+    };
+    if (p->dtype == BF_F32) typed(float());
+    else typed(bf16());
+}
+
 }  // namespace
 
 extern "C" {
 
 size_t bf_linear_xent_kept_bytes(const bf_linear_xent *p)
 {
-    return check_xent(p) ? BF_SIZE_INVALID : plan(p, false).kept;
+    return check_xent(p) ? BF_SIZE_INVALID : kept_bytes_of(p);
 }
 
 size_t bf_linear_xent_fw_workspace_bytes(const bf_linear_xent *p)
 {
-    return check_xent(p) ? BF_SIZE_INVALID : plan(p, false).total;
+    return check_xent(p) ? BF_SIZE_INVALID : workspace_bytes_of(p, false);
 }
 
 size_t bf_linear_xent_bw_workspace_bytes(const bf_linear_xent *p)
 {
-    return check_xent(p) ? BF_SIZE_INVALID : plan(p, true).total;
+    return check_xent(p) ? BF_SIZE_INVALID : workspace_bytes_of(p, true);
 }
 
 int bf_linear_xent_fw(const bf_linear_xent *p, const void *hidden, const void *weight, const int64_t *target, float *loss,
@@ -240,9 +376,18 @@ int bf_linear_xent_fw(const bf_linear_xent *p, const void *hidden, const void *w
     if (p->rows > 0 && (!hidden || !target)) return fail(BF_ERR_INVALID, "hidden or target is NULL");
     if (!weight || (!loss && (p->rows > 0 || p->reduction != BF_XENT_NONE))) return fail(BF_ERR_INVALID, "weight or loss is NULL");
     if (p->rows == 0 && p->reduction == BF_XENT_NONE) return BF_OK;
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    if (few_rows(p)) {
+        const XentFewPlan r = few_plan(p, false);
+        if ((rc = check_memory(r, weight, kept, kept_bytes, workspace, workspace_bytes))) return rc;
+        few_dispatch(p, r, [&](auto type, auto tiles) {
+            few_fw<decltype(type), decltype(tiles)::value>(p, r, hidden, weight, target, loss, kept, workspace, s);
+        });
+        BF_HIP_CHECK(hipGetLastError());
+        return BF_OK;
+    }
     const XentPlan r = plan(p, false);
     if ((rc = check_memory(r, weight, kept, kept_bytes, workspace, workspace_bytes))) return rc;
-    hipStream_t s = static_cast<hipStream_t>(stream);
     MatOperand h, w;
     float *picked = part<float>(workspace, r.picked);
     prepare(p, r, hidden, weight, target, kept, picked, s);
@@ -274,15 +419,25 @@ int bf_linear_xent_fw(const bf_linear_xent *p, const void *hidden, const void *w
     return BF_OK;
 }
 
-int bf_linear_xent_bw(const bf_linear_xent *p, const void *weight, const float *grad, void *kept, size_t kept_bytes, void *d_hidden, void *d_weight, void *workspace, size_t workspace_bytes, void *stream)
+int bf_linear_xent_bw(const bf_linear_xent *p, const void *weight, const float *grad, void *kept, size_t kept_bytes, void *d_hidden,
+                      void *d_weight, void *workspace, size_t workspace_bytes, void *stream)
 {
     int rc = check_xent(p);
     if (rc) return rc;
     if (!weight || (!grad && (p->rows > 0 || p->reduction != BF_XENT_NONE))) return fail(BF_ERR_INVALID, "weight or grad is NULL");
     if (!d_hidden && !d_weight) return BF_OK;
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    if (few_rows(p)) {
+        const XentFewPlan r = few_plan(p, true);
+        if ((rc = check_memory(r, weight, kept, kept_bytes, workspace, workspace_bytes))) return rc;
+        few_dispatch(p, r, [&](auto type, auto tiles) {
+            few_bw<decltype(type), decltype(tiles)::value>(p, r, weight, grad, kept, d_hidden, d_weight, workspace, s);
+        });
+        BF_HIP_CHECK(hipGetLastError());
+        return BF_OK;
+    }
     const XentPlan r = plan(p, true);
     if ((rc = check_memory(r, weight, kept, kept_bytes, workspace, workspace_bytes))) return rc;
-    hipStream_t s = static_cast<hipStream_t>(stream);
     MatOperand h, w;
     operands(p, r, weight, kept, h, w);
     XentScalars *scalars = part<XentScalars>(kept, r.scalars);

@@ -380,6 +380,23 @@ __global__ __launch_bounds__(mat_threads(BM, BN), 1) void xent_logits_kernel(Xen
 
 // ---- a row's log-sum-exp and loss ------------------------------------------------------------------------------
 
+// The maximum of parts of a row and the sum of exponentials over it.
+struct Joined {
+    float top = -INFINITY, sum = 0.0f;
+
+    __device__ __forceinline__ void join(float2 p)
+    {
+        if (p.x > top) {
+            sum = sum * __expf(top - p.x) + p.y;
+            top = p.x;
+        } else {
+            // (all of them minus infinity, or NaN: their sums say so)
+            sum += p.x == top || p.x == -INFINITY ? p.y : p.y * __expf(p.x - top);
+        }
+    }
+    __device__ __forceinline__ float lse() const { return (top == -INFINITY ? 0.0f : top) + logf(sum); }
+};
+
 struct XentJoinArgs {
     const float2 *partial;
     const float *picked;
@@ -397,27 +414,17 @@ __global__ __launch_bounds__(512) void xent_join_kernel(XentJoinArgs a)
     const int64_t row = (int64_t)blockIdx.x * 32 + (threadIdx.x & 31);
     const int run = threadIdx.x >> 5, at = row < a.rows ? a.position[row] : -1;
     const int per = (a.parts + 15) / 16, end = (run + 1) * per < a.parts ? (run + 1) * per : a.parts;
-    float top = -INFINITY, sum = 0.0f;
-    auto join = [&](float2 p) {
-        if (p.x > top) {
-            sum = sum * __expf(top - p.x) + p.y;
-            top = p.x;
-        } else {
-            // (all of them minus infinity, or NaN: their sums say so)
-            sum += p.x == top || p.x == -INFINITY ? p.y : p.y * __expf(p.x - top);
-        }
-    };
+    Joined all;
     if (at >= 0) {
 #pragma unroll 8
-        for (int p = run * per; p < end; ++p) join(a.partial[(int64_t)p * a.rows + at]);
+        for (int p = run * per; p < end; ++p) all.join(a.partial[(int64_t)p * a.rows + at]);
     }
-    lds[run][threadIdx.x & 31] = make_float2(top, sum);
+    lds[run][threadIdx.x & 31] = make_float2(all.top, all.sum);
     __syncthreads();
     if (run != 0 || row >= a.rows) return;
-    top = -INFINITY;
-    sum = 0.0f;
-    for (int i = 0; i < 16; ++i) join(lds[i][threadIdx.x]);
-    const float lse = (top == -INFINITY ? 0.0f : top) + logf(sum);
+    Joined whole;
+    for (int i = 0; i < 16; ++i) whole.join(lds[i][threadIdx.x]);
+    const float lse = whole.lse();
     if (at >= 0) a.lse[at] = a.label[at] < 0 ? __builtin_nanf("") : lse;
     a.losses[row] = at >= 0 ? lse - a.picked[at] : 0.0f;
 }

@@ -284,6 +284,106 @@ def test_same_bits_every_time_on_another_stream_and_in_a_graph(dtype):
             assert torch.equal(a, b)
 
 
+# ---- few rows (up to 64 and no more than features): kernels of their own ----
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,features,vocab", [
+    (1, 1, 1), (1, 7, 33), (2, 2, 31), (3, 3, 5000), (5, 1000, 64), (15, 33, 32), (16, 31, 17), (17, 32, 15), (31, 127, 1001), (32, 2048, 300),
+    (33, 129, 33001), (47, 64, 32768), (48, 520, 40003), (63, 65, 97), (64, 64, 2), (64, 1031, 36001), (7, 4096, 70000)])
+def test_few_rows(rows, features, vocab, dtype):
+    """Each number of 16-row tiles; vocabularies and features around the tiles of 16 and 32, the chunks of 32 and 64, the parts
+    of 64 and 128 columns; vocabularies of both sizes of a workgroup's part (32768 on)."""
+    for seed, reduction in enumerate(("mean", "none", "sum")):
+        check(*make(rows, features, vocab, dtype, seed=seed), reduction)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,features,vocab", [(20, 75, 500), (50, 640, 33000)])
+def test_few_rows_of_any_stride(rows, features, vocab, dtype):
+    hidden, weight, target = make(rows, features, vocab, dtype)
+    first = check(hidden, weight, target)
+    wide = torch.full((rows, features + 13), float("nan"), dtype=dtype, device="cuda")
+    wide[:, 5:5 + features] = hidden
+    tall = torch.full((vocab, features + 11), float("nan"), dtype=dtype, device="cuda")
+    tall[:, :features] = weight
+    for a, b in zip(first, check(wide[:, 5:5 + features], tall[:, :features], target)):
+        assert torch.equal(a, b)
+    same = weight[:1].expand(vocab, features)
+    each = tb.linear_cross_entropy(hidden, same, target, reduction="none")
+    assert (each[target != -100] - torch.log(torch.tensor(float(vocab)))).abs().max() < 1e-5 * 12
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("reduction", ["none", "mean", "sum"])
+def test_few_rows_ignored(reduction, dtype):
+    hidden, weight, target = make(60, 64, 400, dtype, ignored=0.5)
+    first = check(hidden, weight, target, reduction)
+    bad = hidden.clone()
+    bad[target == -100] = float("nan")
+    for a, b in zip(first, check(bad, weight, target, reduction)):
+        assert torch.equal(a, b)
+    h, w = hidden.detach().requires_grad_(), weight.detach().requires_grad_()
+    loss = tb.linear_cross_entropy(h, w, torch.full_like(target, -100), reduction=reduction)
+    assert torch.isnan(loss) if reduction == "mean" else (loss == 0).all()
+    for d in torch.autograd.grad(loss, (h, w), torch.ones_like(loss)):
+        assert (d == 0).all()
+
+
+@pytest.mark.parametrize("up", [1e-25, 1e-6, 1e6, 1e25])
+def test_few_float_rows_of_any_scale(up):
+    hidden, weight, target = make(40, 100, 600, torch.float32)
+    check(hidden * up, weight / up, target)
+    hidden[::2] *= 2.0 ** -20
+    check(hidden, weight, target, "none")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_few_rows_with_large_logits(dtype):
+    hidden, weight, target = make(40, 64, 600, dtype, scale=400.0)
+    h, w = hidden.requires_grad_(), weight.requires_grad_()
+    loss = tb.linear_cross_entropy(h, w, target)
+    want, want_h, want_w = reference(h, w, target, torch.ones((), device="cuda"), "mean")
+    assert abs(float(loss) - float(want)) < 1e-5 * (1 + abs(float(want)))
+    dh, dw = torch.autograd.grad(loss, (h, w))
+    assert err(dh, want_h) < max(2e-3, TOL[dtype]) and err(dw, want_w) < max(2e-3, TOL[dtype])
+
+
+def test_few_rows_gradients_of_one_operand_alone_and_zero_upstream():
+    hidden, weight, target = make(50, 64, 500, torch.float32)
+    h, w = hidden.requires_grad_(), weight.requires_grad_()
+    both = torch.autograd.grad(tb.linear_cross_entropy(h, w, target), (h, w))
+    assert torch.equal(torch.autograd.grad(tb.linear_cross_entropy(h, w.detach(), target), h)[0], both[0])
+    assert torch.equal(torch.autograd.grad(tb.linear_cross_entropy(h.detach(), w, target), w)[0], both[1])
+    for reduction in ("mean", "none"):
+        loss = tb.linear_cross_entropy(h, w, target, reduction=reduction)
+        for d in torch.autograd.grad(loss, (h, w), torch.zeros_like(loss)):
+            assert (d == 0).all()
+    g = torch.logspace(-6, 2, 50, device="cuda")
+    each = tb.linear_cross_entropy(h, w, target, reduction="none")
+    dh, dw = torch.autograd.grad(each, (h, w), g)
+    _, want_h, want_w = reference(h, w, target, g, "none")
+    assert err(dh, want_h) < 5e-5 and err(dw, want_w) < 5e-5
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_few_rows_same_bits_every_time_and_in_a_graph(dtype):
+    hidden, weight, target = make(48, 200, 40000, dtype)
+    first = check(hidden, weight, target)
+    for a, b in zip(first, check(hidden, weight, target)):
+        assert torch.equal(a, b)
+    w = weight.detach().requires_grad_()
+    grad = torch.ones((), device="cuda")
+    step = tb.GraphedStep(lambda h: tb.linear_cross_entropy(h, w, target), hidden, grad, params=(w,))
+    for k in range(3):
+        h = (hidden * (1 + k)).requires_grad_()
+        loss, grads = step(h.detach(), grad)
+        torch.cuda.synchronize()
+        want = tb.linear_cross_entropy(h, w, target)
+        assert torch.equal(loss, want)
+        for a, b in zip(grads, torch.autograd.grad(want, (h, w), grad)):
+            assert torch.equal(a, b)
+
+
 def test_refusals():
     hidden, weight, target = make(8, 16, 50, torch.float32)
     for call in (
