@@ -190,35 +190,47 @@ struct XentFewLogitsArgs {
 };
 
 // A workgroup takes 16 MT entries; its four wavefronts every fourth chunk of the features, and join their sums in LDS.
+// Eight lanes load a row's 128 bytes; the lanes that multiply them get them through the wavefront's own part of LDS
+// (unit u of row r at u ^ (r & 7), so that neither way meets its own banks).
 template <typename T, int NT, int MT>
 __global__ __launch_bounds__(kFewThreads, 2) void xent_few_logits_kernel(XentFewLogitsArgs a)
 {
     using F = Few<T>;
-    __shared__ Acc4 sums[4][MT * NT][64];
+    __shared__ union {
+        Quad staged[4][16 * MT][8];
+        Acc4 sums[4][MT * NT][64];
+    } lds;
     __shared__ float2 tops[MT][NT * 16];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
     const int64_t first = (int64_t)blockIdx.x * (16 * MT);
     const int counted = a.scalars->counted, full = a.features / F::kChunk;
-    const T *row[MT];
+    const T *row[2 * MT];
 #pragma unroll
-    for (int t = 0; t < MT; ++t) {
-        const int64_t v = first + 16 * t + i;
-        row[t] = reinterpret_cast<const T *>(a.weight) + (v < a.vocab ? v : a.vocab - 1) * a.weight_stride;
+    for (int j = 0; j < 2 * MT; ++j) {
+        const int64_t v = first + 8 * j + (lane >> 3);
+        row[j] = reinterpret_cast<const T *>(a.weight) + (v < a.vocab ? v : a.vocab - 1) * a.weight_stride;
     }
     Acc4 acc[MT][NT];
 #pragma unroll
     for (int t = 0; t < MT; ++t)
 #pragma unroll
         for (int n = 0; n < NT; ++n) acc[t][n] = Acc4{0.0f, 0.0f, 0.0f, 0.0f};
-    auto load = [&](int c, Quad (&w)[MT][2]) {
+    auto load = [&](int c, Quad (&w)[2 * MT]) {
 #pragma unroll
-        for (int t = 0; t < MT; ++t) {
-            const T *p = row[t] + c * F::kChunk + F::kEach * g;
-            w[t][0] = *reinterpret_cast<const quad_at_2 *>(p);
-            w[t][1] = *reinterpret_cast<const quad_at_2 *>(p + F::kChunk / 2);
-        }
+        for (int j = 0; j < 2 * MT; ++j) w[j] = *reinterpret_cast<const quad_at_2 *>(row[j] + c * F::kChunk + F::kEach * (lane & 7));
     };
-    auto multiply = [&](int c, const Quad (&w)[MT][2]) {
+    // (a wavefront's LDS accesses are done in their order)
+    auto settle = [] {
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_wave_barrier();
+    };
+    auto stage = [&](const Quad (&w)[2 * MT]) {
+        settle();
+#pragma unroll
+        for (int j = 0; j < 2 * MT; ++j) lds.staged[wave][8 * j + (lane >> 3)][(lane & 7) ^ (lane >> 3)] = w[j];
+        settle();
+    };
+    auto multiply = [&](int c) {
         const Frag *h = reinterpret_cast<const Frag *>(a.by_feature + (int64_t)c * (F::kChunkFrags * NT * 1024)) + lane;
         Frag b[NT][F::kChunkFrags];
 #pragma unroll
@@ -227,10 +239,11 @@ __global__ __launch_bounds__(kFewThreads, 2) void xent_few_logits_kernel(XentFew
             for (int n = 0; n < NT; ++n) b[n][s] = h[(s * NT + n) * 64];
 #pragma unroll
         for (int t = 0; t < MT; ++t) {
+            const Quad w[2] = {lds.staged[wave][16 * t + i][g ^ (i & 7)], lds.staged[wave][16 * t + i][(4 + g) ^ (i & 7)]};
             if constexpr (F::kFloat) {
                 float x[8];
 #pragma unroll
-                for (int k = 0; k < 8; ++k) x[k] = __uint_as_float(w[t][k >> 2][k & 3]);
+                for (int k = 0; k < 8; ++k) x[k] = __uint_as_float(w[k >> 2][k & 3]);
                 Frag f[3];
                 split_bf16(x, f);
 #pragma unroll
@@ -239,41 +252,40 @@ __global__ __launch_bounds__(kFewThreads, 2) void xent_few_logits_kernel(XentFew
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
 #pragma unroll
-                    for (int s = 0; s < 2; ++s) acc[t][n] = mfma_few(__builtin_bit_cast(Frag, w[t][s]), b[n][s], acc[t][n]);
+                    for (int s = 0; s < 2; ++s) acc[t][n] = mfma_few(__builtin_bit_cast(Frag, w[s]), b[n][s], acc[t][n]);
             }
         }
     };
-    Quad now[MT][2], then[MT][2];
+    Quad now[2 * MT], then[2 * MT];
     int c = wave;
     if (c < full) load(c, now);
+    if (c + 4 < full) load(c + 4, then);
     for (; c < full; c += 8) {
-        if (c + 4 < full) load(c + 4, then);
-        multiply(c, now);
-        if (c + 4 >= full) break;
+        stage(now);
         if (c + 8 < full) load(c + 8, now);
-        multiply(c + 4, then);
+        multiply(c);
+        if (c + 4 >= full) break;
+        stage(then);
+        if (c + 12 < full) load(c + 12, then);
+        multiply(c + 4);
     }
     if (full * F::kChunk < a.features && (full & 3) == wave) {
 #pragma unroll
-        for (int t = 0; t < MT; ++t)
-#pragma unroll
-            for (int k = 0; k < 2; ++k)
-                now[t][k] = load_cut(row[t], full * F::kChunk + k * (F::kChunk / 2) + F::kEach * g, a.features);
-        multiply(full, now);
+        for (int j = 0; j < 2 * MT; ++j) now[j] = load_cut(row[j], full * F::kChunk + F::kEach * (lane & 7), a.features);
+        stage(now);
+        multiply(full);
     }
+    __syncthreads();
 #pragma unroll
     for (int t = 0; t < MT; ++t)
 #pragma unroll
-        for (int n = 0; n < NT; ++n) sums[wave][t * NT + n][lane] = acc[t][n];
+        for (int n = 0; n < NT; ++n) lds.sums[wave][t * NT + n][lane] = acc[t][n];
     __syncthreads();
-    // of several tiles of entries each wavefront takes one, of a single one the wavefronts take its tiles of rows
-    const int tile = MT > 1 ? wave : 0;
+    for (int k = wave; k < MT * NT; k += 4) {
+        const int tile = k / NT, n = k % NT;
+        Acc4 l = lds.sums[0][k][lane];
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-        if (MT == 1 && n % 4 != wave) continue;
-        Acc4 l = sums[0][tile * NT + n][lane];
-#pragma unroll
-        for (int w = 1; w < 4; ++w) l += sums[w][tile * NT + n][lane];
+        for (int w = 1; w < 4; ++w) l += lds.sums[w][k][lane];
         const int place = n * 16 + i;
         const int64_t v = first + 16 * tile + 4 * g;
         if (place < counted) *reinterpret_cast<Acc4 *>(a.logits + place * a.stride + v) = l;
