@@ -34,8 +34,8 @@ constexpr int kMatK = 64;          // k's of a step
 
 // Wavefronts of a workgroup, two along m: those of a large tile are two on each SIMD, so that one of them computes while the
 // other one's loads and reads are taken; small tiles leave room for two workgroups a compute unit instead.
-constexpr int mat_waves(int bm, int bn) { return bm * bn >= 256 * 256 ? 8 : 4; }
-constexpr int mat_threads(int bm, int bn) { return 64 * mat_waves(bm, bn); }
+constexpr int mat_waves(int bm, int bn, int buffers) { return bm * bn >= 256 * 256 || buffers > 2 ? 8 : 4; }
+constexpr int mat_threads(int bm, int bn, int buffers) { return 64 * mat_waves(bm, bn, buffers); }
 
 enum MatLayout { kRows, kCols };
 
@@ -195,13 +195,13 @@ __device__ __forceinline__ void mfma_settle(Acc4 (&acc)[MT][NT])
 // asked for, across the boundary between two tiles too, so the next tile's first steps arrive while the
 // sums of the one before are dealt with.  acc[mt][nt][r] is element (m, n) with n = n0 + kPartN wave_n() + 16 nt +
 // lane % 16 and m = m0 + kPartM wave_m() + what tile_row() says.  F16: both operands in two planes.
-template <MatLayout LA, MatLayout LB, bool F16, int BM, int BN, bool SPREAD>
+template <MatLayout LA, MatLayout LB, bool F16, int BM, int BN, int BUFFERS, bool SPREAD>
 struct MatTiles {
-    static constexpr int kWaves = mat_waves(BM, BN), kWavesM = 2, kWavesN = kWaves / kWavesM;
+    static constexpr int kWaves = mat_waves(BM, BN, BUFFERS), kWavesM = 2, kWavesN = kWaves / kWavesM;
     static constexpr int kPartM = BM / kWavesM, kPartN = BN / kWavesN;     // a wavefront's part
     static constexpr int kMT = kPartM / 16, kNT = kPartN / 16, kPasses = F16 ? 3 : 1;
     static constexpr int kBytesA = BM * kMatK * 2, kBytesB = BN * kMatK * 2, kBuffer = kBytesA + kBytesB;
-    static constexpr int kLds = 2 * kBuffer;
+    static constexpr int kLds = BUFFERS * kBuffer;
     static constexpr int kLoadsA = BM / 8 / kWaves, kLoads = (BM + BN) / 8 / kWaves;
     static_assert(kMT >= kNT && kLoads % kMT == 0, "reads and loads are dealt out to rows of MFMAs");
 
@@ -286,10 +286,10 @@ struct MatTiles {
     template <typename Next>
     __device__ __forceinline__ void begin(Next &next)
     {
-        feed(0, next);
-        feed(kBuffer, next);
-        // (the second step's loads may still be on their way)
-        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kLoads) : "memory");
+#pragma unroll
+        for (int i = 0; i < BUFFERS; ++i) feed(i * kBuffer, next);
+        // (the later steps' loads may still be on their way)
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kLoads *(BUFFERS - 1)) : "memory");
         barrier();
 #pragma unroll
         for (int i = 0; i < kMT; ++i) {
@@ -319,11 +319,11 @@ struct MatTiles {
             for (int j = 0; j < kNT; ++j) mfma<F16>(fa[0][i], fb[0][j], acc[i][j]);
             __builtin_amdgcn_sched_barrier(0);
         }
-        // this buffer is read, the other one's loads have landed, for all four wavefronts
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        // this buffer is read, the next one's loads have landed, for all wavefronts
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(kLoads *(BUFFERS - 2)) : "memory");
         barrier();
         feed_begin(next);
-        const unsigned other = kBuffer - buffer;
+        const unsigned other = BUFFERS == 2 ? kBuffer - buffer : buffer + kBuffer == kLds ? 0 : buffer + kBuffer;
 #pragma unroll
         for (int i = 0; i < kMT; ++i) {
 #pragma unroll

@@ -37,29 +37,48 @@ bool weight_in_place(const bf_linear_xent *p)
 }
 
 struct Product {
-    bool large = false;
+    bool large = false, deep = false;   // tiles of 256 x 256, of 128 x 128 in four buffers
     int tiles_m = 0, tiles_n = 0, splits = 1;
+    double time = 0;                    // estimate, microseconds
 };
 
-// Tiles of 256 x 256 where there are enough of them, with the k steps cut into parts of at least 16 if they may be,
-// for three quarters of the compute units; of 128 x 128 otherwise, cut for two workgroups a compute unit.
-Product product(int64_t m, int64_t n, int64_t steps, bool may_split)
+// The shape of tiles that takes less time by this estimate.  At a time the chip holds 256 tiles of 256 x 256 or 512 of
+// 128 x 128; a k step of 64 takes them 1.75 and 1.05 us, a tile's end (exponentials, stores) 8 and 2 us (of two small
+// tiles on a compute unit one computes meanwhile), sums that are split their bytes' way.  Measured, small and large: 8192
+// rows, 1024 features, 32768 entries, bfloat16, forward and backward, 2311 and 1957 us (many tiles: the large ones read
+// less); 572 x 2659 x 24269, float, 1237 and 1536 (285 large tiles are two rounds); 3300 x 70 x 74639, float, 1315 and
+// 1667 (two k steps a tile); 1000 x 1000 x 8000, bfloat16, 121 and 219.
+// Small tiles of which each compute unit has only one are made by eight wavefronts out of four buffers: 129 x 1731 x
+// 1314, float, 157 us beside 194.
+Product product(int64_t m, int64_t n, int64_t steps, int passes, bool may_split)
 {
-    auto tiles = [&](int64_t side) { return ((m + side - 1) / side) * ((n + side - 1) / side); };
-    const int64_t parts = may_split ? std::min<int64_t>(std::max<int64_t>(steps / 16, 1), 32) : 1;
-    Product r;
-    r.large = tiles(256) * parts >= 192;
-    const int64_t t = r.large ? 256 : 128, here = std::max<int64_t>(tiles(t), 1);
-    r.tiles_m = (int)((m + t - 1) / t);
-    r.tiles_n = (int)((n + t - 1) / t);
-    r.splits = (int)std::max<int64_t>(1, std::min<int64_t>(parts, (r.large ? 256 : 512) / here));
-    return r;
+    const int64_t most = may_split ? std::min<int64_t>(std::max<int64_t>(steps / 8, 1), 512) : 1;
+    auto ceil = [](int64_t a, int64_t b) { return (a + b - 1) / b; };
+    auto of = [&](int64_t side, int64_t places, double step, double end) {
+        Product r;
+        r.large = side == 256;
+        r.tiles_m = (int)ceil(m, side);
+        r.tiles_n = (int)ceil(n, side);
+        const int64_t tiles = std::max<int64_t>((int64_t)r.tiles_m * r.tiles_n, 1);
+        auto time = [&](int64_t splits) {
+            const double sums = splits > 1 ? 2 + splits * (double)m * n * 8 / 4.8e6 : 0;
+            return ceil(tiles * splits, places) * (ceil(steps, splits) * passes * step + end) + sums;
+        };
+        const int64_t cut = std::max<int64_t>(1, std::min<int64_t>(most, places / tiles));
+        r.splits = (int)(time(cut) < time(1) ? cut : 1);
+        r.time = time(r.splits);
+        return r;
+    };
+    Product small = of(128, 512, 1.05, 2), large = of(256, 256, 1.75, 8);
+    if (large.time < small.time) return large;
+    small.deep = (int64_t)small.tiles_m * small.tiles_n * small.splits <= 256;
+    return small;
 }
 
 // As many as are at work at a time: one a compute unit for large tiles (128 KiB of LDS), two for small ones.
 unsigned workgroups(const Product &r)
 {
-    return (unsigned)std::min<int64_t>((int64_t)r.tiles_m * r.tiles_n * r.splits, r.large ? 256 : 512);
+    return (unsigned)std::min<int64_t>((int64_t)r.tiles_m * r.tiles_n * r.splits, r.large || r.deep ? 256 : 512);
 }
 
 constexpr size_t kPieceBytes = (size_t)256 << 20;   // d_l of a piece of the vocabulary
@@ -83,6 +102,7 @@ XentPlan plan(const bf_linear_xent *p, bool backward)
 {
     XentPlan r;
     r.planes = p->dtype == BF_F32 ? 2 : 1;
+    const int passes = p->dtype == BF_F32 ? 3 : 1;
     r.features_up = up_to(p->features, kMatK);
     r.rows_up = up_to(std::max<int64_t>(p->rows, 1), 256);
     r.hidden_plane = up256((size_t)r.rows_up * r.features_up * 2);
@@ -104,7 +124,7 @@ XentPlan plan(const bf_linear_xent *p, bool backward)
     r.kept = at;
     at = 0;
     if (!backward) {
-        r.logits = product(p->vocab, p->rows, 0, false);
+        r.logits = product(p->vocab, p->rows, r.features_up / kMatK, passes, false);
         r.picked = take(rows * 4);
         r.losses = take(rows * 4);
         r.partial = take((size_t)2 * r.logits.tiles_m * rows * sizeof(float2));
@@ -113,9 +133,9 @@ XentPlan plan(const bf_linear_xent *p, bool backward)
         r.piece = std::min<int64_t>(up_to(p->vocab, 256), std::max<int64_t>(most, 2048));
         const int64_t pieces = (p->vocab + r.piece - 1) / r.piece;
         r.piece = std::min<int64_t>(up_to((p->vocab + pieces - 1) / pieces, 256), r.piece);
-        r.logits = product(r.piece, p->rows, 0, false);
-        r.to_hidden = product(p->features, p->rows, r.piece / kMatK, true);
-        r.to_weight = product(p->features, r.piece, (p->rows + kMatK - 1) / kMatK, true);
+        r.logits = product(r.piece, p->rows, r.features_up / kMatK, passes, false);
+        r.to_hidden = product(p->features, p->rows, r.piece / kMatK, passes, true);
+        r.to_weight = product(p->features, r.piece, (p->rows + kMatK - 1) / kMatK, passes, true);
         r.share = take(rows * 4);
         r.d_l_plane = up256((size_t)r.rows_up * r.piece * 2);
         r.d_l = take(r.d_l_plane * r.planes);
@@ -215,7 +235,7 @@ void pack(const bf_linear_xent *p, const void *x, char *out, int64_t out_rows, i
 {
     if (p->dtype == BF_F32 && rows > 0) {
         unsigned *largest = which ? &scalars->weight_max : &scalars->hidden_max;
-        xent_largest_kernel<<<dim3((unsigned)std::min<int64_t>((rows + 3) / 4, 1024)), dim3(256), 0, s>>>(
+        xent_largest_kernel<<<dim3((unsigned)std::min<int64_t>((rows * ((p->features + 7) / 8) + 255) / 256, 2048)), dim3(256), 0, s>>>(
             static_cast<const float *>(x), rows, p->features, x_stride, index, scalars, largest);
     }
     const XentPackArgs a = {x, out, out_rows, p->features, x_stride, stride, (int64_t)plane, index, scalars, which};
@@ -255,26 +275,42 @@ void prepare(const bf_linear_xent *p, const XentPlan &r, const void *hidden, con
 template <bool F16, bool BACKWARD>
 void launch_logits(const Product &r, const XentTileArgs &a, hipStream_t s)
 {
-    const dim3 grid(workgroups(r)), threads(r.large ? mat_threads(256, 256) : mat_threads(128, 128));
-    if (r.large) xent_logits_kernel<F16, 256, 256, BACKWARD><<<grid, threads, 0, s>>>(a);
-    else xent_logits_kernel<F16, 128, 128, BACKWARD><<<grid, threads, 0, s>>>(a);
+    const dim3 grid(workgroups(r)), threads(r.large ? mat_threads(256, 256, 2) : mat_threads(128, 128, r.deep ? 4 : 2));
+    if (r.large) xent_logits_kernel<F16, 256, 256, 2, BACKWARD><<<grid, threads, 0, s>>>(a);
+    else if (r.deep) xent_logits_kernel<F16, 128, 128, 4, BACKWARD><<<grid, threads, 0, s>>>(a);
+    else xent_logits_kernel<F16, 128, 128, 2, BACKWARD><<<grid, threads, 0, s>>>(a);
+}
+
+template <typename T, MatLayout LB>
+void launch_grad(const Product &r, const XentGradArgs &a, hipStream_t s)
+{
+    const dim3 grid(workgroups(r)), threads(r.large ? mat_threads(256, 256, 2) : mat_threads(128, 128, r.deep ? 4 : 2));
+    if (r.large) xent_grad_kernel<T, LB, 256, 256, 2><<<grid, threads, 0, s>>>(a);
+    else if (r.deep) xent_grad_kernel<T, LB, 128, 128, 4><<<grid, threads, 0, s>>>(a);
+    else xent_grad_kernel<T, LB, 128, 128, 2><<<grid, threads, 0, s>>>(a);
 }
 
 template <MatLayout LB>
 void launch_grad(const bf_linear_xent *p, const Product &r, const XentGradArgs &a, hipStream_t s)
 {
-    const dim3 grid(workgroups(r)), threads(r.large ? mat_threads(256, 256) : mat_threads(128, 128));
-    if (p->dtype == BF_F32) {
-        if (r.large) xent_grad_kernel<float, LB, 256, 256><<<grid, threads, 0, s>>>(a);
-        else xent_grad_kernel<float, LB, 128, 128><<<grid, threads, 0, s>>>(a);
-    } else {
-        if (r.large) xent_grad_kernel<bf16, LB, 256, 256><<<grid, threads, 0, s>>>(a);
-        else xent_grad_kernel<bf16, LB, 128, 128><<<grid, threads, 0, s>>>(a);
-    }
+    if (p->dtype == BF_F32) launch_grad<float, LB>(r, a, s);
+    else launch_grad<bf16, LB>(r, a, s);
+}
+
+template <typename T, bool SCALED>
+void gather_runs(const XentGatherArgs &a, hipStream_t s)
+{
+    const dim3 grid((unsigned)((a.m + 127) / 128), (unsigned)std::min<int64_t>(a.rows, 4096));
+    xent_gather_runs_kernel<T, SCALED><<<grid, dim3(1024), 0, s>>>(a);
 }
 
 void gather(const bf_linear_xent *p, const XentGatherArgs &a, hipStream_t s)
 {
+    if (a.position && a.splits >= 16) {
+        if (p->dtype == BF_F32) gather_runs<float, true>(a, s);
+        else gather_runs<bf16, false>(a, s);
+        return;
+    }
     const int64_t units = a.rows * ((a.m + 7) / 8);
     const dim3 grid((unsigned)std::min<int64_t>((units + 255) / 256, 8192));
     if (p->dtype == BF_F32) xent_gather_kernel<float><<<grid, dim3(256), 0, s>>>(a);
@@ -334,8 +370,7 @@ void few_bw(const bf_linear_xent *p, const XentFewPlan &r, const void *weight, c
     const int blocks_weight = d_weight ? (r.columns * r.splits_weight + 3) / 4 : 0;
     xent_few_grad_kernel<T, NT><<<dim3((unsigned)(g.blocks_hidden + blocks_weight)), dim3(kFewThreads), 0, s>>>(g);
     if (!d_hidden) return;
-    const XentFewGatherArgs a = {g.partial, part<int>(kept, r.position), scalars, gradient, d_hidden, (int)p->rows, (int)p->features, r.splits_hidden};
-    xent_few_gather_kernel<T><<<dim3((unsigned)((p->features + 127) / 128), (unsigned)p->rows), dim3(1024), 0, s>>>(a);
+    gather_runs<T, false>({g.partial, part<int>(kept, r.position), scalars, gradient, d_hidden, p->rows, p->rows, p->features, r.splits_hidden, 0}, s);
 }
 
 // f(the type, tiles of rows) of a call
@@ -413,7 +448,7 @@ int bf_linear_xent_fw(const bf_linear_xent *p, const void *hidden, const void *w
         else launch_logits<false, false>(r.logits, a, s);
         const XentJoinArgs j = {a.partial, picked, part<int>(kept, r.position), part<int>(kept, r.label), p->rows, 2 * r.logits.tiles_m,
                                 part<float>(kept, r.lse), losses};
-        xent_join_kernel<<<dim3((unsigned)((p->rows + 31) / 32)), dim3(512), 0, s>>>(j);
+        xent_join_kernel<<<dim3((unsigned)((p->rows + 7) / 8)), dim3(1024), 0, s>>>(j);
     }
     if (p->reduction != BF_XENT_NONE)
         xent_total_kernel<<<dim3(1), dim3(kXentThreads), 0, s>>>(losses, p->rows, scalars, p->reduction == BF_XENT_MEAN, loss);

@@ -102,18 +102,17 @@ __global__ __launch_bounds__(256) void xent_largest_kernel(const float *x, int64
                                                            const int *index, const XentScalars *scalars, unsigned *largest)
 {
     __shared__ unsigned lds[4];
-    const int64_t n = index ? scalars->counted : rows;
+    const int units = (int)((cols + 7) / 8);
+    const int64_t total = (index ? scalars->counted : rows) * units;
     unsigned m = 0;
-    for (int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); r < n; r += (int64_t)gridDim.x * 4) {
-        const float *row = x + (index ? index[r] : r) * stride;
-        for (int c = (threadIdx.x & 63) * 8; c < (int)cols; c += 512) {
-            float v[8];
-            load8(row, c, (int)cols, 0.0f, v);
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+        const int64_t r = i / units;
+        float v[8];
+        load8(x + (index ? index[r] : r) * stride, (int)(i - r * units) * 8, (int)cols, 0.0f, v);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const unsigned b = __float_as_uint(v[i]) & 0x7fffffffu;
-                m = b > m ? b : m;
-            }
+        for (int k = 0; k < 8; ++k) {
+            const unsigned b = __float_as_uint(v[k]) & 0x7fffffffu;
+            m = b > m ? b : m;
         }
     }
 #pragma unroll
@@ -249,10 +248,10 @@ __device__ __forceinline__ float rounded_off(float v, float from) { return __bui
 
 // Workgroups stay for tile after tile (grid: as many as the chip holds at a time), so that a tile's exponentials and
 // stores run while the next one's operands arrive.
-template <bool F16, int BM, int BN, bool BACKWARD>
-__global__ __launch_bounds__(mat_threads(BM, BN), 1) void xent_logits_kernel(XentTileArgs a)
+template <bool F16, int BM, int BN, int BUFFERS, bool BACKWARD>
+__global__ __launch_bounds__(mat_threads(BM, BN, BUFFERS), 1) void xent_logits_kernel(XentTileArgs a)
 {
-    using Tile = MatTiles<kRows, kRows, F16, BM, BN, true>;
+    using Tile = MatTiles<kRows, kRows, F16, BM, BN, BUFFERS, true>;
     __shared__ __attribute__((aligned(1024))) char lds[Tile::kLds];
     const int counted = a.scalars->counted;
     const int tiles_n = (counted + BN - 1) / BN, total = a.tiles_m * tiles_n;
@@ -407,21 +406,24 @@ struct XentJoinArgs {
     float *losses;          // (rows), as the caller numbers them; zero where ignored
 };
 
-// 32 rows and 16 runs of partials a workgroup
-__global__ __launch_bounds__(512) void xent_join_kernel(XentJoinArgs a)
+// 8 rows and 128 runs of their parts a workgroup (rows are neighbours in memory)
+__global__ __launch_bounds__(1024) void xent_join_kernel(XentJoinArgs a)
 {
-    __shared__ float2 lds[16][33];
-    const int64_t row = (int64_t)blockIdx.x * 32 + (threadIdx.x & 31);
-    const int run = threadIdx.x >> 5, at = row < a.rows ? a.position[row] : -1;
-    const int per = (a.parts + 15) / 16, end = (run + 1) * per < a.parts ? (run + 1) * per : a.parts;
+    __shared__ float2 lds[16][8];
+    const int lane = threadIdx.x & 63, run = threadIdx.x >> 3;
+    const int64_t row = (int64_t)blockIdx.x * 8 + (lane & 7);
+    const int at = row < a.rows ? a.position[row] : -1;
     Joined all;
     if (at >= 0) {
-#pragma unroll 8
-        for (int p = run * per; p < end; ++p) all.join(a.partial[(int64_t)p * a.rows + at]);
+        const int end = (int)((int64_t)a.parts * (run + 1) / 128);
+#pragma unroll 4
+        for (int p = (int)((int64_t)a.parts * run / 128); p < end; ++p) all.join(a.partial[(int64_t)p * a.rows + at]);
     }
-    lds[run][threadIdx.x & 31] = make_float2(all.top, all.sum);
+#pragma unroll
+    for (int d = 8; d < 64; d *= 2) all.join(make_float2(__shfl_down(all.top, d, 64), __shfl_down(all.sum, d, 64)));
+    if (lane < 8) lds[threadIdx.x >> 6][lane] = make_float2(all.top, all.sum);
     __syncthreads();
-    if (run != 0 || row >= a.rows) return;
+    if (threadIdx.x >= 8 || row >= a.rows) return;
     Joined whole;
     for (int i = 0; i < 16; ++i) whole.join(lds[i][threadIdx.x]);
     const float lse = whole.lse();
@@ -482,11 +484,11 @@ struct XentGradArgs {
 __device__ __forceinline__ int xent_splits(int splits, int steps) { return splits < steps ? splits : steps > 1 ? steps : 1; }
 
 // d_hidden: n are rows, k the vocabulary (d_l row by row); d_weight: n the vocabulary, k the counted rows
-template <typename T, MatLayout LB, int BM, int BN>
-__global__ __launch_bounds__(mat_threads(BM, BN), 1) void xent_grad_kernel(XentGradArgs a)
+template <typename T, MatLayout LB, int BM, int BN, int BUFFERS>
+__global__ __launch_bounds__(mat_threads(BM, BN, BUFFERS), 1) void xent_grad_kernel(XentGradArgs a)
 {
     constexpr bool F16 = sizeof(T) == 4, OF_WEIGHT = LB == kCols;
-    using Tile = MatTiles<kCols, LB, F16, BM, BN, false>;
+    using Tile = MatTiles<kCols, LB, F16, BM, BN, BUFFERS, false>;
     __shared__ __attribute__((aligned(1024))) char lds[Tile::kLds];
     const int counted = a.scalars->counted;
     const int tiles_n = OF_WEIGHT ? a.tiles_n : (counted + BN - 1) / BN, tiles = a.tiles_m * tiles_n;
@@ -598,6 +600,45 @@ __global__ __launch_bounds__(256) void xent_gather_kernel(XentGatherArgs a)
             for (int k = 0; k < 8; ++k) s[k] *= scale;
         }
         store8(reinterpret_cast<T *>(a.out) + row * m, col, m, s);
+    }
+}
+
+// The same for d_hidden's rows in many splits: 128 columns of a row a workgroup, 32 runs of the splits side by side, each and
+// then all of them in ascending order.  SCALED: by the powers of two of the product's operands.
+template <typename T, bool SCALED>
+__global__ __launch_bounds__(1024) void xent_gather_runs_kernel(XentGatherArgs a)
+{
+    __shared__ Acc4 lds[32][32];
+    const int m = (int)a.m, run = threadIdx.x >> 5, col = blockIdx.x * 128 + (threadIdx.x & 31) * 4;
+    for (int64_t row = blockIdx.y; row < a.rows; row += gridDim.y) {
+        const int at = a.position[row];
+        Acc4 s = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (at >= 0 && col < m) {
+            const int begin = a.splits * run / 32, end = a.splits * (run + 1) / 32;
+            const float *p = a.partial + (int64_t)at * m + col;
+            const int64_t stride = a.n * m;
+            if (col + 4 <= m) {
+#pragma unroll 8
+                for (int k = begin; k < end; ++k) s += Acc4(*reinterpret_cast<const quad_at_4 *>(p + k * stride));
+            } else {
+                for (int k = begin; k < end; ++k)
+                    for (int c = 0; c < 4; ++c)
+                        if (col + c < m) s[c] += p[k * stride + c];
+            }
+        }
+        __syncthreads();
+        lds[run][threadIdx.x & 31] = s;
+        __syncthreads();
+        if (run != 0 || col >= m) continue;
+#pragma unroll 4
+        for (int k = 1; k < 32; ++k) s += lds[k][threadIdx.x];
+        float scale = a.grad.scale(a.scalars);
+        if constexpr (SCALED) scale *= 1.0f / 32768.0f / a.scalars->weight_scale;
+        s = s * scale;
+        T *out = reinterpret_cast<T *>(a.out) + row * m + col;
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+            if (col + c < m) out[c] = at >= 0 ? (T)s[c] : (T)0.0f;
     }
 }
 

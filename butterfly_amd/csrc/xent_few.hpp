@@ -586,45 +586,4 @@ __global__ __launch_bounds__(kFewThreads, 2) void xent_few_grad_kernel(XentFewGr
     }
 }
 
-struct XentFewGatherArgs {
-    const float *partial;       // (splits, rows, features)
-    const int *position;
-    const XentScalars *scalars;
-    XentGrad grad;
-    void *out;
-    int rows, features, splits;
-};
-
-// A row's sums of 128 columns: 32 runs of the splits side by side, each and then all of them in ascending order.
-template <typename T>
-__global__ __launch_bounds__(1024) void xent_few_gather_kernel(XentFewGatherArgs a)
-{
-    __shared__ Acc4 lds[32][32];
-    const int at = a.position[blockIdx.y], run = threadIdx.x >> 5, col = blockIdx.x * 128 + (threadIdx.x & 31) * 4;
-    Acc4 s = {0.0f, 0.0f, 0.0f, 0.0f};
-    if (at >= 0 && col < a.features) {
-        const int begin = a.splits * run / 32, end = a.splits * (run + 1) / 32;
-        const float *p = a.partial + (int64_t)at * a.features + col;
-        const int64_t stride = (int64_t)a.rows * a.features;
-        if (col + 4 <= a.features) {
-#pragma unroll 8
-            for (int k = begin; k < end; ++k) s += Acc4(*reinterpret_cast<const quad_at_4 *>(p + k * stride));
-        } else {
-            for (int k = begin; k < end; ++k)
-                for (int c = 0; c < 4; ++c)
-                    if (col + c < a.features) s[c] += p[k * stride + c];
-        }
-    }
-    lds[run][threadIdx.x & 31] = s;
-    __syncthreads();
-    if (run != 0 || col >= a.features) return;
-#pragma unroll 4
-    for (int k = 1; k < 32; ++k) s += lds[k][threadIdx.x];
-    s = s * a.grad.scale(a.scalars);
-    T *out = reinterpret_cast<T *>(a.out) + (int64_t)blockIdx.y * a.features + col;
-#pragma unroll
-    for (int c = 0; c < 4; ++c)
-        if (col + c < a.features) out[c] = at >= 0 ? (T)s[c] : (T)0.0f;
-}
-
 }  // namespace bf
