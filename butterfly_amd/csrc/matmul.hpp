@@ -49,13 +49,14 @@ struct MatOperand {
 
 // lds_addr: where the wavefront's 64 units go (wave-uniform); offsets from the descriptor's base, within 2^31.
 // (m0 is not saved: nothing else in these kernels uses it, and the compiler is told; its warning is that it
-// will not keep it for anybody either)
+// will not keep it for anybody either; with the move of m0 five wait states, which a descriptor or an offset needs that a
+// lane's read has just brought to scalar registers, and which the compiler does not count in front of these lines)
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"
 __device__ __forceinline__ void load_unit_to_lds(MatDesc desc, unsigned lds_addr, int voff, int soff)
 {
     asm volatile("s_mov_b32 m0, %0\n\t"
-                 "s_nop 0\n\t"
+                 "s_nop 3\n\t"
                  "buffer_load_dwordx4 %1, %2, %3 offen lds"
                  :
                  : "s"(lds_addr), "v"(voff), "s"(desc), "s"(soff)
