@@ -34,9 +34,11 @@ struct RecurrencePlan {
     size_t state_bytes = 0, chunk_bytes = 0, run_bytes = 0, workspace = 0;   // of one of chunk_a, chunk_b; run_a, run_b
 };
 
-// Channels times batch make `groups * batch` workgroups.  From 192 of them on (three quarters of the compute units)
-// the sequence stays whole and is read once; below, it is cut until some 512 are at work, in
-// chunks of 16 runs of whole blocks of S steps, at the price of a second read of the gates and inputs.
+// Channels times batch make `groups * batch` workgroups.  A whole sequence is read once, at some 25 ns a step however few
+// of them there are; cut into chunks of 16 runs of whole blocks of S steps, until some 512 are at work, the gates
+// and inputs are read twice and two launches more are made.  Measured in float, forward and backward, whole and cut: 64
+// workgroups of 4096 steps 291 and 173 us, 96 315 and 293, 112 322 and 400; 64 of 512 steps 62 and 79, of 1024
+// 72 and 77, of 2048 132 and 91; 8 (bfloat16) of 16384 steps 1605 and 110.  So below 96 of more than four tiles.
 RecurrencePlan plan(const bf_recurrence *p)
 {
     RecurrencePlan r;
@@ -45,7 +47,7 @@ RecurrencePlan plan(const bf_recurrence *p)
     r.groups = (p->channels + 64 * v - 1) / (64 * v);
     const int64_t whole = r.groups * p->batch, tile = (int64_t)kRecWaves * s;
     r.chunk = std::max<int64_t>(p->steps, 1);
-    if (whole < 192 && p->steps > tile) {
+    if (whole < 96 && p->steps > 4 * tile) {
         const int64_t wanted = std::min<int64_t>((512 + whole - 1) / whole, (p->steps + tile - 1) / tile);
         r.chunk = std::max<int64_t>((p->steps / wanted + tile / 2) / tile, 1) * tile;
         r.chunks = (p->steps + r.chunk - 1) / r.chunk;

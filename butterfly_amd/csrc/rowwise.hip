@@ -12,8 +12,8 @@ namespace {
 
 using namespace bf;
 
+constexpr int kRegisterCols = 8192;              // widest row that the register kernels hold
 constexpr int64_t kMaxCols = (int64_t)1 << 28;   // column numbers and slices stay inside 32 bits
-constexpr int kRegisterCols = 16384;             // widest row that the register kernels hold
 
 int check_rows(const bf_rowwise *p)
 {
@@ -50,9 +50,12 @@ void fill_common(RowArgs &a, const bf_rowwise *p, const void *rng)
     a.wide_params = p->param_dtype == BF_F32;
 }
 
-// Lanes that share a row (L) and chunks of 8 columns each of them holds (K): a wavefront a row up to 1024
-// columns, parts of one for narrow rows, 256 threads up to 8192 (32 columns each), 1024 beyond.
-// (K = 4 in a wavefront for 2048 columns would leave few workgroups at few rows.)
+// Lanes that share a row (L) and chunks of 8 columns each of them holds (K).  Measured (forward, forward with backward):
+// 65536 x 512 float by 32 lanes 41.7 and 128 us, by 64 44.3 and 139; 32768 x 1000 by 64 43.4 and 134, by 128 46.8 and 168;
+// 16384 x 2048 bfloat16 by 256 36.3 and 99, by 64 (K = 4) 40.3 and 97, float 45.5 and 132 beside 47.7 and 146; 8192 x
+// 4096 by 256 44 and 138, by 512 52 and 142; 4096 x 8192 bfloat16 by 512 37 and 108, by 256 43 and 115, by 1024 74 and 134.
+// Wider rows are read again, out of the L2: 2048 x 9000 float 45 and 118, by 512 lanes (K = 4) 60 and 133; 2048 x 16384
+// bfloat16 47 and 120 beside 55 and 139 (float 71 and 223 beside 70 and 199).
 template <typename F>
 void with_row_shape(int cols, F &&f)
 {
@@ -60,12 +63,11 @@ void with_row_shape(int cols, F &&f)
     if (cols <= 64) BF_SHAPE(8, 1);
     else if (cols <= 128) BF_SHAPE(16, 1);
     else if (cols <= 256) BF_SHAPE(32, 1);
-    else if (cols <= 512) BF_SHAPE(64, 1);
+    else if (cols <= 512) BF_SHAPE(32, 2);
     else if (cols <= 1024) BF_SHAPE(64, 2);
     else if (cols <= 2048) BF_SHAPE(256, 1);
     else if (cols <= 4096) BF_SHAPE(256, 2);
-    else if (cols <= 8192) BF_SHAPE(256, 4);
-    else BF_SHAPE(1024, 2);
+    else BF_SHAPE(512, 2);
 #undef BF_SHAPE
 }
 
