@@ -130,6 +130,17 @@ def test_resets(share, dtype, sigmoid):
     check(v, sigmoid, reset[:1].expand(3, 300))
 
 
+@pytest.mark.parametrize("dtype,sigmoid", KINDS)
+@pytest.mark.parametrize("share", [0.5, 1.0])
+def test_resets_in_chunks(share, dtype, sigmoid):
+    v = make(2, 1111, 66, dtype, sigmoid)
+    reset = torch.rand(2, 1111, generator=torch.Generator().manual_seed(4)) < share
+    check(v, sigmoid, reset)
+    reset[:] = False
+    reset[0, 0] = reset[1, 1110] = True
+    check(v, sigmoid, reset)
+
+
 @pytest.mark.parametrize("steps,where", [(40, 13), (300, 200), (1200, 700)])
 @pytest.mark.parametrize("dtype,sigmoid", KINDS)
 def test_nothing_from_before_a_reset_gets_through(steps, where, dtype, sigmoid):
