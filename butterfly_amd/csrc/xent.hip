@@ -235,7 +235,7 @@ void pack(const bf_linear_xent *p, const void *x, char *out, int64_t out_rows, i
 {
     if (p->dtype == BF_F32 && rows > 0) {
         unsigned *largest = which ? &scalars->weight_max : &scalars->hidden_max;
-        xent_largest_kernel<<<dim3((unsigned)std::min<int64_t>((rows * ((p->features + 7) / 8) + 255) / 256, 2048)), dim3(256), 0, s>>>(
+        xent_largest_kernel<<<dim3((unsigned)std::min<int64_t>((rows * ((p->features + 7) / 8) + 1023) / 1024, 1024)), dim3(256), 0, s>>>(
             static_cast<const float *>(x), rows, p->features, x_stride, index, scalars, largest);
     }
     const XentPackArgs a = {x, out, out_rows, p->features, x_stride, stride, (int64_t)plane, index, scalars, which};

@@ -105,6 +105,7 @@ __global__ __launch_bounds__(256) void xent_largest_kernel(const float *x, int64
     const int units = (int)((cols + 7) / 8);
     const int64_t total = (index ? scalars->counted : rows) * units;
     unsigned m = 0;
+#pragma unroll 4
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
         const int64_t r = i / units;
         float v[8];
@@ -120,12 +121,12 @@ __global__ __launch_bounds__(256) void xent_largest_kernel(const float *x, int64
         const unsigned v = (unsigned)__shfl_xor((int)m, d, 64);
         m = v > m ? v : m;
     }
-    // (one atomic a workgroup: all of them go to one address, one after another)
+    // (all of them go to one address, one after another: one a workgroup, and none where a larger number is there)
     if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = m;
     __syncthreads();
     if (threadIdx.x != 0) return;
     for (int w = 1; w < 4; ++w) m = lds[w] > m ? lds[w] : m;
-    if (m > 0) atomicMax(largest, m);
+    if (m > __hip_atomic_load(largest, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)) atomicMax(largest, m);
 }
 
 // 2^e that brings the number to 2^14 .. 2^15 (infinite, NaN or zero: 1)
