@@ -173,8 +173,11 @@ XentFewPlan few_plan(const bf_linear_xent *p, bool backward)
     r.stride = up_to(p->vocab, 64);
     r.steps = (p->vocab + 31) / 32;
     r.columns = (int)((p->features + 16 * each - 1) / (16 * each));
-    // wavefronts for all compute units, of four steps or tiles and more
-    r.splits_hidden = (int)std::max<int64_t>(1, std::min<int64_t>(2048 / r.columns, r.steps / 4));
+    // Wavefronts for all compute units, of four steps or tiles and more; d_hidden's leave sums behind, of which 16 MiB are
+    // enough: 60 rows, 4096 features, 65536 entries, bfloat16, forward and backward, 512 wavefronts 392 us, 2048 453; 33 x 1843 x
+    // 67371 float, 512 607, 1024 509, 2048 518; 6 x 3185 x 32906 bfloat16, 512 198, 2048 180.
+    const int64_t summing = std::min<int64_t>(2048, (16 << 20) / (r.tiles * 16 * 16 * each * 4));
+    r.splits_hidden = (int)std::max<int64_t>(1, std::min<int64_t>(summing / r.columns, r.steps / 4));
     r.splits_weight = (int)std::max<int64_t>(1, std::min<int64_t>(4096 / r.columns, r.steps / 2));
     size_t at = 0;
     auto take = [&](size_t bytes) {
