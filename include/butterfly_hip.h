@@ -376,13 +376,15 @@ int bf_recurrence_bw(const bf_recurrence *p, const void *gate, const void *x, co
 int bf_recurrence_step(const bf_recurrence *p, const void *gate, const void *x, void *state,
                        void *h, void *stream);
 
-/* Softmax cross entropy of logits = hidden weight^T (rows, vocab), which are never held as a whole:
+/* Softmax cross entropy of logits = hidden weight^T (rows, vocab), which are not held as a whole (but those of
+ * up to 64 rows, no more than there are features):
  *   loss_i = log sum_v exp(l_iv) - l_i,target(i);  a row whose target is ignore_index counts for
  *   nothing (loss 0, gradient 0); a target that is no entry of the vocabulary makes loss and
  *   gradients NaN.  Mean: over the rows that count (NaN if there is none).
  * hidden (rows, features), weight (vocab, features), features adjacent, rows `*_stride` elements
  * apart, weight 16-byte aligned.  BF_BF16: products of bfloat16 with sums in float, the logits' gradient in bfloat16.
- * BF_F32: every factor as two float16 numbers of together 22 bits, sums in float.
+ * BF_F32: every factor as two float16 numbers of together 22 bits (few rows: three bfloat16 numbers of together 24), sums in
+ * float.
  * Gradients are dense, summed in a fixed order.                                                 */
 #define BF_XENT_NONE 0
 #define BF_XENT_MEAN 1
@@ -397,16 +399,17 @@ typedef struct bf_linear_xent {
 
 /* kept (256-byte aligned): what the forward call leaves for the backward one, which rows count and the operands in the
  * products' form (and their log-sum-exps): hidden's counted rows and, where it cannot be read as it lies (float, rows that 16
- * bytes do not divide), weight.  A call without a backward one gives it the same room.
- * The workspaces (256-byte aligned) hold 16 bytes for each row and 256 (128) entries forward, and backward the
- * logits' gradient over a piece of the vocabulary, up to some 256 MiB, and the sums of d_hidden's and d_weight's
- * parts.                                                                                         */
+ * bytes do not divide), weight; of few rows hidden and their logits.  A call without a backward one gives it the same
+ * room.  The workspaces (256-byte aligned) hold 16 bytes for each row and 256 (128; few rows: 64 or 16) entries forward,
+ * and backward the logits' gradient over a piece of the vocabulary, up to some 256 MiB (few rows: all of it, twice),
+ * and the sums of d_hidden's and d_weight's parts.                                               */
 size_t bf_linear_xent_kept_bytes(const bf_linear_xent *p);
 size_t bf_linear_xent_fw_workspace_bytes(const bf_linear_xent *p);
 size_t bf_linear_xent_bw_workspace_bytes(const bf_linear_xent *p);
 /* loss: one float, or (rows) with BF_XENT_NONE. */
 int bf_linear_xent_fw(const bf_linear_xent *p, const void *hidden, const void *weight,
-                      const int64_t *target, float *loss, void *kept, size_t kept_bytes, void *workspace, size_t workspace_bytes, void *stream);
+                      const int64_t *target, float *loss, void *kept, size_t kept_bytes,
+                      void *workspace, size_t workspace_bytes, void *stream);
 /* weight, kept: of the forward call.  grad: the loss's gradient, one float or (rows).  d_hidden or
  * d_weight may be NULL.                                                                          */
 int bf_linear_xent_bw(const bf_linear_xent *p, const void *weight, const float *grad, void *kept,
