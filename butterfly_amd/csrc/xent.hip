@@ -152,7 +152,7 @@ XentPlan plan(const bf_linear_xent *p, bool backward)
 bool few_rows(const bf_linear_xent *p) { return p->rows > 0 && p->rows <= kFewRows && p->rows <= p->features; }
 
 struct XentFewPlan {
-    int tiles = 1, entry_tiles = 1, parts = 1;              // of 16 rows; of 16 entries a workgroup; partial maxima and sums
+    int tiles = 1, parts = 1, wide = 0;                     // of 16 rows; workgroups of the logits, those of 64 entries
     int64_t stride = 0, steps = 0;                          // of the logits' rows; of 32 entries
     int columns = 1, splits_hidden = 1, splits_weight = 1;  // parts of the columns, of the vocabulary
     size_t scalars = 0, index = 0, position = 0, label = 0, lse = 0, by_feature = 0, by_row = 0, logits = 0, kept = 0;
@@ -166,10 +166,15 @@ XentFewPlan few_plan(const bf_linear_xent *p, bool backward)
     const int64_t planes = wide ? 3 : 1, each = wide ? 4 : 8, chunk = wide ? 32 : 64, chunk_frags = wide ? 3 : 2;
     XentFewPlan r;
     r.tiles = p->rows <= 16 ? 1 : p->rows <= 32 ? 2 : 4;
-    // (64 entries read hidden a quarter as often: 60 rows, 1000 features, 30001 entries, float: 33 us beside 44; 16 entries are
-    // work for all compute units where 64 are not: 3 rows, 1390 features, 6879 entries: 9.9 us beside 16)
-    r.entry_tiles = p->vocab >= 64 * 256 ? 4 : 1;
-    r.parts = (int)((p->vocab + 16 * r.entry_tiles - 1) / (16 * r.entry_tiles));
+    // Workgroups of 64 entries read hidden a quarter as often as those of 16 (60 rows, 1000 features, 30001 entries, float: 33 us
+    // beside 44), which are work for all compute units where 64 are not (3 rows, 1390 features, 6879 entries: 9.9 us beside
+    // 16).  The chip holds two or three of the former a compute unit; a last round that these would fill by less than
+    // half is made by the latter.
+    if (p->vocab >= 64 * 256) {
+        const int64_t round = wide || r.tiles == 4 ? 512 : 768, all = p->vocab / 64;
+        r.wide = (int)(all % round < round / 2 && all > round ? all / round * round : all);
+    }
+    r.parts = (int)(r.wide + (p->vocab - 64 * (int64_t)r.wide + 15) / 16);
     r.stride = up_to(p->vocab, 64);
     r.steps = (p->vocab + 31) / 32;
     r.columns = (int)((p->features + 16 * each - 1) / (16 * each));
@@ -332,10 +337,10 @@ void few_fw(const bf_linear_xent *p, const XentFewPlan &r, const void *hidden, c
     xent_few_pack_kernel<T><<<dim3((unsigned)std::min<size_t>((slots + kFewThreads - 1) / kFewThreads, 1024)), dim3(kFewThreads), 0, s>>>(pack);
     float *logits = part<float>(kept, r.logits);
     float2 *partial = part<float2>(workspace, r.partial);
-    const XentFewLogitsArgs l = {weight, p->weight_stride, p->vocab, (int)p->features, r.parts, scalars, part<char>(kept, r.by_feature),
-                                 logits, r.stride, partial};
-    if (r.entry_tiles == 4) xent_few_logits_kernel<T, NT, 4><<<dim3((unsigned)r.parts), dim3(kFewThreads), 0, s>>>(l);
-    else xent_few_logits_kernel<T, NT, 1><<<dim3((unsigned)r.parts), dim3(kFewThreads), 0, s>>>(l);
+    const XentFewLogitsArgs l = {weight, p->weight_stride, p->vocab, (int)p->features, r.parts, r.wide, scalars,
+                                 part<char>(kept, r.by_feature), logits, r.stride, partial};
+    if (r.wide > 0) xent_few_logits_kernel<T, NT><<<dim3((unsigned)r.parts), dim3(kFewThreads), 0, s>>>(l);
+    else xent_few_narrow_logits_kernel<T, NT><<<dim3((unsigned)r.parts), dim3(kFewThreads), 0, s>>>(l);
     float *losses = p->reduction == BF_XENT_NONE ? loss : part<float>(workspace, r.losses);
     const XentFewJoinArgs j = {partial, logits, r.stride, index, position, label, scalars, r.parts, part<float>(kept, r.lse), losses};
     xent_few_join_kernel<<<dim3((unsigned)p->rows), dim3(kFewThreads), 0, s>>>(j);

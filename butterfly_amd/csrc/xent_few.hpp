@@ -185,7 +185,7 @@ __global__ __launch_bounds__(kFewThreads) void xent_few_pack_kernel(XentFewPackA
 struct XentFewLogitsArgs {
     const void *weight;
     int64_t weight_stride, vocab;
-    int features, parts;
+    int features, parts, wide;      // parts: workgroups, the first `wide` of them of 64 entries
     const XentScalars *scalars;
     const char *by_feature;
     float *logits;                  // (rows by place, stride)
@@ -193,23 +193,25 @@ struct XentFewLogitsArgs {
     float2 *partial;                // (rows by place, parts): maximum, sum
 };
 
-// A workgroup takes 16 MT entries; its four wavefronts every fourth chunk of the features, and join their sums in LDS.
-// Eight lanes load a row's 128 bytes; the lanes that multiply them get them through the wavefront's own part of LDS
-// (unit u of row r at u ^ (r & 7), so that neither way meets its own banks; 6 rows, 3185 features, 32906 entries,
-// bfloat16 81 us, straight into those lanes, 16 bytes of 16 rows a load, 111).  The weights' bytes bound it: 60 x 4096 x
-// 65536 bfloat16 in 143 .. 162 us (3.3 .. 3.8 TB/s), 33 x 1843 x 67371 float in 193 .. 210 (2.4 .. 2.6; its split
-// and six products keep the other half of the time, two workgroups a compute unit no more).
-template <typename T, int NT, int MT>
-__global__ __launch_bounds__(kFewThreads, 2) void xent_few_logits_kernel(XentFewLogitsArgs a)
-{
-    using F = Few<T>;
-    __shared__ union {
+// LDS of a workgroup of 16 MT entries
+template <int NT, int MT>
+struct FewLds {
+    union {
         Quad staged[4][16 * MT][8];
         Acc4 sums[4][MT * NT][64];
-    } lds;
-    __shared__ float2 tops[MT][NT * 16];
+    };
+    float2 tops[MT][NT * 16];
+};
+
+// 16 MT entries from `first` on by a workgroup; its four wavefronts take every fourth chunk of the features, and join their sums in
+// LDS.  Eight lanes load a row's 128 bytes; the lanes that multiply them get them through the wavefront's own part of LDS
+// (unit u of row r at u ^ (r & 7), so that neither way meets its own banks; 6 rows, 3185 features, 32906 entries,
+// bfloat16 81 us, straight into those lanes, 16 bytes of 16 rows a load, 111).
+template <typename T, int NT, int MT>
+__device__ __forceinline__ void few_logits(const XentFewLogitsArgs &a, int64_t first, int part, FewLds<NT, MT> &lds)
+{
+    using F = Few<T>;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
-    const int64_t first = (int64_t)blockIdx.x * (16 * MT);
     const int counted = a.scalars->counted, full = a.features / F::kChunk;
     const T *row[2 * MT];
 #pragma unroll
@@ -310,14 +312,33 @@ __global__ __launch_bounds__(kFewThreads, 2) void xent_few_logits_kernel(XentFew
         for (int r = 0; r < 4; ++r) sum += __builtin_amdgcn_exp2f(fmaf(l[r], kLog2e, from));
         sum += __shfl_xor(sum, 16, 64);
         sum += __shfl_xor(sum, 32, 64);
-        if (lane < 16) tops[tile][place] = make_float2(top, sum * rounded_off(at, from));
+        if (lane < 16) lds.tops[tile][place] = make_float2(top, sum * rounded_off(at, from));
     }
     __syncthreads();
     if ((int)threadIdx.x >= counted) return;
     Joined all;
 #pragma unroll
-    for (int t = 0; t < MT; ++t) all.join(tops[t][threadIdx.x]);
-    a.partial[(int64_t)threadIdx.x * a.parts + blockIdx.x] = make_float2(all.top, all.sum);
+    for (int t = 0; t < MT; ++t) all.join(lds.tops[t][threadIdx.x]);
+    a.partial[(int64_t)threadIdx.x * a.parts + part] = make_float2(all.top, all.sum);
+}
+
+// Workgroups of 64 entries, and behind them of 16 entries for those that would not fill the chip once more.  The weights' bytes
+// bound it: 60 x 4096 x 65536 bfloat16 in 118 us (4.6 TB/s; without the narrow ones 162), 33 x 1843 x 67371 float in 171 (2.9
+// TB/s; without 210; its split and six products leave the loads two workgroups a compute unit).
+template <typename T, int NT>
+__global__ __launch_bounds__(kFewThreads, 2) void xent_few_logits_kernel(XentFewLogitsArgs a)
+{
+    __shared__ FewLds<NT, 4> lds;
+    const int id = blockIdx.x;
+    if (id < a.wide) few_logits<T, NT, 4>(a, (int64_t)id * 64, id, lds);
+    else few_logits<T, NT, 1>(a, (int64_t)a.wide * 64 + (int64_t)(id - a.wide) * 16, id, reinterpret_cast<FewLds<NT, 1> &>(lds));
+}
+
+template <typename T, int NT>
+__global__ __launch_bounds__(kFewThreads, 2) void xent_few_narrow_logits_kernel(XentFewLogitsArgs a)
+{
+    __shared__ FewLds<NT, 1> lds;
+    few_logits<T, NT, 1>(a, (int64_t)blockIdx.x * 16, blockIdx.x, lds);
 }
 
 struct XentFewJoinArgs {
