@@ -48,23 +48,24 @@ struct RecurrenceArgs {
     int *chunk_cut, *run_cut;           // the same by sequence: a reset inside
 };
 
-// V channels a lane, in registers as V accumulators; S steps a wavefront forward, SB backward.
+// V channels a lane, in registers as V accumulators; S steps a wavefront forward, SB backward, SR where runs are formed (so
+// that 64 registers do and two workgroups fit a compute unit).
 struct RecF32 {
     using Elem = float;
     using Acc = float;
-    static constexpr int V = 1, S = 8, SB = 8;
+    static constexpr int V = 1, S = 8, SB = 8, SR = 8;
     static constexpr bool kExact = true;
 };
 struct RecBF16 {
     using Elem = bf16;
     using Acc = float;
-    static constexpr int V = 2, S = 8, SB = 4;   // (eight steps of four tensors of two channels do not fit 128 registers)
+    static constexpr int V = 2, S = 8, SB = 4, SR = 4;   // (eight steps of four tensors of two channels do not fit 128 registers)
     static constexpr bool kExact = false;   // (the gates have eight bits)
 };
 struct RecC64 {
     using Elem = float2;
     using Acc = float2;
-    static constexpr int V = 1, S = 4, SB = 4;
+    static constexpr int V = 1, S = 4, SB = 4, SR = 4;
     static constexpr bool kExact = true;
 };
 
@@ -77,7 +78,7 @@ __device__ __forceinline__ bool is_zero(float2 v) { return v.x == 0.0f && v.y ==
 struct RecBF16One {
     using Elem = bf16;
     using Acc = float;
-    static constexpr int V = 1, S = 8, SB = 8;
+    static constexpr int V = 1, S = 8, SB = 8, SR = 8;
     static constexpr bool kExact = false;
 };
 
@@ -514,10 +515,10 @@ __global__ __launch_bounds__(64 * kRecWaves) void recurrence_bw_kernel(Recurrenc
 // instead of a launch between, the third launches took 123 and 193.
 
 template <typename Tr, bool SIG, bool BACKWARD>
-__global__ __launch_bounds__(64 * kRecWaves) void recurrence_runs_kernel(RecurrenceArgs p)
+__global__ __launch_bounds__(64 * kRecWaves, 8) void recurrence_runs_kernel(RecurrenceArgs p)
 {
     using A = typename Tr::Acc;
-    constexpr int V = Tr::V, S = Tr::S;
+    constexpr int V = Tr::V, S = Tr::SR;
     __shared__ Runs<Tr> runs;
     const RecPlace<Tr> at(p);
     if (at.chunk >= p.chunks) return;
