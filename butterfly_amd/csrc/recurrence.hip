@@ -36,9 +36,11 @@ struct RecurrencePlan {
 
 // Channels times batch make `groups * batch` workgroups.  A whole sequence is read once, at some 25 ns a step however few
 // of them there are; cut into chunks of 16 runs of whole blocks of S steps, until some 512 are at work, the gates
-// and inputs are read twice and two launches more are made.  Measured in float, forward and backward, whole and cut: 64
-// workgroups of 4096 steps 291 and 173 us, 96 315 and 293, 112 322 and 400; 64 of 512 steps 62 and 79, of 1024
-// 72 and 77, of 2048 132 and 91; 8 (bfloat16) of 16384 steps 1605 and 110.  So below 96 of more than four tiles.
+// and inputs are read twice and two launches more are made.  The chunks are a multiple of eight, one XCD's each in turn:
+// 88 workgroups of 4096 steps, float, forward and backward in 6 chunks 267 us, in 8 246.  Measured in float, forward and
+// backward, whole and cut: 72 workgroups of 4096 steps 301 and 209 us, 96 313 and 276, 104 320 and 325, 128 338 and 403;
+// 96 of 16384 1226 and 1119, 112 1251 and 1330; 64 of 512 62 and 79, 72 of 1024 71 and 68, 40 70 and 50.  In bfloat16 pairs
+// 112 of 4096 455 and 361; 8 of 16384 1605 and 110.  So below 100 (128) of more than four tiles.
 RecurrencePlan plan(const bf_recurrence *p)
 {
     RecurrencePlan r;
@@ -47,8 +49,8 @@ RecurrencePlan plan(const bf_recurrence *p)
     r.groups = (p->channels + 64 * v - 1) / (64 * v);
     const int64_t whole = r.groups * p->batch, tile = (int64_t)kRecWaves * s;
     r.chunk = std::max<int64_t>(p->steps, 1);
-    if (whole < 96 && p->steps > 4 * tile) {
-        const int64_t wanted = std::min<int64_t>((512 + whole - 1) / whole, (p->steps + tile - 1) / tile);
+    if (whole < (pairs ? 128 : 100) && p->steps > 4 * tile) {
+        const int64_t wanted = std::min<int64_t>(((512 + whole - 1) / whole + 7) / 8 * 8, (p->steps + tile - 1) / tile);
         r.chunk = std::max<int64_t>((p->steps / wanted + tile / 2) / tile, 1) * tile;
         r.chunks = (p->steps + r.chunk - 1) / r.chunk;
     }
