@@ -510,8 +510,10 @@ __global__ __launch_bounds__(64 * kRecWaves) void recurrence_bw_kernel(Recurrenc
 // grid (batch x groups, chunks), kRecWaves wavefronts, each with a run of its own: len = chunk / kRecWaves steps.  The first
 // launch forms every run's (A, B) as composed from the chunk's start (backward: end) up to the run, and the chunks';
 // the second one walks those from chunk to chunk; the third one starts each run from there, and the wavefronts need
-// nothing of each other.  65537 steps of 1000 channels, bfloat16: forward 79 + 10 + 74 us (3.3 TB/s, a chain of 65 chunks,
-// 5.3 TB/s), backward 73 + 10 + 167 (3.6 and 4.7 TB/s).  With every wavefront walking the chunks in front of its own,
+// nothing of each other.  65537 steps of 1000 channels, bfloat16: forward 70 + 10 + 75 us (3.7 TB/s, a chain of 65 chunks,
+// 5.2 TB/s), backward 66 + 11 + 167 (4.0 and 4.7 TB/s): memory bounds it, though a copy runs at 4.8.  The first launch's half of
+// the registers took 10 us off each direction; the third one in workgroups of four wavefronts, or the first one walking
+// against the third one's direction (for the caches), gained nothing.  With every wavefront walking the chunks in front of its own,
 // instead of a launch between, the third launches took 123 and 193.
 
 template <typename Tr, bool SIG, bool BACKWARD>

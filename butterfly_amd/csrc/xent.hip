@@ -81,7 +81,8 @@ unsigned workgroups(const Product &r)
     return (unsigned)std::min<int64_t>((int64_t)r.tiles_m * r.tiles_n * r.splits, r.large || r.deep ? 256 : 512);
 }
 
-constexpr size_t kPieceBytes = (size_t)256 << 20;   // d_l of a piece of the vocabulary
+// d_l of a piece of the vocabulary (8192 rows, 1024 features, 32768 entries, bfloat16: 128 MiB 2161 us, 256 2055, 512 2045)
+constexpr size_t kPieceBytes = (size_t)256 << 20;
 
 struct XentPlan {
     int64_t features_up = 0, rows_up = 0;       // padded to k steps, to tiles
