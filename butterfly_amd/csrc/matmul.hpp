@@ -54,85 +54,119 @@ struct MatOperand {
     int64_t bytes;         // of a plane from base on that may be read: loads beyond are zero
 };
 
-// lds_addr: where the wavefront's 64 units go (wave-uniform); offsets from the descriptor's base, within 2^31.
+// lds_addr: where the wavefront's 64 units go (wave-uniform); offset: from the descriptor's base, within 2^31, the sum of a
+// lane's and of the load's own.  The sum is in the lane's register when the load is made: what an instruction adds from a
+// scalar register itself takes no part in the range check.  It is formed in these lines, or the compiler keeps a register
+// for every load's.
 // (m0 is not saved: nothing else in these kernels uses it, and the compiler is told; its warning is that it
-// will not keep it for anybody either; with the move of m0 five wait states, which a descriptor or an offset needs that a
+// will not keep it for anybody either; with the move of m0 and the sum five wait states, which a descriptor needs that a
 // lane's read has just brought to scalar registers, and which the compiler does not count in front of these lines)
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"
-__device__ __forceinline__ void load_unit_to_lds(MatDesc desc, unsigned lds_addr, int voff, int soff)
+__device__ __forceinline__ void load_unit_to_lds(MatDesc desc, unsigned lds_addr, int lane_offset, int load_offset)
 {
-    asm volatile("s_mov_b32 m0, %0\n\t"
-                 "s_nop 3\n\t"
-                 "buffer_load_dwordx4 %1, %2, %3 offen lds"
-                 :
-                 : "s"(lds_addr), "v"(voff), "s"(desc), "s"(soff)
+    int offset;
+    asm volatile("s_mov_b32 m0, %1\n\t"
+                 "v_add_u32_e32 %0, %4, %2\n\t"
+                 "s_nop 2\n\t"
+                 "buffer_load_dwordx4 %0, %3, 0 offen lds"
+                 : "=&v"(offset)
+                 : "s"(lds_addr), "v"(lane_offset), "s"(desc), "s"(load_offset)
                  : "memory", "m0");
 }
 #pragma clang diagnostic pop
 
-// One operand's way into LDS: SIZE rows or columns of it, k step by k step.  From step to step only the lanes' offsets
-// move (a wavefront that is alone on its SIMD has few instructions to spare between MFMAs); the
-// descriptor's base moves every kSteps() steps, before they pass 2^30.
+// Where the loads of one operand read, SIZE rows or columns of it, k step by k step: numbers alone, which the host can go
+// through as well.  From step to step only the lanes' offsets move (a wavefront that is alone on its SIMD has few
+// instructions to spare between MFMAs); the base moves every steps() steps, before they pass 2^30.
 template <MatLayout LAYOUT, int SIZE, bool SPREAD, int WAVES>
-struct MatFeed {
+struct MatPath {
     static constexpr int kLoads = SIZE / 8 / WAVES;          // of a wavefront a step
     static constexpr int kUnits = SIZE / 8;                  // kCols: 16-byte units of a k row
     static constexpr int kPerLoad = LAYOUT == kRows ? 8 : 64 / kUnits;   // rows that a load covers
     static constexpr int kVariants = LAYOUT == kRows ? 1 : kLoads;
-    int stride, wave, first_voff[kVariants], voff[kVariants], soff[kLoads];
-    MatDesc desc;
+    int stride, first_offset[kVariants], lane_offset[kVariants], load_offset[kLoads];   // a load's: the same in all lanes
 
-    __device__ __forceinline__ void init(const MatOperand &o)
+    __host__ __device__ __forceinline__ void init(int64_t stride_, int wave, int lane)
     {
-        const int lane = threadIdx.x & 63;
-        wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-        stride = (int)o.stride;
+        stride = (int)stride_;
         if constexpr (LAYOUT == kRows) {
             // SPREAD: LDS row 16 t + i holds row 64 (t / 4) + 16 (i / 4) + 4 (t % 4) + i % 4, so that the
             // four rows a lane gets of each of four tiles' results are sixteen neighbours
             const int row = SPREAD ? (lane >> 5) * 16 + ((lane >> 3) & 3) : lane >> 3;
-            first_voff[0] = row * stride + ((lane & 7) ^ (lane >> 3)) * 16;
+            first_offset[0] = row * stride + ((lane & 7) ^ (lane >> 3)) * 16;
         } else {
-            const int row = lane / kUnits, unit = lane % kUnits;
+            const int row = lane / kUnits;
 #pragma unroll
             for (int j = 0; j < kLoads; ++j) {
                 const int r = (wave * kLoads + j) * kPerLoad + row, s = (r & 3) | ((r >> 3) & 1) << 2;
-                first_voff[j] = row * stride + (unit ^ s << 1) * 16;
+                first_offset[j] = row * stride + (lane % kUnits ^ s << 1) * 16;
             }
         }
 #pragma unroll
         for (int j = 0; j < kLoads; ++j) {
             const int jj = wave * kLoads + j;
-            soff[j] = (LAYOUT == kRows && SPREAD ? (jj >> 3) * 64 + (jj & 1) * 32 + ((jj >> 1) & 3) * 4 : jj * kPerLoad) * stride;
+            load_offset[j] = (LAYOUT == kRows && SPREAD ? (jj >> 3) * 64 + (jj & 1) * 32 + ((jj >> 1) & 3) * 4 : jj * kPerLoad) * stride;
         }
     }
 
     // steps that one base serves
-    __device__ __forceinline__ int steps() const { return LAYOUT == kRows ? 1 << 20 : max(1, (1 << 30) / (kMatK * stride) - 1); }
+    __host__ __device__ __forceinline__ int steps() const
+    {
+        const int n = LAYOUT == kRows ? 1 << 20 : (1 << 30) / (kMatK * stride) - 1;
+        return n > 1 ? n : 1;
+    }
 
-    // to k step `step`, SIZE rows or columns from `first` on; nothing: loads of zeros from there on
-    __device__ __forceinline__ void start(const MatOperand &o, int first, int64_t step, int plane, bool nothing)
+    // To k step `step`, SIZE rows or columns from `first` on: the base's distance from the operand's, and in `left` the
+    // bytes from there on that may be read (loads beyond are zeros; `nothing`: all of them).
+    __host__ __device__ __forceinline__ int64_t start(const MatOperand &o, int first, int64_t step, bool nothing, int &left)
     {
         const int64_t skip = LAYOUT == kRows ? first * o.stride + step * (kMatK * 2) : step * kMatK * o.stride + (int64_t)first * 2;
+        const int64_t rest = nothing ? 0 : o.bytes - skip;
+        left = (int)(rest < 0 ? 0 : rest < 0x7fffff00 ? rest : 0x7fffff00);
+#pragma unroll
+        for (int v = 0; v < kVariants; ++v) lane_offset[v] = first_offset[v];
+        return skip;
+    }
+    static constexpr __host__ __device__ int variant(int j) { return LAYOUT == kRows ? 0 : j; }
+    // of load j, as the range check sees it
+    __host__ __device__ __forceinline__ int offset(int j) const { return lane_offset[variant(j)] + load_offset[j]; }
+    __host__ __device__ __forceinline__ void advance()
+    {
+#pragma unroll
+        for (int v = 0; v < kVariants; ++v) lane_offset[v] += LAYOUT == kRows ? kMatK * 2 : kMatK * stride;
+    }
+};
+
+// One operand's way into LDS.
+template <MatLayout LAYOUT, int SIZE, bool SPREAD, int WAVES>
+struct MatFeed {
+    MatPath<LAYOUT, SIZE, SPREAD, WAVES> path;
+    int wave;
+    MatDesc desc;
+
+    __device__ __forceinline__ void init(const MatOperand &o)
+    {
+        wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        path.init(o.stride, wave, threadIdx.x & 63);
+    }
+    __device__ __forceinline__ int steps() const { return path.steps(); }
+    __device__ __forceinline__ void start(const MatOperand &o, int first, int64_t step, int plane, bool nothing)
+    {
+        int left;
+        const int64_t skip = path.start(o, first, step, nothing, left);
         const unsigned long long a = (unsigned long long)(o.base + plane * o.plane + skip);
-        const int64_t left = nothing ? 0 : o.bytes - skip;
         desc.x = __builtin_amdgcn_readfirstlane((int)(unsigned)a);
         desc.y = __builtin_amdgcn_readfirstlane((int)((a >> 32) & 0xffff));
-        desc.z = __builtin_amdgcn_readfirstlane((int)(left < 0 ? 0 : left < 0x7fffff00 ? left : 0x7fffff00));
+        desc.z = __builtin_amdgcn_readfirstlane(left);
         desc.w = 0x00020000;
-#pragma unroll
-        for (int v = 0; v < kVariants; ++v) voff[v] = first_voff[v];
     }
     __device__ __forceinline__ void load(unsigned lds, int j) const
     {
-        load_unit_to_lds(desc, lds + (wave * kLoads + j) * 1024, voff[LAYOUT == kRows ? 0 : j], soff[j]);
+        const unsigned to = lds + (wave * path.kLoads + j) * 1024;
+        load_unit_to_lds(desc, to, path.lane_offset[path.variant(j)], path.load_offset[j]);
     }
-    __device__ __forceinline__ void advance()
-    {
-#pragma unroll
-        for (int v = 0; v < kVariants; ++v) voff[v] += LAYOUT == kRows ? kMatK * 2 : kMatK * stride;
-    }
+    __device__ __forceinline__ void advance() { path.advance(); }
 };
 
 // One operand's way out of LDS: the wavefront's 16-wide tiles of a half step (32 k's).
