@@ -473,6 +473,14 @@ int bf_linear_xent_bw(const bf_linear_xent *p, const void *weight, const float *
     if (!weight || (!grad && (p->rows > 0 || p->reduction != BF_XENT_NONE))) return fail(BF_ERR_INVALID, "weight or grad is NULL");
     if (!d_hidden && !d_weight) return BF_OK;
     hipStream_t s = static_cast<hipStream_t>(stream);
+    if (p->rows == 0) {   // (the forward call has left nothing in `kept`)
+        const int64_t count = p->vocab * p->features;
+        const dim3 grid((unsigned)std::min<int64_t>((count + 255) / 256, 8192));
+        if (d_weight && p->dtype == BF_F32) xent_zero_kernel<<<grid, dim3(256), 0, s>>>(static_cast<float *>(d_weight), count);
+        else if (d_weight) xent_zero_kernel<<<grid, dim3(256), 0, s>>>(static_cast<bf16 *>(d_weight), count);
+        BF_HIP_CHECK(hipGetLastError());
+        return BF_OK;
+    }
     if (few_rows(p)) {
         const XentFewPlan r = few_plan(p, true);
         if ((rc = check_memory(r, weight, kept, kept_bytes, workspace, workspace_bytes))) return rc;
@@ -488,7 +496,7 @@ int bf_linear_xent_bw(const bf_linear_xent *p, const void *weight, const float *
     operands(p, r, weight, kept, h, w);
     XentScalars *scalars = part<XentScalars>(kept, r.scalars);
     const XentGrad gradient = {grad, p->reduction == BF_XENT_NONE, p->reduction == BF_XENT_MEAN};
-    if (gradient.each && p->rows > 0)
+    if (gradient.each)
         xent_share_kernel<<<dim3(1), dim3(kXentThreads), 0, s>>>(gradient, part<int>(kept, r.index), scalars,
                                                                  part<float>(workspace, r.share));
     const size_t elem = p->dtype == BF_F32 ? 4 : 2;
@@ -519,11 +527,9 @@ int bf_linear_xent_bw(const bf_linear_xent *p, const void *weight, const float *
         a.d_l = d_l;
         a.stride = d_l_stride;
         a.plane = (int64_t)r.d_l_plane;
-        if (p->rows > 0) {
-            if (p->dtype == BF_F32) launch_logits<true, true>(logits, a, s);
-            else launch_logits<false, true>(logits, a, s);
-        }
-        if (d_hidden && p->rows > 0) {
+        if (p->dtype == BF_F32) launch_logits<true, true>(logits, a, s);
+        else launch_logits<false, true>(logits, a, s);
+        if (d_hidden) {
             XentGradArgs g = {};
             g.a = wp;
             g.b = d_l_operand;
@@ -561,7 +567,7 @@ int bf_linear_xent_bw(const bf_linear_xent *p, const void *weight, const float *
                 gather(p, {g.partial, nullptr, scalars, gradient, out, entries, entries, p->features, g.splits, 1}, s);
         }
     }
-    if (d_hidden && p->rows > 0)
+    if (d_hidden)
         gather(p, {part<float>(workspace, r.sums_hidden), part<int>(kept, r.position), scalars, gradient, d_hidden, p->rows, p->rows,
                    p->features, r.to_hidden.splits, 0}, s);
     BF_HIP_CHECK(hipGetLastError());

@@ -576,6 +576,13 @@ __global__ __launch_bounds__(mat_threads(BM, BN, BUFFERS), 1) void xent_grad_ker
     Tile::end();
 }
 
+// d_weight of no rows at all
+template <typename T>
+__global__ __launch_bounds__(256) void xent_zero_kernel(T *out, int64_t count)
+{
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < count; i += (int64_t)gridDim.x * 256) out[i] = (T)0.0f;
+}
+
 struct XentGatherArgs {
     const float *partial;       // (splits, n, m)
     const int *position;        // rows of the result come from these places (-1: zeros); NULL: as they are

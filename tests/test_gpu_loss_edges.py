@@ -19,3 +19,16 @@ def test_what_lies_behind_the_weight_reaches_nothing(rows, features, vocab, dtyp
     tall[:vocab] = weight
     for a, b in zip(check(hidden, tall[:vocab], target), check(hidden, weight, target)):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("reduction", ["none", "mean", "sum"])
+def test_no_rows_give_the_weight_no_gradient(reduction, dtype):
+    hidden, weight, target = make(0, 40, 777, dtype)
+    # (memory that the operators take next is not zero)
+    used = [torch.full((1 << k,), float("nan"), device="cuda") for k in range(8, 22)]
+    del used
+    h, w = hidden.requires_grad_(), weight.requires_grad_()
+    loss = tb.linear_cross_entropy(h, w, target, reduction=reduction)
+    dh, dw = torch.autograd.grad(loss, (h, w), torch.ones_like(loss))
+    assert dh.shape == (0, 40) and torch.equal(dw, torch.zeros_like(weight))
