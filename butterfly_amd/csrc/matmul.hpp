@@ -52,7 +52,10 @@ struct MatOperand {
     int64_t plane;         // bytes between planes
     int64_t stride;        // bytes between rows
     int64_t bytes;         // of a plane from base on that may be read: loads beyond are zero
+    int tail;              // kRows: bytes of a row's last k step that are the row's (multiples of 16): what is behind, to 128, is zero
 };
+
+constexpr int kWholeTail = kMatK * 2;
 
 // lds_addr: where the wavefront's 64 units go (wave-uniform); offset: from the descriptor's base, within 2^31, the sum of a
 // lane's and of the load's own.  The sum is in the lane's register when the load is made: what an instruction adds from a
@@ -128,6 +131,15 @@ struct MatPath {
         for (int v = 0; v < kVariants; ++v) lane_offset[v] = first_offset[v];
         return skip;
     }
+    // In front of a row's last k step: the lanes whose unit lies behind the row's end read nothing (in rows that lie as a
+    // caller has them there may be anything, NaN too, which the other operand's zeros would not undo).
+    __host__ __device__ __forceinline__ void cut(const MatOperand &o, int lane)
+    {
+        if constexpr (LAYOUT == kRows) {
+            if (((lane & 7) ^ (lane >> 3)) * 16 >= o.tail) lane_offset[0] = kRefused;
+        }
+    }
+    static constexpr int kRefused = (int)0x80000000u;   // (as the range check takes it: behind everything, with a load's own offset too)
     static constexpr __host__ __device__ int variant(int j) { return LAYOUT == kRows ? 0 : j; }
     // of load j, as the range check sees it
     __host__ __device__ __forceinline__ int offset(int j) const { return lane_offset[variant(j)] + load_offset[j]; }
@@ -167,6 +179,10 @@ struct MatFeed {
         load_unit_to_lds(desc, to, path.lane_offset[path.variant(j)], path.load_offset[j]);
     }
     __device__ __forceinline__ void advance() { path.advance(); }
+    __device__ __forceinline__ void cut(const MatOperand &o)
+    {
+        if (LAYOUT == kRows && o.tail < kWholeTail) path.cut(o, threadIdx.x & 63);
+    }
 };
 
 // One operand's way out of LDS: the wavefront's 16-wide tiles of a half step (32 k's).
@@ -296,7 +312,10 @@ struct MatTiles {
             feed_b.start(b, n0, first + (nothing ? 0 : fed), F16 && pass == 0, nothing);
             until = min(count - fed, min(feed_a.steps(), feed_b.steps())) + fed;
         }
-        ++fed;
+        if (++fed == count) {
+            feed_a.cut(a);
+            feed_b.cut(b);
+        }
     }
     __device__ __forceinline__ void feed_load(unsigned to, int i)
     {

@@ -259,11 +259,12 @@ void operands(const bf_linear_xent *p, const XentPlan &r, const void *weight, vo
 {
     char *hp = part<char>(kept, r.hidden), *wp = part<char>(kept, r.weight);
     const int64_t stride = r.features_up * 2;
-    h = {hp, (int64_t)r.hidden_plane, stride, r.rows_up * stride};
+    h = {hp, (int64_t)r.hidden_plane, stride, r.rows_up * stride, kWholeTail};
     if (weight_in_place(p))
-        w = {static_cast<const char *>(weight), 0, p->weight_stride * 2, ((p->vocab - 1) * p->weight_stride + p->features) * 2};
+        w = {static_cast<const char *>(weight), 0, p->weight_stride * 2, ((p->vocab - 1) * p->weight_stride + p->features) * 2,
+             p->features % kMatK ? (int)(p->features % kMatK) * 2 : kWholeTail};
     else
-        w = {wp, (int64_t)r.weight_plane, stride, p->vocab * stride};
+        w = {wp, (int64_t)r.weight_plane, stride, p->vocab * stride, kWholeTail};
 }
 
 // The counted rows, and both operands in that form, for both directions.
@@ -502,7 +503,7 @@ int bf_linear_xent_bw(const bf_linear_xent *p, const void *weight, const float *
     const size_t elem = p->dtype == BF_F32 ? 4 : 2;
     char *d_l = part<char>(workspace, r.d_l);
     const int64_t d_l_stride = r.piece * 2;
-    const MatOperand d_l_operand = {d_l, (int64_t)r.d_l_plane, d_l_stride, r.rows_up * d_l_stride};
+    const MatOperand d_l_operand = {d_l, (int64_t)r.d_l_plane, d_l_stride, r.rows_up * d_l_stride, kWholeTail};
     for (int64_t first = 0; first < p->vocab; first += r.piece) {
         const int64_t entries = std::min<int64_t>(r.piece, p->vocab - first);
         MatOperand wp = w;

@@ -1,6 +1,6 @@
 // Where the loads of the loss's matrix products read (MatPath), gone through on the host for every tile size and layout: each
 // load lies inside its operand or is refused by the range check, which sees a lane's register and nothing else, and
-// what is inside arrives once.
+// what is inside arrives once; of rows that lie as a caller has them nothing behind a row's end is read.
 #include "../../butterfly_amd/csrc/matmul.hpp"
 
 #include <cstdio>
@@ -22,7 +22,7 @@ template <MatLayout LAYOUT, int SIZE, bool SPREAD, int WAVES>
 static void walk(int64_t rows, int64_t cols, int64_t stride)
 {
     using Path = MatPath<LAYOUT, SIZE, SPREAD, WAVES>;
-    MatOperand o = {nullptr, 0, stride * 2, ((rows - 1) * stride + cols) * 2};
+    MatOperand o = {nullptr, 0, stride * 2, ((rows - 1) * stride + cols) * 2, cols % kMatK ? (int)(cols % kMatK) * 2 : kWholeTail};
     // the row and 16-byte unit of its tile that a load brings, from rows that are far apart
     constexpr int per = LAYOUT == kRows ? 8 : SIZE / 8, far = 1 << 21;
     std::vector<int> place(64 * WAVES * Path::kLoads);
@@ -30,7 +30,7 @@ static void walk(int64_t rows, int64_t cols, int64_t stride)
         Path p;
         int all;
         p.init(far, t / 64, t % 64);
-        p.start({nullptr, 0, far, (int64_t)1 << 40}, 0, 0, false, all);
+        p.start({nullptr, 0, far, (int64_t)1 << 40, kWholeTail}, 0, 0, false, all);
         for (int j = 0; j < Path::kLoads; ++j) place[t * Path::kLoads + j] = p.offset(j) / far * per + p.offset(j) % far / 16;
     }
     const int64_t m = LAYOUT == kRows ? rows : cols, k = LAYOUT == kRows ? cols : rows, steps = (k + kMatK - 1) / kMatK;
@@ -47,18 +47,22 @@ static void walk(int64_t rows, int64_t cols, int64_t stride)
                 }
                 for (int64_t step = from; step < steps + 2; ++step) {
                     std::vector<int> seen(SIZE * 8);
+                    if (step == steps - 1)
+                        for (int t = 0; t < 64 * WAVES; ++t) lanes[t].cut(o, t % 64);
                     for (int t = 0; t < 64 * WAVES; ++t) {
                         for (int j = 0; j < Path::kLoads; ++j) {
                             const int64_t sum = (int64_t)lanes[t].lane_offset[Path::variant(j)] + lanes[t].load_offset[j];
                             const int at = lanes[t].offset(j);
-                            if (sum != at || at < 0) fail("offset", SIZE, WAVES, rows, cols, stride, first, step);
-                            if (at + 16 > left[t]) continue;   // refused: zeros
+                            const bool cut = lanes[t].lane_offset[Path::variant(j)] < 0;
+                            if (sum != at || (at < 0 && !cut)) fail("offset", SIZE, WAVES, rows, cols, stride, first, step);
+                            if ((unsigned)at + 16 > (unsigned)left[t]) continue;   // refused: zeros
                             const int64_t byte = skip + at;
                             if (nothing || byte < 0 || byte + 16 > o.bytes) fail("outside", SIZE, WAVES, rows, cols, stride, first, step);
                             const int i = place[t * Path::kLoads + j];
                             const int64_t row = i / per + (LAYOUT == kRows ? first : step * kMatK);
                             const int64_t unit = i % per + (LAYOUT == kRows ? step * 8 : first / 8);
                             if (byte != row * o.stride + unit * 16) fail("elsewhere", SIZE, WAVES, rows, cols, stride, first, step);
+                            if (LAYOUT == kRows && step < steps && unit * 8 >= cols) fail("behind a row", SIZE, WAVES, rows, cols, stride, first, step);
                             ++seen[i];
                         }
                         lanes[t].advance();

@@ -32,3 +32,27 @@ def test_no_rows_give_the_weight_no_gradient(reduction, dtype):
     loss = tb.linear_cross_entropy(h, w, target, reduction=reduction)
     dh, dw = torch.autograd.grad(loss, (h, w), torch.ones_like(loss))
     assert dh.shape == (0, 40) and torch.equal(dw, torch.zeros_like(weight))
+
+
+@pytest.mark.parametrize("gap", [8, 24, 64])
+@pytest.mark.parametrize("rows,features,vocab", [(70, 40, 1000), (300, 200, 515), (2048, 72, 16390), (3000, 1000, 4100)])
+def test_what_lies_between_the_weights_rows_reaches_nothing(rows, features, vocab, gap):
+    """bfloat16 rows that 16 bytes divide are read where they lie, by steps of 64 features that end inside the gap."""
+    hidden, weight, target = make(rows, features, vocab, torch.bfloat16)
+    wide = torch.full((vocab, features + gap), float("nan"), dtype=torch.bfloat16, device="cuda")
+    wide[:, :features] = weight
+    for a, b in zip(check(hidden, wide[:, :features], target), check(hidden, weight, target)):
+        assert torch.equal(a, b)
+
+
+def test_an_entry_of_no_probability_spoils_no_other_entry():
+    """Weight rows with an entry of minus infinity give a logit of minus infinity (positive hidden features): nothing of
+    them may reach the entry in front, whose last k step ends where they begin."""
+    hidden, weight, target = make(80, 72, 500, torch.bfloat16)
+    hidden = hidden.abs() + 0.125
+    target = target.masked_fill(target == 7, 8)
+    weight[7, 3] = float("-inf")
+    loss = tb.linear_cross_entropy(hidden, weight, target, reduction="none")
+    logits = hidden.double() @ weight.double().t()
+    want = torch.nn.functional.cross_entropy(logits, target, reduction="none")
+    assert (loss.double() - want).abs().max() < 1e-5 * (1 + want.abs().max())
