@@ -4,7 +4,7 @@ import pytest
 import torch
 
 import butterfly_amd as tb
-from test_gpu_linear_cross_entropy import DTYPES, check, make
+from test_gpu_linear_cross_entropy import DTYPES, TOL, check, err, make, reference
 
 pytestmark = pytest.mark.gpu
 
@@ -56,3 +56,23 @@ def test_an_entry_of_no_probability_spoils_no_other_entry():
     logits = hidden.double() @ weight.double().t()
     want = torch.nn.functional.cross_entropy(logits, target, reduction="none")
     assert (loss.double() - want).abs().max() < 1e-5 * (1 + want.abs().max())
+
+
+@pytest.mark.parametrize("up", [1e-6, 1e-3, 1.0, 1e5])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows", [40, 90, 700])
+def test_a_row_that_is_not_finite_spoils_no_other(rows, dtype, up):
+    """Losses and hidden gradients of the other rows; every row of the weight's gradient sums over all of them."""
+    hidden, weight, target = make(rows, 64, 1000, dtype, ignored=0.0)
+    hidden, weight = hidden * up, weight / up
+    good = torch.ones(rows, dtype=torch.bool, device="cuda")
+    good[[3, 11, rows - 1]] = False
+    h, w = hidden.clone(), weight.requires_grad_()
+    h[3, 5], h[11, 0], h[rows - 1, 63] = float("nan"), float("inf"), float("-inf")
+    h.requires_grad_()
+    each = tb.linear_cross_entropy(h, w, target, reduction="none")
+    dh, dw = torch.autograd.grad(each, (h, w), torch.ones_like(each))
+    want, want_h, _ = reference(hidden[good], weight, target[good], torch.ones(int(good.sum()), device="cuda"), "none")
+    assert (each[good].double() - want).abs().max() <= 1e-5 * (1 + want.abs().max())
+    assert err(dh[good], want_h) < TOL[dtype]
+    assert not torch.isfinite(each[~good]).any() and not torch.isfinite(dh[~good]).any() and not torch.isfinite(dw).any()
