@@ -458,20 +458,24 @@ __global__ __launch_bounds__(kXentThreads) void xent_total_kernel(const float *l
 }
 
 // ---- backward: what the rows' d_l are multiplied by ---------------------------------------------------------------
-// g_i = scale share_i.  One gradient for all: shares of one.  One a row: scale is the largest |g_i|.
+// g_i = scale share_i.  One gradient for all: shares of one.  One a row: scale is the largest finite |g_i| (one that is not
+// finite stays its row's own).
 __global__ __launch_bounds__(kXentThreads) void xent_share_kernel(XentGrad g, const int *index, XentScalars *scalars, float *share)
 {
     __shared__ float sums[kXentThreads / 64];
     const int n = scalars->counted;
     float most = 0.0f;
-    for (int i = threadIdx.x; i < n; i += kXentThreads) most = fmaxf(most, fabsf(g.grad[index[i]]));
+    for (int i = threadIdx.x; i < n; i += kXentThreads) {
+        const float v = fabsf(g.grad[index[i]]);
+        most = v < INFINITY ? fmaxf(most, v) : most;
+    }
 #pragma unroll
     for (int d = 1; d < 64; d *= 2) most = fmaxf(most, __shfl_xor(most, d, 64));
     if ((threadIdx.x & 63) == 0) sums[threadIdx.x >> 6] = most;
     __syncthreads();
     for (int w = 0; w < kXentThreads / 64; ++w) most = fmaxf(most, sums[w]);
     if (threadIdx.x == 0) scalars->grad_scale = most;
-    // (all zero: the numbers themselves, zeros and NaN)
+    // (none but zeros: the numbers themselves)
     for (int i = threadIdx.x; i < n; i += kXentThreads) share[i] = most == 0.0f ? g.grad[index[i]] : g.grad[index[i]] / most;
 }
 

@@ -76,3 +76,22 @@ def test_a_row_that_is_not_finite_spoils_no_other(rows, dtype, up):
     assert (each[good].double() - want).abs().max() <= 1e-5 * (1 + want.abs().max())
     assert err(dh[good], want_h) < TOL[dtype]
     assert not torch.isfinite(each[~good]).any() and not torch.isfinite(dh[~good]).any() and not torch.isfinite(dw).any()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows", [40, 90, 700])
+def test_a_rows_gradient_that_is_not_finite_spoils_no_other_row(rows, dtype):
+    hidden, weight, target = make(rows, 64, 1000, dtype, ignored=0.0)
+    good = torch.ones(rows, dtype=torch.bool, device="cuda")
+    good[[3, 11, rows - 1]] = False
+    g = torch.linspace(0.5, 2.0, rows, device="cuda")
+    _, want_h, _ = reference(hidden, weight, target, g, "none")
+    g[3], g[11], g[rows - 1] = float("nan"), float("inf"), float("-inf")
+    h, w = hidden.requires_grad_(), weight.requires_grad_()
+    dh, dw = torch.autograd.grad(tb.linear_cross_entropy(h, w, target, reduction="none"), (h, w), g)
+    assert err(dh[good], want_h[good]) < TOL[dtype]
+    assert not torch.isfinite(dh[~good]).any() and not torch.isfinite(dw).any()
+    # nothing but zeros beside it
+    g[good] = 0.0
+    dh, = torch.autograd.grad(tb.linear_cross_entropy(h, w, target, reduction="none"), h, g)
+    assert (dh[good] == 0).all() and not torch.isfinite(dh[~good]).any()
