@@ -95,7 +95,7 @@ struct XentPlan {
     // offsets into what the forward call leaves for the backward one, and into the workspaces
     size_t scalars = 0, index = 0, position = 0, label = 0, lse = 0, hidden = 0, weight = 0, kept = 0;
     size_t picked = 0, losses = 0, partial = 0;
-    size_t share = 0, d_l = 0, d_l_plane = 0, sums_hidden = 0, sums_weight = 0;
+    size_t share = 0, shared = 0, d_l = 0, d_l_plane = 0, sums_hidden = 0, sums_weight = 0;
     size_t total = 0;
 };
 
@@ -138,6 +138,7 @@ XentPlan plan(const bf_linear_xent *p, bool backward)
         r.to_hidden = product(p->features, p->rows, r.piece / kMatK, passes, true);
         r.to_weight = product(p->features, r.piece, (p->rows + kMatK - 1) / kMatK, passes, true);
         r.share = take(rows * 4);
+        if (p->dtype == BF_F32 && p->reduction == BF_XENT_NONE) r.shared = take(r.hidden_plane * r.planes);
         r.d_l_plane = up256((size_t)r.rows_up * r.piece * 2);
         r.d_l = take(r.d_l_plane * r.planes);
         r.sums_hidden = take((size_t)r.to_hidden.splits * rows * p->features * sizeof(float));
@@ -380,7 +381,8 @@ void few_bw(const bf_linear_xent *p, const XentFewPlan &r, const void *weight, c
     const int blocks_weight = d_weight ? (r.columns * r.splits_weight + 3) / 4 : 0;
     xent_few_grad_kernel<T, NT><<<dim3((unsigned)(g.blocks_hidden + blocks_weight)), dim3(kFewThreads), 0, s>>>(g);
     if (!d_hidden) return;
-    gather_runs<T, false>({g.partial, part<int>(kept, r.position), scalars, gradient, d_hidden, p->rows, p->rows, p->features, r.splits_hidden, 0}, s);
+    gather_runs<T, false>({g.partial, part<int>(kept, r.position), scalars, gradient, d_hidden, p->rows, p->rows, p->features, r.splits_hidden, 0,
+                           nullptr}, s);
 }
 
 // f(the type, tiles of rows) of a call
@@ -500,6 +502,13 @@ int bf_linear_xent_bw(const bf_linear_xent *p, const void *weight, const float *
     if (gradient.each)
         xent_share_kernel<<<dim3(1), dim3(kXentThreads), 0, s>>>(gradient, part<int>(kept, r.index), scalars,
                                                                  part<float>(workspace, r.share));
+    const bool shared = gradient.each && p->dtype == BF_F32;
+    MatOperand rows = h;   // hidden as d_weight's product takes it
+    if (shared && d_weight) {
+        rows.base = part<char>(workspace, r.shared);
+        const XentSharedArgs a = {h.base, part<char>(workspace, r.shared), r.rows_up, h.stride, h.plane, part<float>(workspace, r.share), scalars};
+        xent_shared_kernel<<<dim3((unsigned)std::min<int64_t>((r.rows_up * (h.stride / 16) + 255) / 256, 8192)), dim3(256), 0, s>>>(a);
+    }
     const size_t elem = p->dtype == BF_F32 ? 4 : 2;
     char *d_l = part<char>(workspace, r.d_l);
     const int64_t d_l_stride = r.piece * 2;
@@ -551,7 +560,7 @@ int bf_linear_xent_bw(const bf_linear_xent *p, const void *weight, const float *
             Product to_weight = r.to_weight;
             const int64_t t = to_weight.large ? 256 : 128;
             to_weight.tiles_n = (int)((entries + t - 1) / t);
-            g.a = h;
+            g.a = rows;
             g.b = d_l_operand;
             g.scalars = scalars;
             g.grad = gradient;
@@ -565,12 +574,12 @@ int bf_linear_xent_bw(const bf_linear_xent *p, const void *weight, const float *
             else g.out = out;
             launch_grad<kCols>(p, to_weight, g, s);
             if (g.splits > 1)
-                gather(p, {g.partial, nullptr, scalars, gradient, out, entries, entries, p->features, g.splits, 1}, s);
+                gather(p, {g.partial, nullptr, scalars, gradient, out, entries, entries, p->features, g.splits, 1, nullptr}, s);
         }
     }
     if (d_hidden)
         gather(p, {part<float>(workspace, r.sums_hidden), part<int>(kept, r.position), scalars, gradient, d_hidden, p->rows, p->rows,
-                   p->features, r.to_hidden.splits, 0}, s);
+                   p->features, r.to_hidden.splits, 0, shared ? grad : nullptr}, s);
     BF_HIP_CHECK(hipGetLastError());
     return BF_OK;
 }

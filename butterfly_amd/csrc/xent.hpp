@@ -20,9 +20,11 @@
 // Number formats.  bfloat16 operands multiply as they are; d_l is rounded to bfloat16 (2^-9), like every gradient
 // of such a model.  float operands are split, x 2^e = hi + lo in two float16 numbers of together 22 bits,
 // e the power of two that brings the operand's largest number to 2^14 .. 2^15 (one for hidden, one for
-// weight; d_l is at most one times the largest g, e = 15), and a product is hi lo + lo hi + hi hi with sums in float: three
+// weight; d_l is at most one, e = 15), and a product is hi lo + lo hi + hi hi with sums in float: three
 // products at the 16-bit rate, 16 times that of float ones on this card, for a relative error of 2^-22 a factor, as long as
-// numbers are within 2^-17 of the largest (below that an absolute error of 2^-39 of it).
+// numbers are within 2^-17 of the largest (below that an absolute error of 2^-39 of it).  With one gradient a row d_l is
+// without it in float (rows of small ones would lose their bits): d_hidden's rows are multiplied at the end, and d_weight's
+// product takes hidden's rows times their share of the largest.
 #pragma once
 
 #include "matmul.hpp"
@@ -226,7 +228,7 @@ struct XentTileArgs {
     float2 *partial;            // (2 tiles_m, rows): maximum, sum
     float *picked;
     // backward
-    const float *lse, *share;   // by place; share NULL: ones
+    const float *lse, *share;   // by place; share NULL: ones; float: only whether it is zero
     char *d_l;                  // (rows, stride bytes), in F16 two planes
     int64_t stride, plane;
 };
@@ -353,7 +355,7 @@ __global__ __launch_bounds__(mat_threads(BM, BN, BUFFERS), 1) void xent_logits_k
                         for (int r = 0; r < 4; ++r)
                             if (mw + Tile::tile_row(i) + r >= a.vocab) acc[i][j][r] = 0.0f;
                 }
-                const float factor = share * exact * (F16 ? 32768.0f : 1.0f);
+                const float factor = F16 ? share != 0.0f ? 32768.0f * exact : 0.0f : share * exact;
                 char *out = a.d_l + (int64_t)row * a.stride + (mw + Tile::tile_row(0)) * 2;
                 // sixteen neighbouring entries from four tiles
 #pragma unroll
@@ -479,6 +481,34 @@ __global__ __launch_bounds__(kXentThreads) void xent_share_kernel(XentGrad g, co
     for (int i = threadIdx.x; i < n; i += kXentThreads) share[i] = most == 0.0f ? g.grad[index[i]] : g.grad[index[i]] / most;
 }
 
+// Hidden's two planes times the rows' shares, zeros behind the counted rows (float).
+struct XentSharedArgs {
+    const char *hidden;
+    char *out;
+    int64_t rows, stride, plane;
+    const float *share;
+    const XentScalars *scalars;
+};
+
+__global__ __launch_bounds__(256) void xent_shared_kernel(XentSharedArgs a)
+{
+    const int units = (int)(a.stride / 16), counted = a.scalars->counted;
+    const int64_t total = a.rows * units;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+        const int64_t r = i / units, at = i * 16;
+        uint32_t w[4] = {}, low[4] = {};
+        if (r < counted) {
+            const float share = a.share[r];
+            const f16x8 h = *reinterpret_cast<const f16x8 *>(a.hidden + at), l = *reinterpret_cast<const f16x8 *>(a.hidden + a.plane + at);
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                split_f16(((float)h[2 * k] + (float)l[2 * k]) * share, ((float)h[2 * k + 1] + (float)l[2 * k + 1]) * share, w[k], low[k]);
+        }
+        *reinterpret_cast<uint4 *>(a.out + at) = make_uint4(w[0], w[1], w[2], w[3]);
+        *reinterpret_cast<uint4 *>(a.out + a.plane + at) = make_uint4(low[0], low[1], low[2], low[3]);
+    }
+}
+
 // ---- backward: the gradients' products -----------------------------------------------------------------------------
 
 struct XentGradArgs {
@@ -595,6 +625,7 @@ struct XentGatherArgs {
     void *out;
     int64_t rows, n, m;         // rows of the result, of a split
     int splits, of_weight;
+    const float *row_grad;      // what each row of the result is multiplied by instead of grad's; NULL: nothing
 };
 
 // The splits' sums in ascending order, scaled and rounded once: eight neighbours a thread.  Memory bounds it: 8 splits of
@@ -603,7 +634,7 @@ template <typename T>
 __global__ __launch_bounds__(256) void xent_gather_kernel(XentGatherArgs a)
 {
     constexpr bool F16 = sizeof(T) == 4;
-    float scale = a.grad.scale(a.scalars);
+    float scale = a.row_grad ? 1.0f : a.grad.scale(a.scalars);
     if constexpr (F16) scale *= 1.0f / 32768.0f / (a.of_weight ? a.scalars->hidden_scale : a.scalars->weight_scale);
     const int splits = a.of_weight ? xent_splits(a.splits, (a.scalars->counted + kMatK - 1) / kMatK) : a.splits;
     const int m = (int)a.m, units = (m + 7) / 8;
@@ -619,8 +650,9 @@ __global__ __launch_bounds__(256) void xent_gather_kernel(XentGatherArgs a)
 #pragma unroll
                 for (int k = 0; k < 8; ++k) s[k] += v[k];
             }
+            const float row_grad = a.row_grad ? a.row_grad[row] : 1.0f;
 #pragma unroll
-            for (int k = 0; k < 8; ++k) s[k] *= scale;
+            for (int k = 0; k < 8; ++k) s[k] = s[k] * scale * row_grad;
         }
         store8(reinterpret_cast<T *>(a.out) + row * m, col, m, s);
     }
@@ -655,9 +687,9 @@ __global__ __launch_bounds__(1024) void xent_gather_runs_kernel(XentGatherArgs a
         if (run != 0 || col >= m) continue;
 #pragma unroll 4
         for (int k = 1; k < 32; ++k) s += lds[k][threadIdx.x];
-        float scale = a.grad.scale(a.scalars);
+        float scale = a.row_grad ? 1.0f : a.grad.scale(a.scalars);
         if constexpr (SCALED) scale *= 1.0f / 32768.0f / a.scalars->weight_scale;
-        s = s * scale;
+        s = s * scale * (a.row_grad ? a.row_grad[row] : 1.0f);
         T *out = reinterpret_cast<T *>(a.out) + row * m + col;
 #pragma unroll
         for (int c = 0; c < 4; ++c)

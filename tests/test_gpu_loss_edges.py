@@ -95,3 +95,18 @@ def test_a_rows_gradient_that_is_not_finite_spoils_no_other_row(rows, dtype):
     g[good] = 0.0
     dh, = torch.autograd.grad(tb.linear_cross_entropy(h, w, target, reduction="none"), h, g)
     assert (dh[good] == 0).all() and not torch.isfinite(dh[~good]).any()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,vocab", [(50, 1000), (300, 1000), (700, 9000)])
+def test_every_row_keeps_its_bits_whatever_the_others_gradients(rows, vocab, dtype):
+    """A row of d_hidden is g (sum_v p_v W_v - W_t): off by the tolerance times g and the largest weight, its own g, be it
+    10^-30 of the largest."""
+    hidden, weight, target = make(rows, 64, vocab, dtype)
+    h, w = hidden.requires_grad_(), weight.requires_grad_()
+    g = torch.logspace(-30, 0, rows, device="cuda")[torch.randperm(rows, generator=torch.Generator().manual_seed(1)).cuda()]
+    g[5] = 0.0
+    dh, dw = torch.autograd.grad(tb.linear_cross_entropy(h, w, target, reduction="none"), (h, w), g)
+    _, want_h, want_w = reference(h, w, target, g, "none")
+    off = (dh.double() - want_h).abs().amax(1) / (g.double() * float(w.detach().abs().max())).clamp(min=1e-300)
+    assert off.max() < TOL[dtype] and (dh[5] == 0).all() and err(dw, want_w) < TOL[dtype]
