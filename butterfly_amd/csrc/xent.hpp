@@ -266,8 +266,8 @@ __global__ __launch_bounds__(mat_threads(BM, BN, BUFFERS), 1) void xent_logits_k
     const int counted = a.scalars->counted;
     const int tiles_n = (counted + BN - 1) / BN, total = a.tiles_m * tiles_n;
     const int lane = threadIdx.x & 63, part = Tile::wave_m();
-    // (powers of two, each within the range of float)
-    const float scale_h = F16 ? 1.0f / a.scalars->hidden_scale : 1.0f, scale_w = F16 ? 1.0f / a.scalars->weight_scale : 1.0f;
+    // (powers of two, each within the range of float, and their product where the logits are)
+    const float scale = F16 ? 1.0f / a.scalars->hidden_scale * (1.0f / a.scalars->weight_scale) : 1.0f;
     if ((int)blockIdx.x >= total) return;
     Tile tiles(a.weight, a.hidden, lds);
     int ahead = blockIdx.x;
@@ -299,7 +299,7 @@ __global__ __launch_bounds__(mat_threads(BM, BN, BUFFERS), 1) void xent_logits_k
             const bool labelled = __any(label >= 0 && label < Tile::kPartM);
             if constexpr (F16) {
 #pragma unroll
-                for (int i = 0; i < Tile::kMT; ++i) acc[i][j] = acc[i][j] * scale_h * scale_w;
+                for (int i = 0; i < Tile::kMT; ++i) acc[i][j] = acc[i][j] * scale;
             }
             if constexpr (!BACKWARD) {
                 if (labelled) {

@@ -110,3 +110,13 @@ def test_every_row_keeps_its_bits_whatever_the_others_gradients(rows, vocab, dty
     _, want_h, want_w = reference(h, w, target, g, "none")
     off = (dh.double() - want_h).abs().amax(1) / (g.double() * float(w.detach().abs().max())).clamp(min=1e-300)
     assert off.max() < TOL[dtype] and (dh[5] == 0).all() and err(dw, want_w) < TOL[dtype]
+
+
+@pytest.mark.parametrize("rows", [40, 90, 700])
+def test_float_operands_far_apart(rows):
+    """Hidden rows of some 2^112 and weights of some 2^-100: logits of some 2^15, off by 2^-20 of that (1e-5 of the losses)."""
+    hidden, weight, target = make(rows, 64, 1000, torch.float32, ignored=0.0)
+    hidden, weight = hidden * 2.0 ** 112, weight * 2.0 ** -100
+    each = tb.linear_cross_entropy(hidden, weight, target, reduction="none")
+    want, _, _ = reference(hidden, weight, target, torch.ones(rows, device="cuda"), "none")
+    assert (each.double() - want).abs().max() <= 1e-5 * (1 + want.abs().max())
