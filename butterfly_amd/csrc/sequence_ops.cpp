@@ -574,12 +574,13 @@ bf_linear_xent describe(const Xent &o, const Tensor &hidden, const Tensor &weigh
     return d;
 }
 
-// (loss, kept operands)
-std::tuple<Tensor, Tensor> xent_fw(const Xent &o)
+// (loss, kept operands); what the call was, for its backward one, in *desc
+std::tuple<Tensor, Tensor> xent_fw(const Xent &o, bf_linear_xent *desc)
 {
     const Guard guard(o.hidden.device());
     const Tensor hidden = rows_of(o.hidden), weight = aligned_rows_of(o.weight), target = o.target.contiguous();
     const bf_linear_xent d = describe(o, hidden, weight);
+    if (desc) *desc = d;
     const auto options = hidden.options().dtype(at::kFloat);
     Tensor loss = o.reduction == BF_XENT_NONE ? at::empty(o.target.sizes(), options) : at::empty({}, options);
     const size_t bytes = valid_size(bf_linear_xent_fw_workspace_bytes(&d));
@@ -653,15 +654,14 @@ Tensor linear_cross_entropy(Tensor hidden, Tensor weight, Tensor target, int64_t
     refuse_tangents({hidden, weight}, who);
     if (!any_wants_grad({hidden, weight})) {
         at::AutoDispatchBelowADInplaceOrView below;
-        return std::get<0>(xent_fw(o));
+        return std::get<0>(xent_fw(o, nullptr));
     }
     std::shared_ptr<XentNode> node(new XentNode(), torch::autograd::deleteNode);
     node->set_next_edges(torch::autograd::collect_next_edges(hidden, weight));
     Tensor loss, kept;
     {
         at::AutoDispatchBelowADInplaceOrView below;
-        std::tie(loss, kept) = xent_fw(o);
-        node->desc = describe(o, rows_of(hidden), rows_of(weight));
+        std::tie(loss, kept) = xent_fw(o, &node->desc);
     }
     node->hidden_shape = hidden.sizes();
     node->weight.set(weight);

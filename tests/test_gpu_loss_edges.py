@@ -120,3 +120,12 @@ def test_float_operands_far_apart(rows):
     each = tb.linear_cross_entropy(hidden, weight, target, reduction="none")
     want, _, _ = reference(hidden, weight, target, torch.ones(rows, device="cuda"), "none")
     assert (each.double() - want).abs().max() <= 1e-5 * (1 + want.abs().max())
+
+
+def test_a_weight_whose_features_are_not_adjacent_is_copied_once():
+    hidden, weight, target = make(70, 256, 20000, torch.bfloat16)
+    columns = weight.t().contiguous().t().requires_grad_()
+    tb.linear_cross_entropy(hidden, columns, target)
+    before = torch.cuda.memory_stats()["allocated_bytes.all.allocated"]
+    tb.linear_cross_entropy(hidden, columns, target)
+    assert torch.cuda.memory_stats()["allocated_bytes.all.allocated"] - before < 1.5 * weight.numel() * 2
