@@ -175,11 +175,19 @@ __device__ __forceinline__ A step_of(bool cut, A a, A h, A b)
     return cut ? b : mac(b, a, h);
 }
 
-// Chunks compose by products of many factors, which may overflow where nothing is there to be multiplied.
+// Runs and chunks compose by products of many gates, which may overflow where nothing is there to be multiplied (leading
+// zeros under gates above one): zero through them is zero, as it is step by step.  (A number below one may be infinite
+// behind a product that has passed 2^128 where step by step it is not yet.)
 template <typename A>
 __device__ __forceinline__ A chunk_of(bool cut, A a, A h, A b)
 {
     return cut || is_zero(h) ? b : mac(b, a, h);
+}
+// the gates' product of two of them
+template <typename A>
+__device__ __forceinline__ A gates_of(bool cut, A a, A b)
+{
+    return cut || is_zero(a) || is_zero(b) ? zero_of(A()) : mul(a, b);
 }
 
 // carry behind the composition in a slot (columns past the end repeat the last one)
@@ -223,7 +231,7 @@ __device__ __forceinline__ void exchange(Runs<Tr> &runs, int turn, int wave, int
         for (int v = 0; v < Tr::V; ++v) {
             const A ca = runs.a[turn][w][v][lane], cb = runs.b[turn][w][v][lane];
             if (w == wave) mine[v] = carry[v];
-            carry[v] = step_of(cut_w, ca, carry[v], cb);
+            carry[v] = chunk_of(cut_w, ca, carry[v], cb);
         }
     }
 }
@@ -609,8 +617,8 @@ __global__ __launch_bounds__(64 * kRecWaves, 8) void recurrence_runs_kernel(Recu
 #pragma unroll
         for (int v = 0; v < V; ++v) {
             const A ca = runs.a[0][w][v][at.lane], cb = runs.b[0][w][v][at.lane];
-            pb[v] = step_of(cut_w, ca, pb[v], cb);
-            pa[v] = cut_w ? zero_of(A()) : mul(pa[v], ca);
+            pb[v] = chunk_of(cut_w, ca, pb[v], cb);
+            pa[v] = gates_of(cut_w, pa[v], ca);
         }
     };
     for (int i = 0; i < turn; ++i) add_run(i);
