@@ -87,6 +87,11 @@ int64_t backward_groups(const bf_rowwise *p)
     return std::max<int64_t>(1, std::min<int64_t>((p->rows + g - 1) / g, 512));
 }
 
+size_t slice_bytes(const bf_rowwise *p)
+{
+    return (size_t)backward_groups(p) * 2 * (size_t)((p->cols + 7) / 8 * 8) * sizeof(float);
+}
+
 template <typename T>
 void launch_fw(const RowArgs &a, hipStream_t stream)
 {
@@ -110,8 +115,7 @@ template <typename T>
 void launch_bw(const RowArgs &a, int64_t blocks, hipStream_t stream)
 {
     if (a.cols > kRegisterCols) {
-        if (a.d_x || a.d_residual)
-            norm_bw_wide_kernel<T><<<dim3((unsigned)std::min<int64_t>(a.rows, 512)), dim3(kWideThreads), 0, stream>>>(a);
+        norm_bw_wide_kernel<T><<<dim3((unsigned)std::min<int64_t>(a.rows, 512)), dim3(kWideThreads), 0, stream>>>(a);
         if (a.partial)
             norm_param_partial_kernel<T><<<dim3((unsigned)((a.cols + 511) / 512), (unsigned)blocks), dim3(256), 0, stream>>>(a);
     } else {
@@ -180,7 +184,8 @@ size_t bf_rowwise_bw_workspace_bytes(const bf_rowwise *p)
 {
     if (check_rows(p)) return BF_SIZE_INVALID;
     if (p->rows == 0 || p->cols == 0) return 0;
-    return (size_t)backward_groups(p) * 2 * (size_t)((p->cols + 7) / 8 * 8) * sizeof(float);
+    // the slices of column sums; rows that are read again: what each one's u is off by
+    return slice_bytes(p) + (p->cols > kRegisterCols ? (size_t)p->rows * sizeof(float) : 0);
 }
 
 int bf_rowwise_bw(const bf_rowwise *p, const void *sum, const void *grad_y, const void *grad_sum, const int64_t *rng,
@@ -205,6 +210,7 @@ int bf_rowwise_bw(const bf_rowwise *p, const void *sum, const void *grad_y, cons
             return fail(BF_ERR_WORKSPACE, "workspace of %zu bytes needed, %zu given", need, workspace ? workspace_bytes : 0);
         if (reinterpret_cast<uintptr_t>(workspace) & 15) return fail(BF_ERR_WORKSPACE, "workspace must be 16-byte aligned");
         a.partial = static_cast<float *>(workspace);
+        if (p->cols > kRegisterCols) a.shift = reinterpret_cast<float *>(static_cast<char *>(workspace) + slice_bytes(p));
     }
     a.x = sum;
     a.grad_y = grad_y;

@@ -33,6 +33,7 @@ struct RowArgs {
     void *d_x, *d_residual;             // d_residual NULL: not wanted
     float2 *stats;                      // (mean, rstd) of each row; NULL forward: not wanted
     float *partial;                     // backward: (workgroups, 2, slice) column sums; NULL: not wanted
+    float *shift;                       // backward, rows read again, with partial: what each row's u is off by
     const int64_t *rng;                 // (seed, call); NULL: nothing is dropped
     int64_t rows;
     int64_t x_stride, residual_stride, grad_y_stride, grad_sum_stride;
@@ -282,13 +283,17 @@ __device__ __forceinline__ void store_sums(const float (&v)[K][8], float *joined
     }
 }
 
+// u is formed from the row's float mean, which is off by its rounding (2^-24 of an offset in front of the deviations): by
+// delta = mean(u), since the true u have none.  So the row's sums are those of gw, gw u and u, and u, and mean(gw u) by
+// delta mean(gw), are put right behind them, before the columns take their share.  (The sum behind a dropout in bfloat16 is
+// its rounded self here, the statistics those of the unrounded one: 2^-9 of a gradient that has no more bits.)
 // 32768 x 4096 float 292 us (1.61 GB, 5.5 TB/s); 8192 x 2048 float with dropout and three gradients 64 (336 MB, 5.2 TB/s); 3001 x
 // 1000 bfloat16 12.3.
 template <typename T, int L, int K>
 __global__ __launch_bounds__(row_threads<L>()) void norm_bw_kernel(RowArgs a)
 {
     constexpr int B = row_threads<L>(), G = B / L, W = L < 64 ? L : 64;
-    __shared__ float2 lds[2][16];
+    __shared__ float4 lds[2][16];
     __shared__ float joined[G > 1 ? B * K * 8 : 1];
     const Dropper drop(a);
     const int lane = threadIdx.x % L, group = threadIdx.x / L;
@@ -299,43 +304,54 @@ __global__ __launch_bounds__(row_threads<L>()) void norm_bw_kernel(RowArgs a)
     int turn = 0;
     for (int64_t row = (int64_t)blockIdx.x * G + group; row < a.rows; row += (int64_t)gridDim.x * G) {
         float u[K][8], g[K][8];
+        const float2 st = a.stats[row];
 #pragma unroll
         for (int k = 0; k < K; ++k) {
             const int col = 8 * (k * L + lane);
-            load8(reinterpret_cast<const T *>(a.x) + row * a.x_stride, col, a.cols, 0.0f, u[k]);
+            // (past the row's end u and g are zero)
+            load8(reinterpret_cast<const T *>(a.x) + row * a.x_stride, col, a.cols, st.x, u[k]);
             load8(reinterpret_cast<const T *>(a.grad_y) + row * a.grad_y_stride, col, a.cols, 0.0f, g[k]);
         }
-        const float2 st = a.stats[row];
-        float c1 = 0.0f, c2 = 0.0f;
+        float c1 = 0.0f, c2 = 0.0f, delta = 0.0f;
 #pragma unroll
         for (int k = 0; k < K; ++k)
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                // (past the row's end u is some number and g zero)
                 u[k][i] = (u[k][i] - st.x) * st.y;
-                dw[k][i] = fmaf(g[k][i], u[k][i], dw[k][i]);
-                db[k][i] += g[k][i];
-                g[k][i] *= w[k][i];
-                c1 += g[k][i];
-                c2 = fmaf(g[k][i], u[k][i], c2);
+                const float gw = g[k][i] * w[k][i];
+                c1 += gw;
+                c2 = fmaf(gw, u[k][i], c2);
+                delta += u[k][i];
             }
         c1 = lanes_sum<W>(c1);
         c2 = lanes_sum<W>(c2);
+        delta = lanes_sum<W>(delta);
         if constexpr (L > 64) {
-            if ((lane & 63) == 0) lds[turn][lane >> 6] = make_float2(c1, c2);
+            if ((lane & 63) == 0) lds[turn][lane >> 6] = make_float4(c1, c2, delta, 0.0f);
             __syncthreads();
-            c1 = c2 = 0.0f;
+            c1 = c2 = delta = 0.0f;
 #pragma unroll
-            for (int i = 0; i < L / 64; ++i) { c1 += lds[turn][i].x; c2 += lds[turn][i].y; }
+            for (int i = 0; i < L / 64; ++i) {
+                const float4 p = lds[turn][i];
+                c1 += p.x;
+                c2 += p.y;
+                delta += p.z;
+            }
             turn ^= 1;
         }
         c1 *= inv;
-        c2 *= inv;
+        delta *= inv;
+        c2 = fmaf(-delta, c1, c2 * inv);
 #pragma unroll
         for (int k = 0; k < K; ++k) {
             const int col = 8 * (k * L + lane);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) g[k][i] = st.y * (g[k][i] - c1 - u[k][i] * c2);
+            for (int i = 0; i < 8; ++i) {
+                const float v = u[k][i] - delta;
+                dw[k][i] = fmaf(g[k][i], v, dw[k][i]);
+                db[k][i] += g[k][i];
+                g[k][i] = st.y * (g[k][i] * w[k][i] - c1 - v * c2);
+            }
             if (a.grad_sum) {
                 float more[8];
                 load8(reinterpret_cast<const T *>(a.grad_sum) + row * a.grad_sum_stride, col, a.cols, 0.0f, more);
@@ -360,45 +376,52 @@ __global__ __launch_bounds__(row_threads<L>()) void norm_bw_kernel(RowArgs a)
 
 constexpr int kWideThreads = 1024;
 
-__device__ __forceinline__ float2 block_sum(float2 v, float2 (*lds)[16], int turn)
+template <int N>
+__device__ __forceinline__ void block_sum(float (&v)[N], float (*lds)[16][N], int turn)
 {
-    v = make_float2(lanes_sum<64>(v.x), lanes_sum<64>(v.y));
-    if ((threadIdx.x & 63) == 0) lds[turn][threadIdx.x >> 6] = v;
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+        v[n] = lanes_sum<64>(v[n]);
+        if ((threadIdx.x & 63) == 0) lds[turn][threadIdx.x >> 6][n] = v[n];
+    }
     __syncthreads();
-    v = make_float2(0.0f, 0.0f);
-    for (int i = 0; i < kWideThreads / 64; ++i) v = make_float2(v.x + lds[turn][i].x, v.y + lds[turn][i].y);
-    return v;
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+        v[n] = 0.0f;
+        for (int i = 0; i < kWideThreads / 64; ++i) v[n] += lds[turn][i][n];
+    }
 }
 
 template <typename T>
 __global__ __launch_bounds__(kWideThreads) void norm_fw_wide_kernel(RowArgs a)
 {
-    __shared__ float2 lds[2][16];
+    __shared__ float lds[2][16][2];
     const Dropper drop(a);
     const float inv = 1.0f / (float)a.cols;
     for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
         float v[8];
-        float2 s = make_float2(0.0f, 0.0f);
+        float s[2] = {};
         for (int col = threadIdx.x * 8; col < a.cols; col += kWideThreads * 8) {
             total8<T>(a, drop, row, col, v);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) s.x += v[i];
+            for (int i = 0; i < 8; ++i) s[0] += v[i];
         }
         Moments m;
-        m.base = block_sum(s, lds, 0).x * inv;
-        s = make_float2(0.0f, 0.0f);
+        block_sum(s, lds, 0);
+        m.base = s[0] * inv;
+        s[0] = s[1] = 0.0f;
         for (int col = threadIdx.x * 8; col < a.cols; col += kWideThreads * 8) {
             total8<T>(a, drop, row, col, v);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 const float d = col + i < a.cols ? v[i] - m.base : 0.0f;
-                s.x += d;
-                s.y = fmaf(d, d, s.y);
+                s[0] += d;
+                s[1] = fmaf(d, d, s[1]);
             }
         }
-        s = block_sum(s, lds, 1);
-        m.shift = s.x * inv;
-        m.m2 = s.y - s.x * m.shift;
+        block_sum(s, lds, 1);
+        m.shift = s[0] * inv;
+        m.m2 = s[1] - s[0] * m.shift;
         if (m.m2 < 0.0f) m.m2 = 0.0f;
         const float rstd = 1.0f / sqrtf(m.m2 * inv + a.eps);
         if (a.stats && threadIdx.x == 0) a.stats[row] = make_float2(m.mean(), rstd);
@@ -418,7 +441,7 @@ __global__ __launch_bounds__(kWideThreads) void norm_fw_wide_kernel(RowArgs a)
 template <typename T>
 __global__ __launch_bounds__(kWideThreads) void norm_bw_wide_kernel(RowArgs a)
 {
-    __shared__ float2 lds[2][16];
+    __shared__ float lds[2][16][3];
     const Dropper drop(a);
     const float inv = 1.0f / (float)a.cols;
     int turn = 0;
@@ -427,26 +450,31 @@ __global__ __launch_bounds__(kWideThreads) void norm_bw_wide_kernel(RowArgs a)
         const T *gy = reinterpret_cast<const T *>(a.grad_y) + row * a.grad_y_stride;
         const float2 st = a.stats[row];
         float u[8], g[8], w[8];
-        float2 c = make_float2(0.0f, 0.0f);
+        float c[3] = {};   // of gw, gw u and u
         for (int col = threadIdx.x * 8; col < a.cols; col += kWideThreads * 8) {
-            load8(x, col, a.cols, 0.0f, u);
+            load8(x, col, a.cols, st.x, u);
             load8(gy, col, a.cols, 0.0f, g);
             param8<T>(a.weight, a.wide_params, col, a.cols, 1.0f, w);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 g[i] *= w[i];
-                c.x += g[i];
-                c.y = fmaf(g[i], (u[i] - st.x) * st.y, c.y);
+                u[i] = (u[i] - st.x) * st.y;
+                c[0] += g[i];
+                c[1] = fmaf(g[i], u[i], c[1]);
+                c[2] += u[i];
             }
         }
-        c = block_sum(c, lds, turn);
+        block_sum(c, lds, turn);
         turn ^= 1;
+        const float c1 = c[0] * inv, delta = c[2] * inv, c2 = fmaf(-delta, c1, c[1] * inv);
+        if (a.shift && threadIdx.x == 0) a.shift[row] = delta;
+        if (!a.d_x && !a.d_residual) continue;
         for (int col = threadIdx.x * 8; col < a.cols; col += kWideThreads * 8) {
             load8(x, col, a.cols, 0.0f, u);
             load8(gy, col, a.cols, 0.0f, g);
             param8<T>(a.weight, a.wide_params, col, a.cols, 1.0f, w);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) g[i] = st.y * (g[i] * w[i] - c.x * inv - (u[i] - st.x) * st.y * (c.y * inv));
+            for (int i = 0; i < 8; ++i) g[i] = st.y * (g[i] * w[i] - c1 - fmaf(u[i] - st.x, st.y, -delta) * c2);
             if (a.grad_sum) {
                 load8(reinterpret_cast<const T *>(a.grad_sum) + row * a.grad_sum_stride, col, a.cols, 0.0f, u);
 #pragma unroll
@@ -471,12 +499,13 @@ __global__ __launch_bounds__(256) void norm_param_partial_kernel(RowArgs a)
     if (col < a.cols) {
         for (int64_t row = (int64_t)blockIdx.y * 4 + group; row < a.rows; row += (int64_t)gridDim.y * 4) {
             const float2 st = a.stats[row];
+            const float delta = a.shift[row];
             float u[8], g[8];
             load8(reinterpret_cast<const T *>(a.x) + row * a.x_stride, col, a.cols, 0.0f, u);
             load8(reinterpret_cast<const T *>(a.grad_y) + row * a.grad_y_stride, col, a.cols, 0.0f, g);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                dw[i] = fmaf(g[i], (u[i] - st.x) * st.y, dw[i]);
+                dw[i] = fmaf(g[i], fmaf(u[i] - st.x, st.y, -delta), dw[i]);
                 db[i] += g[i];
             }
         }

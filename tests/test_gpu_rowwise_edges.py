@@ -1,0 +1,26 @@
+"""Norms of rows whose offset is large beside their spread, in the backward pass.  Error measure and tolerances are those of the
+row operators' other tests."""
+import pytest
+import torch
+
+import butterfly_amd as tb
+from test_gpu_rowwise import err, randn, reference
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("offset", [0.0, 1000.0, 10000.0, -30000.0])
+@pytest.mark.parametrize("cols", [7, 100, 500, 1000, 2000, 3000, 8000, 9000, 20000])
+def test_gradients_of_rows_with_large_offsets(cols, offset):
+    """The inputs' own rounding is the reference's too; what is left are roundings of deviations from the row's mean."""
+    x = (randn(40, cols, seed=1) + offset).requires_grad_()
+    w, b = randn(cols, seed=2, scale=0.3, shift=1.0).requires_grad_(), randn(cols, seed=3).requires_grad_()
+    g = randn(40, cols, seed=4)
+    y = tb.layer_norm(x, w, b)
+    ref = reference(x, g, weight=w, bias=b)
+    assert err(y, ref["y"]) < 1e-5
+    for got, name in zip(torch.autograd.grad(y, (x, w, b), g, retain_graph=True), ("d_x", "d_weight", "d_bias")):
+        assert err(got, ref[name]) < 1e-5, name
+    # the parameters' gradients alone
+    dw, = torch.autograd.grad(y, w, g)
+    assert err(dw, ref["d_weight"]) < 1e-5
