@@ -9,6 +9,7 @@
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/saved_variable.h>
 #include <torch/library.h>
@@ -66,6 +67,22 @@ bool any_wants_grad(std::initializer_list<Tensor> tensors)
     for (const Tensor &t : tensors)
         if (t.defined() && t.requires_grad()) return true;
     return false;
+}
+
+// Gradients that are to be differentiated again (create_graph) come with a history that says, once it is followed, that there
+// is no second derivative; without one they would count as constants.
+void refuse_second(variable_list &out, const torch::autograd::Node &node, std::initializer_list<Tensor> grads, const char *who)
+{
+    if (!at::GradMode::is_enabled()) return;
+    torch::autograd::edge_list edges;
+    for (const auto &edge : node.next_edges())
+        if (edge.is_valid()) edges.push_back(edge);
+    for (const Tensor &t : grads)
+        if (t.defined() && t.requires_grad()) edges.push_back(torch::autograd::impl::gradient_edge(t));
+    std::shared_ptr<torch::autograd::Node> error(
+        new torch::autograd::Error(std::string(who) + ": no second derivative", std::move(edges)), torch::autograd::deleteNode);
+    for (Tensor &t : out)
+        if (t.defined()) torch::autograd::set_history(t, error);
 }
 
 int dtype_code(const Tensor &t, bool complex_too, const char *who)
@@ -193,6 +210,8 @@ Tensor rows_fw(const Rows &o, bool want_sum, Tensor *sum, Tensor *stats)
     return o.norm ? y : total;
 }
 
+std::tuple<Tensor, Tensor> rows_op(const Rows &o, bool two);
+
 struct RowsNode : public torch::autograd::Node {
     SavedSlot total, stats, weight, rng;
     c10::SmallVector<int64_t, 6> shape;
@@ -216,19 +235,27 @@ struct RowsNode : public torch::autograd::Node {
         o.p = p;
         o.eps = eps;
         o.who = who;
-        at::AutoDispatchBelowADInplaceOrView below;
         if (!norm || !gy.defined()) {
-            // the gradient itself, through the mask for x
+            // the gradient itself, through the mask for x: the operator itself, with derivatives of its own
             const Tensor g = gy.defined() ? gy : gs;
             if (want_residual) out[1] = g;
             if (want_x) {
                 o.x = g;
-                out[0] = o.rng.defined() ? rows_fw(o, true, nullptr, nullptr) : g;
+                out[0] = o.rng.defined() ? std::get<0>(rows_op(o, false)) : g;
             }
             return out;
         }
         o.weight = weight.get(self);
         const Tensor sum = total.get(self), st = stats.get(self);
+        apply_norm(o, gy, gs, sum, st, out);
+        refuse_second(out, *this, {gy, gs}, who);
+        return out;
+    }
+
+    void apply_norm(const Rows &o, const Tensor &gy, const Tensor &gs, const Tensor &sum, const Tensor &st, variable_list &out)
+    {
+        const bool want_x = task_should_compute_output(0), want_residual = task_should_compute_output(1);
+        at::AutoDispatchBelowADInplaceOrView below;
         const bool want_weight = task_should_compute_output(2), want_bias = task_should_compute_output(3);
         const Guard guard(sum.device());
         bf_rowwise d = describe(o, sum);
@@ -251,7 +278,6 @@ struct RowsNode : public torch::autograd::Node {
                  who);
         if (want_x) out[0] = dx.defined() ? dx : dr;
         if (want_residual) out[1] = dr;
-        return out;
     }
 
     void release_variables() override
@@ -476,6 +502,7 @@ struct RecurrenceNode : public torch::autograd::Node {
                                   before.data_ptr(), ptr(g), ptr(gl), out[0].data_ptr(), out[1].data_ptr(), ptr(out[2]), ptr(ws),
                                   bytes, current_stream()),
                  who);
+        refuse_second(out, *this, {grads[0], grads[1]}, who);
         return out;
     }
 
@@ -618,6 +645,7 @@ struct XentNode : public torch::autograd::Node {
         check_rc(bf_linear_xent_bw(&d, w.data_ptr(), g.data_ptr<float>(), operands.data_ptr(),
                                    (size_t)operands.numel(), ptr(out[0]), ptr(out[1]), ptr(ws), bytes, current_stream()),
                  "linear_cross_entropy");
+        refuse_second(out, *this, {grads[0]}, "linear_cross_entropy");
         return out;
     }
 
