@@ -31,7 +31,7 @@ SYMBOLS = [
     "bf_butterfly_multiply_base4_saved_bytes", "bf_butterfly_multiply_base4_fw_saving",
     "bf_butterfly_multiply_base4_bw_saved_workspace_bytes", "bf_butterfly_multiply_base4_bw_saved",
     "bf_layer_takes_real", "bf_layer_kept_bytes", "bf_layer_fw_workspace_bytes", "bf_layer_fw", "bf_layer_bw_workspace_bytes", "bf_layer_bw",
-    "bf_rng_next", "bf_rowwise_fw", "bf_rowwise_bw_workspace_bytes", "bf_rowwise_bw",
+    "bf_rng_next", "bf_rng_next_of", "bf_rowwise_fw", "bf_rowwise_bw_workspace_bytes", "bf_rowwise_bw",
     "bf_recurrence_workspace_bytes", "bf_recurrence_fw", "bf_recurrence_bw", "bf_recurrence_step",
     "bf_linear_xent_kept_bytes", "bf_linear_xent_fw_workspace_bytes", "bf_linear_xent_bw_workspace_bytes", "bf_linear_xent_fw",
     "bf_linear_xent_bw",
@@ -154,6 +154,7 @@ def lib():
         L.bf_layer_bw.argtypes = [pl, vp, vp, vp, sz, vp, vp, vp, vp, vp, sz, vp]
         pr, pc, px = ctypes.POINTER(Rowwise), ctypes.POINTER(Recurrence), ctypes.POINTER(LinearXent)
         L.bf_rng_next.argtypes = [vp, vp, vp]
+        L.bf_rng_next_of.argtypes = [vp, vp, ctypes.c_int64, vp]
         L.bf_rowwise_fw.argtypes = [pr] + [vp] * 9
         L.bf_rowwise_bw_workspace_bytes.argtypes = [pr]
         L.bf_rowwise_bw_workspace_bytes.restype = sz

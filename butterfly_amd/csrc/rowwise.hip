@@ -134,10 +134,10 @@ void launch_sums(const ColumnSumArgs &c, hipStream_t s)
     else column_sums_kernel<P, 4><<<dim3((unsigned)((entries + 15) / 16)), dim3(1024), 0, s>>>(c);
 }
 
-__global__ void rng_next_kernel(int64_t *state, int64_t *taken)
+__global__ void rng_next_kernel(int64_t *state, int64_t *taken, uint64_t add)
 {
     const int64_t seed = state[0], call = state[1];
-    taken[0] = seed;
+    taken[0] = (int64_t)((uint64_t)seed + add);
     taken[1] = call;
     state[1] = (int64_t)((uint64_t)call + 1);
 }
@@ -146,10 +146,13 @@ __global__ void rng_next_kernel(int64_t *state, int64_t *taken)
 
 extern "C" {
 
-int bf_rng_next(int64_t *state, int64_t *taken, void *stream)
+int bf_rng_next(int64_t *state, int64_t *taken, void *stream) { return bf_rng_next_of(state, taken, 0, stream); }
+
+int bf_rng_next_of(int64_t *state, int64_t *taken, int64_t replica, void *stream)
 {
     if (!state || !taken) return fail(BF_ERR_INVALID, "state or taken is NULL");
-    rng_next_kernel<<<dim3(1), dim3(1), 0, static_cast<hipStream_t>(stream)>>>(state, taken);
+    // (2^64 over the golden ratio, odd: seeds of neighbouring replicas lie far apart)
+    rng_next_kernel<<<dim3(1), dim3(1), 0, static_cast<hipStream_t>(stream)>>>(state, taken, (uint64_t)replica * 0x9E3779B97F4A7C15ull);
     BF_HIP_CHECK(hipGetLastError());
     return BF_OK;
 }

@@ -374,8 +374,8 @@ std::tuple<Tensor, Tensor> dropout_add_layer_norm(Tensor x, OptTensor rng, doubl
     return rows_op(o, true);
 }
 
-// The generator's present (seed, call), whose call number then goes up by one, in stream order.
-Tensor rng_next(Tensor rng)
+// The generator's present (seed of the replica, call), whose call number then goes up by one, in stream order.
+Tensor rng_next(Tensor rng, int64_t replica)
 {
     const char *who = "rng_next";
     require_device(rng, who);
@@ -384,7 +384,7 @@ Tensor rng_next(Tensor rng)
     at::AutoDispatchBelowADInplaceOrView below;
     const Guard guard(rng.device());
     Tensor taken = at::empty_like(rng);
-    check_rc(bf_rng_next(rng.data_ptr<int64_t>(), taken.data_ptr<int64_t>(), current_stream()), who);
+    check_rc(bf_rng_next_of(rng.data_ptr<int64_t>(), taken.data_ptr<int64_t>(), replica, current_stream()), who);
     rng.unsafeGetTensorImpl()->bump_version();
     return taken;
 }
@@ -705,7 +705,7 @@ TORCH_LIBRARY_FRAGMENT(torch_butterfly, m)
     m.def("layer_norm", layer_norm);
     m.def("dropout_add", dropout_add);
     m.def("dropout_add_layer_norm", dropout_add_layer_norm);
-    m.def("rng_next", rng_next);
+    m.def("rng_next(Tensor rng, int replica=0) -> Tensor", rng_next);
     m.def("gated_recurrence", gated_recurrence);
     m.def("gated_recurrence_step", gated_recurrence_step);
     m.def("linear_cross_entropy", linear_cross_entropy);

@@ -8,7 +8,7 @@ rows' dtype; statistics are formed in float32.  Host tensors run as tensor opera
 
 No counterpart in the reference, whose users take these from PyTorch."""
 import torch
-from torch import nn
+from torch import distributed as dist, nn
 
 ops = torch.ops.torch_butterfly
 
@@ -36,12 +36,15 @@ def dropout_add_layer_norm(x, rng, p, residual=None, weight=None, bias=None, eps
     return _host_norm(total, weight, bias, eps), total
 
 
-def rng_next(rng):
+def rng_next(rng, replica=0):
     """A copy of ``rng``, whose call number then goes up by one (on the device, in stream order: recorded in a HIP
-    graph, every replay takes the next number)."""
+    graph, every replay takes the next number).  ``replica``: which of several copies of a model that hold the same
+    ``rng`` draws; each has a seed of its own."""
     if rng.is_cuda:
-        return ops.rng_next(rng)
+        return ops.rng_next(rng, replica)
     taken = rng.clone()
+    # (2^64 over the golden ratio, modulo 2^64, as a signed number)
+    taken[0] += (replica * 0x9E3779B97F4A7C15 + (1 << 63)) % (1 << 64) - (1 << 63)
     rng[1] += 1
     return taken
 
@@ -108,20 +111,34 @@ class LayerNorm(nn.Module):
 
 
 class _Dropping(nn.Module):
-    """Holds ``p`` and the generator's (seed, call), part of the state dict: a resumed run goes on where it stopped."""
+    """Holds ``p`` and the generator's (seed, call), part of the state dict: a resumed run goes on where it stopped.
 
-    def __init__(self, p):
+    ``replica``: the number of the model's copy that this process trains.  Copies on several GPUs hold the same ``rng``
+    (``DistributedDataParallel`` sees to it, and a state dict that all of them load) and drop elements of their own by
+    this number: by default the process's rank in ``torch.distributed``, where that is initialised.  Processes
+    that work on the same activations give the same one.  A deep copy within a process drops what its original drops,
+    until one of them is given another seed (``reseed``)."""
+
+    def __init__(self, p, replica=None):
         super().__init__()
         if not 0 <= p <= 1:
             raise ValueError(f"p must be between 0 and 1, got {p}")
-        self.p = p
+        self.p, self.replica = p, replica
         self.register_buffer("rng", torch.stack((torch.randint(1 << 62, ()), torch.zeros((), dtype=torch.int64))))
+
+    def reseed(self, seed=None):
+        """Another seed (by default one from PyTorch's generator), calls counted from zero."""
+        seed = torch.randint(1 << 62, ()) if seed is None else torch.tensor(seed)
+        self.rng.copy_(torch.stack((seed, torch.zeros_like(seed))))
 
     def _draw(self):
         """(rng of this call, p): nothing is dropped outside of training."""
         if not self.training or self.p == 0:
             return None, 0.0
-        return rng_next(self.rng), self.p
+        replica = self.replica
+        if replica is None:
+            replica = dist.get_rank() if dist.is_available() and dist.is_initialized() else 0
+        return rng_next(self.rng, replica), self.p
 
 
 class DropoutAdd(_Dropping):
@@ -135,8 +152,8 @@ class DropoutAdd(_Dropping):
 class DropoutAddLayerNorm(_Dropping):
     """``(layer_norm(sum), sum)`` with ``sum = residual + dropout(x)``: the end of one block and the norm of the next."""
 
-    def __init__(self, size, p=0.1, eps=1e-5):
-        super().__init__(p)
+    def __init__(self, size, p=0.1, eps=1e-5, replica=None):
+        super().__init__(p, replica)
         self.size, self.eps = size, eps
         self.weight = nn.Parameter(torch.ones(size))
         self.bias = nn.Parameter(torch.zeros(size))

@@ -327,8 +327,11 @@ typedef struct bf_rowwise {
  * 65536 / (65536 - t).  No mask is stored: forward and backward make the same one from rng, two
  * device integers.
  * bf_rng_next: taken = state, then state[1] += 1, in stream order: what a module draws per call
- * (also from a recorded graph, whose every replay then drops other elements).                   */
+ * (also from a recorded graph, whose every replay then drops other elements).
+ * bf_rng_next_of: for one of several replicas of a model that hold the same state: taken[0] = state[0] +
+ * replica * 0x9E3779B97F4A7C15 (modulo 2^64), so that each drops elements of its own.            */
 int bf_rng_next(int64_t *state, int64_t *taken, void *stream);
+int bf_rng_next_of(int64_t *state, int64_t *taken, int64_t replica, void *stream);
 
 /* residual, rng (when drop_probability is 0), weight (ones), bias (zeros) may be NULL; sum or y may be NULL
  * (not wanted; without y there is no norm and no weight, bias or stats).  stats: (rows, 2) floats,

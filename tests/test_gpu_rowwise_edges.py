@@ -1,4 +1,4 @@
-"""Norms of rows whose offset is large beside their spread, in the backward pass.  Error measure and tolerances are those of the
+"""Norms of rows whose offset is large beside their spread, in the backward pass; generators of several replicas.  Error measure and tolerances are those of the
 row operators' other tests."""
 import pytest
 import torch
@@ -24,3 +24,16 @@ def test_gradients_of_rows_with_large_offsets(cols, offset):
     # the parameters' gradients alone
     dw, = torch.autograd.grad(y, w, g)
     assert err(dw, ref["d_weight"]) < 1e-5
+
+
+@pytest.mark.parametrize("replica", [0, 1, 7, -3, 1 << 40])
+def test_replicas_of_a_generator(replica):
+    host = torch.tensor([-0x123456789ABCDEF, 0x7FEDCBA987654321])
+    device = host.cuda()
+    for _ in range(2):
+        assert tb.rng_next(device, replica).tolist() == tb.rng_next(host, replica).tolist()
+    assert device.tolist() == host.tolist()
+    layer = tb.DropoutAdd(0.5, replica=replica).cuda()
+    taken = tb.rng_next(layer.rng.clone(), replica)
+    x = randn(9, 70, seed=5)
+    assert torch.equal(layer(x), tb.dropout_add(x, taken, 0.5))
