@@ -7,6 +7,9 @@ of stored.  Rows are float32 or bfloat16, of any width and row stride; ``weight`
 rows' dtype; statistics are formed in float32.  Host tensors run as tensor operations.
 
 No counterpart in the reference, whose users take these from PyTorch."""
+import collections
+import weakref
+
 import torch
 from torch import distributed as dist, nn
 
@@ -110,6 +113,18 @@ class LayerNorm(nn.Module):
         return layer_norm(x, self.weight, self.bias, self.eps)
 
 
+# What forward calls drew that a backward pass may run again (torch.utils.checkpoint), by module and by a number from PyTorch's
+# generator: the recomputation restores that generator, not a module's own, and so finds the number again.
+_drawn = weakref.WeakKeyDictionary()
+_DRAWN_AT_MOST = 1024       # of a module
+
+
+def _may_run_again():
+    """Whether somebody keeps the present call's inputs instead of what it saves: no gradient in training, or hooks on what
+    is saved."""
+    return not torch.is_grad_enabled() or torch._C._autograd._top_saved_tensors_default_hooks(False) is not None
+
+
 class _Dropping(nn.Module):
     """Holds ``p`` and the generator's (seed, call), part of the state dict: a resumed run goes on where it stopped.
 
@@ -132,13 +147,27 @@ class _Dropping(nn.Module):
         self.rng.copy_(torch.stack((seed, torch.zeros_like(seed))))
 
     def _draw(self):
-        """(rng of this call, p): nothing is dropped outside of training."""
+        """(rng of this call, p): nothing is dropped outside of training; a call that is run again draws what it drew."""
         if not self.training or self.p == 0:
             return None, 0.0
+        again = torch._C._current_graph_task_id() != -1     # (a forward call inside of a backward pass)
+        if not again and not _may_run_again():
+            return self._next(), self.p
+        calls, number = _drawn.setdefault(self, collections.OrderedDict()), int(torch.empty((), dtype=torch.int64).random_())
+        if not again:
+            calls[number] = self._next()
+            if len(calls) > _DRAWN_AT_MOST:
+                calls.popitem(last=False)
+        elif number not in calls:
+            raise RuntimeError("dropout: this forward call runs again inside of a backward pass and cannot tell which call it was: "
+                               f"checkpoint with preserve_rng_state=True, at most {_DRAWN_AT_MOST} calls of a module at a time")
+        return calls[number], self.p
+
+    def _next(self):
         replica = self.replica
         if replica is None:
             replica = dist.get_rank() if dist.is_available() and dist.is_initialized() else 0
-        return rng_next(self.rng, replica), self.p
+        return rng_next(self.rng, replica)
 
 
 class DropoutAdd(_Dropping):

@@ -1,9 +1,14 @@
-"""Norms of rows whose offset is large beside their spread, in the backward pass; generators of several replicas.  Error measure and tolerances are those of the
+"""Norms of rows whose offset is large beside their spread, in the backward pass; generators of several replicas; forward
+calls that a backward pass runs again.  Error measure and tolerances are those of the
 row operators' other tests."""
+import copy
+
 import pytest
 import torch
+from torch.utils.checkpoint import checkpoint
 
 import butterfly_amd as tb
+from butterfly_amd.sequence_model import ButterflyLM
 from test_gpu_rowwise import err, randn, reference
 
 pytestmark = pytest.mark.gpu
@@ -37,3 +42,23 @@ def test_replicas_of_a_generator(replica):
     taken = tb.rng_next(layer.rng.clone(), replica)
     x = randn(9, 70, seed=5)
     assert torch.equal(layer(x), tb.dropout_add(x, taken, 0.5))
+
+
+@pytest.mark.parametrize("reentrant", [False, True])
+def test_recomputed_blocks_give_the_gradients_of_kept_ones(reentrant):
+    """The same kernels on the same numbers; gradients of the embedding's rows may be added in another order."""
+    torch.manual_seed(0)
+    kept = ButterflyLM(200, 48, 2, dropout=0.3).cuda()
+    again = copy.deepcopy(kept)
+    for module in [*again.mixers, *again.mixed, *again.fed]:
+        module.forward = (lambda run: lambda *args: checkpoint(run, *args, use_reentrant=reentrant))(module.forward)
+    tokens, target = torch.randint(0, 200, (2, 3, 50), device="cuda")
+    results = []
+    for m in (kept, again):
+        for _ in range(2):
+            loss = m.loss(tokens, target)
+            m.zero_grad()
+            loss.backward()
+        results.append([loss.detach(), *(p.grad for p in m.parameters()), *m.buffers()])
+    for a, b in zip(*results):
+        assert float((a.double() - b.double()).abs().max()) <= 1e-6 * float(a.double().abs().max())

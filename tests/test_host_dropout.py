@@ -1,11 +1,13 @@
-"""Dropout modules in several processes and as copies, on the host."""
+"""Dropout modules in several processes, as copies and in forward calls that a backward pass runs again, on the host."""
 import copy
 import os
 import tempfile
 
+import pytest
 import torch
 import torch.distributed as dist
 import torch.multiprocessing as mp
+from torch.utils.checkpoint import checkpoint
 
 import butterfly_amd as tb
 from butterfly_amd.rowwise import dropout_mask
@@ -69,3 +71,76 @@ def test_a_copy_with_a_seed_of_its_own():
     assert not torch.equal(layer(x), twin(x))
     twin.reseed(5)
     assert twin.rng.tolist() == [5, 0]
+
+
+@pytest.mark.parametrize("reentrant", [False, True])
+def test_a_call_that_is_run_again_drops_what_it_dropped(reentrant):
+    layer = tb.DropoutAdd(0.5)
+    x = torch.ones(16, 64, requires_grad=True)
+    y = checkpoint(layer, x, use_reentrant=reentrant)
+    y.sum().backward()
+    # (ones through the same mask, both ways)
+    assert torch.equal(x.grad, y.detach())
+    assert int(layer.rng[1]) == 1
+
+
+@pytest.mark.parametrize("reentrant", [False, True])
+def test_recomputed_blocks_give_the_gradients_of_kept_ones(reentrant):
+    torch.manual_seed(0)
+    blocks = torch.nn.ModuleList(torch.nn.Sequential(torch.nn.Linear(24, 24), tb.DropoutAdd(0.3), torch.nn.Tanh(), torch.nn.Linear(24, 24))
+                                 for _ in range(3))
+    shared = tb.DropoutAdd(0.2)     # called once a block and batch
+    x = torch.randn(5, 24)
+
+    def block(i, v):
+        return shared(blocks[i](v), v)
+
+    def step(again):
+        leaf = x.clone().requires_grad_()
+        outs = []
+        for scale in (1.0, 2.0):    # two batches in front of the backward pass
+            v = leaf * scale
+            for i in range(3):
+                v = checkpoint(block, i, v, use_reentrant=reentrant) if again else block(i, v)
+            outs.append(v)
+        total = outs[0].sum() + (outs[1] ** 2).sum()
+        blocks.zero_grad()
+        total.backward()
+        return [total.detach(), leaf.grad, *(p.grad.clone() for p in blocks.parameters())]
+
+    state = {k: v.clone() for k, v in blocks.state_dict().items()}, shared.rng.clone()
+    kept = step(False)
+    blocks.load_state_dict(state[0])
+    shared.rng.copy_(state[1])
+    for a, b in zip(kept, step(True)):
+        assert torch.allclose(a, b, rtol=1e-6, atol=1e-7)
+    assert int(shared.rng[1]) == int(state[1][1]) + 6
+
+
+def test_a_call_run_twice_again_and_calls_in_any_order():
+    layer = tb.DropoutAdd(0.5)
+    x = torch.ones(8, 64, requires_grad=True)
+    ys = [checkpoint(layer, x, use_reentrant=False) for _ in range(3)]
+    assert not torch.equal(ys[0], ys[1])
+    for k in (1, 1, 0, 2, 1):
+        dx, = torch.autograd.grad(ys[k], x, torch.ones_like(x), retain_graph=True)
+        assert torch.equal(dx, ys[k].detach())
+    assert int(layer.rng[1]) == 3
+
+
+def test_a_call_run_again_without_its_generator_is_refused():
+    layer = tb.DropoutAdd(0.5)
+    x = torch.ones(8, 64, requires_grad=True)
+    y = checkpoint(torch.nn.Sequential(layer, torch.nn.Tanh()), x, use_reentrant=False, preserve_rng_state=False)
+    torch.rand(1)
+    with pytest.raises(RuntimeError, match="preserve_rng_state"):
+        y.sum().backward()
+
+
+def test_ordinary_calls_draw_nothing_from_pytorch():
+    layer = tb.DropoutAdd(0.5)
+    torch.manual_seed(3)
+    want = torch.rand(4)
+    torch.manual_seed(3)
+    layer(torch.ones(4, 4, requires_grad=True)).sum().backward()
+    assert torch.equal(torch.rand(4), want)
