@@ -18,10 +18,20 @@ def linear_cross_entropy(hidden, weight, target, ignore_index=-100, reduction="m
         raise ValueError(f"reduction must be 'none', 'mean' or 'sum', got {reduction!r}")
     if hidden.is_cuda:
         return torch.ops.torch_butterfly.linear_cross_entropy(hidden, weight, target, ignore_index, _REDUCTIONS[reduction])
-    logits = F.linear(hidden, weight)
-    logits = logits if logits.dtype == torch.float64 else logits.float()
-    return F.cross_entropy(logits.flatten(0, -2), target.flatten(), ignore_index=ignore_index,
-                           reduction=reduction).reshape(target.shape if reduction == "none" else ())
+    return _host_loss(hidden, weight, target, ignore_index, reduction)
+
+
+def _host_loss(hidden, weight, target, ignore_index, reduction):
+    wide = torch.float64 if hidden.dtype == torch.float64 else torch.float32
+    logits, labels = F.linear(hidden.to(wide), weight.to(wide)).reshape(-1, weight.shape[0]), target.reshape(-1)
+    wrong = (labels != ignore_index) & ((labels < 0) | (labels >= weight.shape[0]))
+    if not wrong.any():
+        loss = F.cross_entropy(logits, labels, ignore_index=ignore_index, reduction=reduction)
+    else:
+        # (any entry that counts, times NaN)
+        loss = F.cross_entropy(logits, labels.masked_fill(wrong, int(ignore_index == 0)), ignore_index=ignore_index, reduction=reduction)
+        loss = loss * (torch.where(wrong, torch.nan, 1.0).to(wide) if reduction == "none" else torch.nan)
+    return loss.reshape(target.shape if reduction == "none" else ())
 
 
 class LinearCrossEntropy(nn.Module):
