@@ -28,7 +28,7 @@ def dropout_add(x, rng, p, residual=None):
     the inverse of the probability to stay.  A dropped element contributes zero whatever it is."""
     if x.is_cuda:
         return ops.dropout_add(x, rng, p, residual)
-    return _host_total(x, rng, p, residual)
+    return _host_total(x, rng, p, residual).to(x.dtype)
 
 
 def dropout_add_layer_norm(x, rng, p, residual=None, weight=None, bias=None, eps=1e-5):
@@ -36,7 +36,7 @@ def dropout_add_layer_norm(x, rng, p, residual=None, weight=None, bias=None, eps
     if x.is_cuda:
         return ops.dropout_add_layer_norm(x, rng, p, residual, weight, bias, eps)
     total = _host_total(x, rng, p, residual)
-    return _host_norm(total, weight, bias, eps), total
+    return _host_norm(total, weight, bias, eps).to(x.dtype), total.to(x.dtype)
 
 
 def rng_next(rng, replica=0):
@@ -76,20 +76,27 @@ def dropout_mask(rng, rows, cols, p):
     return torch.stack((words & 0xFFFF, words >> 16), -1).reshape(rows, groups * 8)[:, :cols] >= round(65536 * p)
 
 
+def _wide(x):
+    return x if x.dtype == torch.float64 else x.float()
+
+
 def _host_total(x, rng, p, residual):
+    """In float where the device's kernels are, to be rounded once."""
     if not 0 <= p <= 1:
         raise ValueError(f"p must be between 0 and 1, got {p}")
+    if p > 0 and rng is None:
+        raise RuntimeError("dropout: p > 0 needs rng")
     threshold = round(65536 * p)
-    total = x
+    total = _wide(x)
     if threshold > 0:
         keep = dropout_mask(rng, x.numel() // max(1, x.shape[-1]), x.shape[-1], p).reshape(x.shape)
         scale = 65536 / (65536 - threshold) if threshold < 65536 else 0.0
-        total = torch.where(keep, x * scale, torch.zeros((), dtype=x.dtype))
-    return total if residual is None else residual + total
+        total = torch.where(keep, total * scale, torch.zeros((), dtype=total.dtype))
+    return total if residual is None else _wide(residual) + total
 
 
 def _host_norm(x, weight, bias, eps):
-    wide = x if x.dtype == torch.float64 else x.float()
+    wide = _wide(x)
     centred = wide - wide.mean(-1, keepdim=True)
     y = centred * torch.rsqrt(centred.square().mean(-1, keepdim=True) + eps)
     if weight is not None:

@@ -1,4 +1,5 @@
-"""Dropout modules in several processes, as copies and in forward calls that a backward pass runs again, on the host."""
+"""Dropout modules in several processes, as copies in forward calls that a backward pass runs again, and in bfloat16, on the
+host."""
 import copy
 import os
 import tempfile
@@ -144,3 +145,26 @@ def test_ordinary_calls_draw_nothing_from_pytorch():
     torch.manual_seed(3)
     layer(torch.ones(4, 4, requires_grad=True)).sum().backward()
     assert torch.equal(torch.rand(4), want)
+
+
+def test_bfloat16_is_rounded_once():
+    """As in the device's kernels: product, sum and norm in float."""
+    gen = torch.Generator().manual_seed(0)
+    x, r = (torch.randn(40, 70, generator=gen).bfloat16() for _ in range(2))
+    w, b = torch.randn(2, 70, generator=gen)
+    rng, p = torch.tensor([3, 4]), 0.1
+    keep = dropout_mask(rng, 40, 70, p)
+    want = r.double() + keep * x.double() * (65536 / (65536 - round(65536 * p)))
+    assert torch.equal(tb.dropout_add(x, rng, p, r), want.float().bfloat16())
+    y, total = tb.dropout_add_layer_norm(x, rng, p, r, w, b)
+    assert y.dtype == total.dtype == torch.bfloat16
+    assert torch.equal(total, want.float().bfloat16())
+    norm = torch.nn.functional.layer_norm(want, (70,), w.double(), b.double())
+    # one rounding to eight bits (seven behind the leading one: half of 2^-7), and 2^-20 of float beside it
+    assert ((y.double() - norm).abs() <= (2.0 ** -8 + 2.0 ** -20) * norm.abs() + 2.0 ** -20).all()
+
+
+def test_a_probability_without_a_generator_is_refused():
+    with pytest.raises(RuntimeError, match="needs rng"):
+        tb.dropout_add(torch.ones(3, 4), None, 0.5)
+    assert torch.equal(tb.dropout_add(torch.ones(3, 4), None, 0.0), torch.ones(3, 4))
