@@ -101,10 +101,16 @@ int64_t row_count(const Tensor &t)
     return n;
 }
 
+// What the memory holds is what the tensor is (views of conjugates may say otherwise).
+Tensor plain(const Tensor &t) { return t.resolve_conj().resolve_neg(); }
+
+Tensor dense(const Tensor &t) { return t.defined() ? plain(t).contiguous() : Tensor(); }
+
 // A 2-d view (rows, columns) of a tensor with adjacent columns, or a copy.
 Tensor rows_of(const Tensor &t)
 {
-    Tensor r = t.dim() == 2 ? t : t.reshape({row_count(t), t.size(-1)});
+    Tensor r = plain(t);
+    if (r.dim() != 2) r = r.reshape({row_count(r), r.size(-1)});
     return r.size(1) > 1 && r.stride(1) != 1 ? r.contiguous() : r;
 }
 
@@ -194,9 +200,7 @@ Tensor rows_fw(const Rows &o, bool want_sum, Tensor *sum, Tensor *stats)
     bf_rowwise d = describe(o, o.x);
     d.x_stride = row_stride(x);
     if (residual.defined()) d.residual_stride = row_stride(residual);
-    const Tensor weight = o.weight.defined() ? o.weight.contiguous() : Tensor();
-    const Tensor bias = o.bias.defined() ? o.bias.contiguous() : Tensor();
-    const Tensor rng = o.rng.defined() ? o.rng.contiguous() : Tensor();
+    const Tensor weight = dense(o.weight), bias = dense(o.bias), rng = dense(o.rng);
     Tensor y, total;
     const auto options = o.x.options();
     if (o.norm) y = at::empty(o.x.sizes(), options);
@@ -264,7 +268,7 @@ struct RowsNode : public torch::autograd::Node {
         d.x_stride = row_stride(x);
         d.grad_y_stride = row_stride(g);
         if (more.defined()) d.grad_sum_stride = row_stride(more);
-        const Tensor w = o.weight.defined() ? o.weight.contiguous() : Tensor();
+        const Tensor w = dense(o.weight);
         // (without dropout the gradients of x and of the residual are one tensor)
         Tensor dx, dr;
         if (want_x && o.rng.defined()) dx = at::empty(shape, options);
@@ -399,7 +403,7 @@ struct Recurrence {
 
 Tensor adjacent(const Tensor &t)
 {
-    const Tensor r = t.resolve_conj();
+    const Tensor r = plain(t);
     return r.size(-1) > 1 && r.stride(-1) != 1 ? r.contiguous() : r;
 }
 
@@ -452,7 +456,7 @@ std::tuple<Tensor, Tensor> recurrence_fw(const Recurrence &o)
 {
     const Guard guard(o.x.device());
     const Tensor gate = adjacent(o.gate), x = adjacent(o.x);
-    const Tensor state = o.state.defined() ? o.state.resolve_conj().contiguous() : Tensor();
+    const Tensor state = dense(o.state);
     bf_recurrence d = describe(o, gate, x);
     Tensor h = at::empty(x.sizes(), x.options());
     Tensor last = at::empty({d.batch, d.channels}, x.options().dtype(state_type(x)));
@@ -488,9 +492,9 @@ struct RecurrenceNode : public torch::autograd::Node {
         at::AutoDispatchBelowADInplaceOrView below;
         const Guard guard(o.x.device());
         const Tensor z = adjacent(o.gate), v = adjacent(o.x), before = out_h.contiguous();
-        const Tensor first = o.state.defined() ? o.state.resolve_conj().contiguous() : Tensor();
+        const Tensor first = dense(o.state);
         const Tensor g = grads[0].defined() ? adjacent(grads[0]) : Tensor();
-        const Tensor gl = grads[1].defined() ? grads[1].resolve_conj().contiguous() : Tensor();
+        const Tensor gl = dense(grads[1]);
         bf_recurrence d = describe(o, z, v);
         if (g.defined()) batch_steps(d.grad_stride, g);
         out[0] = at::empty(v.sizes(), v.options());
@@ -561,7 +565,7 @@ Tensor gated_recurrence_step(Tensor gate, Tensor x, Tensor state, bool sigmoid)
     check_recurrence(o, 2);
     refuse_tangents({o.gate, o.x, o.state}, o.who);
     TORCH_CHECK(!any_wants_grad({o.gate, o.x, o.state}), o.who, ": has no gradient (use gated_recurrence, or torch.no_grad)");
-    TORCH_CHECK(state.is_contiguous() && !state.is_conj(), o.who, ": state must be contiguous, it is updated in place");
+    TORCH_CHECK(state.is_contiguous() && !state.is_conj() && !state.is_neg(), o.who, ": state must be contiguous, it is updated in place");
     at::AutoDispatchBelowADInplaceOrView below;
     const Guard guard(x.device());
     const Tensor z = adjacent(gate), v = adjacent(x);
@@ -635,7 +639,7 @@ struct XentNode : public torch::autograd::Node {
         const bool want_hidden = task_should_compute_output(0), want_weight = task_should_compute_output(1);
         at::AutoDispatchBelowADInplaceOrView below;
         const Guard guard(saved.device());
-        const Tensor w = aligned_rows_of(saved), g = grads[0].contiguous();
+        const Tensor w = aligned_rows_of(saved), g = dense(grads[0]);
         bf_linear_xent d = desc;
         d.weight_stride = row_stride(w);
         if (want_hidden) out[0] = at::empty(hidden_shape, w.options());
