@@ -268,7 +268,7 @@ struct RowsNode : public torch::autograd::Node {
         d.x_stride = row_stride(x);
         d.grad_y_stride = row_stride(g);
         if (more.defined()) d.grad_sum_stride = row_stride(more);
-        const Tensor w = dense(o.weight);
+        const Tensor w = dense(o.weight), state = dense(o.rng);
         // (without dropout the gradients of x and of the residual are one tensor)
         Tensor dx, dr;
         if (want_x && o.rng.defined()) dx = at::empty(shape, options);
@@ -277,7 +277,7 @@ struct RowsNode : public torch::autograd::Node {
         if (want_bias) out[3] = at::empty({d.cols}, options.dtype(param_type));
         const size_t bytes = want_weight || want_bias ? valid_size(bf_rowwise_bw_workspace_bytes(&d)) : 0;
         const Tensor ws = workspace_like(x, bytes);
-        check_rc(bf_rowwise_bw(&d, x.data_ptr(), g.data_ptr(), ptr(more), static_cast<const int64_t *>(ptr(o.rng)), ptr(w),
+        check_rc(bf_rowwise_bw(&d, x.data_ptr(), g.data_ptr(), ptr(more), static_cast<const int64_t *>(ptr(state)), ptr(w),
                                st.data_ptr<float>(), ptr(dx), ptr(dr), ptr(out[2]), ptr(out[3]), ptr(ws), bytes, current_stream()),
                  who);
         if (want_x) out[0] = dx.defined() ? dx : dr;

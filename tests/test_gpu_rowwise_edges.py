@@ -1,5 +1,5 @@
-"""Norms of rows whose offset is large beside their spread, in the backward pass; generators of several replicas; forward
-calls that a backward pass runs again.  Error measure and tolerances are those of the
+"""Norms of rows whose offset is large beside their spread, in the backward pass; generators of several replicas, and ones whose
+two numbers are not adjacent; forward calls that a backward pass runs again.  Error measure and tolerances are those of the
 row operators' other tests."""
 import copy
 
@@ -62,3 +62,14 @@ def test_recomputed_blocks_give_the_gradients_of_kept_ones(reentrant):
         results.append([loss.detach(), *(p.grad for p in m.parameters()), *m.buffers()])
     for a, b in zip(*results):
         assert float((a.double() - b.double()).abs().max()) <= 1e-6 * float(a.double().abs().max())
+
+
+def test_a_generator_whose_numbers_are_not_adjacent():
+    apart = torch.tensor([[3, 100], [4, 200]], device="cuda")[:, 0]
+    x, r, w, b = (randn(*s, seed=k).requires_grad_() for k, s in enumerate(((30, 70), (30, 70), (70,), (70,))))
+    results = []
+    for rng in (apart, apart.contiguous()):
+        y, total = tb.dropout_add_layer_norm(x, rng, 0.5, r, w, b)
+        results.append([y, total, *torch.autograd.grad(y, (x, r, w, b), torch.ones_like(y) + total.detach())])
+    for a, c in zip(*results):
+        assert torch.equal(a, c)
