@@ -108,6 +108,13 @@ int check_grid(const bf_recurrence *p, const RecurrencePlan &r)
     return BF_OK;
 }
 
+// Workgroups of sequences that stay whole, of up to 2^10 threads each: a dimension of a grid has less than 2^32 threads.
+dim3 whole_grid(const bf_recurrence *p, const RecurrencePlan &r)
+{
+    const int64_t total = r.groups * p->batch, x = std::min<int64_t>(total, 1 << 21);
+    return dim3((unsigned)x, (unsigned)((total + x - 1) / x));
+}
+
 // f(traits, sigmoid as a type)
 template <typename F>
 void with_kind(const bf_recurrence *p, F &&f)
@@ -174,7 +181,7 @@ int bf_recurrence_fw(const bf_recurrence *p, const void *gate, const void *x, co
             recurrence_enter_kernel<Tr, false><<<enter, dim3(64), 0, s>>>(a);
             recurrence_chunk_fw_kernel<Tr, SIG><<<grid, threads, 0, s>>>(a);
         } else {
-            recurrence_fw_kernel<Tr, SIG><<<dim3(x_blocks), dim3(64 * r.waves), 0, s>>>(a);
+            recurrence_fw_kernel<Tr, SIG><<<whole_grid(p, r), dim3(64 * r.waves), 0, s>>>(a);
         }
     });
     BF_HIP_CHECK(hipGetLastError());
@@ -216,7 +223,7 @@ int bf_recurrence_bw(const bf_recurrence *p, const void *gate, const void *x, co
             recurrence_enter_kernel<Tr, true><<<enter, dim3(64), 0, s>>>(a);
             recurrence_chunk_bw_kernel<Tr, SIG><<<grid, threads, 0, s>>>(a);
         } else {
-            recurrence_bw_kernel<Tr, SIG><<<dim3(x_blocks), dim3(64 * r.waves_bw), 0, s>>>(a);
+            recurrence_bw_kernel<Tr, SIG><<<whole_grid(p, r), dim3(64 * r.waves_bw), 0, s>>>(a);
         }
     });
     BF_HIP_CHECK(hipGetLastError());

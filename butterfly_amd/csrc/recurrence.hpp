@@ -252,6 +252,7 @@ struct RecPlace {
     using A = typename Tr::Acc;
     int lane, wave, waves, chunk, c, n;
     int64_t b, begin, end;     // the workgroup's steps
+    bool there;                // whether it has any (a grid in two dimensions may have more than there is work for)
 
     // Workgroups go to the eight XCDs in turn.  Rows seldom begin at a cache line, so the groups of channels of one
     // chunk belong on one XCD, behind each other, where a line that two of them share is in one L2: chunk k is XCD k % 8's
@@ -264,10 +265,12 @@ struct RecPlace {
         if (p.chunks > 1) {
             chunk = (int)(id / 8 / gridDim.x * 8 + xcd);
             x = (unsigned)(id / 8 % gridDim.x);
+            there = chunk < p.chunks;
         } else {
-            const unsigned per = gridDim.x / 8, over = gridDim.x % 8;
+            const uint64_t total = (uint64_t)p.batch * p.groups, per = total / 8, over = total % 8;
             chunk = 0;
             x = (unsigned)(xcd * per + (xcd < over ? xcd : over) + id / 8);
+            there = id < total;
         }
         b = x / (unsigned)p.groups;
         c = ((int)(x % (unsigned)p.groups) * 64 + lane) * Tr::V;
@@ -314,7 +317,7 @@ __device__ __forceinline__ void by_kind(bool plain, F &&f)
 }
 
 // ---- sequences that stay whole ---------------------------------------------------------------------------
-// grid (batch x groups); 64 x waves threads.  16 sequences of 2048 steps and 1024 channels, float: 83 us (402 MB, 4.8 TB/s),
+// grid: batch x groups workgroups in one or two dimensions; 64 x waves threads.  16 sequences of 2048 steps and 1024 channels, float: 83 us (402 MB, 4.8 TB/s),
 // backward 155 (805 MB, 5.2 TB/s): memory bounds both.
 template <typename Tr, bool SIG>
 __global__ __launch_bounds__(64 * kRecWaves) void recurrence_fw_kernel(RecurrenceArgs p)
@@ -324,6 +327,7 @@ __global__ __launch_bounds__(64 * kRecWaves) void recurrence_fw_kernel(Recurrenc
     constexpr int V = Tr::V, S = Tr::S;
     __shared__ Runs<Tr> runs;
     const RecPlace<Tr> at(p);
+    if (!at.there) return;
     const int c = at.c, n = at.n;
     const int64_t end = at.end;
     const RecLoad<Tr> in(c, n);
@@ -477,6 +481,7 @@ __global__ __launch_bounds__(64 * kRecWaves) void recurrence_bw_kernel(Recurrenc
     constexpr int V = Tr::V, S = Tr::SB;
     __shared__ Runs<Tr> runs;
     const RecPlace<Tr> at(p);
+    if (!at.there) return;
     const int64_t end = at.end;
     const RecLoad<Tr> in(at.c, at.n);
     A carry[V];
@@ -531,7 +536,7 @@ __global__ __launch_bounds__(64 * kRecWaves, 8) void recurrence_runs_kernel(Recu
     constexpr int V = Tr::V, S = Tr::SR;
     __shared__ Runs<Tr> runs;
     const RecPlace<Tr> at(p);
-    if (at.chunk >= p.chunks) return;
+    if (!at.there) return;
     const RecLoad<Tr> in(at.c, at.n);
     const int64_t len = p.chunk / kRecWaves, begin = at.begin + at.wave * len;
     const int64_t end = begin + len < at.end ? begin + len : at.end;
@@ -678,7 +683,7 @@ __global__ __launch_bounds__(64 * kRecWaves) void recurrence_chunk_fw_kernel(Rec
     using E = typename Tr::Elem;
     constexpr int V = Tr::V, S = Tr::S;
     const RecPlace<Tr> at(p);
-    if (at.chunk >= p.chunks) return;
+    if (!at.there) return;
     const int c = at.c, n = at.n;
     const RecLoad<Tr> in(c, n);
     const int64_t len = p.chunk / kRecWaves, begin = at.begin + at.wave * len;
@@ -730,7 +735,7 @@ __global__ __launch_bounds__(64 * kRecWaves) void recurrence_chunk_bw_kernel(Rec
     using A = typename Tr::Acc;
     constexpr int V = Tr::V, S = Tr::SB;
     const RecPlace<Tr> at(p);
-    if (at.chunk >= p.chunks) return;
+    if (!at.there) return;
     const RecLoad<Tr> in(at.c, at.n);
     const int64_t len = p.chunk / kRecWaves, begin = at.begin + at.wave * len;
     const int64_t end = begin + len < at.end ? begin + len : at.end;

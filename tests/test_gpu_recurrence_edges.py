@@ -1,4 +1,4 @@
-"""Linear gates above one: their products over a run of steps pass the range of the numbers long before a sequence does that has
+"""More sequences than one dimension of a grid has workgroups for.  Linear gates above one: their products over a run of steps pass the range of the numbers long before a sequence does that has
 nothing to be multiplied.  Tolerances are those of the recurrence's other tests."""
 import pytest
 import torch
@@ -69,3 +69,20 @@ def test_a_gate_of_zero_ends_what_grew(dtype):
     ref = reference(v, False)
     close(h, ref["h"], TOL[dtype], "h")
     close(last, ref["last"], 1e-5, "last")
+
+
+def test_more_sequences_than_a_dimension_of_a_grid():
+    """Workgroups of 1024 threads: 2^22 of them are 2^32 threads."""
+    batch, steps = (1 << 22) + 5, 130
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    gate, x, grad = (torch.randn(batch, steps, 1, device="cuda", generator=gen) for _ in range(3))
+    some = torch.cat((torch.arange(70), torch.arange((1 << 21) - 70, (1 << 21) + 70), torch.arange(batch - 70, batch))).cuda()
+
+    def run(gate, x, grad):
+        gate, x = gate.requires_grad_(), x.requires_grad_()
+        h, last = tb.gated_recurrence(gate, x)
+        return h.detach(), last.detach(), *torch.autograd.grad(h, (gate, x), grad)
+
+    alone = run(gate[some], x[some], grad[some])
+    for a, b in zip(run(gate, x, grad), alone):
+        assert torch.equal(a[some], b)
