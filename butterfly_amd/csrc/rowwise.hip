@@ -28,6 +28,8 @@ int check_rows(const bf_rowwise *p)
         return fail(BF_ERR_INVALID, "strides must be non-negative");
     if (!(p->drop_probability >= 0.0 && p->drop_probability <= 1.0))
         return fail(BF_ERR_INVALID, "drop_probability must be in [0, 1]");
+    // (the generator's counter takes a row's number in 32 bits)
+    if (p->drop_probability > 0.0 && p->rows > ((int64_t)1 << 32)) return fail(BF_ERR_UNSUPPORTED, "dropout of more than 2^32 rows is not supported");
     if (!(p->eps >= 0.0)) return fail(BF_ERR_INVALID, "eps must be non-negative");
     return BF_OK;
 }

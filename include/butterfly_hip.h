@@ -322,7 +322,7 @@ typedef struct bf_rowwise {
 } bf_rowwise;
 
 /* The generator of dropped elements is Philox4x32-10: key = the 64 bits of rng[0] (a seed), counter =
- * (column / 8, row, low and high half of rng[1] (the number of the call)); column c of a row takes
+ * (column / 8, row (of up to 2^32), low and high half of rng[1] (the number of the call)); column c of a row takes
  * bits 16 (c % 2) .. + 15 of word (c % 8) / 2 and is kept where they are >= t, scaled by
  * 65536 / (65536 - t).  No mask is stored: forward and backward make the same one from rng, two
  * device integers.
