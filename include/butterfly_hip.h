@@ -404,8 +404,9 @@ typedef struct bf_linear_xent {
  * products' form (and their log-sum-exps): hidden's counted rows and, where it cannot be read as it lies (float, rows that 16
  * bytes do not divide), weight; of few rows hidden and their logits.  A call without a backward one gives it the same
  * room.  The workspaces (256-byte aligned) hold 16 bytes for each row and 256 (128; few rows: 64 or 16) entries forward,
- * and backward the logits' gradient over a piece of the vocabulary, up to some 256 MiB (few rows: all of it, twice),
- * and the sums of d_hidden's and d_weight's parts.                                               */
+ * and backward the logits' gradient over a piece of the vocabulary of some 256 MiB, or of 2048 entries where those are more
+ * (4 KiB a row, float 8; few rows: all of it, twice), the sums of d_hidden's and d_weight's parts and, float with
+ * BF_XENT_NONE, hidden's counted rows once more.                                                 */
 size_t bf_linear_xent_kept_bytes(const bf_linear_xent *p);
 size_t bf_linear_xent_fw_workspace_bytes(const bf_linear_xent *p);
 size_t bf_linear_xent_bw_workspace_bytes(const bf_linear_xent *p);

@@ -16,3 +16,18 @@ def test_masks_of_more_rows_than_the_generator_counts_are_refused():
     assert L.bf_rowwise_bw_workspace_bytes(ctypes.byref(r)) < _capi.SIZE_INVALID
     r.drop_probability, r.rows = 0.5, 1 << 32
     assert L.bf_rowwise_bw_workspace_bytes(ctypes.byref(r)) < _capi.SIZE_INVALID
+
+
+def test_workspace_of_a_loss_of_many_rows():
+    """A piece of the vocabulary has 2048 entries at least: 4 KiB a row and 8 of float pairs, whatever the vocabulary."""
+    L = _capi.lib()
+    for dtype, elem in ((2, 2), (0, 4)):
+        for rows in (1 << 16, 1 << 20):
+            x = _capi.LinearXent(dtype=dtype, reduction=1, rows=rows, features=1024, vocab=1 << 17, hidden_stride=1024, weight_stride=1024)
+            d_l = max(256 << 20, rows * 2048 * elem)
+            # d_hidden's sums (one part), d_weight's over the piece (some parts), a number a row
+            sums = rows * 1024 * 4 + (64 << 20) + rows * 4
+            assert L.bf_linear_xent_bw_workspace_bytes(ctypes.byref(x)) < d_l + sums + (1 << 20)
+            x.reduction = 0
+            shared = rows * 1024 * 4 if dtype == 0 else 0
+            assert L.bf_linear_xent_bw_workspace_bytes(ctypes.byref(x)) < d_l + sums + shared + (1 << 20)
