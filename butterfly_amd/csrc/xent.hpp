@@ -255,6 +255,9 @@ constexpr float kLog2e = 1.44269504088896340736f;
 // exp(l - v) is formed as exp2(l log2(e) + from), from = -v log2(e) rounded; the factor that undoes the rounding.
 __device__ __forceinline__ float rounded_off(float v, float from) { return __builtin_amdgcn_exp2f(-fmaf(v, kLog2e, from)); }
 
+// Beyond it that factor, 2^(half a unit of v log2(e)), would itself pass the range (from 2^31 on): there v is taken off first.
+__device__ __forceinline__ bool is_far(float v) { return fabsf(v) > 0x1p24f && fabsf(v) < INFINITY; }
+
 // Workgroups stay for tile after tile (grid: as many as the chip holds at a time), so that a tile's exponentials and
 // stores run while the next one's operands arrive: 512 rows (461 counted), 4096 features, 65536 entries, bfloat16 in 230 us
 // (1.08 PFLOP/s; 1.20 with the rows that only fill up a tile), 572 (515) x 2659 x 24269 float by small tiles in 271.
@@ -323,7 +326,13 @@ __global__ __launch_bounds__(mat_threads(BM, BN, BUFFERS), 1) void xent_logits_k
                 top = fmaxf(top, __shfl_xor(top, 16, 64));
                 top = fmaxf(top, __shfl_xor(top, 32, 64));
                 // (NaN is no maximum, and an infinite one would make NaN of its own term: both show in the sum)
-                const float at = top == -INFINITY ? 0.0f : top, from = -at * kLog2e;
+                float at = top == -INFINITY ? 0.0f : top;
+                if (__any(is_far(at))) {
+#pragma unroll
+                    for (int i = 0; i < Tile::kMT; ++i) acc[i][j] = acc[i][j] - at;
+                    at = 0.0f;
+                }
+                const float from = -at * kLog2e;
                 float sum = 0.0f;
 #pragma unroll
                 for (int i = 0; i < Tile::kMT; ++i)
@@ -335,7 +344,14 @@ __global__ __launch_bounds__(mat_threads(BM, BN, BUFFERS), 1) void xent_logits_k
             } else {
                 const float share = there ? a.share ? a.share[row] : 1.0f : 0.0f;
                 // (no share: the exponentials of minus infinity, zeros)
-                const float lse = share != 0.0f ? a.lse[row] : INFINITY, from = -lse * kLog2e;
+                float lse = share != 0.0f ? a.lse[row] : INFINITY;
+                if (__any(is_far(lse))) {
+                    const float off = is_far(lse) ? lse : 0.0f;
+#pragma unroll
+                    for (int i = 0; i < Tile::kMT; ++i) acc[i][j] = acc[i][j] - off;
+                    lse -= off;
+                }
+                const float from = -lse * kLog2e;
                 const float exact = share != 0.0f ? rounded_off(lse, from) : 1.0f;
 #pragma unroll
                 for (int i = 0; i < Tile::kMT; ++i)

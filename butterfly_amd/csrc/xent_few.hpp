@@ -306,7 +306,12 @@ __device__ __forceinline__ void few_logits(const XentFewLogitsArgs &a, int64_t f
         }
         top = fmaxf(top, __shfl_xor(top, 16, 64));
         top = fmaxf(top, __shfl_xor(top, 32, 64));
-        const float at = top == -INFINITY ? 0.0f : top, from = -at * kLog2e;
+        float at = top == -INFINITY ? 0.0f : top;
+        if (is_far(at)) {
+            l = l - at;
+            at = 0.0f;
+        }
+        const float from = -at * kLog2e;
         float sum = 0.0f;
 #pragma unroll
         for (int r = 0; r < 4; ++r) sum += __builtin_amdgcn_exp2f(fmaf(l[r], kLog2e, from));
@@ -405,10 +410,11 @@ __global__ __launch_bounds__(64 * NT) void xent_few_dl_kernel(XentFewDlArgs a)
     if (place < a.scalars->counted) {
         const float share = a.grad.each ? a.grad.grad[a.index[place]] : 1.0f;
         if (share != 0.0f) {
-            const float lse = a.lse[place], from = -lse * kLog2e, exact = rounded_off(lse, from);
+            const float far = is_far(a.lse[place]) ? a.lse[place] : 0.0f;
+            const float lse = a.lse[place] - far, from = -lse * kLog2e, exact = rounded_off(lse, from);
             const int64_t label = a.label[place] - v;
             const Acc4 *l = reinterpret_cast<const Acc4 *>(a.logits + place * a.stride + v);
-            const Acc4 lo = l[0], hi = l[1];
+            const Acc4 lo = l[0] - far, hi = l[1] - far;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 const float p = __builtin_amdgcn_exp2f(fmaf(j < 4 ? lo[j & 3] : hi[j & 3], kLog2e, from)) * exact;

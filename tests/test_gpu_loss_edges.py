@@ -129,3 +129,19 @@ def test_a_weight_whose_features_are_not_adjacent_is_copied_once():
     before = torch.cuda.memory_stats()["allocated_bytes.all.allocated"]
     tb.linear_cross_entropy(hidden, columns, target)
     assert torch.cuda.memory_stats()["allocated_bytes.all.allocated"] - before < 1.5 * weight.numel() * 2
+
+
+@pytest.mark.parametrize("up", [1e5, 1e7, 1e10, 1e15])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows", [40, 90, 700])
+def test_logits_of_any_size(rows, dtype, up):
+    """A softmax of far larger logits is one-hot but for ties: losses off by 2^-20 of the logits (1e-5 of the largest loss), and
+    gradients of at most two rows' sum."""
+    hidden, weight, target = make(rows, 64, 1000, dtype, ignored=0.0)
+    h, w = (hidden * up).requires_grad_(), (weight * up).requires_grad_()
+    each = tb.linear_cross_entropy(h, w, target, reduction="none")
+    want, _, _ = reference(h, w, target, torch.ones(rows, device="cuda"), "none")
+    assert (each.double() - want).abs().max() <= 1e-5 * (1 + want.abs().max())
+    dh, dw = torch.autograd.grad(each, (h, w), torch.ones_like(each))
+    assert torch.isfinite(dh).all() and float(dh.abs().max()) <= 2.1 * float(w.abs().max())
+    assert torch.isfinite(dw).all() and float(dw.abs().max()) <= 1.1 * rows * float(h.abs().max())
