@@ -52,7 +52,7 @@ struct MatOperand {
     int64_t plane;         // bytes between planes
     int64_t stride;        // bytes between rows
     int64_t bytes;         // of a plane from base on that may be read: loads beyond are zero
-    int tail;              // kRows: bytes of a row's last k step that are the row's (multiples of 16): what is behind, to 128, is zero
+    int tail;              // kRows, the first operand: bytes of a row's last k step that are the row's (multiples of 16): what is behind, to 128, is zero
 };
 
 constexpr int kWholeTail = kMatK * 2;
@@ -179,9 +179,10 @@ struct MatFeed {
         load_unit_to_lds(desc, to, path.lane_offset[path.variant(j)], path.load_offset[j]);
     }
     __device__ __forceinline__ void advance() { path.advance(); }
+    // (the lane's number made anew: no register holds it until here)
     __device__ __forceinline__ void cut(const MatOperand &o)
     {
-        if (LAYOUT == kRows && o.tail < kWholeTail) path.cut(o, threadIdx.x & 63);
+        if (LAYOUT == kRows && o.tail < kWholeTail) path.cut(o, __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0)));
     }
 };
 
@@ -312,10 +313,8 @@ struct MatTiles {
             feed_b.start(b, n0, first + (nothing ? 0 : fed), F16 && pass == 0, nothing);
             until = min(count - fed, min(feed_a.steps(), feed_b.steps())) + fed;
         }
-        if (++fed == count) {
-            feed_a.cut(a);
-            feed_b.cut(b);
-        }
+        // (float operands and b have rows of whole steps)
+        if (++fed == count && !F16) feed_a.cut(a);
     }
     __device__ __forceinline__ void feed_load(unsigned to, int i)
     {
