@@ -145,3 +145,22 @@ def test_logits_of_any_size(rows, dtype, up):
     dh, dw = torch.autograd.grad(each, (h, w), torch.ones_like(each))
     assert torch.isfinite(dh).all() and float(dh.abs().max()) <= 2.1 * float(w.abs().max())
     assert torch.isfinite(dw).all() and float(dw.abs().max()) <= 1.1 * rows * float(h.abs().max())
+
+
+@pytest.mark.parametrize("rows", [50, 100, 1000])
+def test_unlikely_entries_keep_their_bits(rows):
+    """Every entry of the weight's gradient by itself: sums of the entry's probabilities, all of one size.  float32: 2^-20 of a
+    logit of up to 28, and pairs of 22 bits for probabilities from 2^-28 up, of 11 down to 2^-40."""
+    gen = torch.Generator().manual_seed(rows)
+    logits = -torch.linspace(0, 40, 401, dtype=torch.float64) * torch.log(torch.tensor(2.0, dtype=torch.float64))
+    h, w = torch.zeros(rows, 64), torch.zeros(401, 64)
+    h[:, 0], w[:, 0] = 1.0, logits.float()
+    h[:, 1:] = torch.rand(rows, 63, generator=gen)      # (against weights of zero)
+    h, w = h.cuda().requires_grad_(), w.cuda().requires_grad_()
+    target = torch.zeros(rows, dtype=torch.int64, device="cuda")
+    dw, = torch.autograd.grad(tb.linear_cross_entropy(h, w, target, reduction="sum"), w)
+    _, _, want = reference(h, w, target, torch.ones((), device="cuda"), "sum")
+    off = ((dw.double() - want).abs() / want.abs()).amax(1).cpu()
+    p = torch.softmax(w.detach()[:, 0].double(), 0).cpu()
+    assert off[p >= 2.0 ** -28].max() < 5e-5
+    assert off[p >= 2.0 ** -40].max() < 2.0 ** -11
