@@ -46,8 +46,8 @@ constexpr int mat_threads(int bm, int bn, int buffers) { return 64 * mat_waves(b
 
 enum MatLayout { kRows, kCols };
 
-// Values in two f16 halves (hi + lo) are two planes; a product then runs over hi lo + lo hi + hi hi.  The second operand's lower
-// halves may be kept times 2^kRaised (MatTiles' RAISED), so that they reach further below the upper ones.
+// Values in two f16 halves (hi + lo) are two planes; a product then runs over hi lo + lo hi + hi hi.  The lower halves are kept
+// times 2^kRaised, so that they reach further below the upper ones; the sums of the first two products are divided by it.
 constexpr int kRaised = 11;
 
 struct MatOperand {
@@ -257,7 +257,7 @@ __device__ __forceinline__ void mfma_settle(Acc4 (&acc)[MT][NT])
 // asked for, across the boundary between two tiles too, so the next tile's first steps arrive while the
 // sums of the one before are dealt with.  acc[mt][nt][r] is element (m, n) with n = n0 + kPartN wave_n() + 16 nt +
 // lane % 16 and m = m0 + kPartM wave_m() + what tile_row() says.  F16: both operands in two planes.
-template <MatLayout LA, MatLayout LB, bool F16, int BM, int BN, int BUFFERS, bool SPREAD, bool RAISED = false>
+template <MatLayout LA, MatLayout LB, bool F16, int BM, int BN, int BUFFERS, bool SPREAD>
 struct MatTiles {
     static constexpr int kWaves = mat_waves(BM, BN, BUFFERS), kWavesM = 2, kWavesN = kWaves / kWavesM;
     static constexpr int kPartM = BM / kWavesM, kPartN = BN / kWavesN;     // a wavefront's part
@@ -417,8 +417,7 @@ struct MatTiles {
         mfma_settle(acc);
         for (int s = 0; s < steps * kPasses; ++s) {
             step(next, acc);
-            // the first pass is b's lower halves
-            if (RAISED && s == steps - 1) {
+            if (F16 && s == 2 * steps - 1) {
                 mfma_settle(acc);
 #pragma unroll
                 for (int i = 0; i < kMT; ++i)

@@ -21,9 +21,8 @@
 // of such a model.  float operands are split, x 2^e = hi + lo in two float16 numbers of together 22 bits,
 // e the power of two that brings the operand's largest number to 2^14 .. 2^15 (one for hidden, one for
 // weight; d_l is at most one, e = 15), and a product is hi lo + lo hi + hi hi with sums in float: three
-// products at the 16-bit rate, 16 times that of float ones on this card, for a relative error of 2^-22 a factor, as long as
-// numbers are within 2^-17 of the largest (below that an absolute error of 2^-39 of it).  d_l, which spans far more, has its
-// lower halves times 2^11, undone on the sums between the products: 22 bits from 2^-28 up, 11 from 2^-40, none below 2^-51.
+// products at the 16-bit rate, 16 times that of float ones on this card, for a relative error of 2^-22 a factor.  The lower
+// halves are kept times 2^11: numbers from 2^-28 of the largest up have their 22 bits, from 2^-40 eleven, below 2^-51 none.
 // With one gradient a row d_l is
 // without it in float (rows of small ones would lose their bits): d_hidden's rows are multiplied at the end, and d_weight's
 // product takes hidden's rows times their share of the largest.
@@ -147,13 +146,12 @@ __device__ __forceinline__ float scale_of(unsigned bits)
     return __uint_as_float((unsigned)((up > 100 ? 100 : up) + 127) << 23);
 }
 
-// Two numbers' upper and lower float16 halves, the lower ones times 2^RAISED.  The numbers are hidden from the compiler: rounded from the
+// Two numbers' upper and lower float16 halves, the lower ones times 2^kRaised.  The numbers are hidden from the compiler: rounded from the
 // product that made one of them, not from the number itself, an upper half could be another one than
 // the lower half is the rest to.
-template <int RAISED = 0>
 __device__ __forceinline__ void split_f16(float a, float b, uint32_t &high, uint32_t &low)
 {
-    constexpr float kFactor = 1 << RAISED;
+    constexpr float kFactor = 1 << kRaised;
     typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
     asm("" : "+v"(a), "+v"(b));
     const f16x2 h = {(_Float16)a, (_Float16)b};
@@ -161,6 +159,8 @@ __device__ __forceinline__ void split_f16(float a, float b, uint32_t &high, uint
     high = __builtin_bit_cast(uint32_t, h);
     low = __builtin_bit_cast(uint32_t, l);
 }
+
+__device__ __forceinline__ float whole(_Float16 high, _Float16 low) { return fmaf((float)low, 1.0f / (1 << kRaised), (float)high); }
 
 struct XentPackArgs {
     const void *x;
@@ -385,8 +385,8 @@ __global__ __launch_bounds__(mat_threads(BM, BN, BUFFERS), 1) void xent_logits_k
                     for (int k = 0; k < 4; ++k) {
                         const Acc4 p = acc[i + k][j] * factor;
                         if constexpr (F16) {
-                            split_f16<kRaised>(p[0], p[1], w[2 * k], low[2 * k]);
-                            split_f16<kRaised>(p[2], p[3], w[2 * k + 1], low[2 * k + 1]);
+                            split_f16(p[0], p[1], w[2 * k], low[2 * k]);
+                            split_f16(p[2], p[3], w[2 * k + 1], low[2 * k + 1]);
                         } else {
                             w[2 * k] = pack_bf16(p[0], p[1]);
                             w[2 * k + 1] = pack_bf16(p[2], p[3]);
@@ -522,7 +522,7 @@ __global__ __launch_bounds__(256) void xent_shared_kernel(XentSharedArgs a)
             const f16x8 h = *reinterpret_cast<const f16x8 *>(a.hidden + at), l = *reinterpret_cast<const f16x8 *>(a.hidden + a.plane + at);
 #pragma unroll
             for (int k = 0; k < 4; ++k)
-                split_f16(((float)h[2 * k] + (float)l[2 * k]) * share, ((float)h[2 * k + 1] + (float)l[2 * k + 1]) * share, w[k], low[k]);
+                split_f16(whole(h[2 * k], l[2 * k]) * share, whole(h[2 * k + 1], l[2 * k + 1]) * share, w[k], low[k]);
         }
         *reinterpret_cast<uint4 *>(a.out + at) = make_uint4(w[0], w[1], w[2], w[3]);
         *reinterpret_cast<uint4 *>(a.out + a.plane + at) = make_uint4(low[0], low[1], low[2], low[3]);
@@ -553,7 +553,7 @@ template <typename T, MatLayout LB, int BM, int BN, int BUFFERS>
 __global__ __launch_bounds__(mat_threads(BM, BN, BUFFERS), 1) void xent_grad_kernel(XentGradArgs a)
 {
     constexpr bool F16 = sizeof(T) == 4, OF_WEIGHT = LB == kCols;
-    using Tile = MatTiles<kCols, LB, F16, BM, BN, BUFFERS, false, F16>;
+    using Tile = MatTiles<kCols, LB, F16, BM, BN, BUFFERS, false>;
     __shared__ __attribute__((aligned(1024))) char lds[Tile::kLds];
     const int counted = a.scalars->counted;
     const int tiles_n = OF_WEIGHT ? a.tiles_n : (counted + BN - 1) / BN, tiles = a.tiles_m * tiles_n;

@@ -164,3 +164,29 @@ def test_unlikely_entries_keep_their_bits(rows):
     p = torch.softmax(w.detach()[:, 0].double(), 0).cpu()
     assert off[p >= 2.0 ** -28].max() < 5e-5
     assert off[p >= 2.0 ** -40].max() < 2.0 ** -11
+
+
+@pytest.mark.parametrize("rows", [50, 100, 700])
+def test_float_rows_and_features_of_unlike_scale(rows):
+    """Numbers from 2^-28 of the operand's largest up keep 22 bits, and a few below that 20."""
+    hidden, weight, target = make(rows, 64, 1000, torch.float32, ignored=0.0)
+    ones = torch.ones(rows, device="cuda")
+    # features: every product as it was
+    scale = torch.full((64,), 2.0 ** 13, device="cuda")
+    scale[::2] = 2.0 ** -13
+    h, w = (hidden * scale).requires_grad_(), (weight / scale).requires_grad_()
+    each = tb.linear_cross_entropy(h, w, target, reduction="none")
+    want, want_h, want_w = reference(h, w, target, ones, "none")
+    assert (each.double() - want).abs().max() <= 1e-5 * (1 + want.abs().max())
+    dh, dw = torch.autograd.grad(each, (h, w), ones)
+    for part in (slice(0, None, 2), slice(1, None, 2)):
+        assert err(dh[:, part], want_h[:, part]) < TOL[torch.float32] and err(dw[:, part], want_w[:, part]) < TOL[torch.float32]
+    # rows: ordinary logits beside enormous ones
+    h, w = hidden * 2.0 ** 13, (weight * 2.0 ** 13).requires_grad_()
+    h[::2] = hidden[::2] * 2.0 ** -13
+    h.requires_grad_()
+    each = tb.linear_cross_entropy(h, w, target, reduction="none")
+    want, want_h, _ = reference(h, w, target, ones, "none")
+    assert (each[::2].double() - want[::2]).abs().max() <= 1e-5 * (1 + want[::2].abs().max())
+    dh, = torch.autograd.grad(each, h, ones)
+    assert err(dh[::2], want_h[::2]) < TOL[torch.float32]
