@@ -376,52 +376,59 @@ __global__ __launch_bounds__(row_threads<L>()) void norm_bw_kernel(RowArgs a)
 
 constexpr int kWideThreads = 1024;
 
-template <int N>
-__device__ __forceinline__ void block_sum(float (&v)[N], float (*lds)[16][N], int turn)
+__device__ __forceinline__ float2 block_sum(float2 v, float2 (*lds)[16], int turn)
 {
-#pragma unroll
-    for (int n = 0; n < N; ++n) {
-        v[n] = lanes_sum<64>(v[n]);
-        if ((threadIdx.x & 63) == 0) lds[turn][threadIdx.x >> 6][n] = v[n];
-    }
+    v = make_float2(lanes_sum<64>(v.x), lanes_sum<64>(v.y));
+    if ((threadIdx.x & 63) == 0) lds[turn][threadIdx.x >> 6] = v;
     __syncthreads();
-#pragma unroll
-    for (int n = 0; n < N; ++n) {
-        v[n] = 0.0f;
-        for (int i = 0; i < kWideThreads / 64; ++i) v[n] += lds[turn][i][n];
+    v = make_float2(0.0f, 0.0f);
+    for (int i = 0; i < kWideThreads / 64; ++i) v = make_float2(v.x + lds[turn][i].x, v.y + lds[turn][i].y);
+    return v;
+}
+
+// (three sums; the fourth is nothing)
+__device__ __forceinline__ float4 block_sum(float4 v, float4 (*lds)[16], int turn)
+{
+    v = make_float4(lanes_sum<64>(v.x), lanes_sum<64>(v.y), lanes_sum<64>(v.z), 0.0f);
+    if ((threadIdx.x & 63) == 0) lds[turn][threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int i = 0; i < kWideThreads / 64; ++i) {
+        const float4 p = lds[turn][i];
+        v = make_float4(v.x + p.x, v.y + p.y, v.z + p.z, 0.0f);
     }
+    return v;
 }
 
 template <typename T>
 __global__ __launch_bounds__(kWideThreads) void norm_fw_wide_kernel(RowArgs a)
 {
-    __shared__ float lds[2][16][2];
+    __shared__ float2 lds[2][16];
     const Dropper drop(a);
     const float inv = 1.0f / (float)a.cols;
     for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
         float v[8];
-        float s[2] = {};
+        float2 s = make_float2(0.0f, 0.0f);
         for (int col = threadIdx.x * 8; col < a.cols; col += kWideThreads * 8) {
             total8<T>(a, drop, row, col, v);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) s[0] += v[i];
+            for (int i = 0; i < 8; ++i) s.x += v[i];
         }
         Moments m;
-        block_sum(s, lds, 0);
-        m.base = s[0] * inv;
-        s[0] = s[1] = 0.0f;
+        m.base = block_sum(s, lds, 0).x * inv;
+        s = make_float2(0.0f, 0.0f);
         for (int col = threadIdx.x * 8; col < a.cols; col += kWideThreads * 8) {
             total8<T>(a, drop, row, col, v);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 const float d = col + i < a.cols ? v[i] - m.base : 0.0f;
-                s[0] += d;
-                s[1] = fmaf(d, d, s[1]);
+                s.x += d;
+                s.y = fmaf(d, d, s.y);
             }
         }
-        block_sum(s, lds, 1);
-        m.shift = s[0] * inv;
-        m.m2 = s[1] - s[0] * m.shift;
+        s = block_sum(s, lds, 1);
+        m.shift = s.x * inv;
+        m.m2 = s.y - s.x * m.shift;
         if (m.m2 < 0.0f) m.m2 = 0.0f;
         const float rstd = 1.0f / sqrtf(m.m2 * inv + a.eps);
         if (a.stats && threadIdx.x == 0) a.stats[row] = make_float2(m.mean(), rstd);
@@ -441,7 +448,7 @@ __global__ __launch_bounds__(kWideThreads) void norm_fw_wide_kernel(RowArgs a)
 template <typename T>
 __global__ __launch_bounds__(kWideThreads) void norm_bw_wide_kernel(RowArgs a)
 {
-    __shared__ float lds[2][16][3];
+    __shared__ float4 lds[2][16];
     const Dropper drop(a);
     const float inv = 1.0f / (float)a.cols;
     int turn = 0;
@@ -450,7 +457,7 @@ __global__ __launch_bounds__(kWideThreads) void norm_bw_wide_kernel(RowArgs a)
         const T *gy = reinterpret_cast<const T *>(a.grad_y) + row * a.grad_y_stride;
         const float2 st = a.stats[row];
         float u[8], g[8], w[8];
-        float c[3] = {};   // of gw, gw u and u
+        float4 c = make_float4(0.0f, 0.0f, 0.0f, 0.0f);   // of gw, gw u and u
         for (int col = threadIdx.x * 8; col < a.cols; col += kWideThreads * 8) {
             load8(x, col, a.cols, st.x, u);
             load8(gy, col, a.cols, 0.0f, g);
@@ -459,14 +466,14 @@ __global__ __launch_bounds__(kWideThreads) void norm_bw_wide_kernel(RowArgs a)
             for (int i = 0; i < 8; ++i) {
                 g[i] *= w[i];
                 u[i] = (u[i] - st.x) * st.y;
-                c[0] += g[i];
-                c[1] = fmaf(g[i], u[i], c[1]);
-                c[2] += u[i];
+                c.x += g[i];
+                c.y = fmaf(g[i], u[i], c.y);
+                c.z += u[i];
             }
         }
-        block_sum(c, lds, turn);
+        c = block_sum(c, lds, turn);
         turn ^= 1;
-        const float c1 = c[0] * inv, delta = c[2] * inv, c2 = fmaf(-delta, c1, c[1] * inv);
+        const float c1 = c.x * inv, delta = c.z * inv, c2 = fmaf(-delta, c1, c.y * inv);
         if (a.shift && threadIdx.x == 0) a.shift[row] = delta;
         if (!a.d_x && !a.d_residual) continue;
         for (int col = threadIdx.x * 8; col < a.cols; col += kWideThreads * 8) {
