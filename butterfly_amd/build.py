@@ -37,6 +37,9 @@ def _run(cmd):
 # between request and wait, i.e. while nothing spills to scratch memory.  (Scalar registers that the
 # compiler parks in the lanes of a vector register -- "SGPRs Spill" with a scratch size of 0 -- move
 # no memory and are allowed: the forward variants compiled for eight wavefronts per SIMD have a few.)
+# The matrix products of the loss count their loads into LDS too and are not among them: their counts say how many
+# of the newest operations may still be on their way, operations complete in order, and spilled registers only add newer
+# ones, so that the wait covers more than it must.
 GATED_KERNELS = ("fast_fw_kernel", "fast_bw_kernel", "wide_fw_kernel", "fast4_fw_kernel", "fast4_bw_kernel",
                  "fast4g_fw_kernel", "fast4g_bw_kernel")
 RESOURCES = os.path.join(PKG, "kernel_resources.txt")

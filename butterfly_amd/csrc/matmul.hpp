@@ -12,7 +12,7 @@
 // there are enough of them.
 //
 // What bounds it: the matrix units at the clock that the card's power leaves them.  7370 x 1024 x 32768 in bfloat16 runs at
-// 1.04 PFLOP/s (logits, exponentials included), 0.91 (d_hidden), 1.11 (d_weight), a library's products of 8192 rows
+// 0.99 PFLOP/s (logits, exponentials included), 1.01 (d_hidden), 1.12 (d_weight), a library's products of 8192 rows
 // at 1.05, 1.29 and 1.47, the same MFMAs without any load at 1.5.  Steps of 32 in four buffers, loads in clumps, other row
 // orders and a stride off the powers of two changed nothing by more than 3%.
 //
@@ -55,7 +55,8 @@ struct MatOperand {
     int64_t plane;         // bytes between planes
     int64_t stride;        // bytes between rows
     int64_t bytes;         // of a plane from base on that may be read: loads beyond are zero
-    int tail;              // kRows, the first operand: bytes of a row's last k step that are the row's (multiples of 16): what is behind, to 128, is zero
+    int tail;              // kRows, the first operand: bytes of a row's last k step that are the row's, a multiple of 16; the
+                           // others of 128 are zero
 };
 
 constexpr int kWholeTail = kMatK * 2;
@@ -382,7 +383,9 @@ struct MatTiles {
             for (int j = 0; j < kNT; ++j) mfma<F16>(fa[0][i], fb[0][j], acc[i][j]);
             __builtin_amdgcn_sched_barrier(0);
         }
-        // this buffer is read, the next one's loads have landed, for all wavefronts
+        // This buffer is read, the next one's loads have landed, for all wavefronts.  Memory operations complete in order here, so the
+        // count stays right beside others that it does not know (stores of a tile's end, registers that the compiler keeps in
+        // scratch memory): with them in front or behind, it waits for more.
         asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(kLoads *(BUFFERS - 2)) : "memory");
         barrier();
         feed_begin(next);

@@ -36,7 +36,8 @@ struct RecurrencePlan {
 
 // Channels times batch make `groups * batch` workgroups.  A whole sequence is read once, at some 25 ns a step however few
 // of them there are; cut into chunks of 16 runs of whole blocks of S steps, until some 512 are at work, the gates
-// and inputs are read twice and two launches more are made.  The chunks are a multiple of eight, one XCD's each in turn:
+// and inputs are read twice and two launches more are made.  A multiple of eight chunks is wanted, one XCD's each in turn
+// (whole tiles of steps make them a few more or less: 65537 steps, 65 chunks, the last one of a single step):
 // 88 workgroups of 4096 steps, float, forward and backward in 6 chunks 267 us, in 8 246.  Measured in float, forward and
 // backward, whole and cut: 72 workgroups of 4096 steps 301 and 209 us, 96 313 and 276, 104 320 and 325, 128 338 and 403;
 // 96 of 16384 1226 and 1119, 112 1251 and 1330; 64 of 512 62 and 79, 72 of 1024 71 and 68, 40 70 and 50.  In bfloat16 pairs

@@ -19,7 +19,8 @@
 // starts each run from there (a fixed order: the same sums at every call).
 //
 // h is kept in float (complex64: two) whatever the rows' type; 1 - a is s(-gate), not a difference,
-// or decays close to one would lose it.
+// or decays close to one would lose it.  Backward h_{t-1} is what the forward call wrote, rounded where the rows
+// are bfloat16: d_gate then has 2^-9 of h beside its own rounding, and no second copy of h in float is written and read.
 #pragma once
 
 #include <type_traits>
@@ -318,7 +319,8 @@ __device__ __forceinline__ void by_kind(bool plain, F &&f)
 
 // ---- sequences that stay whole ---------------------------------------------------------------------------
 // grid: batch x groups workgroups in one or two dimensions; 64 x waves threads.  16 sequences of 2048 steps and 1024 channels, float: 83 us (402 MB, 4.8 TB/s),
-// backward 155 (805 MB, 5.2 TB/s): memory bounds both.
+// backward 155 (805 MB, 5.2 TB/s): memory bounds both.  As many steps of 512 channels, complex64 (the same bytes, half the
+// workgroups): 147 and 213; of 1024 channels, bfloat16 (half the bytes, half the workgroups): 86 and 159.
 template <typename Tr, bool SIG>
 __global__ __launch_bounds__(64 * kRecWaves) void recurrence_fw_kernel(RecurrenceArgs p)
 {
@@ -524,7 +526,8 @@ __global__ __launch_bounds__(64 * kRecWaves) void recurrence_bw_kernel(Recurrenc
 // launch forms every run's (A, B) as composed from the chunk's start (backward: end) up to the run, and the chunks';
 // the second one walks those from chunk to chunk; the third one starts each run from there, and the wavefronts need
 // nothing of each other.  65537 steps of 1000 channels, bfloat16: forward 70 + 10 + 75 us (3.7 TB/s, a chain of 65 chunks,
-// 5.2 TB/s), backward 66 + 11 + 167 (4.0 and 4.7 TB/s): memory bounds it, though a copy runs at 4.8.  The first launch's half of
+// 5.2 TB/s), backward 66 + 11 + 167 (4.0 and 4.7 TB/s): memory bounds it, though a copy runs at 4.8.  Of 500 channels,
+// complex64 (twice the bytes): 140 + 12 + 153 and 133 + 12 + 271.  The first launch's half of
 // the registers took 10 us off each direction; the third one in workgroups of four wavefronts, or the first one walking
 // against the third one's direction (for the caches), gained nothing.  With every wavefront walking the chunks in front of its own,
 // instead of a launch between, the third launches took 123 and 193.

@@ -372,7 +372,7 @@ __global__ __launch_bounds__(row_threads<L>()) void norm_bw_kernel(RowArgs a)
 }
 
 // ---- rows too wide for the registers of a workgroup: read again instead -----------------------------
-// 2048 x 9000 float: 44 us forward, 118 with backward; 2048 x 16384 70 and 224 (the second read out of the L2).
+// 2048 x 9000 float: 47 us forward, 123 with backward; 2048 x 16384 71 and 225 (the second read out of the L2).
 
 constexpr int kWideThreads = 1024;
 

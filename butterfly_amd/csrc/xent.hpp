@@ -9,13 +9,13 @@
 // two products with that buffer, d_hidden's partial sums over the pieces and d_weight's rows of the piece.
 // 2 rows x vocabulary x features operations forward and 6 backward, all on the matrix units (matmul.hpp),
 // which bound every call but those of a few rows (there the weights' bytes do: xent_few.hpp).
-// Measured at 8192 rows (7370 of them counted), 1024 features, 32768 entries, bfloat16: 1845 us forward and backward, of which
-// the logits take 476 (1.04 PFLOP/s), d_l 2 x 250 (two pieces; the same product and 2 x 241 MB written), d_hidden 2 x
-// 273, d_weight 2 x 222, everything else 50.  At 2000 (1800) x 1000 x 30001, float: 1390 us: 350, 394, 335, 319 (three products
-// each: 0.93 PFLOP/s), the largest numbers and the copies in two planes 85.
+// Measured at 8192 rows (7370 of them counted), 1024 features, 32768 entries, bfloat16: 1890 us forward and backward, of which
+// the logits take 499 (0.99 PFLOP/s), d_l 2 x 258 (two pieces; the same product and 2 x 241 MB written), d_hidden 2 x
+// 244, d_weight 2 x 220, everything else 50.  At 2000 (1800) x 1000 x 30001, float: 1452 us: 367, 402, 331, 347 (three products
+// each: 0.81 to 0.98 PFLOP/s), the largest numbers and the copies in two planes 88.
 //
 // Rows whose target is ignored are left out before anything else: the others' hidden rows are gathered, so
-// ignored ones cost nothing and what they hold (NaN too) reaches nothing.
+// what ignored ones hold (NaN too) reaches nothing, and they cost nothing but the tiles that the counted ones leave unfilled.
 //
 // Number formats.  bfloat16 operands multiply as they are; d_l is rounded to bfloat16 (2^-9), like every gradient
 // of such a model.  float operands are split, x 2^e = hi + lo in two float16 numbers of together 22 bits,
@@ -23,9 +23,8 @@
 // weight; d_l is at most one, e = 15), and a product is hi lo + lo hi + hi hi with sums in float: three
 // products at the 16-bit rate, 16 times that of float ones on this card, for a relative error of 2^-22 a factor.  The lower
 // halves are kept times 2^11: numbers from 2^-28 of the largest up have their 22 bits, from 2^-40 eleven, below 2^-51 none.
-// With one gradient a row d_l is
-// without it in float (rows of small ones would lose their bits): d_hidden's rows are multiplied at the end, and d_weight's
-// product takes hidden's rows times their share of the largest.
+// With one gradient a row d_l is without it in float (rows of small ones would lose their bits): d_hidden's rows are multiplied
+// at the end, and d_weight's product takes hidden's rows times their share of the largest.
 #pragma once
 
 #include "matmul.hpp"
@@ -36,7 +35,7 @@ constexpr int kXentThreads = 1024;   // of the single-workgroup kernels
 
 struct XentScalars {
     float hidden_scale, weight_scale;   // the powers of two
-    float grad_scale;                   // one gradient a row: the largest |g_i| (d_l is kept over it)
+    float grad_scale;                   // one gradient a row: the largest finite |g_i| (shares are kept over it)
     unsigned hidden_max, weight_max;    // bits of the largest magnitudes
     int counted;                        // rows whose target is not ignored
 };

@@ -13,7 +13,12 @@ def linear_cross_entropy(hidden, weight, target, ignore_index=-100, reduction="m
     features), ``target`` (*) int64, both float32 or both bfloat16; the loss is float32, (*) for ``reduction="none"``.
 
     Rows whose target is ``ignore_index`` count for nothing (the mean is over the others, NaN if there are none); a target
-    that is no entry of the vocabulary makes loss and gradients NaN."""
+    that is no entry of the vocabulary makes loss and gradients NaN.
+
+    On the device sums are float32.  float32 operands of up to 64 rows (no more than features) are multiplied with 24
+    bits; with more rows with 22 bits, which numbers (the probabilities of the backward pass among them) from 2^-28 of
+    the operand's largest finite one up keep, and from 2^-40 up eleven.  Gradients of bfloat16 operands go through the logits'
+    gradient in bfloat16.  There is no second derivative: following a gradient's history raises."""
     if reduction not in _REDUCTIONS:
         raise ValueError(f"reduction must be 'none', 'mean' or 'sum', got {reduction!r}")
     if hidden.is_cuda:

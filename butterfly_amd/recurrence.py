@@ -13,7 +13,7 @@ def gated_recurrence(gate, x, state=None, reset=None, sigmoid=True):
     ``sigmoid``: ``a = sigmoid(gate)``, ``b = (1 - a) * x``; otherwise ``a = gate``, ``b = x``.  ``gate`` and ``x`` are
     (batch, steps, channels), float32, bfloat16 or (not sigmoid) complex64; states (batch, channels), float32 (complex64
     for complex rows).  ``reset`` (batch, steps), bool: there ``h[:, t-1]`` counts as zero (a packed document
-    starts)."""
+    starts).  On the device there is no second derivative: following a gradient's history raises."""
     if x.is_cuda:
         return ops.gated_recurrence(gate, x, state, reset, sigmoid)
     wide = x.dtype if x.dtype.is_complex or x.dtype == torch.float64 else torch.float32

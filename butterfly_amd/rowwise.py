@@ -4,7 +4,8 @@
 Dropout is counter-based: ``rng`` is a tensor of two int64, a seed and the number of the call, and the mask is a
 function of those, the row and the column (see ``dropout_mask``), made again in the backward pass instead
 of stored.  Rows are float32 or bfloat16, of any width and row stride; ``weight`` and ``bias`` float32 or the
-rows' dtype; statistics are formed in float32.  Host tensors run as tensor operations.
+rows' dtype; statistics are formed in float32.  Host tensors run as tensor operations.  On the device the norms have no
+second derivative (following a gradient's history raises), ``dropout_add`` has all of them.
 
 No counterpart in the reference, whose users take these from PyTorch."""
 import collections

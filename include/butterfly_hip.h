@@ -386,8 +386,8 @@ int bf_recurrence_step(const bf_recurrence *p, const void *gate, const void *x, 
  *   gradients NaN.  Mean: over the rows that count (NaN if there is none).
  * hidden (rows, features), weight (vocab, features), features adjacent, rows `*_stride` elements
  * apart, weight 16-byte aligned.  BF_BF16: products of bfloat16 with sums in float, the logits' gradient in bfloat16.
- * BF_F32: every factor as two float16 numbers of together 22 bits (few rows: three bfloat16 numbers of together 24), sums in
- * float.
+ * BF_F32: every factor as two float16 numbers of together 22 bits, from 2^-28 of the operand's largest finite number up (from
+ * 2^-40 up eleven, below 2^-51 none); few rows: three bfloat16 numbers of together 24 bits at any scale.  Sums in float.
  * Gradients are dense, summed in a fixed order.                                                 */
 #define BF_XENT_NONE 0
 #define BF_XENT_MEAN 1
