@@ -35,8 +35,9 @@ HBM_PEAK_GBS = 8000.0
 TRAFFIC_TABLE = os.path.join(ROOT, "profiles", "hbm_traffic_all_configs.md")
 KERNEL_SOURCES = os.path.join(ROOT, "butterfly_amd", "csrc")
 # (the operators beside the multiply, none of whose sources the multiply's kernels include)
-OTHER_SOURCES = {"matmul.hpp", "recurrence.hip", "recurrence.hpp", "rowwise.hip", "rowwise.hpp", "sequence_ops.cpp", "vec8.hpp",
-                 "xent.hip", "xent.hpp", "xent_few.hpp"}
+OTHER_SOURCES = {"attention_ops.cpp", "linear_attention.hip", "linear_attention.hpp", "matmul.hpp", "recurrence.hip", "recurrence.hpp",
+                 "rotary.hip", "rotary.hpp", "rowwise.hip", "rowwise.hpp", "sample.hip", "sample.hpp", "sequence_ops.cpp", "shim.hpp",
+                 "vec8.hpp", "xent.hip", "xent.hpp", "xent_few.hpp"}
 
 
 def kernel_source_digest():

@@ -26,6 +26,7 @@ def _load_native():
 
 _load_native()
 
+from .attention import linear_attention, linear_attention_step  # noqa: E402
 from .multiply import butterfly_multiply  # noqa: E402
 from .multiply_base4 import butterfly_multiply_base4  # noqa: E402
 from .butterfly import Butterfly, ButterflyBmm, ButterflyUnitary  # noqa: E402
@@ -33,9 +34,11 @@ from .butterfly_base4 import ButterflyBase4  # noqa: E402
 from .graphed import GraphedStep  # noqa: E402
 from .loss import LinearCrossEntropy, linear_cross_entropy  # noqa: E402
 from .recurrence import gated_recurrence, gated_recurrence_step  # noqa: E402
+from .positions import rotary, rotary_frequencies  # noqa: E402
+from .sampling import sample  # noqa: E402
 from .rowwise import (DropoutAdd, DropoutAddLayerNorm, LayerNorm, dropout_add, dropout_add_layer_norm,  # noqa: E402
                       layer_norm, rng_next)
-from . import combine, complex_utils, diagonal, kops, legacy, legacy_permutation, loss, multiply, multiply_base4, permutation, recurrence, rowwise, sequence_model, special  # noqa: E402,F401
+from . import attention, combine, complex_utils, diagonal, kops, legacy, legacy_permutation, loss, multiply, multiply_base4, permutation, positions, recurrence, rowwise, sampling, sequence_model, special  # noqa: E402,F401
 
 __all__ = [
     "Butterfly",
@@ -54,7 +57,12 @@ __all__ = [
     "gated_recurrence",
     "gated_recurrence_step",
     "layer_norm",
+    "linear_attention",
+    "linear_attention_step",
     "linear_cross_entropy",
     "rng_next",
+    "rotary",
+    "rotary_frequencies",
+    "sample",
     "__version__",
 ]

@@ -35,6 +35,8 @@ SYMBOLS = [
     "bf_recurrence_workspace_bytes", "bf_recurrence_fw", "bf_recurrence_bw", "bf_recurrence_step",
     "bf_linear_xent_kept_bytes", "bf_linear_xent_fw_workspace_bytes", "bf_linear_xent_bw_workspace_bytes", "bf_linear_xent_fw",
     "bf_linear_xent_bw",
+    "bf_linear_attention_kept_bytes", "bf_linear_attention_fw_workspace_bytes", "bf_linear_attention_bw_workspace_bytes",
+    "bf_linear_attention_fw", "bf_linear_attention_bw", "bf_linear_attention_step", "bf_rotary_apply", "bf_sample_tokens",
 ]
 
 NOALLOC_SCRATCH_BYTES = 48 << 20
@@ -88,6 +90,25 @@ class LinearXent(ctypes.Structure):
     _fields_ = [("dtype", ctypes.c_int32), ("reduction", ctypes.c_int32), ("rows", ctypes.c_int64), ("features", ctypes.c_int64),
                 ("vocab", ctypes.c_int64), ("hidden_stride", ctypes.c_int64), ("weight_stride", ctypes.c_int64),
                 ("ignore_index", ctypes.c_int64)]
+
+
+class LinearAttention(ctypes.Structure):
+    _fields_ = [("dtype", ctypes.c_int32), ("batch", ctypes.c_int64), ("steps", ctypes.c_int64), ("heads", ctypes.c_int64),
+                ("groups", ctypes.c_int64), ("features", ctypes.c_int64), ("values", ctypes.c_int64),
+                ("q_stride", ctypes.c_int64 * 3), ("k_stride", ctypes.c_int64 * 3), ("v_stride", ctypes.c_int64 * 3),
+                ("grad_stride", ctypes.c_int64 * 3), ("decay_stride", ctypes.c_int64 * 3), ("reset_stride", ctypes.c_int64 * 2),
+                ("scale", ctypes.c_double)]
+
+
+class Rotary(ctypes.Structure):
+    _fields_ = [("dtype", ctypes.c_int32), ("interleaved", ctypes.c_int32), ("batch", ctypes.c_int64), ("steps", ctypes.c_int64),
+                ("heads", ctypes.c_int64), ("features", ctypes.c_int64), ("rotated", ctypes.c_int64),
+                ("x_stride", ctypes.c_int64 * 3), ("position_stride", ctypes.c_int64 * 2), ("magnitude", ctypes.c_double)]
+
+
+class Sample(ctypes.Structure):
+    _fields_ = [("dtype", ctypes.c_int32), ("rows", ctypes.c_int64), ("vocab", ctypes.c_int64), ("logits_stride", ctypes.c_int64),
+                ("temperature", ctypes.c_double), ("top_p", ctypes.c_double), ("min_p", ctypes.c_double), ("top_k", ctypes.c_int64)]
 
 
 _lib = None
@@ -169,6 +190,15 @@ def lib():
             getattr(L, name).restype = sz
         L.bf_linear_xent_fw.argtypes = [px] + [vp] * 5 + [sz, vp, sz, vp]
         L.bf_linear_xent_bw.argtypes = [px] + [vp] * 3 + [sz, vp, vp, vp, sz, vp]
+        pa = ctypes.POINTER(LinearAttention)
+        for name in ("bf_linear_attention_kept_bytes", "bf_linear_attention_fw_workspace_bytes", "bf_linear_attention_bw_workspace_bytes"):
+            getattr(L, name).argtypes = [pa]
+            getattr(L, name).restype = sz
+        L.bf_linear_attention_fw.argtypes = [pa] + [vp] * 9 + [sz, vp, sz, vp]
+        L.bf_linear_attention_bw.argtypes = [pa] + [vp] * 6 + [sz] + [vp] * 8 + [sz, vp]
+        L.bf_linear_attention_step.argtypes = [pa] + [vp] * 7
+        L.bf_rotary_apply.argtypes = [ctypes.POINTER(Rotary), vp, vp, vp, vp, i32, vp]
+        L.bf_sample_tokens.argtypes = [ctypes.POINTER(Sample)] + [vp] * 8
         _lib = L
     return _lib
 

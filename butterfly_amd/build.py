@@ -125,7 +125,7 @@ def _torch_flags():
 
 def build_ops():
     flags, libs = _torch_flags()
-    _run(["g++"] + flags + [os.path.join(CSRC, name) for name in ("butterfly_ops.cpp", "sequence_ops.cpp")] +
+    _run(["g++"] + flags + [os.path.join(CSRC, name) for name in ("butterfly_ops.cpp", "sequence_ops.cpp", "attention_ops.cpp")] +
          ["-o", LIB_OPS] + libs +
          ["-ltorch_hip", "-lc10_hip", f"-L{PKG}", "-lbutterfly_hip", "-Wl,-rpath,$ORIGIN"])
     return LIB_OPS

@@ -1,0 +1,440 @@
+// A token for each row of logits, from one random number in [0, 1): with w_i = exp((z_i - max z) / temperature), of the top_k
+// largest logits (ties: the lowest indexes) the likeliest ones until their sum reaches top_p of it, of those the ones with
+// w_i >= min_p; the token is the first index whose cumulated w, in the order of indexes, exceeds uniform * total.
+//
+// A workgroup takes a row and keeps it in registers (up to 256 KiB; longer ones are read again, out of the caches).  There is no
+// sort: what is kept is "logit above t, and the first m of those equal to t", and t is found by histograms of 2048 bins, first
+// over the values from the maximum down, then over the logits' bits within the bin where the sum crosses its goal.
+//
+// Weights are whole numbers, w in units of 2^-44: sums do not depend on their order (so the histograms may be filled by
+// atomics, and every call gives the same token), and are off by 2^-45 an entry, where borders between tokens are
+// decided as in 64 bits.  The exponential is a polynomial in double for the same reason: a float one moves each border by
+// some 1e-8 of the total, which with 50000 entries of similar weight is 1e-3 of the distance between two borders.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "vec8.hpp"
+
+namespace bf {
+
+struct SampleArgs {
+    const void *logits;
+    const float *uniform, *temperature, *top_p, *min_p;   // one a row; settings NULL: the ones below for all rows
+    const int64_t *top_k;
+    double temperature_all, top_p_all, min_p_all;
+    int64_t top_k_all;
+    int64_t *token;
+    int64_t stride;
+    int vocab;
+};
+
+constexpr int kSampleThreads = 1024, kSampleWaves = kSampleThreads / 64, kSampleBins = 2 * kSampleThreads;
+constexpr int kSampleBits = 44;
+
+struct SampleLds {
+    unsigned long long bins[kSampleBins];
+    unsigned long long sums[kSampleWaves];
+    float low[kSampleWaves], high[kSampleWaves];
+    unsigned long long counts[kSampleWaves];
+    unsigned long long above;
+    int at;
+};
+
+// Order of floats as an order of whole numbers (of bfloat16: 16 bits).
+template <typename T>
+__device__ __forceinline__ uint32_t sample_key(float v)
+{
+    const uint32_t bits = __builtin_bit_cast(uint32_t, v);
+    const uint32_t key = bits ^ (bits >> 31 ? 0xffffffffu : 0x80000000u);
+    return sizeof(T) == 2 ? key >> 16 : key;
+}
+template <typename T>
+__device__ __forceinline__ float sample_value(uint32_t key)
+{
+    if (sizeof(T) == 2) key = key << 16 | (key >> 15 ? 0u : 0xffffu);
+    return __builtin_bit_cast(float, key >> 31 ? key ^ 0x80000000u : ~key);
+}
+
+// 16 bytes of a row, NaN and what lies behind its end as -inf, -0 as 0.
+template <typename T>
+__device__ __forceinline__ uint4 sample_load(const T *row, int64_t col, int vocab)
+{
+    constexpr int E = 16 / sizeof(T);
+    using Quad = std::conditional_t<sizeof(T) == 4, quad_at_4, quad_at_2>;
+    uint32_t out[4];
+    T part[E];
+    if (col + E <= vocab) {
+        const Quad v = *reinterpret_cast<const Quad *>(row + col);
+        __builtin_memcpy(part, &v, 16);
+    } else {
+#pragma unroll
+        for (int i = 0; i < E; ++i) part[i] = col + i < vocab ? row[col + i] : (T)-INFINITY;
+    }
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+        const float f = to_float(part[i]);
+        const uint32_t bits = __builtin_bit_cast(uint32_t, f == f ? f + 0.0f : -INFINITY);
+        if constexpr (sizeof(T) == 4) out[i] = bits;
+        else if (i % 2 == 0) out[i / 2] = bits >> 16;
+        else out[i / 2] |= bits & 0xffff0000u;
+    }
+    return make_uint4(out[0], out[1], out[2], out[3]);
+}
+template <typename T>
+__device__ __forceinline__ float sample_element(const uint4 &v, int i)
+{
+    const uint32_t words[4] = {v.x, v.y, v.z, v.w};
+    if constexpr (sizeof(T) == 4) return __builtin_bit_cast(float, words[i]);
+    else return __builtin_bit_cast(float, i % 2 ? words[i / 2] & 0xffff0000u : words[i / 2] << 16);
+}
+
+struct SampleWeight {
+    float top = 0.0f;
+    double per_nat = 0.0;              // log2 e / temperature
+    float range = 0.0f;                // farther below the maximum a weight is zero
+    unsigned long long least = 1;      // smallest weight that min_p leaves
+
+    __device__ __forceinline__ float below(float v) const { return v == top ? 0.0f : top - v; }
+
+    // 2^44 exp((v - top) / temperature), rounded
+    __device__ __forceinline__ unsigned long long operator()(float v) const
+    {
+        if (!(below(v) <= range)) return 0;
+        const double y = v == top ? 0.0 : ((double)v - (double)top) * per_nat, n = rint(y), x = (y - n) * 0.6931471805599453;
+        // Taylor polynomial, |x| <= log(2) / 2: off by x^12 / 12! < 7e-15
+        double p = 1.0 / 39916800.0;
+        p = fma(p, x, 1.0 / 3628800.0);
+        p = fma(p, x, 1.0 / 362880.0);
+        p = fma(p, x, 1.0 / 40320.0);
+        p = fma(p, x, 1.0 / 5040.0);
+        p = fma(p, x, 1.0 / 720.0);
+        p = fma(p, x, 1.0 / 120.0);
+        p = fma(p, x, 1.0 / 24.0);
+        p = fma(p, x, 1.0 / 6.0);
+        p = fma(p, x, 0.5);
+        p = fma(p, x, 1.0);
+        p = fma(p, x, 1.0);
+        return (unsigned long long)(ldexp(p, (int)n + kSampleBits) + 0.5);
+    }
+};
+
+__device__ __forceinline__ unsigned long long sample_wave_sum(unsigned long long v)
+{
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) v += __shfl_xor(v, d, 64);
+    return v;
+}
+__device__ __forceinline__ unsigned long long sample_wave_scan(unsigned long long v)
+{
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+        const unsigned long long before = __shfl_up(v, d, 64);
+        if (lane >= d) v += before;
+    }
+    return v;
+}
+
+// Sum over the threads in front of this one; total: over all.  (Ends behind a barrier of its own.)
+__device__ __forceinline__ unsigned long long sample_before(SampleLds &lds, unsigned long long v, unsigned long long &total)
+{
+    const int wave = threadIdx.x >> 6;
+    const unsigned long long inside = sample_wave_scan(v);
+    if ((threadIdx.x & 63) == 63) lds.sums[wave] = inside;
+    __syncthreads();
+    unsigned long long before = 0;
+    total = 0;
+    for (int w = 0; w < kSampleWaves; ++w) {
+        if (w == wave) before = total;
+        total += lds.sums[w];
+    }
+    __syncthreads();
+    return before + inside - v;
+}
+
+// The bin in which the sum from the first bin on reaches the goal; lds.above: the sum in front of it.  -1: it is never reached.
+__device__ __forceinline__ int sample_crossing(SampleLds &lds, unsigned long long goal)
+{
+    if (threadIdx.x == 0) lds.at = -1;
+    const unsigned long long one = lds.bins[2 * threadIdx.x], two = lds.bins[2 * threadIdx.x + 1];
+    unsigned long long total;
+    const unsigned long long before = sample_before(lds, one + two, total);
+    if (before < goal && goal <= before + one + two) {
+        const bool second = goal > before + one;
+        lds.at = 2 * threadIdx.x + second;
+        lds.above = second ? before + one : before;
+    }
+    __syncthreads();
+    return lds.at;
+}
+
+// VECTORS: 16-byte pieces of the row that a thread holds; 0: the row is read again in each pass.
+template <typename T, int VECTORS>
+struct SampleRow {
+    static constexpr int E = 16 / sizeof(T);
+    const T *row;
+    int vocab, span;             // span: pieces of a wavefront, side by side
+    uint4 held[VECTORS > 0 ? VECTORS : 1];
+
+    __device__ __forceinline__ int64_t piece(int n) const { return (int64_t)(threadIdx.x >> 6) * span + n * 64 + (threadIdx.x & 63); }
+
+    __device__ __forceinline__ void init(const T *r, int v)
+    {
+        row = r;
+        vocab = v;
+        const int pieces = (vocab + E - 1) / E;
+        span = VECTORS > 0 ? VECTORS * 64 : (pieces + 64 * kSampleWaves - 1) / (64 * kSampleWaves) * 64;
+        if constexpr (VECTORS > 0) {
+#pragma unroll
+            for (int n = 0; n < VECTORS; ++n) held[n] = sample_load(row, piece(n) * E, vocab);
+        }
+    }
+
+    template <typename Fn>
+    __device__ __forceinline__ void each(Fn &&f) const
+    {
+        if constexpr (VECTORS > 0) {
+#pragma unroll
+            for (int n = 0; n < VECTORS; ++n)
+#pragma unroll
+                for (int i = 0; i < E; ++i) f(sample_element<T>(held[n], i), (int)piece(n) * E + i);
+        } else {
+            for (int n = 0; n < span / 64; ++n) {
+                const int64_t at = piece(n);
+                if (at * E >= vocab) break;
+                const uint4 v = sample_load(row, at * E, vocab);
+#pragma unroll
+                for (int i = 0; i < E; ++i) f(sample_element<T>(v, i), (int)at * E + i);
+            }
+        }
+    }
+};
+
+// The largest key t such that the weights of the logits from t up sum to the goal at least; lds.above: the sum of those above t.
+// False: all of them do not.
+template <typename T, typename Row, typename W>
+__device__ __forceinline__ bool sample_threshold(SampleLds &lds, const Row &row, const SampleWeight &weight, unsigned long long goal, W &&of,
+                                                 uint32_t &t)
+{
+    auto clear = [&] {
+        lds.bins[2 * threadIdx.x] = lds.bins[2 * threadIdx.x + 1] = 0;
+        __syncthreads();
+    };
+    const float per = weight.range > 0.0f ? kSampleBins / weight.range : 0.0f;
+    auto bin_of = [&](float v) { return min((int)(weight.below(v) * per), kSampleBins - 1); };
+    clear();
+    row.each([&](float v, int) {
+        if (!(weight.below(v) <= weight.range)) return;
+        const unsigned long long w = of(v);
+        if (w) atomicAdd(&lds.bins[bin_of(v)], w);
+    });
+    __syncthreads();
+    const int bin = sample_crossing(lds, goal);
+    if (bin < 0) return false;
+    unsigned long long above = lds.above;
+    // (bins are off by rounding: a hundredth more on both sides)
+    const float width = per > 0.0f ? 1.0f / per : 0.0f;
+    uint32_t high = sample_key<T>(fminf(weight.top, weight.top - (bin - 0.01f) * width));
+    uint32_t low = bin == kSampleBins - 1 ? sample_key<T>(weight.top - weight.range * 1.001f) : sample_key<T>(weight.top - (bin + 1.01f) * width);
+    for (;;) {
+        const uint32_t length = high - low;
+        const int shift = length < (uint32_t)kSampleBins ? 0 : 32 - __clz((int)length) - 11;
+        __syncthreads();
+        clear();
+        row.each([&](float v, int) {
+            const uint32_t key = sample_key<T>(v);
+            if (key < low || key > high || !(weight.below(v) <= weight.range) || bin_of(v) != bin) return;
+            const unsigned long long w = of(v);
+            if (w) atomicAdd(&lds.bins[(high - key) >> shift], w);
+        });
+        __syncthreads();
+        const int at = sample_crossing(lds, goal - above);
+        if (at < 0) return false;   // (cannot be: the bin held it)
+        above += lds.above;
+        high -= (uint32_t)at << shift;
+        if (shift == 0) break;
+        const uint32_t lowest = high - ((1u << shift) - 1);
+        low = max(low, lowest > high ? 0u : lowest);
+    }
+    t = high;
+    __syncthreads();
+    if (threadIdx.x == 0) lds.above = above;
+    __syncthreads();
+    return true;
+}
+
+template <typename T, int VECTORS>
+__global__ __launch_bounds__(kSampleThreads) void sample_kernel(const SampleArgs a)
+{
+    __shared__ SampleLds lds;
+    constexpr int E = 16 / sizeof(T);
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const int64_t r = blockIdx.x;
+    SampleRow<T, VECTORS> row;
+    row.init(static_cast<const T *>(a.logits) + r * a.stride, a.vocab);
+
+    float high = -INFINITY, low = INFINITY;
+    row.each([&](float v, int) {
+        high = fmaxf(high, v);
+        low = fminf(low, v == -INFINITY ? INFINITY : v);
+    });
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+        high = fmaxf(high, __shfl_xor(high, d, 64));
+        low = fminf(low, __shfl_xor(low, d, 64));
+    }
+    if (lane == 0) {
+        lds.high[wave] = high;
+        lds.low[wave] = low;
+    }
+    __syncthreads();
+    for (int w = 0; w < kSampleWaves; ++w) {
+        high = fmaxf(high, lds.high[w]);
+        low = fminf(low, lds.low[w]);
+    }
+    if (high == -INFINITY) {
+        // nothing is possible
+        if (threadIdx.x == 0) a.token[r] = -1;
+        return;
+    }
+    // (beyond 2^100 the differences of all finite logits are nearly nothing, and below what a float range holds)
+    const double temperature = fmin(a.temperature ? (double)a.temperature[r] : a.temperature_all, 0x1p100);
+    if (!(temperature > 0.0)) {
+        // the first of the largest
+        int first = a.vocab;
+        row.each([&](float v, int at) { if (v == high) first = min(first, at); });
+#pragma unroll
+        for (int d = 1; d < 64; d *= 2) first = min(first, __shfl_xor(first, d, 64));
+        if (lane == 0) lds.counts[wave] = (unsigned long long)first;
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            unsigned long long least = lds.counts[0];
+            for (int w = 1; w < kSampleWaves; ++w) least = min(least, lds.counts[w]);
+            a.token[r] = (int64_t)least;
+        }
+        return;
+    }
+    SampleWeight weight;
+    weight.top = high;
+    weight.per_nat = 1.4426950408889634 / temperature;
+    weight.range = high == INFINITY ? 0.0f : fminf(high - low, (float)(temperature * ((kSampleBits + 2) * 0.6931471805599453)));
+    const double min_p = a.min_p ? (double)a.min_p[r] : a.min_p_all;
+    const double top_p = a.top_p ? (double)a.top_p[r] : a.top_p_all;
+    const int64_t top_k = a.top_k ? a.top_k[r] : a.top_k_all;
+    const unsigned long long one = 1ull << kSampleBits;
+    if (min_p > 0.0) weight.least = max(1ull, (unsigned long long)ceil(fmin(min_p, 1.0) * (double)one));
+
+    // kept: keys above t, and the first m of those equal to it
+    uint32_t t = 0;
+    unsigned long long m = 0;
+    auto kept_sums = [&](unsigned long long least, unsigned long long &sum, unsigned long long &ties) {
+        sum = ties = 0;
+        row.each([&](float v, int) {
+            const uint32_t key = sample_key<T>(v);
+            if (key > t) {
+                const unsigned long long w = weight(v);
+                sum += w >= least ? w : 0;
+            } else if (key == t) {
+                ++ties;
+            }
+        });
+    };
+    if (top_k > 0 && top_k < a.vocab &&
+        sample_threshold<T>(lds, row, weight, (unsigned long long)top_k, [](float) { return 1ull; }, t))
+        m = (unsigned long long)top_k - lds.above;
+    if (top_p < 1.0) {
+        unsigned long long sum, ties, total;
+        kept_sums(1, sum, ties);
+        sample_before(lds, sum, total);
+        if (m > 0) total += m * weight(sample_value<T>(t));
+        const double share = ceil(fmax(top_p, 0.0) * (double)total);
+        const unsigned long long goal = max(1ull, min(total, (unsigned long long)share));
+        uint32_t tp;
+        if (sample_threshold<T>(lds, row, weight, goal, [&](float v) { return weight(v); }, tp)) {
+            const unsigned long long w = weight(sample_value<T>(tp));
+            t = tp;
+            m = (goal - lds.above + w - 1) / w;
+        }
+    }
+    const unsigned long long tie = m > 0 ? weight(sample_value<T>(t)) : 0;
+    if (tie < weight.least) m = 0;
+    unsigned long long sum, ties;
+    kept_sums(weight.least, sum, ties);
+    sum = sample_wave_sum(sum);
+    ties = sample_wave_sum(ties);
+    __syncthreads();
+    if (lane == 0) {
+        lds.sums[wave] = sum;
+        lds.counts[wave] = ties;
+    }
+    __syncthreads();
+    unsigned long long total = 0, ties_before = 0;
+    for (int w = 0; w < kSampleWaves; ++w) {
+        const unsigned long long left = m > ties_before ? m - ties_before : 0;
+        total += lds.sums[w] + min(left, lds.counts[w]) * tie;
+        ties_before += lds.counts[w];
+    }
+    const double u = fmin(fmax((double)a.uniform[r], 0.0), 1.0);
+    unsigned long long target = min((unsigned long long)(u * (double)total), total - 1);
+    // the wavefront's part of the row that holds it, read again by all threads in the order of indexes
+    int where = 0;
+    unsigned long long left = m;
+    for (; where < kSampleWaves - 1; ++where) {
+        const unsigned long long here = lds.sums[where] + min(left, lds.counts[where]) * tie;
+        if (target < here) break;
+        target -= here;
+        left -= min(left, lds.counts[where]);
+    }
+    __syncthreads();
+    for (int start = 0; start < row.span; start += kSampleThreads) {
+        const int64_t piece = (int64_t)where * row.span + start + threadIdx.x;
+        const bool mine = start + (int)threadIdx.x < row.span && piece * E < a.vocab;
+        const uint4 v = mine ? sample_load(row.row, piece * E, a.vocab) : make_uint4(0, 0, 0, 0);
+        unsigned long long mass = 0, equal = 0;
+        if (mine) {
+#pragma unroll
+            for (int i = 0; i < E; ++i) {
+                const float x = sample_element<T>(v, i);
+                const uint32_t key = sample_key<T>(x);
+                if (key > t) {
+                    const unsigned long long w = weight(x);
+                    mass += w >= weight.least ? w : 0;
+                }
+                equal += key == t;
+            }
+        }
+        unsigned long long all_equal, all;
+        const unsigned long long equal_before = sample_before(lds, equal, all_equal);
+        const unsigned long long allowed = left > equal_before ? min(left - equal_before, equal) : 0;
+        const unsigned long long before = sample_before(lds, mass + allowed * tie, all);
+        if (target < all) {
+            if (before <= target && target < before + mass + allowed * tie) {
+                unsigned long long rest = target - before, used = 0;
+                for (int i = 0; i < E; ++i) {
+                    const float x = sample_element<T>(v, i);
+                    const uint32_t key = sample_key<T>(x);
+                    unsigned long long w = 0;
+                    if (key > t) {
+                        w = weight(x);
+                        if (w < weight.least) w = 0;
+                    } else if (key == t && used < allowed) {
+                        w = tie;
+                        ++used;
+                    }
+                    if (rest < w) {
+                        a.token[r] = piece * E + i;
+                        break;
+                    }
+                    rest -= w;
+                }
+            }
+            return;
+        }
+        target -= all;
+        left -= min(left, all_equal);
+    }
+}
+
+}  // namespace bf

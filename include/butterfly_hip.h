@@ -25,7 +25,7 @@ extern "C" {
 
 #define BF_F32 0
 #define BF_C64 1
-#define BF_BF16 2 /* the operators beside the multiply only (bf_rowwise_*, bf_recurrence_*, bf_linear_xent_*) */
+#define BF_BF16 2 /* the operators beside the multiply only */
 
 #define BF_OK 0
 #define BF_ERR_INVALID (-1)     /* bad shape / stride / argument                      */
@@ -419,6 +419,79 @@ int bf_linear_xent_fw(const bf_linear_xent *p, const void *hidden, const void *w
 int bf_linear_xent_bw(const bf_linear_xent *p, const void *weight, const float *grad, void *kept,
                       size_t kept_bytes, void *d_hidden, void *d_weight, void *workspace,
                       size_t workspace_bytes, void *stream);
+
+/* Linear attention with a decay for each head: S_t = exp(log_decay_t) S_{t-1} + k_t^T v_t from S_{-1} = state and
+ * o_t = scale q_t S_t, S of (features, values) floats for each sequence and head.  q, k are (batch, steps, groups,
+ * features), v (batch, steps, heads, values), log_decay (batch, steps, heads) floats; heads is a multiple of groups, and
+ * heads / groups neighbouring heads share queries and keys.  The last dimension is adjacent (log_decay: the strides
+ * say it all), the others have the given strides; o and every gradient are dense, states dense (batch, heads,
+ * features, values).  reset (bytes, (batch, steps), may be NULL): where set, S_{t-1} counts as zero whatever it is
+ * (a packed document starts).  features and values: 1 to 128.                                    */
+typedef struct bf_linear_attention {
+    int32_t dtype; /* BF_F32 or BF_BF16: q, k, v, o and their gradients */
+    int64_t batch, steps, heads, groups, features, values;
+    int64_t q_stride[3], k_stride[3], v_stride[3], grad_stride[3], decay_stride[3]; /* (batch, step, head or group) */
+    int64_t reset_stride[2];                                                        /* (batch, step)                */
+    double scale;
+} bf_linear_attention;
+
+/* kept (16-byte aligned): the states in front of every chunk of 64 steps (float with more than 64 features or values: 32), for
+ * the backward call.  Workspaces (16-byte aligned): 0 where sequences and heads fill the chip; otherwise the states
+ * between segments of the sequences; backward with shared queries and keys also the gradients of each head as floats. */
+size_t bf_linear_attention_kept_bytes(const bf_linear_attention *p);
+size_t bf_linear_attention_fw_workspace_bytes(const bf_linear_attention *p);
+size_t bf_linear_attention_bw_workspace_bytes(const bf_linear_attention *p);
+/* state (zeros), reset, last and kept (not wanted) may be NULL. */
+int bf_linear_attention_fw(const bf_linear_attention *p, const void *q, const void *k, const void *v,
+                           const float *log_decay, const float *state, const uint8_t *reset, void *o,
+                           float *last, void *kept, size_t kept_bytes, void *workspace,
+                           size_t workspace_bytes, void *stream);
+/* grad (of o; strides grad_stride), grad_last (zeros), reset and d_state (not wanted) may be NULL. */
+int bf_linear_attention_bw(const bf_linear_attention *p, const void *q, const void *k, const void *v,
+                           const float *log_decay, const uint8_t *reset, const void *kept,
+                           size_t kept_bytes, const void *grad, const float *grad_last, void *d_q,
+                           void *d_k, void *d_v, float *d_log_decay, float *d_state, void *workspace,
+                           size_t workspace_bytes, void *stream);
+/* One step of every sequence, for serving: the state is updated in place.  steps and the strides of
+ * steps are not read.                                                                            */
+int bf_linear_attention_step(const bf_linear_attention *p, const void *q, const void *k, const void *v,
+                             const float *log_decay, float *state, void *o, void *stream);
+
+/* Rotary positions: of each head's first `rotated` features pair p is turned by position * frequencies[p] (radians; formed in
+ * double) and scaled by magnitude: (a, b) -> magnitude (a cos - b sin, a sin + b cos); a pair is features p and p + rotated / 2,
+ * or 2 p and 2 p + 1 (interleaved).  The other features are copied.  x is (batch, steps, heads, features) with adjacent
+ * features, y dense, positions (batch, steps).  back: by the opposite angle (the gradient of x from that of y). */
+typedef struct bf_rotary {
+    int32_t dtype; /* BF_F32 or BF_BF16 */
+    int32_t interleaved;
+    int64_t batch, steps, heads, features, rotated;
+    int64_t x_stride[3], position_stride[2];
+    double magnitude;
+} bf_rotary;
+
+/* positions and frequencies (rotated / 2) may be NULL where nothing is rotated. */
+int bf_rotary_apply(const bf_rotary *p, const void *x, const int64_t *positions, const double *frequencies,
+                    void *y, int32_t back, void *stream);
+
+/* A token for each row of logits (rows, vocab), entries adjacent, from one random number a row.  With
+ * w_i = exp((z_i - max z) / temperature): of the top_k largest logits (<= 0: all; ties: lowest indexes first) the likeliest
+ * ones until their sum reaches top_p of all of theirs (>= 1: all; at least one), of those the ones with w_i >= min_p (<= 0: all;
+ * at most 1); the token is the first index whose cumulated w, in the order of indexes, exceeds uniform * total (uniform in [0, 1)).
+ * temperature <= 0: the first of the largest logits.  NaN counts as -inf, which is never drawn; a row of nothing else gives
+ * -1; with +inf among the logits only those are drawn.  w is rounded to whole multiples of 2^-44: the same token at every call.
+ * Up to 2^19 entries. */
+typedef struct bf_sample {
+    int32_t dtype; /* BF_F32 or BF_BF16: logits */
+    int64_t rows, vocab;
+    int64_t logits_stride;
+    double temperature, top_p, min_p; /* of all rows, where the call has no array of one a row */
+    int64_t top_k;
+} bf_sample;
+
+/* temperature, top_k, top_p, min_p: one a row, or NULL. */
+int bf_sample_tokens(const bf_sample *p, const void *logits, const float *uniform, const float *temperature,
+                     const int64_t *top_k, const float *top_p, const float *min_p, int64_t *token,
+                     void *stream);
 
 #ifdef __cplusplus
 }
