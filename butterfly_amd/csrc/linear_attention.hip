@@ -149,7 +149,7 @@ extern "C" {
 size_t bf_linear_attention_kept_bytes(const bf_linear_attention *p)
 {
     if (check_attention(p)) return BF_SIZE_INVALID;
-    return (size_t)p->batch * (size_t)p->heads * (size_t)chunk_count(p) * (size_t)square(p) * sizeof(float);
+    return (size_t)p->batch * (size_t)p->heads * (size_t)chunk_count(p) * (size_t)p->features * (size_t)la_line((int)p->values) * sizeof(float);
 }
 
 size_t bf_linear_attention_fw_workspace_bytes(const bf_linear_attention *p)
@@ -190,10 +190,10 @@ int bf_linear_attention_fw(const bf_linear_attention *p, const void *q, const vo
         using T = decltype(type);
         constexpr int D = decltype(widest)::value;
         if (a.segments > 1) {
-            la_walk_kernel<T, D, false, false><<<walk_grid(a), dim3(4 * D), 0, s>>>(a);
+            la_walk_kernel<T, D, false, false><<<walk_grid(a), dim3(LaShape<T, D>::THREADS), 0, s>>>(a);
             la_enter_kernel<false><<<enter_grid(a), dim3(256), 0, s>>>(a);
         }
-        la_walk_kernel<T, D, true, false><<<walk_grid(a), dim3(4 * D), 0, s>>>(a);
+        la_walk_kernel<T, D, true, false><<<walk_grid(a), dim3(LaShape<T, D>::THREADS), 0, s>>>(a);
     });
     BF_HIP_CHECK(hipGetLastError());
     return BF_OK;
@@ -234,10 +234,10 @@ int bf_linear_attention_bw(const bf_linear_attention *p, const void *q, const vo
         using T = decltype(type);
         constexpr int D = decltype(widest)::value;
         if (a.segments > 1) {
-            la_walk_kernel<T, D, false, true><<<walk_grid(a), dim3(4 * D), 0, s>>>(a);
+            la_walk_kernel<T, D, false, true><<<walk_grid(a), dim3(LaShape<T, D>::THREADS), 0, s>>>(a);
             la_enter_kernel<true><<<enter_grid(a), dim3(256), 0, s>>>(a);
         }
-        la_back_kernel<T, D><<<walk_grid(a), dim3(4 * D), 0, s>>>(a);
+        la_back_kernel<T, D><<<walk_grid(a), dim3(LaShape<T, D>::THREADS), 0, s>>>(a);
         if (a.wide) {
             const int64_t rows = p->batch * p->steps, count = rows * p->groups * p->features;
             const dim3 grid((unsigned)std::min<int64_t>((count + 255) / 256, 1 << 16));

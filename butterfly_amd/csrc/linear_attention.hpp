@@ -53,6 +53,7 @@ struct LaArgs {
 };
 
 typedef float LaAcc __attribute__((ext_vector_type(4)));
+typedef int LaParts __attribute__((ext_vector_type(4)));
 typedef bf16 LaHalf4 __attribute__((ext_vector_type(4)));
 typedef bf16 LaHalf8 __attribute__((ext_vector_type(8)));
 
@@ -64,17 +65,25 @@ template <> struct LaFrag<float> { using type = LaAcc; };
 template <typename T, int D>
 struct LaShape {
     static constexpr int C = sizeof(T) == 4 && D == 128 ? 32 : 64;
-    static constexpr int W = D / 16;                 // wavefronts: each owns 16 columns of a state
-    static constexpr int TT = C / 16, DT = D / 16;   // tiles
+    static constexpr int SLICES = D / 16;            // of 16 columns of a state or a result
+    // wavefronts of a slice: two of 64 columns share the steps and the rows of the state (two wavefronts on each SIMD), the
+    // state's operands then go through LDS, where there is no room for those of 128
+    static constexpr int HALVES = D == 64 ? 2 : 1;
+    static constexpr int W = SLICES * HALVES, THREADS = 64 * W;
+    static constexpr int TT = C / 16, DT = D / 16;   // tiles of a chunk, of a state
+    static constexpr int OWN_T = TT / HALVES, OWN_D = DT / HALVES;
     static constexpr int E = 16 / sizeof(T);         // elements of a load
     static constexpr int LD = D + E, LDC = C + E;    // rows in LDS: 16 bytes more, so that sixteen of them start in different banks
-    static constexpr int LOADS = C * D / E / (64 * W);
+    static constexpr int LOADS = C * D / E / THREADS;
     // pairs of tiles (i, j) with j <= i, and those above the diagonal that a product of 32 steps reads
-    static constexpr int PAIRS = TT == 4 ? 12 : 4;
+    static constexpr int PAIRS = TT == 4 ? 12 : 4, EACH = (PAIRS + W - 1) / W;
     static constexpr int INNER = sizeof(T) == 4 ? 1 : 2;   // numbers that an inner factor or a state is split into
     static constexpr int ADDED = sizeof(T) == 4 ? 1 : 3;   // and what is added to a state
-    // the state's gradient in LDS (for dV): there is no room for a second number beside rows of 128
-    static constexpr int HELD = sizeof(T) == 4 || D == 128 ? 1 : 2;
+
+    // A wavefront's tiles of steps: all, or the first and last or the two in between, which meet equally many others.
+    static __device__ __forceinline__ int tile(int half, int u) { return HALVES == 1 ? u : u == 0 ? half : 3 - half; }
+    // The pair of tiles that holds it: pairs of earlier steps are those up to it, of later ones those from it on.
+    static constexpr int pair_of(int u) { return HALVES == 1 ? u / 2 : u; }
 };
 
 __device__ __forceinline__ LaAcc la_mma(LaHalf4 a0, LaHalf4 a1, LaHalf4 b0, LaHalf4 b1, LaAcc c)
@@ -146,22 +155,6 @@ __device__ __forceinline__ float la_sum16(float v)
     return v;
 }
 
-// 16 bytes of a row; what lies behind its end is zero.
-template <typename T>
-__device__ __forceinline__ uint4 la_load(const T *row, int col, int cols)
-{
-    constexpr int E = 16 / sizeof(T);
-    using Quad = std::conditional_t<sizeof(T) == 4, quad_at_4, quad_at_2>;
-    if (col + E <= cols) {
-        const Quad v = *reinterpret_cast<const Quad *>(row + col);
-        return __builtin_bit_cast(uint4, v);
-    }
-    T part[E];
-#pragma unroll
-    for (int i = 0; i < E; ++i) part[i] = col + i < cols ? row[col + i] : (T)0.0f;
-    return __builtin_bit_cast(uint4, part);
-}
-
 // The largest magnitude among the numbers of v, as bits; at least la_infinite<T> where one is not finite.
 typedef uint16_t LaShort2 __attribute__((ext_vector_type(2)));
 template <typename T>
@@ -185,91 +178,212 @@ __device__ __forceinline__ bool la_not_finite(uint32_t m)
     else return (m & 0xffffu) >= 0x7f80u || (m >> 16) >= 0x7f80u;
 }
 
-// The steps of a chunk that a lane brings into LDS, on their way in registers.
+// The steps of a chunk that a lane brings into LDS, on their way in registers: 16 bytes of a row each, always the same columns.
+// Nothing depends on what is loaded until it is stored, and nothing branches: rows behind the last step read that one, columns
+// behind a row's end its first ones, and the 16 bytes that a row's end cuts are read as the row's last 16 and moved down.
+// What does not exist is zero in LDS.
 template <typename T, int D>
 struct LaPiece {
     using S = LaShape<T, D>;
-    uint4 v[S::LOADS];
+    using Quad = std::conditional_t<sizeof(T) == 4, quad_at_4, quad_at_2>;
+    static constexpr int ROWS = S::THREADS / (D / S::E);   // between a lane's rows
+    Quad v[S::LOADS];
+    const T *base;
+    int64_t stride, offset;   // offset: of the lane's first 16 bytes from a chunk's first row
+    int cols, col, row, from; // col: where the 16 bytes go; from: and come from
+    int shift;                // bits that they move down
 
-    __device__ __forceinline__ void fetch(const T *base, int64_t stride, int rows, int cols)
+    __device__ __forceinline__ void init(const T *start, int64_t step, int columns)
     {
+        base = start;
+        stride = step;
+        cols = columns;
+        col = (int)threadIdx.x % (D / S::E) * S::E;
+        row = (int)threadIdx.x / (D / S::E);
+        const bool cut = col < cols && col + S::E > cols && cols >= S::E;
+        from = col >= cols ? 0 : cut ? cols - S::E : col;
+        shift = cut ? (col - from) * 8 * (int)sizeof(T) : 0;
+        offset = row * stride + from;
+    }
+    // whole chunks of rows of at least 16 bytes
+    __device__ __forceinline__ void fetch_whole(int64_t t0)
+    {
+        const T *start = base + t0 * stride;
+#pragma unroll
+        for (int n = 0; n < S::LOADS; ++n) v[n] = *reinterpret_cast<const Quad *>(start + n * ROWS * stride + offset);
+    }
+    __device__ __forceinline__ void fetch_any(int64_t t0, int rows)
+    {
+        const T *start = base + t0 * stride;
 #pragma unroll
         for (int n = 0; n < S::LOADS; ++n) {
-            const int at = threadIdx.x + n * 64 * S::W, row = at / (D / S::E), col = at % (D / S::E) * S::E;
-            v[n] = base && row < rows && col < cols ? la_load(base + row * stride, col, cols) : make_uint4(0, 0, 0, 0);
+            const T *at = start + min(row + n * ROWS, rows - 1) * stride;
+            if (cols >= S::E) {
+                v[n] = *reinterpret_cast<const Quad *>(at + from);
+            } else {
+                // (narrower than 16 bytes: one by one)
+                T x[S::E];
+#pragma unroll
+                for (int i = 0; i < S::E; ++i) x[i] = i < cols ? at[i] : (T)0.0f;
+                v[n] = __builtin_bit_cast(Quad, x);
+            }
         }
     }
-    __device__ __forceinline__ void store(T *lds, uint32_t &m) const
+    // magnitude: of what is stored, see la_magnitude
+    template <bool EVEN>
+    __device__ __forceinline__ void store(T *lds, int rows, uint32_t &magnitude) const
     {
 #pragma unroll
         for (int n = 0; n < S::LOADS; ++n) {
-            const int at = threadIdx.x + n * 64 * S::W, row = at / (D / S::E), col = at % (D / S::E) * S::E;
-            *reinterpret_cast<uint4 *>(lds + row * S::LD + col) = v[n];
-            la_magnitude<T>(v[n], m);
+            uint4 x = __builtin_bit_cast(uint4, v[n]);
+            if constexpr (!EVEN) {
+                uint64_t low = (uint64_t)x.y << 32 | x.x, high = (uint64_t)x.w << 32 | x.z;
+                low = shift >= 64 ? high >> (shift - 64) : low >> shift | (high << 1) << (63 - shift);
+                high = shift >= 64 ? 0 : high >> shift;
+                x = make_uint4((uint32_t)low, (uint32_t)(low >> 32), (uint32_t)high, (uint32_t)(high >> 32));
+            }
+            const bool there = (row + n * ROWS < rows) & (col < cols);
+            x.x = there ? x.x : 0;
+            x.y = there ? x.y : 0;
+            x.z = there ? x.z : 0;
+            x.w = there ? x.w : 0;
+            *reinterpret_cast<uint4 *>(lds + (row + n * ROWS) * S::LD + col) = x;
+            la_magnitude<T>(x, magnitude);
         }
     }
 };
 
-// Sums of a chunk's log decays, to the base 2, as two floats of together 48 bits: their differences keep the bits of the
-// decays between two steps, whatever the steps in front have summed up to.  part: resets so far.
+// What the products take from a chunk's decays.  Sums of log decays, to the base 2, as two floats of together 48 bits: their
+// differences keep the bits of the decays between two steps, whatever the steps in front have summed up to.  part: resets
+// so far.  start, end: what steps meet of the states in front of and behind the chunk (scale exp(L_i), exp(L_C - L_j)), -1 where a
+// reset lies between.
 template <int C>
 struct LaLevels {
-    float hi[C], lo[C];
+    float hi[C], lo[C], start[C], end[C];
     int part[C];
+    float decay;   // over the whole chunk; -1: a reset lies within
 
-    __device__ __forceinline__ float from_start(int i) const { return __builtin_amdgcn_exp2f(hi[i] + lo[i]); }
-    __device__ __forceinline__ float between(int i, int j) const { return __builtin_amdgcn_exp2f((hi[i] - hi[j]) + (lo[i] - lo[j])); }
+    __device__ __forceinline__ LaAcc quad(const float (&v)[C], int at) const { return *reinterpret_cast<const LaAcc *>(v + at); }
+    // scale exp(L_i - L_j) for four neighbouring steps i or j and one other one
+    __device__ __forceinline__ LaAcc between(LaAcc hi0, LaAcc lo0, float hi1, float lo1, float sign) const
+    {
+        LaAcc f;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) f[r] = __builtin_amdgcn_exp2f(sign * ((hi0[r] - hi1) + (lo0[r] - lo1)));
+        return f;
+    }
 };
+
+// (-1: nothing, whatever x is)
+__device__ __forceinline__ LaAcc la_times(LaAcc x, LaAcc factor)
+{
+#pragma unroll
+    for (int r = 0; r < 4; ++r) x[r] = factor[r] < 0.0f ? 0.0f : x[r] * factor[r];
+    return x;
+}
+__device__ __forceinline__ LaAcc la_times(LaAcc x, float factor) { return la_times(x, LaAcc{factor, factor, factor, factor}); }
+
+// Lanes' values moved up: by 1, 2, 4, 8 within rows of 16, then the last of a row to the next one, the last of two rows to the
+// next two.  Lanes that get nothing keep `none`.
+template <int STEP>
+__device__ __forceinline__ int la_up(int none, int v)
+{
+    constexpr int ctrl = STEP < 16 ? 0x110 + STEP : STEP == 16 ? 0x142 : 0x143;
+    return __builtin_amdgcn_update_dpp(none, v, ctrl, STEP == 16 ? 0xa : STEP == 32 ? 0xc : 0xf, 0xf, false);
+}
+template <int STEP>
+__device__ __forceinline__ float la_up(float none, float v)
+{
+    return __builtin_bit_cast(float, la_up<STEP>(__builtin_bit_cast(int, none), __builtin_bit_cast(int, v)));
+}
+template <int STEP>
+__device__ __forceinline__ double la_up(double none, double v)
+{
+    typedef int Two __attribute__((ext_vector_type(2)));
+    const Two n = __builtin_bit_cast(Two, none), x = __builtin_bit_cast(Two, v);
+    return __builtin_bit_cast(double, Two{la_up<STEP>(n[0], x[0]), la_up<STEP>(n[1], x[1])});
+}
+
+// One round of a sum over the lanes up to this one that lie in its part (parts grow with the lanes; -1: no lane).
+template <int STEP, typename V>
+__device__ __forceinline__ void la_scan_round(V &sum, int part)
+{
+    const V before = la_up<STEP>((V)0, sum);
+    if (la_up<STEP>(-1, part) == part) sum += before;
+}
+template <typename V>
+__device__ __forceinline__ void la_scan(V &sum, int part)
+{
+    la_scan_round<1>(sum, part);
+    la_scan_round<2>(sum, part);
+    la_scan_round<4>(sum, part);
+    la_scan_round<8>(sum, part);
+    la_scan_round<16>(sum, part);
+    la_scan_round<32>(sum, part);
+}
 
 // One step a lane.  A decay below 2^-160 is zero beside anything in 32 bits and counts as that.
 template <int C>
-__device__ __forceinline__ void la_levels(LaLevels<C> &out, float log_decay, bool reset)
+__device__ __forceinline__ void la_levels(LaLevels<C> &out, float log_decay, bool reset, float scale)
 {
     const int lane = threadIdx.x & 63;
     const double x = (double)log_decay * 1.4426950408889634;
     double level = reset ? 0.0 : x < -160.0 ? -160.0 : x;
-    int part = reset;
-#pragma unroll
-    for (int d = 1; d < C; d *= 2) {
-        const double before = __shfl_up(level, d, 64);
-        const int resets = __shfl_up(part, d, 64);
-        if (lane >= d) {
-            if (part == 0) level += before;
-            part += resets;
-        }
-    }
+    const uint64_t resets = __ballot(reset), below = ((uint64_t)2 << lane) - 1;
+    const int part = __popcll(resets & below), parts = __popcll(resets);
+    la_scan(level, part);
+    const float hi = (float)level, from_start = __builtin_amdgcn_exp2f(hi);
+    const double last = __shfl(level, C - 1, 64);
+    const float to_end = __builtin_amdgcn_exp2f((float)(last - level));
     if (lane < C) {
-        const float hi = (float)level;
         out.hi[lane] = hi;
-        // (not finite: the difference of two of them is what it is)
         out.lo[lane] = (float)(level - (double)hi);
+        out.start[lane] = part == 0 ? scale * from_start : -1.0f;
+        out.end[lane] = part == parts ? to_end : -1.0f;
         out.part[lane] = part;
+        if (lane == C - 1) out.decay = part == 0 ? from_start : -1.0f;
     }
 }
 
+// A chunk's decays and resets, one step a lane, on their way in registers (by every wavefront: no branch).
+template <int C>
 struct LaDecay {
-    float log_decay = 0.0f;
-    bool reset = false;
+    const float *log_decay;
+    const uint8_t *reset;
+    int64_t stride, reset_stride;
+    float x;
+    uint8_t flag;
+    bool inside, resets;
 
-    __device__ __forceinline__ void fetch(const LaArgs &a, const float *log_decay_row, const uint8_t *reset_row, int64_t t0, int rows)
+    __device__ __forceinline__ void init(const LaArgs &a, int64_t b, int h)
     {
-        const int lane = threadIdx.x & 63;
-        log_decay = lane < rows ? log_decay_row[(t0 + lane) * a.decay_stride[1]] : 0.0f;
-        reset = reset_row && lane < rows && reset_row[(t0 + lane) * a.reset_stride[1]] != 0;
+        log_decay = a.log_decay + b * a.decay_stride[0] + h * a.decay_stride[2];
+        stride = a.decay_stride[1];
+        resets = a.reset != nullptr;
+        reset = resets ? a.reset + b * a.reset_stride[0] : reinterpret_cast<const uint8_t *>(log_decay);
+        reset_stride = resets ? a.reset_stride[1] : 0;
+    }
+    __device__ __forceinline__ void fetch(int64_t t0, int rows)
+    {
+        const int lane = threadIdx.x & 63, at = min(lane, rows - 1);
+        x = log_decay[(t0 + at) * stride];
+        flag = reset[(t0 + at) * reset_stride];
+        inside = lane < rows && lane < C;
+    }
+    __device__ __forceinline__ void levels(LaLevels<C> &out, float scale) const
+    {
+        la_levels<C>(out, inside ? x : 0.0f, inside && resets && flag != 0, scale);
     }
 };
 
-// (ti, tj) of pair n
-template <int TT>
+// Values of a row of the kept states: whole quads (those behind the last value are zero)
+__host__ __device__ __forceinline__ int la_line(int values) { return (values + 3) / 4 * 4; }
+
+// (ti, tj) of pair n: those with j <= i of two rows of tiles, then of the next two, out of a number for each (two bits a pair)
 __device__ __forceinline__ void la_pair(int n, int &ti, int &tj)
 {
-    if (n < 4) {
-        ti = n >> 1;
-        tj = n & 1;
-    } else {
-        ti = 2 + ((n - 4) >> 2);
-        tj = (n - 4) & 3;
-    }
+    ti = 0xffaa50 >> 2 * n & 3;
+    tj = 0xe4e444 >> 2 * n & 3;
 }
 
 // The pieces of step t alone: the others count as zero whatever they are.
@@ -283,31 +397,65 @@ __device__ __forceinline__ F la_only(F f, int t)
     return f;
 }
 
-// Sum over the steps of tiles first .. last of a(part, tile) x b(tile), onto c (rows: steps row0 + 4 g + r of the chunk).
-// bad: something is not finite.  Then step by step, and only onto the rows that `meets(row, step)`: what a factor of
+// Sum over the steps of the pairs of tiles first .. last of a(part, tile) x b(tile), onto c (rows: steps of the chunk).
+// BAD: something in the chunk is not finite.  Then step by step, and only onto the rows that `meets(row, step)`: what a factor of
 // zero stands for must not turn into NaN.
-template <int N, int TT, typename F, typename A, typename B, typename M>
-__device__ __forceinline__ void la_over_steps(LaAcc &c, int first, int last, bool bad, A &&a, B &&b, M &&meets)
+template <bool BAD, int N, int TT, typename F, typename A, typename B, typename M>
+__device__ __forceinline__ void la_over_steps(LaAcc &c, int first, int last, A &&a, B &&b, M &&meets)
 {
-    if (!bad) {
+    if constexpr (!BAD) {
 #pragma unroll
-        for (int p = 0; p < TT; p += 2)
-            if (p + 1 >= first && p <= last) {
+        for (int p = 0; p < TT / 2; ++p)
+            if (p >= first && p <= last) {
 #pragma unroll
-                for (int n = 0; n < N; ++n) c = la_mma(a(n, p), a(n, p + 1), b(p), b(p + 1), c);
+                for (int n = 0; n < N; ++n) c = la_mma(a(n, 2 * p), a(n, 2 * p + 1), b(2 * p), b(2 * p + 1), c);
             }
-        return;
-    }
-    const F zero = {};
-    for (int tile = first; tile <= last; ++tile)
-        for (int t = 16 * tile; t < 16 * tile + 16; ++t) {
+    } else {
+        const F zero = {};
+#pragma unroll 1
+        for (int t = 32 * first; t < 32 * last + 32; ++t) {
             LaAcc d = {};
-            for (int n = 0; n < N; ++n) d = la_mma(la_only(a(n, tile), t), zero, la_only(b(tile), t), zero, d);
+#pragma unroll 1
+            for (int n = 0; n < N; ++n) d = la_mma(la_only(a(n, t >> 4), t), zero, la_only(b(t >> 4), t), zero, d);
 #pragma unroll
             for (int r = 0; r < 4; ++r)
                 if (meets(r, t)) c[r] += d[r];
         }
+    }
 }
+
+// A chunk's rows of a dense result: 16-bit or 32-bit stores of a tile, whose range check drops rows behind the last step and
+// columns behind the last one, so that nothing branches.  (The whole offset is in the lane's register, where the check sees it.)
+struct LaOut {
+    __amdgpu_buffer_rsrc_t to;
+    unsigned at;
+    unsigned row_bytes;
+
+    template <typename T>
+    __device__ __forceinline__ void init(T *row0, int rows, int row_elements, int col, int cols)
+    {
+        row_bytes = (unsigned)(row_elements * (int)sizeof(T));
+        to = __builtin_amdgcn_make_buffer_rsrc(row0, 0, (int)(rows * row_bytes), 0x00020000);
+        at = col < cols ? 4 * ((threadIdx.x & 63) >> 4) * row_bytes + col * (unsigned)sizeof(T) : 0x80000000u;
+    }
+    __device__ __forceinline__ void store(int tile, LaAcc x, float) const
+    {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const float y = x[r];
+            __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, y), to, (int)(at + (16 * tile + r) * row_bytes), 0, 0);
+        }
+    }
+    __device__ __forceinline__ void store(int tile, LaAcc x, bf16) const
+    {
+        const LaHalf4 half = __builtin_convertvector(x, LaHalf4);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const bf16 y = half[r];
+            __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(unsigned short, y), to, (int)(at + (16 * tile + r) * row_bytes), 0, 0);
+        }
+    }
+};
 
 __device__ __forceinline__ int64_t la_offset(const int64_t (&stride)[3], int64_t b, int64_t t, int64_t h)
 {
@@ -326,182 +474,220 @@ __device__ __forceinline__ int64_t la_unit(int64_t units)
 // A head's walk over its chunks.  OUT: outputs, and the states in front of the chunks where they are kept; otherwise
 // what a segment adds to the state: of k^T w v forward, of q^T b grad with BACK (from the end).
 template <typename T, int D, bool OUT, bool BACK>
-__global__ __launch_bounds__(4 * D) void la_walk_kernel(const LaArgs a)
+__global__ __launch_bounds__((LaShape<T, D>::THREADS)) void la_walk_kernel(const LaArgs a)
 {
     using S = LaShape<T, D>;
     using F = typename LaFrag<T>::type;
-    constexpr int C = S::C, W = S::W, TT = S::TT, DT = S::DT, LD = S::LD, LDC = S::LDC;
+    constexpr int C = S::C, W = S::W, TT = S::TT, DT = S::DT, OT = S::OWN_T, OD = S::OWN_D, LD = S::LD, LDC = S::LDC;
+    constexpr bool SHARED = OUT && S::HALVES > 1;   // the state's operands in LDS
     __shared__ __align__(16) T ks[C * LD];
     __shared__ __align__(16) T vs[C * LD];
     __shared__ __align__(16) T qs[OUT ? C * LD : 16];
     __shared__ __align__(16) T ps[OUT ? S::INNER * C * LDC : 16];
-    __shared__ __align__(16) LaLevels<C> levels;
+    __shared__ __align__(16) T ss[SHARED ? S::INNER * D * LD : 16];   // S, rows are values
+    __shared__ __align__(16) LaLevels<C> both_levels[2];
     __shared__ int bad_chunk[2];
 
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, i16 = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, i16 = lane & 15, g = lane >> 4;
+    const int slice = wave % S::SLICES, half = wave / S::SLICES;
     const int64_t heads = a.batch * a.heads, unit = la_unit(heads * a.segments);
     if (unit >= heads * a.segments) return;
     const int64_t segment = unit / heads, bh = unit % heads, b = bh / a.heads;
     const int h = (int)(bh % a.heads);
     const int64_t first = segment * a.segment_chunks, end = min(first + a.segment_chunks, a.chunks);
     const int count = (int)(end - first), features = a.features, values = a.values;
-    const T *q = static_cast<const T *>(a.q) + (OUT ? la_offset(a.q_stride, b, 0, h / a.shared) : 0);
-    const T *k = BACK ? static_cast<const T *>(a.q) + la_offset(a.q_stride, b, 0, h / a.shared)
-                      : static_cast<const T *>(a.k) + la_offset(a.k_stride, b, 0, h / a.shared);
-    const T *v = BACK ? (a.grad ? static_cast<const T *>(a.grad) + la_offset(a.grad_stride, b, 0, h) : nullptr)
-                      : static_cast<const T *>(a.v) + la_offset(a.v_stride, b, 0, h);
-    const int64_t k_step = BACK ? a.q_stride[1] : a.k_stride[1], v_step = BACK ? a.grad_stride[1] : a.v_stride[1];
-    const float *decay_row = a.log_decay + la_offset(a.decay_stride, b, 0, h);
-    const uint8_t *reset_row = a.reset ? a.reset + b * a.reset_stride[0] : nullptr;
+    const bool nothing = BACK && !a.grad;   // (no gradient of o: zeros, whatever is read)
 
-    // rows: features 16 t + 4 g + r, column: value 16 wave + lane % 16
-    LaAcc s[DT];
-    const int col = 16 * wave + i16;
+    // rows: features 16 (half OD + t) + 4 g + r, column: value 16 slice + lane % 16
+    LaAcc s[OD];
+    const int col = 16 * slice + i16, row0 = 16 * half * OD + 4 * g;
     const float *start = !OUT ? nullptr : a.segments > 1 ? a.segment_state + (segment * heads + bh) * features * values
                                        : a.state ? a.state + bh * features * values : nullptr;
 #pragma unroll
-    for (int t = 0; t < DT; ++t)
+    for (int t = 0; t < OD; ++t)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            const int row = 16 * t + 4 * g + r;
+            const int row = row0 + 16 * t + r;
             s[t][r] = start && row < features && col < values ? start[row * values + col] : 0.0f;
         }
 
     LaPiece<T, D> nk, nv, nq;
-    LaDecay nd;
+    if constexpr (BACK) {
+        nk.init(static_cast<const T *>(a.q) + la_offset(a.q_stride, b, 0, h / a.shared), a.q_stride[1], features);
+        nv.init(static_cast<const T *>(nothing ? a.v : a.grad) + la_offset(nothing ? a.v_stride : a.grad_stride, b, 0, h),
+                nothing ? a.v_stride[1] : a.grad_stride[1], values);
+    } else {
+        nk.init(static_cast<const T *>(a.k) + la_offset(a.k_stride, b, 0, h / a.shared), a.k_stride[1], features);
+        nv.init(static_cast<const T *>(a.v) + la_offset(a.v_stride, b, 0, h), a.v_stride[1], values);
+    }
+    if constexpr (OUT) nq.init(static_cast<const T *>(a.q) + la_offset(a.q_stride, b, 0, h / a.shared), a.q_stride[1], features);
+    LaDecay<C> nd;
+    nd.init(a, b, h);
+    auto chunk_of = [&](int n) { return BACK ? end - 1 - n : first + n; };
+    auto rows_of = [&](int n) { return (int)min((int64_t)C, a.steps - chunk_of(n) * C); };
+    const bool wide = features >= S::E && values >= S::E, even = features % S::E == 0 && values % S::E == 0;
     auto fetch = [&](int n) {
-        const int64_t chunk = BACK ? end - 1 - n : first + n, t0 = chunk * C;
-        const int rows = (int)min((int64_t)C, a.steps - t0);
-        nk.fetch(k + t0 * k_step, k_step, rows, features);
-        nv.fetch(v ? v + t0 * v_step : nullptr, v_step, rows, values);
-        if constexpr (OUT) nq.fetch(q + t0 * a.q_stride[1], a.q_stride[1], rows, features);
-        if (wave == 0) nd.fetch(a, decay_row, reset_row, t0, rows);
+        const int64_t t0 = chunk_of(n) * C;
+        const int rows = rows_of(n);
+        if (__builtin_expect(wide && rows == C, 1)) {
+            nk.fetch_whole(t0);
+            nv.fetch_whole(t0);
+            if constexpr (OUT) nq.fetch_whole(t0);
+        } else {
+            nk.fetch_any(t0, rows);
+            nv.fetch_any(t0, rows);
+            if constexpr (OUT) nq.fetch_any(t0, rows);
+        }
     };
     if (threadIdx.x < 2) bad_chunk[threadIdx.x] = 0;
+    nd.fetch(chunk_of(0) * C, rows_of(0));
     fetch(0);
+    if (wave == W - 1) nd.levels(both_levels[0], a.scale);
+    nd.fetch(chunk_of(min(1, count - 1)) * C, rows_of(min(1, count - 1)));
     __syncthreads();
     double total = 0.0;
     int cuts = 0;
     for (int n = 0; n < count; ++n) {
-        const int64_t chunk = BACK ? end - 1 - n : first + n, t0 = chunk * C;
+        const int64_t chunk = chunk_of(n), t0 = chunk * C;
+        const int rows = rows_of(n);
+        const LaLevels<C> &levels = both_levels[n & 1];
         uint32_t magnitude = 0;
-        nk.store(ks, magnitude);
-        nv.store(vs, magnitude);
-        if constexpr (OUT) nq.store(qs, magnitude);
+        auto store = [&](auto even_type) {
+            constexpr bool EVEN = decltype(even_type)::value;
+            nk.template store<EVEN>(ks, rows, magnitude);
+            nv.template store<EVEN>(vs, nothing ? 0 : rows, magnitude);
+            if constexpr (OUT) nq.template store<EVEN>(qs, rows, magnitude);
+        };
+        if (__builtin_expect(even, 1)) store(std::true_type());
+        else store(std::false_type());
+        if constexpr (SHARED) {
+#pragma unroll
+            for (int t = 0; t < OD; ++t) {
+                F f[S::INNER];
+                la_split(s[t], f);
+#pragma unroll
+                for (int m = 0; m < S::INNER; ++m) *reinterpret_cast<F *>(ss + (m * D + col) * LD + row0 + 16 * t) = f[m];
+            }
+        }
         if (la_not_finite<T>(magnitude)) bad_chunk[n & 1] = 1;
-        if (wave == 0) la_levels<C>(levels, nd.log_decay, nd.reset);
         __syncthreads();
         const bool bad = bad_chunk[n & 1] != 0;
         if (threadIdx.x == 0) bad_chunk[(n + 1) & 1] = 0;
-        if (n + 1 < count) fetch(n + 1);
+        // (behind the last chunk: that one once more)
+        fetch(min(n + 1, count - 1));
+        if (wave == W - 1 && n + 1 < count) nd.levels(both_levels[(n + 1) & 1], a.scale);
+        nd.fetch(chunk_of(min(n + 2, count - 1)) * C, rows_of(min(n + 2, count - 1)));
 
-        if constexpr (OUT) {
-            // Q K^T . D, transposed in the sums: rows are steps j
-            for (int p = wave; p < S::PAIRS; p += W) {
-                int ti, tj;
-                la_pair<TT>(p, ti, tj);
-                LaAcc c = {};
-                if (tj <= ti) {
+        auto products = [&](auto bad_type) {
+            constexpr bool BAD = decltype(bad_type)::value;
+            if constexpr (OUT) {
+                // Q K^T . D, transposed in the sums: rows are steps j
+#pragma unroll
+                for (int u = 0; u < S::EACH; ++u) {
+                    const int p = wave + u * W;
+                    if (S::PAIRS % W != 0 && p >= S::PAIRS) break;
+                    int ti, tj;
+                    la_pair(p, ti, tj);
+                    LaAcc c = {};
 #pragma unroll
                     for (int x = 0; x < D; x += 32)
                         c = la_mma(la_rows<F>(ks, LD, 16 * tj, x), la_rows<F>(ks, LD, 16 * tj, x + 16), la_rows<F>(qs, LD, 16 * ti, x),
                                    la_rows<F>(qs, LD, 16 * ti, x + 16), c);
-                }
-                const int i = 16 * ti + i16;
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int j = 16 * tj + 4 * g + r;
-                    c[r] = j <= i && levels.part[j] == levels.part[i] ? c[r] * (a.scale * levels.between(i, j)) : 0.0f;
-                }
-                F f[S::INNER];
-                la_split(c, f);
-#pragma unroll
-                for (int m = 0; m < S::INNER; ++m) *reinterpret_cast<F *>(ps + (m * C + i) * LDC + 16 * tj + 4 * g) = f[m];
-            }
-        }
-        F vf[TT];
-#pragma unroll
-        for (int t = 0; t < TT; ++t) vf[t] = la_cols(vs, LD, 16 * t, 16 * wave);
-        if constexpr (OUT) {
-            if (a.kept) {
-                float *to = a.kept + (bh * a.chunks + chunk) * features * values;
-#pragma unroll
-                for (int t = 0; t < DT; ++t)
+                    const int i = 16 * ti + i16, j = 16 * tj + 4 * g, part = levels.part[i];
+                    const LaAcc f_ij = levels.between(levels.quad(levels.hi, j), levels.quad(levels.lo, j), levels.hi[i], levels.lo[i], -1.0f);
+                    const LaParts parts = *reinterpret_cast<const LaParts *>(levels.part + j);
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
-                        const int row = 16 * t + 4 * g + r;
-                        if (row < features && col < values) to[row * values + col] = s[t][r];
+                        const float x = c[r] * (a.scale * f_ij[r]);
+                        c[r] = (j + r <= i) & (parts[r] == part) ? x : 0.0f;
                     }
-            }
-            LaAcc o[TT] = {};
+                    F f[S::INNER];
+                    la_split(c, f);
 #pragma unroll
-            for (int x = 0; x < DT; x += 2) {
-                F s0[S::INNER], s1[S::INNER];
-                la_split(s[x], s0);
-                la_split(s[x + 1], s1);
-#pragma unroll
-                for (int t = 0; t < TT; ++t) {
-                    const F q0 = la_rows<F>(qs, LD, 16 * t, 16 * x), q1 = la_rows<F>(qs, LD, 16 * t, 16 * x + 16);
-#pragma unroll
-                    for (int m = 0; m < S::INNER; ++m) o[t] = la_mma(q0, q1, s0[m], s1[m], o[t]);
+                    for (int m = 0; m < S::INNER; ++m) *reinterpret_cast<F *>(ps + (m * C + i) * LDC + j) = f[m];
                 }
             }
-            __syncthreads();
-            T *out = static_cast<T *>(a.o) + ((b * a.steps + t0) * a.heads + h) * values;
-            const int rows = (int)min((int64_t)C, a.steps - t0);
+            F vf[TT];
 #pragma unroll
-            for (int t = 0; t < TT; ++t) {
+            for (int t = 0; t < TT; ++t) vf[t] = la_cols(vs, LD, 16 * t, 16 * slice);
+            if constexpr (OUT) {
+                if (a.kept) {
+                    LaOut to;
+                    to.init(a.kept + (bh * a.chunks + chunk) * features * la_line(values), features, la_line(values), col, la_line(values));
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int i = 16 * t + 4 * g + r;
-                    o[t][r] = levels.part[i] == 0 ? o[t][r] * (a.scale * levels.from_start(i)) : 0.0f;
+                    for (int t = 0; t < OD; ++t) to.store(half * OD + t, s[t], 0.0f);
                 }
-                la_over_steps<S::INNER, TT, F>(
-                    o[t], 0, t, bad, [&](int m, int j) { return la_rows<F>(ps + m * C * LDC, LDC, 16 * t, 16 * j); },
-                    [&](int j) { return la_cols(vs, LD, 16 * j, 16 * wave); },
-                    [&](int r, int j) { const int i = 16 * t + 4 * g + r; return j <= i && levels.part[j] == levels.part[i]; });
+                LaAcc o[OT] = {};
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int i = 16 * t + 4 * g + r;
-                    if (i < rows && col < values) out[(int64_t)i * a.heads * values + col] = (T)o[t][r];
-                }
-            }
-        }
-        // the state behind the chunk (BACK: its gradient in front of it)
-        const int part = levels.part[C - 1];
-        const float decay = levels.from_start(C - 1);
+                for (int x = 0; x < DT; x += 2) {
+                    F s0[S::INNER], s1[S::INNER];
+                    if constexpr (SHARED) {
 #pragma unroll
-        for (int t = 0; t < DT; ++t) s[t] = part == 0 ? s[t] * decay : LaAcc{0.f, 0.f, 0.f, 0.f};
+                        for (int m = 0; m < S::INNER; ++m) {
+                            s0[m] = la_rows<F>(ss + m * D * LD, LD, 16 * slice, 16 * x);
+                            s1[m] = la_rows<F>(ss + m * D * LD, LD, 16 * slice, 16 * x + 16);
+                        }
+                    } else {
+                        la_split(s[x], s0);
+                        la_split(s[x + 1], s1);
+                    }
 #pragma unroll
-        for (int t = 0; t < TT; t += 2) {
-            F w[2][S::ADDED];
+                    for (int u = 0; u < OT; ++u) {
+                        const int t = S::tile(half, u);
+                        const F q0 = la_rows<F>(qs, LD, 16 * t, 16 * x), q1 = la_rows<F>(qs, LD, 16 * t, 16 * x + 16);
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                LaAcc x = la_float(vf[t + u]);
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int j = 16 * (t + u) + 4 * g + r;
-                    x[r] = levels.part[j] != (BACK ? 0 : part) ? 0.0f : x[r] * (BACK ? a.scale * levels.from_start(j) : levels.between(C - 1, j));
-                }
-                la_split(x, w[u]);
-            }
-#pragma unroll
-            for (int x = 0; x < DT; ++x) {
-                F k0 = la_cols(ks, LD, 16 * t, 16 * x), k1 = la_cols(ks, LD, 16 * t + 16, 16 * x);
-                if (bad) {
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        if (levels.part[16 * t + 4 * g + r] != (BACK ? 0 : part)) k0[r] = 0.0f;
-                        if (levels.part[16 * t + 16 + 4 * g + r] != (BACK ? 0 : part)) k1[r] = 0.0f;
+                        for (int m = 0; m < S::INNER; ++m) o[u] = la_mma(q0, q1, s0[m], s1[m], o[u]);
                     }
                 }
+                __syncthreads();
+                LaOut to;
+                to.init(static_cast<T *>(a.o) + ((b * a.steps + t0) * a.heads + h) * values, rows, a.heads * values, col, values);
 #pragma unroll
-                for (int m = 0; m < S::ADDED; ++m) s[x] = la_mma(k0, k1, w[0][m], w[1][m], s[x]);
+                for (int u = 0; u < OT; ++u) {
+                    const int t = S::tile(half, u);
+                    o[u] = la_times(o[u], levels.quad(levels.start, 16 * t + 4 * g));
+                    la_over_steps<BAD, S::INNER, TT, F>(
+                        o[u], 0, S::pair_of(u), [&](int m, int j) { return la_rows<F>(ps + m * C * LDC, LDC, 16 * t, 16 * j); },
+                        [&](int j) { return BAD ? la_cols(vs, LD, 16 * j, 16 * slice) : vf[j]; },
+                        [&](int r, int j) { const int i = 16 * t + 4 * g + r; return j <= i && levels.part[j] == levels.part[i]; });
+                }
+#pragma unroll
+                for (int u = 0; u < OT; ++u) to.store(S::tile(half, u), o[u], T());
             }
-        }
+            // the state behind the chunk (BACK: its gradient in front of it)
+            const float decay = levels.decay;
+#pragma unroll
+            for (int t = 0; t < OD; ++t) s[t] = la_times(s[t], decay);
+#pragma unroll
+            for (int t = 0; t < TT; t += 2) {
+                F w[2][S::ADDED];
+                LaAcc factor[2];
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    factor[u] = levels.quad(BACK ? levels.start : levels.end, 16 * (t + u) + 4 * g);
+                    la_split(la_times(la_float(vf[t + u]), factor[u]), w[u]);
+                }
+#pragma unroll
+                for (int x = 0; x < OD; ++x) {
+                    const int at = 16 * (half * OD + x);
+                    F k0 = la_cols(ks, LD, 16 * t, at), k1 = la_cols(ks, LD, 16 * t + 16, at);
+                    if constexpr (BAD) {
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            if (factor[0][r] < 0.0f) k0[r] = 0.0f;
+                            if (factor[1][r] < 0.0f) k1[r] = 0.0f;
+                        }
+                    }
+#pragma unroll
+                    for (int m = 0; m < S::ADDED; ++m) s[x] = la_mma(k0, k1, w[0][m], w[1][m], s[x]);
+                }
+            }
+        };
+        if (__builtin_expect(bad, 0)) products(std::true_type());
+        else products(std::false_type());
         if constexpr (!OUT) {
             total += (double)levels.hi[C - 1] + (double)levels.lo[C - 1];
-            cuts |= part;
+            cuts |= levels.part[C - 1];
         }
         __syncthreads();
     }
@@ -509,10 +695,10 @@ __global__ __launch_bounds__(4 * D) void la_walk_kernel(const LaArgs a)
                     : a.segment_state + (segment * heads + bh) * features * values;
     if (to) {
 #pragma unroll
-        for (int t = 0; t < DT; ++t)
+        for (int t = 0; t < OD; ++t)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const int row = 16 * t + 4 * g + r;
+                const int row = row0 + 16 * t + r;
                 if (row < features && col < values) to[row * values + col] = s[t][r];
             }
     }
@@ -550,304 +736,407 @@ __global__ __launch_bounds__(256) void la_copy_kernel(const float *from, float *
 
 // The gradients, chunk by chunk from a segment's end, with the states that the forward call kept.
 template <typename T, int D>
-__global__ __launch_bounds__(4 * D) void la_back_kernel(const LaArgs a)
+__global__ __launch_bounds__((LaShape<T, D>::THREADS)) void la_back_kernel(const LaArgs a)
 {
     using S = LaShape<T, D>;
     using F = typename LaFrag<T>::type;
-    constexpr int C = S::C, W = S::W, TT = S::TT, DT = S::DT, LD = S::LD, LDC = S::LDC;
+    constexpr int C = S::C, W = S::W, TT = S::TT, DT = S::DT, OT = S::OWN_T, OD = S::OWN_D, LD = S::LD, LDC = S::LDC;
+    constexpr bool SHARED = S::HALVES > 1;             // E's operands for dK in LDS too, to the chunk's end
+    constexpr int EP = SHARED ? S::ADDED : S::INNER;   // numbers of E in LDS
+    constexpr int HELD = EP * D * LD, FACTORS = 2 * S::INNER * C * LDC;
     __shared__ __align__(16) T qs[C * LD];
     __shared__ __align__(16) T ks[C * LD];
     __shared__ __align__(16) T vs[C * LD];
     __shared__ __align__(16) T gs[C * LD];
-    __shared__ __align__(16) T es[S::HELD * D * LD];         // E, rows are features
-    __shared__ __align__(16) T ps[S::INNER * C * LDC];       // (Q K^T . D)^T, rows are steps j
-    __shared__ __align__(16) T ds[S::INNER * C * LDC];       // (dO V^T . D)^T
-    __shared__ __align__(16) LaLevels<C> levels;
-    __shared__ float row_sums[TT][C], col_sums[TT][C], start_sums[W][C], end_sums[W][C], through[W];
+    // E, rows are features; (Q K^T . D)^T and (dO V^T . D)^T, rows are steps j, in its place where it is not needed any more
+    __shared__ __align__(16) T room[SHARED ? HELD + FACTORS : HELD > FACTORS ? HELD : FACTORS];
+    T *const es = room, *const ps = room + (SHARED ? HELD : 0), *const ds = ps + S::INNER * C * LDC;
+    __shared__ __align__(16) LaLevels<C> both_levels[2];
+    struct Sums {
+        float row[TT][C], col[TT][C], start[S::SLICES][C], end[S::SLICES][C], through[W];
+    };
+    __shared__ __align__(16) Sums sums;
     __shared__ int bad_chunk[2];
 
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, i16 = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, i16 = lane & 15, g = lane >> 4;
+    const int slice = wave % S::SLICES, half = wave / S::SLICES;
     const int64_t heads = a.batch * a.heads, unit = la_unit(heads * a.segments);
     if (unit >= heads * a.segments) return;
     const int64_t segment = unit / heads, bh = unit % heads, b = bh / a.heads;
     const int h = (int)(bh % a.heads);
     const int64_t first = segment * a.segment_chunks, end = min(first + a.segment_chunks, a.chunks);
     const int count = (int)(end - first), features = a.features, values = a.values;
-    const T *q = static_cast<const T *>(a.q) + la_offset(a.q_stride, b, 0, h / a.shared);
-    const T *k = static_cast<const T *>(a.k) + la_offset(a.k_stride, b, 0, h / a.shared);
-    const T *v = static_cast<const T *>(a.v) + la_offset(a.v_stride, b, 0, h);
-    const T *go = a.grad ? static_cast<const T *>(a.grad) + la_offset(a.grad_stride, b, 0, h) : nullptr;
-    const float *decay_row = a.log_decay + la_offset(a.decay_stride, b, 0, h);
-    const uint8_t *reset_row = a.reset ? a.reset + b * a.reset_stride[0] : nullptr;
 
-    // E transposed: rows are values 16 t + 4 g + r, column: feature 16 wave + lane % 16; S likewise
-    LaAcc e[DT], before[DT];
-    const int col = 16 * wave + i16;
-    auto fetch_square = [&](const float *from, LaAcc (&to)[DT]) {
+    // E transposed: rows are values 16 (half OD + t) + 4 g + r, column: feature 16 slice + lane % 16
+    LaAcc e[OD];
+    const int col = 16 * slice + i16, value0 = 16 * half * OD + 4 * g;
+    const float *behind = a.segments > 1 ? a.segment_state + (segment * heads + bh) * features * values
+                          : a.grad_last ? a.grad_last + bh * features * values : nullptr;
 #pragma unroll
-        for (int t = 0; t < DT; ++t) {
-            const int row = 16 * t + 4 * g;
-            if (from && col < features && row + 4 <= values) {
-                const quad_at_4 x = *reinterpret_cast<const quad_at_4 *>(from + (int64_t)col * values + row);
-                to[t] = LaAcc{x[0], x[1], x[2], x[3]};
-            } else {
+    for (int t = 0; t < OD; ++t)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) to[t][r] = from && col < features && row + r < values ? from[(int64_t)col * values + row + r] : 0.0f;
-            }
+        for (int r = 0; r < 4; ++r) {
+            const int row = value0 + 16 * t + r;
+            e[t][r] = behind && col < features && row < values ? behind[col * values + row] : 0.0f;
+        }
+
+    const bool nothing = !a.grad;   // (no gradient of o: zeros, whatever is read)
+    LaPiece<T, D> nq, nk, nv, ng;
+    nq.init(static_cast<const T *>(a.q) + la_offset(a.q_stride, b, 0, h / a.shared), a.q_stride[1], features);
+    nk.init(static_cast<const T *>(a.k) + la_offset(a.k_stride, b, 0, h / a.shared), a.k_stride[1], features);
+    nv.init(static_cast<const T *>(a.v) + la_offset(a.v_stride, b, 0, h), a.v_stride[1], values);
+    ng.init(static_cast<const T *>(nothing ? a.v : a.grad) + la_offset(nothing ? a.v_stride : a.grad_stride, b, 0, h),
+            nothing ? a.v_stride[1] : a.grad_stride[1], values);
+    LaDecay<C> nd;
+    nd.init(a, b, h);
+    auto chunk_of = [&](int n) { return end - 1 - n; };
+    auto rows_of = [&](int n) { return (int)min((int64_t)C, a.steps - chunk_of(n) * C); };
+    const bool wide = features >= S::E && values >= S::E, even = features % S::E == 0 && values % S::E == 0;
+    auto fetch = [&](int n) {
+        const int64_t t0 = chunk_of(n) * C;
+        const int rows = rows_of(n);
+        if (__builtin_expect(wide && rows == C, 1)) {
+            nq.fetch_whole(t0);
+            nk.fetch_whole(t0);
+            nv.fetch_whole(t0);
+            ng.fetch_whole(t0);
+        } else {
+            nq.fetch_any(t0, rows);
+            nk.fetch_any(t0, rows);
+            nv.fetch_any(t0, rows);
+            ng.fetch_any(t0, rows);
         }
     };
-    fetch_square(a.segments > 1 ? a.segment_state + (segment * heads + bh) * features * values
-                                : a.grad_last ? a.grad_last + bh * features * values : nullptr, e);
+    const int line = la_line(values);
 
-    LaPiece<T, D> nq, nk, nv, ng;
-    LaDecay nd;
-    auto fetch = [&](int n) {
-        const int64_t chunk = end - 1 - n, t0 = chunk * C;
-        const int rows = (int)min((int64_t)C, a.steps - t0);
-        nq.fetch(q + t0 * a.q_stride[1], a.q_stride[1], rows, features);
-        nk.fetch(k + t0 * a.k_stride[1], a.k_stride[1], rows, features);
-        nv.fetch(v + t0 * a.v_stride[1], a.v_stride[1], rows, values);
-        ng.fetch(go ? go + t0 * a.grad_stride[1] : nullptr, a.grad_stride[1], rows, values);
-        if (wave == 0) nd.fetch(a, decay_row, reset_row, t0, rows);
+    // The decays' gradients of a chunk, one step a lane: sums over the later steps of its document, sums over the earlier ones.
+    auto decays = [&](int n) {
+        const LaLevels<C> &levels = both_levels[n & 1];
+        const int mine = levels.part[min(lane, C - 1)], parts = levels.part[C - 1], part_before = __shfl_up(mine, 1, 64);
+        // later steps: lanes reversed, so that they are the earlier ones
+        const int t = C - 1 - min(lane, C - 1), reversed = parts - levels.part[t];
+        float later = 0.0f, earlier = 0.0f;
+#pragma unroll
+        for (int x = 0; x < TT; ++x) {
+            later += x <= ((t >> 4) | 1) ? sums.row[x][t] : 0.0f;
+            later -= x >= ((t >> 4) & ~1) ? sums.col[x][t] : 0.0f;
+        }
+#pragma unroll
+        for (int x = 0; x < S::SLICES; ++x) {
+            later += sums.start[x][t];
+            earlier += sums.end[x][min(lane, C - 1)];
+        }
+        la_scan(later, reversed);
+        la_scan(earlier, mine);
+        later = __shfl(later, C - 1 - min(lane, C - 1), 64);
+        float ahead = __shfl_up(earlier, 1, 64);
+        if (lane == 0 || part_before != mine) ahead = 0.0f;
+        float crossing = 0.0f;
+        if (parts == 0) {
+#pragma unroll
+            for (int x = 0; x < W; ++x) crossing += sums.through[x];
+            crossing *= levels.decay;
+        }
+        // (the decay of a reset step meets nothing)
+        const bool starts = mine != (lane == 0 ? 0 : part_before);
+        if (lane < rows_of(n)) a.d_log_decay[((b * a.steps + chunk_of(n) * C + lane) * a.heads) + h] = starts ? 0.0f : later + ahead + crossing;
     };
+
     if (threadIdx.x < 2) bad_chunk[threadIdx.x] = 0;
+    nd.fetch(chunk_of(0) * C, rows_of(0));
     fetch(0);
+    if (wave == W - 1) nd.levels(both_levels[0], a.scale);
+    nd.fetch(chunk_of(min(1, count - 1)) * C, rows_of(min(1, count - 1)));
     __syncthreads();
     for (int n = 0; n < count; ++n) {
-        const int64_t chunk = end - 1 - n, t0 = chunk * C;
-        const int rows = (int)min((int64_t)C, a.steps - t0);
+        const int64_t chunk = chunk_of(n), t0 = chunk * C;
+        const int rows = rows_of(n);
+        const LaLevels<C> &levels = both_levels[n & 1];
         uint32_t magnitude = 0;
-        nq.store(qs, magnitude);
-        nk.store(ks, magnitude);
-        nv.store(vs, magnitude);
-        ng.store(gs, magnitude);
+        auto store_all = [&](auto even_type) {
+            constexpr bool EVEN = decltype(even_type)::value;
+            nq.template store<EVEN>(qs, rows, magnitude);
+            nk.template store<EVEN>(ks, rows, magnitude);
+            nv.template store<EVEN>(vs, rows, magnitude);
+            ng.template store<EVEN>(gs, nothing ? 0 : rows, magnitude);
+        };
+        if (__builtin_expect(even, 1)) store_all(std::true_type());
+        else store_all(std::false_type());
         if (la_not_finite<T>(magnitude)) bad_chunk[n & 1] = 1;
 #pragma unroll
-        for (int t = 0; t < DT; ++t) {
-            F f[S::HELD];
+        for (int t = 0; t < OD; ++t) {
+            F f[EP];
             la_split(e[t], f);
 #pragma unroll
-            for (int m = 0; m < S::HELD; ++m) *reinterpret_cast<F *>(es + (m * D + col) * LD + 16 * t + 4 * g) = f[m];
+            for (int m = 0; m < EP; ++m) *reinterpret_cast<F *>(es + (m * D + col) * LD + value0 + 16 * t) = f[m];
         }
-        if (wave == 0) la_levels<C>(levels, nd.log_decay, nd.reset);
         __syncthreads();
         const bool bad = bad_chunk[n & 1] != 0;
         if (threadIdx.x == 0) bad_chunk[(n + 1) & 1] = 0;
-        fetch_square(a.kept + (bh * a.chunks + chunk) * features * values, before);
-        if (n + 1 < count) fetch(n + 1);
-
-        for (int p = wave; p < S::PAIRS; p += W) {
-            int ti, tj;
-            la_pair<TT>(p, ti, tj);
-            LaAcc c = {}, d = {}, gg = {};
-            if (tj <= ti) {
+        // the state in front of the chunk (what lies outside of it: some address inside, zero when it is used)
+        LaAcc before[DT];
+        {
+            const float *from = a.kept + (bh * a.chunks + chunk) * features * line + (col < features ? col * line : 0);
 #pragma unroll
-                for (int x = 0; x < D; x += 32) {
-                    c = la_mma(la_rows<F>(qs, LD, 16 * ti, x), la_rows<F>(qs, LD, 16 * ti, x + 16), la_rows<F>(ks, LD, 16 * tj, x),
-                               la_rows<F>(ks, LD, 16 * tj, x + 16), c);
-                    d = la_mma(la_rows<F>(gs, LD, 16 * ti, x), la_rows<F>(gs, LD, 16 * ti, x + 16), la_rows<F>(vs, LD, 16 * tj, x),
-                               la_rows<F>(vs, LD, 16 * tj, x + 16), d);
-                }
+            for (int t = 0; t < DT; ++t) before[t] = *reinterpret_cast<const LaAcc *>(from + (16 * t + 4 * g < line ? 16 * t + 4 * g : 0));
+        }
+        fetch(min(n + 1, count - 1));
+        if (n > 0 && wave == W - 2) decays(n - 1);
+
+        // dV, rows are steps j, columns this wavefront's values: w K E
+        LaAcc dv[OT] = {};
+#pragma unroll
+        for (int x = 0; x < D; x += 32) {
+            F e0[S::INNER], e1[S::INNER];
+#pragma unroll
+            for (int m = 0; m < S::INNER; ++m) {
+                e0[m] = la_cols(es + m * D * LD, LD, x, 16 * slice);
+                e1[m] = la_cols(es + m * D * LD, LD, x + 16, 16 * slice);
             }
-            const int j = 16 * tj + i16;
+#pragma unroll
+            for (int u = 0; u < OT; ++u) {
+                const int t = S::tile(half, u);
+                const F k0 = la_rows<F>(ks, LD, 16 * t, x), k1 = la_rows<F>(ks, LD, 16 * t, x + 16);
+#pragma unroll
+                for (int m = 0; m < S::INNER; ++m) dv[u] = la_mma(k0, k1, e0[m], e1[m], dv[u]);
+            }
+        }
+        // the inner factors and G
+        constexpr int EACH = S::EACH;
+        LaAcc cs[EACH], dds[EACH], gg[EACH];
+        int tis[EACH], tjs[EACH];
+#pragma unroll
+        for (int u = 0; u < EACH; ++u) {
+            const int p = wave + u * W;
+            if (S::PAIRS % W != 0 && p >= S::PAIRS) break;
+            int ti, tj;
+            la_pair(p, ti, tj);
+            LaAcc c = {}, d = {};
+#pragma unroll
+            for (int x = 0; x < D; x += 32) {
+                c = la_mma(la_rows<F>(qs, LD, 16 * ti, x), la_rows<F>(qs, LD, 16 * ti, x + 16), la_rows<F>(ks, LD, 16 * tj, x),
+                           la_rows<F>(ks, LD, 16 * tj, x + 16), c);
+                d = la_mma(la_rows<F>(gs, LD, 16 * ti, x), la_rows<F>(gs, LD, 16 * ti, x + 16), la_rows<F>(vs, LD, 16 * tj, x),
+                           la_rows<F>(vs, LD, 16 * tj, x + 16), d);
+            }
+            const int j = 16 * tj + i16, i = 16 * ti + 4 * g, part = levels.part[j];
+            const LaAcc f_ij = levels.between(levels.quad(levels.hi, i), levels.quad(levels.lo, i), levels.hi[j], levels.lo[j], 1.0f);
+            const LaParts parts = *reinterpret_cast<const LaParts *>(levels.part + i);
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const int i = 16 * ti + 4 * g + r;
-                const bool there = j <= i && levels.part[j] == levels.part[i];
-                const float f = a.scale * levels.between(i, j);
-                c[r] = there ? c[r] * f : 0.0f;
-                gg[r] = there && j < i ? c[r] * d[r] : 0.0f;
-                d[r] = there ? d[r] * f : 0.0f;
+                const bool there = (j <= i + r) & (parts[r] == part);
+                const float f = a.scale * f_ij[r], x = c[r] * f, y = d[r] * f, z = x * d[r];
+                c[r] = there ? x : 0.0f;
+                gg[u][r] = there & (j < i + r) ? z : 0.0f;
+                d[r] = there ? y : 0.0f;
             }
+            cs[u] = c;
+            dds[u] = d;
+            tis[u] = ti;
+            tjs[u] = tj;
+        }
+        if constexpr (!SHARED) __syncthreads();
+#pragma unroll
+        for (int u = 0; u < EACH; ++u) {
+            if (S::PAIRS % W != 0 && wave + u * W >= S::PAIRS) break;
+            const int ti = tis[u], tj = tjs[u], j = 16 * tj + i16, i = 16 * ti + 4 * g;
             F f[S::INNER];
-            la_split(c, f);
+            la_split(cs[u], f);
 #pragma unroll
-            for (int m = 0; m < S::INNER; ++m) *reinterpret_cast<F *>(ps + (m * C + j) * LDC + 16 * ti + 4 * g) = f[m];
-            la_split(d, f);
+            for (int m = 0; m < S::INNER; ++m) *reinterpret_cast<F *>(ps + (m * C + j) * LDC + i) = f[m];
+            la_split(dds[u], f);
 #pragma unroll
-            for (int m = 0; m < S::INNER; ++m) *reinterpret_cast<F *>(ds + (m * C + j) * LDC + 16 * ti + 4 * g) = f[m];
-            float column = (gg[0] + gg[1]) + (gg[2] + gg[3]);
+            for (int m = 0; m < S::INNER; ++m) *reinterpret_cast<F *>(ds + (m * C + j) * LDC + i) = f[m];
+            float column = (gg[u][0] + gg[u][1]) + (gg[u][2] + gg[u][3]);
             column += __shfl_xor(column, 16, 64);
             column += __shfl_xor(column, 32, 64);
-            if (g == 0) col_sums[ti][j] = column;
+            sums.col[ti][j] = column;   // (the same from four lanes)
+            LaAcc row;
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const float sum = la_sum16(gg[r]);
-                if (i16 == 0) row_sums[tj][16 * ti + 4 * g + r] = sum;
-            }
+            for (int r = 0; r < 4; ++r) row[r] = la_sum16(gg[u][r]);
+            *reinterpret_cast<LaAcc *>(&sums.row[tj][i]) = row;   // (from sixteen)
         }
+        if (wave == W - 1 && n + 1 < count) nd.levels(both_levels[(n + 1) & 1], a.scale);
+        nd.fetch(chunk_of(min(n + 2, count - 1)) * C, rows_of(min(n + 2, count - 1)));
         __syncthreads();
 
-        const int part = levels.part[C - 1];
-        const float decay = levels.from_start(C - 1);
-        auto to_end = [&](int j, float x) { return levels.part[j] == part ? x * levels.between(C - 1, j) : 0.0f; };
-        auto to_start = [&](int i, float x) { return levels.part[i] == 0 ? x * (a.scale * levels.from_start(i)) : 0.0f; };
-        auto meets = [&](int i, int j) { return j <= i && levels.part[j] == levels.part[i]; };
-        const int64_t row0 = (b * a.steps + t0) * a.heads + h, row_step = a.heads;
-
-        // dV: rows are steps j, columns this wavefront's values
-        {
-            LaAcc c[TT] = {};
+        const float decay = levels.decay;
+        const int64_t row0 = (b * a.steps + t0) * a.heads + h;
+        auto products = [&](auto bad_type) {
+            constexpr bool BAD = decltype(bad_type)::value;
+            auto meets = [&](int i, int j) { return j <= i && levels.part[j] == levels.part[i]; };
 #pragma unroll
-            for (int x = 0; x < D; x += 32)
-#pragma unroll
-                for (int m = 0; m < S::HELD; ++m) {
-                    const F e0 = la_cols(es + m * D * LD, LD, x, 16 * wave), e1 = la_cols(es + m * D * LD, LD, x + 16, 16 * wave);
-#pragma unroll
-                    for (int t = 0; t < TT; ++t) c[t] = la_mma(la_rows<F>(ks, LD, 16 * t, x), la_rows<F>(ks, LD, 16 * t, x + 16), e0, e1, c[t]);
-                }
-            T *out = static_cast<T *>(a.d_v) + row0 * values + col;
-#pragma unroll
-            for (int t = 0; t < TT; ++t) {
-#pragma unroll
-                for (int r = 0; r < 4; ++r) c[t][r] = to_end(16 * t + 4 * g + r, c[t][r]);
-                la_over_steps<S::INNER, TT, F>(
-                    c[t], t, TT - 1, bad, [&](int m, int i) { return la_rows<F>(ps + m * C * LDC, LDC, 16 * t, 16 * i); },
-                    [&](int i) { return la_cols(gs, LD, 16 * i, 16 * wave); },
+            for (int u = 0; u < OT; ++u) {
+                const int t = S::tile(half, u);
+                dv[u] = la_times(dv[u], levels.quad(levels.end, 16 * t + 4 * g));
+                la_over_steps<BAD, S::INNER, TT, F>(
+                    dv[u], S::pair_of(u), TT / 2 - 1, [&](int m, int i) { return la_rows<F>(ps + m * C * LDC, LDC, 16 * t, 16 * i); },
+                    [&](int i) { return la_cols(gs, LD, 16 * i, 16 * slice); },
                     [&](int r, int i) { return meets(i, 16 * t + 4 * g + r); });
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int j = 16 * t + 4 * g + r;
-                    if (j < rows && col < values) out[j * row_step * values] = (T)c[t][r];
-                }
             }
-        }
-        F qf[TT];
+            {
+                LaOut to;
+                to.init(static_cast<T *>(a.d_v) + row0 * values, rows, a.heads * values, col, values);
 #pragma unroll
-        for (int t = 0; t < TT; ++t) qf[t] = la_cols(qs, LD, 16 * t, 16 * wave);
-        auto store = [&](void *to, int step, float x) {
-            if (step >= rows || col >= features) return;
-            const int64_t at = (row0 + step * row_step) * features + col;
-            if (a.wide) static_cast<float *>(to)[at] = x;
-            else static_cast<T *>(to)[at] = (T)x;
-        };
-        // dK: rows are steps j, columns this wavefront's features
-        {
-            F kf[TT];
+                for (int u = 0; u < OT; ++u) to.store(S::tile(half, u), dv[u], T());
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            // dQ, rows are steps i, columns this wavefront's features: b dO S^T
+            LaAcc d[OT] = {};
 #pragma unroll
-            for (int t = 0; t < TT; ++t) kf[t] = la_cols(ks, LD, 16 * t, 16 * wave);
-            LaAcc c[TT] = {}, d[TT] = {};
+            for (int x = 0; x < DT; ++x) {
+                const bool there = (col < features) & (16 * x + 4 * g < line);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) before[x][r] = there ? before[x][r] : 0.0f;
+            }
 #pragma unroll
             for (int x = 0; x < DT; x += 2) {
-                F e0[S::INNER], e1[S::INNER], s0[S::INNER], s1[S::INNER];
-                la_split(e[x], e0);
-                la_split(e[x + 1], e1);
+                F s0[S::ADDED], s1[S::ADDED];
                 la_split(before[x], s0);
                 la_split(before[x + 1], s1);
 #pragma unroll
-                for (int t = 0; t < TT; ++t) {
-                    const F v0 = la_rows<F>(vs, LD, 16 * t, 16 * x), v1 = la_rows<F>(vs, LD, 16 * t, 16 * x + 16);
+                for (int u = 0; u < OT; ++u) {
+                    const int t = S::tile(half, u);
                     const F g0 = la_rows<F>(gs, LD, 16 * t, 16 * x), g1 = la_rows<F>(gs, LD, 16 * t, 16 * x + 16);
 #pragma unroll
-                    for (int m = 0; m < S::INNER; ++m) {
-                        c[t] = la_mma(v0, v1, e0[m], e1[m], c[t]);
-                        d[t] = la_mma(g0, g1, s0[m], s1[m], d[t]);
-                    }
+                    for (int m = 0; m < S::ADDED; ++m) d[u] = la_mma(g0, g1, s0[m], s1[m], d[u]);
                 }
             }
+            F qf[TT], kf[TT];
 #pragma unroll
             for (int t = 0; t < TT; ++t) {
-                const LaAcc kx = la_float(kf[t]), qx = la_float(qf[t]);
+                qf[t] = la_cols(qs, LD, 16 * t, 16 * slice);
+                kf[t] = la_cols(ks, LD, 16 * t, 16 * slice);
+            }
+            // <E, S>
+            float sum = 0.0f;
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int j = 16 * t + 4 * g + r;
-                    c[t][r] = to_end(j, c[t][r]);
-                    d[t][r] = to_start(j, d[t][r]);
-                    const float at_end = la_sum16(levels.part[j] == part ? c[t][r] * kx[r] : 0.0f);
-                    const float at_start = la_sum16(levels.part[j] == 0 ? d[t][r] * qx[r] : 0.0f);
-                    if (i16 == 0) end_sums[wave][j] = at_end;
-                    if (i16 == 1) start_sums[wave][j] = at_start;
-                }
-                la_over_steps<S::INNER, TT, F>(
-                    c[t], t, TT - 1, bad, [&](int m, int i) { return la_rows<F>(ds + m * C * LDC, LDC, 16 * t, 16 * i); },
-                    [&](int i) { return la_cols(qs, LD, 16 * i, 16 * wave); },
-                    [&](int r, int i) { return meets(i, 16 * t + 4 * g + r); });
-                // dQ: rows are steps i
-                la_over_steps<S::INNER, TT, F>(
-                    d[t], 0, t, bad, [&](int m, int j) { return la_cols(ds + m * C * LDC, LDC, 16 * j, 16 * t); },
-                    [&](int j) { return la_cols(ks, LD, 16 * j, 16 * wave); },
+            for (int t = 0; t < OD; ++t)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) sum += e[t][r] * (S::HALVES == 1 || half == 0 ? before[t][r] : before[(DT - OD) + t][r]);
+            sum = la_sum16(sum);
+            sum += __shfl_xor(sum, 16, 64);
+            sum += __shfl_xor(sum, 32, 64);
+            sums.through[wave] = sum;
+            // (of the wavefront's tile u; the operands are those of all tiles)
+            auto mine = [&](const F (&f)[TT], int u) {
+                if constexpr (S::HALVES == 1) return la_float(f[u]);
+                else return la_float(u == 0 ? (half == 0 ? f[0] : f[1]) : (half == 0 ? f[3] : f[2]));
+            };
+#pragma unroll
+            for (int u = 0; u < OT; ++u) {
+                const int t = S::tile(half, u), i = 16 * t + 4 * g;
+                const LaAcc to_start = levels.quad(levels.start, i);
+                d[u] = la_times(d[u], to_start);
+                // (a step that a reset parts from the state: zero times what may not be finite)
+                LaAcc at_start = d[u] * mine(qf, u);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) at_start[r] = la_sum16(to_start[r] < 0.0f ? 0.0f : at_start[r]);
+                *reinterpret_cast<LaAcc *>(&sums.start[slice][i]) = at_start;
+                la_over_steps<BAD, S::INNER, TT, F>(
+                    d[u], 0, S::pair_of(u), [&](int m, int j) { return la_cols(ds + m * C * LDC, LDC, 16 * j, 16 * t); },
+                    [&](int j) { return BAD ? la_cols(ks, LD, 16 * j, 16 * slice) : kf[j]; },
                     [&](int r, int j) { return meets(16 * t + 4 * g + r, j); });
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    store(a.d_k, 16 * t + 4 * g + r, c[t][r]);
-                    store(a.d_q, 16 * t + 4 * g + r, d[t][r]);
-                }
             }
-        }
-        // <E, S>, and E in front of the chunk
-        float sum = 0.0f;
+            LaOut to;
+            if (a.wide) {
+                to.init(static_cast<float *>(a.d_q) + row0 * features, rows, a.heads * features, col, features);
 #pragma unroll
-        for (int t = 0; t < DT; ++t) {
+                for (int u = 0; u < OT; ++u) to.store(S::tile(half, u), d[u], 0.0f);
+            } else {
+                to.init(static_cast<T *>(a.d_q) + row0 * features, rows, a.heads * features, col, features);
 #pragma unroll
-            for (int r = 0; r < 4; ++r) sum += e[t][r] * before[t][r];
-            e[t] = part == 0 ? e[t] * decay : LaAcc{0.f, 0.f, 0.f, 0.f};
-        }
-        sum = la_sum16(sum);
-        sum += __shfl_xor(sum, 16, 64);
-        sum += __shfl_xor(sum, 32, 64);
-        if (lane == 0) through[wave] = sum;
-#pragma unroll
-        for (int t = 0; t < TT; t += 2) {
-            F w[2][S::ADDED];
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                LaAcc x = la_float(qf[t + u]);
-#pragma unroll
-                for (int r = 0; r < 4; ++r) x[r] = to_start(16 * (t + u) + 4 * g + r, x[r]);
-                la_split(x, w[u]);
+                for (int u = 0; u < OT; ++u) to.store(S::tile(half, u), d[u], T());
             }
+            __builtin_amdgcn_sched_barrier(0);
+            // dK, rows are steps j: w V E^T
+            LaAcc c[OT] = {};
 #pragma unroll
-            for (int x = 0; x < DT; ++x) {
-                F g0 = la_cols(gs, LD, 16 * t, 16 * x), g1 = la_cols(gs, LD, 16 * t + 16, 16 * x);
-                if (bad) {
+            for (int x = 0; x < DT; x += 2) {
+                F e0[S::ADDED], e1[S::ADDED];
+                if constexpr (SHARED) {
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        if (levels.part[16 * t + 4 * g + r] != 0) g0[r] = 0.0f;
-                        if (levels.part[16 * t + 16 + 4 * g + r] != 0) g1[r] = 0.0f;
+                    for (int m = 0; m < S::ADDED; ++m) {
+                        e0[m] = la_rows<F>(es + m * D * LD, LD, 16 * slice, 16 * x);
+                        e1[m] = la_rows<F>(es + m * D * LD, LD, 16 * slice, 16 * x + 16);
                     }
+                } else {
+                    la_split(e[x], e0);
+                    la_split(e[x + 1], e1);
                 }
 #pragma unroll
-                for (int m = 0; m < S::ADDED; ++m) e[x] = la_mma(g0, g1, w[0][m], w[1][m], e[x]);
-            }
-        }
-        __syncthreads();
-        if (wave == 0) {
-            // one step a lane: sums over the later steps of its document, sums over the earlier ones
-            const int t = min(lane, C - 1);
-            float later = 0.0f, earlier = 0.0f;
-            for (int x = 0; x <= ((t >> 4) | 1); ++x) later += row_sums[x][t];
-            for (int x = (t >> 4) & ~1; x < TT; ++x) later -= col_sums[x][t];
-            for (int x = 0; x < W; ++x) {
-                later += start_sums[x][t];
-                earlier += end_sums[x][t];
-            }
-            const int mine = levels.part[t];
-            float crossing = 0.0f;
-            if (part == 0)
-                for (int x = 0; x < W; ++x) crossing += decay * through[x];
+                for (int u = 0; u < OT; ++u) {
+                    const int t = S::tile(half, u);
+                    const F v0 = la_rows<F>(vs, LD, 16 * t, 16 * x), v1 = la_rows<F>(vs, LD, 16 * t, 16 * x + 16);
 #pragma unroll
-            for (int d = 1; d < C; d *= 2) {
-                const float down = __shfl_down(later, d, 64), up = __shfl_up(earlier, d, 64);
-                const int part_down = __shfl_down(mine, d, 64), part_up = __shfl_up(mine, d, 64);
-                if (lane + d < C && part_down == mine) later += down;
-                if (lane >= d && part_up == mine) earlier += up;
+                    for (int m = 0; m < S::ADDED; ++m) c[u] = la_mma(v0, v1, e0[m], e1[m], c[u]);
+                }
             }
-            float before_t = __shfl_up(earlier, 1, 64);
-            const int part_before = __shfl_up(mine, 1, 64);
-            if (lane == 0 || part_before != mine) before_t = 0.0f;
-            // (the decay of a reset step meets nothing)
-            const bool starts = mine != (lane == 0 ? 0 : part_before);
-            if (lane < rows) a.d_log_decay[row0 + lane * row_step] = starts ? 0.0f : later + before_t + crossing;
-        }
+#pragma unroll
+            for (int u = 0; u < OT; ++u) {
+                const int t = S::tile(half, u), j = 16 * t + 4 * g;
+                const LaAcc to_end = levels.quad(levels.end, j);
+                c[u] = la_times(c[u], to_end);
+                LaAcc at_end = c[u] * mine(kf, u);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) at_end[r] = la_sum16(to_end[r] < 0.0f ? 0.0f : at_end[r]);
+                *reinterpret_cast<LaAcc *>(&sums.end[slice][j]) = at_end;
+                la_over_steps<BAD, S::INNER, TT, F>(
+                    c[u], S::pair_of(u), TT / 2 - 1, [&](int m, int i) { return la_rows<F>(ds + m * C * LDC, LDC, 16 * t, 16 * i); },
+                    [&](int i) { return BAD ? la_cols(qs, LD, 16 * i, 16 * slice) : qf[i]; },
+                    [&](int r, int i) { return meets(i, 16 * t + 4 * g + r); });
+            }
+            if (a.wide) {
+                to.init(static_cast<float *>(a.d_k) + row0 * features, rows, a.heads * features, col, features);
+#pragma unroll
+                for (int u = 0; u < OT; ++u) to.store(S::tile(half, u), c[u], 0.0f);
+            } else {
+                to.init(static_cast<T *>(a.d_k) + row0 * features, rows, a.heads * features, col, features);
+#pragma unroll
+                for (int u = 0; u < OT; ++u) to.store(S::tile(half, u), c[u], T());
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            // E in front of the chunk
+#pragma unroll
+            for (int t = 0; t < OD; ++t) e[t] = la_times(e[t], decay);
+#pragma unroll
+            for (int t = 0; t < TT; t += 2) {
+                F w[2][S::ADDED];
+                LaAcc factor[2];
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    factor[u] = levels.quad(levels.start, 16 * (t + u) + 4 * g);
+                    la_split(la_times(la_float(qf[t + u]), factor[u]), w[u]);
+                }
+#pragma unroll
+                for (int x = 0; x < OD; ++x) {
+                    const int at = 16 * (half * OD + x);
+                    F g0 = la_cols(gs, LD, 16 * t, at), g1 = la_cols(gs, LD, 16 * t + 16, at);
+                    if constexpr (BAD) {
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            if (factor[0][r] < 0.0f) g0[r] = 0.0f;
+                            if (factor[1][r] < 0.0f) g1[r] = 0.0f;
+                        }
+                    }
+#pragma unroll
+                    for (int m = 0; m < S::ADDED; ++m) e[x] = la_mma(g0, g1, w[0][m], w[1][m], e[x]);
+                }
+            }
+        };
+        if (__builtin_expect(bad, 0)) products(std::true_type());
+        else products(std::false_type());
+        __syncthreads();
     }
+    if (wave == W - 2) decays(count - 1);
     if (segment == 0 && a.d_state) {
         float *to = a.d_state + bh * features * values;
 #pragma unroll
-        for (int t = 0; t < DT; ++t)
+        for (int t = 0; t < OD; ++t)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const int row = 16 * t + 4 * g + r;
-                if (col < features && row < values) to[(int64_t)col * values + row] = e[t][r];
+                const int row = value0 + 16 * t + r;
+                if (col < features && row < values) to[col * values + row] = e[t][r];
             }
     }
 }
