@@ -100,26 +100,35 @@ __device__ __forceinline__ LaAcc la_mma(LaAcc a0, LaAcc a1, LaAcc b0, LaAcc b1, 
     return c;
 }
 
+// The lane's number, of TIGHT kernels as something that the compiler knows nothing of: what is computed from it is computed where
+// it is needed.  (Left to itself it forms every address of a chunk in front of the loop and keeps them all, in scratch memory
+// where registers end.)
+template <bool TIGHT>
+__device__ __forceinline__ int la_lane()
+{
+    int lane = threadIdx.x & 63;
+    if constexpr (TIGHT) asm volatile("" : "+v"(lane));
+    return lane;
+}
+
 // Element s is [row0 + lane % 16][col0 + 4 g + s]: the sum runs over neighbours in memory.
 template <typename F, typename T>
-__device__ __forceinline__ F la_rows(const T *lds, int stride, int row0, int col0)
+__device__ __forceinline__ F la_rows(int lane, const T *lds, int stride, int row0, int col0)
 {
-    const int lane = threadIdx.x & 63;
     return *reinterpret_cast<const F *>(lds + (row0 + (lane & 15)) * stride + col0 + 4 * (lane >> 4));
 }
 // Element s is [row0 + 4 g + s][col0 + lane % 16]: the sum runs over rows.
-__device__ __forceinline__ LaHalf4 la_cols(const bf16 *lds, int stride, int row0, int col0)
+__device__ __forceinline__ LaHalf4 la_cols(int lane, const bf16 *lds, int stride, int row0, int col0)
 {
     typedef short Quad16 __attribute__((ext_vector_type(4)));
     typedef __attribute__((address_space(3))) Quad16 LdsQuad;
-    const int lane = threadIdx.x & 63, i = lane & 15;
+    const int i = lane & 15;
     // (16 lanes hand in 4 rows of 16 columns and get them by columns)
     const bf16 *p = lds + (row0 + 4 * (lane >> 4) + (i >> 2)) * stride + col0 + 4 * (i & 3);
     return __builtin_bit_cast(LaHalf4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsQuad *)p));
 }
-__device__ __forceinline__ LaAcc la_cols(const float *lds, int stride, int row0, int col0)
+__device__ __forceinline__ LaAcc la_cols(int lane, const float *lds, int stride, int row0, int col0)
 {
-    const int lane = threadIdx.x & 63;
     const float *p = lds + (row0 + 4 * (lane >> 4)) * stride + col0 + (lane & 15);
     return LaAcc{p[0], p[stride], p[2 * stride], p[3 * stride]};
 }
@@ -322,6 +331,17 @@ __device__ __forceinline__ void la_scan(V &sum, int part)
     la_scan_round<32>(sum, part);
 }
 
+template <typename V>
+__device__ __forceinline__ void la_scan(V &sum)
+{
+    sum += la_up<1>((V)0, sum);
+    sum += la_up<2>((V)0, sum);
+    sum += la_up<4>((V)0, sum);
+    sum += la_up<8>((V)0, sum);
+    sum += la_up<16>((V)0, sum);
+    sum += la_up<32>((V)0, sum);
+}
+
 // One step a lane.  A decay below 2^-160 is zero beside anything in 32 bits and counts as that.
 template <int C>
 __device__ __forceinline__ void la_levels(LaLevels<C> &out, float log_decay, bool reset, float scale)
@@ -331,7 +351,8 @@ __device__ __forceinline__ void la_levels(LaLevels<C> &out, float log_decay, boo
     double level = reset ? 0.0 : x < -160.0 ? -160.0 : x;
     const uint64_t resets = __ballot(reset), below = ((uint64_t)2 << lane) - 1;
     const int part = __popcll(resets & below), parts = __popcll(resets);
-    la_scan(level, part);
+    if (resets == 0) la_scan(level);
+    else la_scan(level, part);
     const float hi = (float)level, from_start = __builtin_amdgcn_exp2f(hi);
     const double last = __shfl(level, C - 1, 64);
     const float to_end = __builtin_amdgcn_exp2f((float)(last - level));
@@ -345,14 +366,14 @@ __device__ __forceinline__ void la_levels(LaLevels<C> &out, float log_decay, boo
     }
 }
 
-// A chunk's decays and resets, one step a lane, on their way in registers (by every wavefront: no branch).
+// A chunk's decays and resets, one step a lane, on their way in registers.
 template <int C>
 struct LaDecay {
     const float *log_decay;
     const uint8_t *reset;
     int64_t stride, reset_stride;
     float x;
-    uint8_t flag;
+    uint8_t flag = 0;
     bool inside, resets;
 
     __device__ __forceinline__ void init(const LaArgs &a, int64_t b, int h)
@@ -360,14 +381,14 @@ struct LaDecay {
         log_decay = a.log_decay + b * a.decay_stride[0] + h * a.decay_stride[2];
         stride = a.decay_stride[1];
         resets = a.reset != nullptr;
-        reset = resets ? a.reset + b * a.reset_stride[0] : reinterpret_cast<const uint8_t *>(log_decay);
-        reset_stride = resets ? a.reset_stride[1] : 0;
+        reset = resets ? a.reset + b * a.reset_stride[0] : nullptr;
+        reset_stride = a.reset_stride[1];
     }
     __device__ __forceinline__ void fetch(int64_t t0, int rows)
     {
         const int lane = threadIdx.x & 63, at = min(lane, rows - 1);
         x = log_decay[(t0 + at) * stride];
-        flag = reset[(t0 + at) * reset_stride];
+        if (resets) flag = reset[(t0 + at) * reset_stride];
         inside = lane < rows && lane < C;
     }
     __device__ __forceinline__ void levels(LaLevels<C> &out, float scale) const
@@ -425,34 +446,36 @@ __device__ __forceinline__ void la_over_steps(LaAcc &c, int first, int last, A &
 }
 
 // A chunk's rows of a dense result: 16-bit or 32-bit stores of a tile, whose range check drops rows behind the last step and
-// columns behind the last one, so that nothing branches.  (The whole offset is in the lane's register, where the check sees it.)
+// columns behind the last one, so that nothing branches.  Each tile has a descriptor of its own (scalars), for one descriptor the
+// lanes' offsets of all tiles would be kept in registers from chunk to chunk.  (What the check is to see is in the lane's
+// register.)
+template <typename T>
 struct LaOut {
-    __amdgpu_buffer_rsrc_t to;
-    unsigned at;
-    unsigned row_bytes;
+    T *row0;
+    int rows;
+    unsigned at, row_bytes;
 
-    template <typename T>
-    __device__ __forceinline__ void init(T *row0, int rows, int row_elements, int col, int cols)
+    __device__ __forceinline__ LaOut(T *to, int count, int row_elements, int g, int col, int cols)
     {
+        row0 = to;
+        rows = count;
         row_bytes = (unsigned)(row_elements * (int)sizeof(T));
-        to = __builtin_amdgcn_make_buffer_rsrc(row0, 0, (int)(rows * row_bytes), 0x00020000);
-        at = col < cols ? 4 * ((threadIdx.x & 63) >> 4) * row_bytes + col * (unsigned)sizeof(T) : 0x80000000u;
+        at = col < cols ? 4 * g * row_bytes + col * (unsigned)sizeof(T) : 0x80000000u;
     }
-    __device__ __forceinline__ void store(int tile, LaAcc x, float) const
+    __device__ __forceinline__ void store(int tile, LaAcc x) const
     {
+        char *base = reinterpret_cast<char *>(row0) + (int64_t)(16 * tile) * row_bytes;
+        const __amdgpu_buffer_rsrc_t to = __builtin_amdgcn_make_buffer_rsrc(base, 0, max(rows - 16 * tile, 0) * (int)row_bytes, 0x00020000);
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             const float y = x[r];
-            __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, y), to, (int)(at + (16 * tile + r) * row_bytes), 0, 0);
-        }
-    }
-    __device__ __forceinline__ void store(int tile, LaAcc x, bf16) const
-    {
-        const LaHalf4 half = __builtin_convertvector(x, LaHalf4);
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const bf16 y = half[r];
-            __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(unsigned short, y), to, (int)(at + (16 * tile + r) * row_bytes), 0, 0);
+            const int offset = (int)(at + r * row_bytes);
+            if constexpr (sizeof(T) == 4) {
+                __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, y), to, offset, 0, 0);
+            } else {
+                const bf16 z = (bf16)y;
+                __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(unsigned short, z), to, offset, 0, 0);
+            }
         }
     }
 };
@@ -540,14 +563,19 @@ __global__ __launch_bounds__((LaShape<T, D>::THREADS)) void la_walk_kernel(const
         }
     };
     if (threadIdx.x < 2) bad_chunk[threadIdx.x] = 0;
-    nd.fetch(chunk_of(0) * C, rows_of(0));
+    // The decays are fetched two chunks ahead, in front of the next chunk's rows: once those have arrived, they have, too.
+    auto fetch_decays = [&](int n) { nd.fetch(chunk_of(min(n, count - 1)) * C, rows_of(min(n, count - 1))); };
+    if (wave == W - 1) {
+        fetch_decays(0);
+        nd.levels(both_levels[0], a.scale);
+        fetch_decays(1);
+    }
     fetch(0);
-    if (wave == W - 1) nd.levels(both_levels[0], a.scale);
-    nd.fetch(chunk_of(min(1, count - 1)) * C, rows_of(min(1, count - 1)));
     __syncthreads();
     double total = 0.0;
     int cuts = 0;
     for (int n = 0; n < count; ++n) {
+        const int lane = la_lane<(D > 64)>(), i16 = lane & 15, g = lane >> 4, col = 16 * slice + i16;
         const int64_t chunk = chunk_of(n), t0 = chunk * C;
         const int rows = rows_of(n);
         const LaLevels<C> &levels = both_levels[n & 1];
@@ -566,17 +594,19 @@ __global__ __launch_bounds__((LaShape<T, D>::THREADS)) void la_walk_kernel(const
                 F f[S::INNER];
                 la_split(s[t], f);
 #pragma unroll
-                for (int m = 0; m < S::INNER; ++m) *reinterpret_cast<F *>(ss + (m * D + col) * LD + row0 + 16 * t) = f[m];
+                for (int m = 0; m < S::INNER; ++m) *reinterpret_cast<F *>(ss + (m * D + col) * LD + 16 * half * OD + 4 * g + 16 * t) = f[m];
             }
         }
         if (la_not_finite<T>(magnitude)) bad_chunk[n & 1] = 1;
         __syncthreads();
         const bool bad = bad_chunk[n & 1] != 0;
         if (threadIdx.x == 0) bad_chunk[(n + 1) & 1] = 0;
+        if (wave == W - 1) {
+            if (n + 1 < count) nd.levels(both_levels[(n + 1) & 1], a.scale);
+            fetch_decays(n + 2);
+        }
         // (behind the last chunk: that one once more)
         fetch(min(n + 1, count - 1));
-        if (wave == W - 1 && n + 1 < count) nd.levels(both_levels[(n + 1) & 1], a.scale);
-        nd.fetch(chunk_of(min(n + 2, count - 1)) * C, rows_of(min(n + 2, count - 1)));
 
         auto products = [&](auto bad_type) {
             constexpr bool BAD = decltype(bad_type)::value;
@@ -591,8 +621,8 @@ __global__ __launch_bounds__((LaShape<T, D>::THREADS)) void la_walk_kernel(const
                     LaAcc c = {};
 #pragma unroll
                     for (int x = 0; x < D; x += 32)
-                        c = la_mma(la_rows<F>(ks, LD, 16 * tj, x), la_rows<F>(ks, LD, 16 * tj, x + 16), la_rows<F>(qs, LD, 16 * ti, x),
-                                   la_rows<F>(qs, LD, 16 * ti, x + 16), c);
+                        c = la_mma(la_rows<F>(lane, ks, LD, 16 * tj, x), la_rows<F>(lane, ks, LD, 16 * tj, x + 16), la_rows<F>(lane, qs, LD, 16 * ti, x),
+                                   la_rows<F>(lane, qs, LD, 16 * ti, x + 16), c);
                     const int i = 16 * ti + i16, j = 16 * tj + 4 * g, part = levels.part[i];
                     const LaAcc f_ij = levels.between(levels.quad(levels.hi, j), levels.quad(levels.lo, j), levels.hi[i], levels.lo[i], -1.0f);
                     const LaParts parts = *reinterpret_cast<const LaParts *>(levels.part + j);
@@ -609,13 +639,12 @@ __global__ __launch_bounds__((LaShape<T, D>::THREADS)) void la_walk_kernel(const
             }
             F vf[TT];
 #pragma unroll
-            for (int t = 0; t < TT; ++t) vf[t] = la_cols(vs, LD, 16 * t, 16 * slice);
+            for (int t = 0; t < TT; ++t) vf[t] = la_cols(lane, vs, LD, 16 * t, 16 * slice);
             if constexpr (OUT) {
                 if (a.kept) {
-                    LaOut to;
-                    to.init(a.kept + (bh * a.chunks + chunk) * features * la_line(values), features, la_line(values), col, la_line(values));
+                    const LaOut<float> to(a.kept + (bh * a.chunks + chunk) * features * la_line(values), features, la_line(values), g, col, la_line(values));
 #pragma unroll
-                    for (int t = 0; t < OD; ++t) to.store(half * OD + t, s[t], 0.0f);
+                    for (int t = 0; t < OD; ++t) to.store(half * OD + t, s[t]);
                 }
                 LaAcc o[OT] = {};
 #pragma unroll
@@ -624,8 +653,8 @@ __global__ __launch_bounds__((LaShape<T, D>::THREADS)) void la_walk_kernel(const
                     if constexpr (SHARED) {
 #pragma unroll
                         for (int m = 0; m < S::INNER; ++m) {
-                            s0[m] = la_rows<F>(ss + m * D * LD, LD, 16 * slice, 16 * x);
-                            s1[m] = la_rows<F>(ss + m * D * LD, LD, 16 * slice, 16 * x + 16);
+                            s0[m] = la_rows<F>(lane, ss + m * D * LD, LD, 16 * slice, 16 * x);
+                            s1[m] = la_rows<F>(lane, ss + m * D * LD, LD, 16 * slice, 16 * x + 16);
                         }
                     } else {
                         la_split(s[x], s0);
@@ -634,25 +663,24 @@ __global__ __launch_bounds__((LaShape<T, D>::THREADS)) void la_walk_kernel(const
 #pragma unroll
                     for (int u = 0; u < OT; ++u) {
                         const int t = S::tile(half, u);
-                        const F q0 = la_rows<F>(qs, LD, 16 * t, 16 * x), q1 = la_rows<F>(qs, LD, 16 * t, 16 * x + 16);
+                        const F q0 = la_rows<F>(lane, qs, LD, 16 * t, 16 * x), q1 = la_rows<F>(lane, qs, LD, 16 * t, 16 * x + 16);
 #pragma unroll
                         for (int m = 0; m < S::INNER; ++m) o[u] = la_mma(q0, q1, s0[m], s1[m], o[u]);
                     }
                 }
                 __syncthreads();
-                LaOut to;
-                to.init(static_cast<T *>(a.o) + ((b * a.steps + t0) * a.heads + h) * values, rows, a.heads * values, col, values);
+                const LaOut<T> to(static_cast<T *>(a.o) + ((b * a.steps + t0) * a.heads + h) * values, rows, a.heads * values, g, col, values);
 #pragma unroll
                 for (int u = 0; u < OT; ++u) {
                     const int t = S::tile(half, u);
                     o[u] = la_times(o[u], levels.quad(levels.start, 16 * t + 4 * g));
                     la_over_steps<BAD, S::INNER, TT, F>(
-                        o[u], 0, S::pair_of(u), [&](int m, int j) { return la_rows<F>(ps + m * C * LDC, LDC, 16 * t, 16 * j); },
-                        [&](int j) { return BAD ? la_cols(vs, LD, 16 * j, 16 * slice) : vf[j]; },
+                        o[u], 0, S::pair_of(u), [&](int m, int j) { return la_rows<F>(lane, ps + m * C * LDC, LDC, 16 * t, 16 * j); },
+                        [&](int j) { return BAD ? la_cols(lane, vs, LD, 16 * j, 16 * slice) : vf[j]; },
                         [&](int r, int j) { const int i = 16 * t + 4 * g + r; return j <= i && levels.part[j] == levels.part[i]; });
                 }
 #pragma unroll
-                for (int u = 0; u < OT; ++u) to.store(S::tile(half, u), o[u], T());
+                for (int u = 0; u < OT; ++u) to.store(S::tile(half, u), o[u]);
             }
             // the state behind the chunk (BACK: its gradient in front of it)
             const float decay = levels.decay;
@@ -670,7 +698,7 @@ __global__ __launch_bounds__((LaShape<T, D>::THREADS)) void la_walk_kernel(const
 #pragma unroll
                 for (int x = 0; x < OD; ++x) {
                     const int at = 16 * (half * OD + x);
-                    F k0 = la_cols(ks, LD, 16 * t, at), k1 = la_cols(ks, LD, 16 * t + 16, at);
+                    F k0 = la_cols(lane, ks, LD, 16 * t, at), k1 = la_cols(lane, ks, LD, 16 * t + 16, at);
                     if constexpr (BAD) {
 #pragma unroll
                         for (int r = 0; r < 4; ++r) {
@@ -751,7 +779,7 @@ __global__ __launch_bounds__((LaShape<T, D>::THREADS)) void la_back_kernel(const
     // E, rows are features; (Q K^T . D)^T and (dO V^T . D)^T, rows are steps j, in its place where it is not needed any more
     __shared__ __align__(16) T room[SHARED ? HELD + FACTORS : HELD > FACTORS ? HELD : FACTORS];
     T *const es = room, *const ps = room + (SHARED ? HELD : 0), *const ds = ps + S::INNER * C * LDC;
-    __shared__ __align__(16) LaLevels<C> both_levels[2];
+    __shared__ __align__(16) LaLevels<C> three_levels[3];   // of the chunk, the next one, and the last one's for its decays' gradients
     struct Sums {
         float row[TT][C], col[TT][C], start[S::SLICES][C], end[S::SLICES][C], through[W];
     };
@@ -780,6 +808,8 @@ __global__ __launch_bounds__((LaShape<T, D>::THREADS)) void la_back_kernel(const
             e[t][r] = behind && col < features && row < values ? behind[col * values + row] : 0.0f;
         }
 
+    // (nothing is moved ahead of it: with 128 columns the operands of later products would push others out of the registers)
+    auto hold = [] { if constexpr (D > 64) __builtin_amdgcn_sched_barrier(0); };
     const bool nothing = !a.grad;   // (no gradient of o: zeros, whatever is read)
     LaPiece<T, D> nq, nk, nv, ng;
     nq.init(static_cast<const T *>(a.q) + la_offset(a.q_stride, b, 0, h / a.shared), a.q_stride[1], features);
@@ -811,7 +841,7 @@ __global__ __launch_bounds__((LaShape<T, D>::THREADS)) void la_back_kernel(const
 
     // The decays' gradients of a chunk, one step a lane: sums over the later steps of its document, sums over the earlier ones.
     auto decays = [&](int n) {
-        const LaLevels<C> &levels = both_levels[n & 1];
+        const LaLevels<C> &levels = three_levels[n % 3];
         const int mine = levels.part[min(lane, C - 1)], parts = levels.part[C - 1], part_before = __shfl_up(mine, 1, 64);
         // later steps: lanes reversed, so that they are the earlier ones
         const int t = C - 1 - min(lane, C - 1), reversed = parts - levels.part[t];
@@ -843,15 +873,21 @@ __global__ __launch_bounds__((LaShape<T, D>::THREADS)) void la_back_kernel(const
     };
 
     if (threadIdx.x < 2) bad_chunk[threadIdx.x] = 0;
-    nd.fetch(chunk_of(0) * C, rows_of(0));
+    // The decays are fetched two chunks ahead, in front of the next chunk's rows: once those have arrived, they have, too.
+    auto fetch_decays = [&](int n) { nd.fetch(chunk_of(min(n, count - 1)) * C, rows_of(min(n, count - 1))); };
+    if (wave == W - 1) {
+        fetch_decays(0);
+        nd.levels(three_levels[0], a.scale);
+        fetch_decays(1);
+    }
     fetch(0);
-    if (wave == W - 1) nd.levels(both_levels[0], a.scale);
-    nd.fetch(chunk_of(min(1, count - 1)) * C, rows_of(min(1, count - 1)));
     __syncthreads();
     for (int n = 0; n < count; ++n) {
+        const int lane = la_lane<(D > 64)>(), i16 = lane & 15, g = lane >> 4, col = 16 * slice + i16;
         const int64_t chunk = chunk_of(n), t0 = chunk * C;
         const int rows = rows_of(n);
-        const LaLevels<C> &levels = both_levels[n & 1];
+        const LaLevels<C> &levels = three_levels[n % 3];
+        LaLevels<C> &next_levels = three_levels[(n + 1) % 3];
         uint32_t magnitude = 0;
         auto store_all = [&](auto even_type) {
             constexpr bool EVEN = decltype(even_type)::value;
@@ -868,19 +904,29 @@ __global__ __launch_bounds__((LaShape<T, D>::THREADS)) void la_back_kernel(const
             F f[EP];
             la_split(e[t], f);
 #pragma unroll
-            for (int m = 0; m < EP; ++m) *reinterpret_cast<F *>(es + (m * D + col) * LD + value0 + 16 * t) = f[m];
+            for (int m = 0; m < EP; ++m) *reinterpret_cast<F *>(es + (m * D + col) * LD + 16 * half * OD + 4 * g + 16 * t) = f[m];
         }
         __syncthreads();
         const bool bad = bad_chunk[n & 1] != 0;
         if (threadIdx.x == 0) bad_chunk[(n + 1) & 1] = 0;
         // the state in front of the chunk (what lies outside of it: some address inside, zero when it is used)
-        LaAcc before[DT];
-        {
+        LaAcc before[DT] = {};
+        auto fetch_state = [&] {
             const float *from = a.kept + (bh * a.chunks + chunk) * features * line + (col < features ? col * line : 0);
 #pragma unroll
             for (int t = 0; t < DT; ++t) before[t] = *reinterpret_cast<const LaAcc *>(from + (16 * t + 4 * g < line ? 16 * t + 4 * g : 0));
+        };
+        // (behind the last chunk: that one once more)
+        auto fetch_next = [&] {
+            if (wave == W - 1) fetch_decays(n + 2);
+            fetch(min(n + 1, count - 1));
+        };
+        if (wave == W - 1 && n + 1 < count) nd.levels(next_levels, a.scale);
+        // (128 columns leave no registers for what is not needed yet)
+        if constexpr (SHARED) {
+            fetch_state();
+            fetch_next();
         }
-        fetch(min(n + 1, count - 1));
         if (n > 0 && wave == W - 2) decays(n - 1);
 
         // dV, rows are steps j, columns this wavefront's values: w K E
@@ -890,21 +936,21 @@ __global__ __launch_bounds__((LaShape<T, D>::THREADS)) void la_back_kernel(const
             F e0[S::INNER], e1[S::INNER];
 #pragma unroll
             for (int m = 0; m < S::INNER; ++m) {
-                e0[m] = la_cols(es + m * D * LD, LD, x, 16 * slice);
-                e1[m] = la_cols(es + m * D * LD, LD, x + 16, 16 * slice);
+                e0[m] = la_cols(lane, es + m * D * LD, LD, x, 16 * slice);
+                e1[m] = la_cols(lane, es + m * D * LD, LD, x + 16, 16 * slice);
             }
 #pragma unroll
             for (int u = 0; u < OT; ++u) {
                 const int t = S::tile(half, u);
-                const F k0 = la_rows<F>(ks, LD, 16 * t, x), k1 = la_rows<F>(ks, LD, 16 * t, x + 16);
+                const F k0 = la_rows<F>(lane, ks, LD, 16 * t, x), k1 = la_rows<F>(lane, ks, LD, 16 * t, x + 16);
 #pragma unroll
                 for (int m = 0; m < S::INNER; ++m) dv[u] = la_mma(k0, k1, e0[m], e1[m], dv[u]);
             }
+            hold();
         }
         // the inner factors and G
         constexpr int EACH = S::EACH;
-        LaAcc cs[EACH], dds[EACH], gg[EACH];
-        int tis[EACH], tjs[EACH];
+        LaAcc cs[EACH] = {}, dds[EACH] = {}, gg[EACH] = {};
 #pragma unroll
         for (int u = 0; u < EACH; ++u) {
             const int p = wave + u * W;
@@ -914,10 +960,11 @@ __global__ __launch_bounds__((LaShape<T, D>::THREADS)) void la_back_kernel(const
             LaAcc c = {}, d = {};
 #pragma unroll
             for (int x = 0; x < D; x += 32) {
-                c = la_mma(la_rows<F>(qs, LD, 16 * ti, x), la_rows<F>(qs, LD, 16 * ti, x + 16), la_rows<F>(ks, LD, 16 * tj, x),
-                           la_rows<F>(ks, LD, 16 * tj, x + 16), c);
-                d = la_mma(la_rows<F>(gs, LD, 16 * ti, x), la_rows<F>(gs, LD, 16 * ti, x + 16), la_rows<F>(vs, LD, 16 * tj, x),
-                           la_rows<F>(vs, LD, 16 * tj, x + 16), d);
+                c = la_mma(la_rows<F>(lane, qs, LD, 16 * ti, x), la_rows<F>(lane, qs, LD, 16 * ti, x + 16), la_rows<F>(lane, ks, LD, 16 * tj, x),
+                           la_rows<F>(lane, ks, LD, 16 * tj, x + 16), c);
+                d = la_mma(la_rows<F>(lane, gs, LD, 16 * ti, x), la_rows<F>(lane, gs, LD, 16 * ti, x + 16), la_rows<F>(lane, vs, LD, 16 * tj, x),
+                           la_rows<F>(lane, vs, LD, 16 * tj, x + 16), d);
+                hold();
             }
             const int j = 16 * tj + i16, i = 16 * ti + 4 * g, part = levels.part[j];
             const LaAcc f_ij = levels.between(levels.quad(levels.hi, i), levels.quad(levels.lo, i), levels.hi[j], levels.lo[j], 1.0f);
@@ -930,16 +977,17 @@ __global__ __launch_bounds__((LaShape<T, D>::THREADS)) void la_back_kernel(const
                 gg[u][r] = there & (j < i + r) ? z : 0.0f;
                 d[r] = there ? y : 0.0f;
             }
+            hold();
             cs[u] = c;
             dds[u] = d;
-            tis[u] = ti;
-            tjs[u] = tj;
         }
         if constexpr (!SHARED) __syncthreads();
 #pragma unroll
         for (int u = 0; u < EACH; ++u) {
             if (S::PAIRS % W != 0 && wave + u * W >= S::PAIRS) break;
-            const int ti = tis[u], tj = tjs[u], j = 16 * tj + i16, i = 16 * ti + 4 * g;
+            int ti, tj;
+            la_pair(wave + u * W, ti, tj);
+            const int j = 16 * tj + i16, i = 16 * ti + 4 * g;
             F f[S::INNER];
             la_split(cs[u], f);
 #pragma unroll
@@ -956,31 +1004,40 @@ __global__ __launch_bounds__((LaShape<T, D>::THREADS)) void la_back_kernel(const
             for (int r = 0; r < 4; ++r) row[r] = la_sum16(gg[u][r]);
             *reinterpret_cast<LaAcc *>(&sums.row[tj][i]) = row;   // (from sixteen)
         }
-        if (wave == W - 1 && n + 1 < count) nd.levels(both_levels[(n + 1) & 1], a.scale);
-        nd.fetch(chunk_of(min(n + 2, count - 1)) * C, rows_of(min(n + 2, count - 1)));
         __syncthreads();
+        if constexpr (!SHARED) fetch_state();
 
         const float decay = levels.decay;
         const int64_t row0 = (b * a.steps + t0) * a.heads + h;
         auto products = [&](auto bad_type) {
             constexpr bool BAD = decltype(bad_type)::value;
             auto meets = [&](int i, int j) { return j <= i && levels.part[j] == levels.part[i]; };
+            auto store = [&](void *rows_of_all, const LaAcc (&x)[OT]) {
+                if (a.wide) {
+                    const LaOut<float> to(static_cast<float *>(rows_of_all) + row0 * features, rows, a.heads * features, g, col, features);
+#pragma unroll
+                    for (int u = 0; u < OT; ++u) to.store(S::tile(half, u), x[u]);
+                } else {
+                    const LaOut<T> to(static_cast<T *>(rows_of_all) + row0 * features, rows, a.heads * features, g, col, features);
+#pragma unroll
+                    for (int u = 0; u < OT; ++u) to.store(S::tile(half, u), x[u]);
+                }
+            };
 #pragma unroll
             for (int u = 0; u < OT; ++u) {
                 const int t = S::tile(half, u);
                 dv[u] = la_times(dv[u], levels.quad(levels.end, 16 * t + 4 * g));
                 la_over_steps<BAD, S::INNER, TT, F>(
-                    dv[u], S::pair_of(u), TT / 2 - 1, [&](int m, int i) { return la_rows<F>(ps + m * C * LDC, LDC, 16 * t, 16 * i); },
-                    [&](int i) { return la_cols(gs, LD, 16 * i, 16 * slice); },
+                    dv[u], S::pair_of(u), TT / 2 - 1, [&](int m, int i) { return la_rows<F>(lane, ps + m * C * LDC, LDC, 16 * t, 16 * i); },
+                    [&](int i) { return la_cols(lane, gs, LD, 16 * i, 16 * slice); },
                     [&](int r, int i) { return meets(i, 16 * t + 4 * g + r); });
             }
             {
-                LaOut to;
-                to.init(static_cast<T *>(a.d_v) + row0 * values, rows, a.heads * values, col, values);
+                const LaOut<T> to(static_cast<T *>(a.d_v) + row0 * values, rows, a.heads * values, g, col, values);
 #pragma unroll
-                for (int u = 0; u < OT; ++u) to.store(S::tile(half, u), dv[u], T());
+                for (int u = 0; u < OT; ++u) to.store(S::tile(half, u), dv[u]);
             }
-            __builtin_amdgcn_sched_barrier(0);
+            hold();
             // dQ, rows are steps i, columns this wavefront's features: b dO S^T
             LaAcc d[OT] = {};
 #pragma unroll
@@ -997,16 +1054,17 @@ __global__ __launch_bounds__((LaShape<T, D>::THREADS)) void la_back_kernel(const
 #pragma unroll
                 for (int u = 0; u < OT; ++u) {
                     const int t = S::tile(half, u);
-                    const F g0 = la_rows<F>(gs, LD, 16 * t, 16 * x), g1 = la_rows<F>(gs, LD, 16 * t, 16 * x + 16);
+                    const F g0 = la_rows<F>(lane, gs, LD, 16 * t, 16 * x), g1 = la_rows<F>(lane, gs, LD, 16 * t, 16 * x + 16);
 #pragma unroll
                     for (int m = 0; m < S::ADDED; ++m) d[u] = la_mma(g0, g1, s0[m], s1[m], d[u]);
                 }
+                hold();
             }
             F qf[TT], kf[TT];
 #pragma unroll
             for (int t = 0; t < TT; ++t) {
-                qf[t] = la_cols(qs, LD, 16 * t, 16 * slice);
-                kf[t] = la_cols(ks, LD, 16 * t, 16 * slice);
+                qf[t] = la_cols(lane, qs, LD, 16 * t, 16 * slice);
+                kf[t] = la_cols(lane, ks, LD, 16 * t, 16 * slice);
             }
             // <E, S>
             float sum = 0.0f;
@@ -1034,21 +1092,13 @@ __global__ __launch_bounds__((LaShape<T, D>::THREADS)) void la_back_kernel(const
                 for (int r = 0; r < 4; ++r) at_start[r] = la_sum16(to_start[r] < 0.0f ? 0.0f : at_start[r]);
                 *reinterpret_cast<LaAcc *>(&sums.start[slice][i]) = at_start;
                 la_over_steps<BAD, S::INNER, TT, F>(
-                    d[u], 0, S::pair_of(u), [&](int m, int j) { return la_cols(ds + m * C * LDC, LDC, 16 * j, 16 * t); },
-                    [&](int j) { return BAD ? la_cols(ks, LD, 16 * j, 16 * slice) : kf[j]; },
+                    d[u], 0, S::pair_of(u), [&](int m, int j) { return la_cols(lane, ds + m * C * LDC, LDC, 16 * j, 16 * t); },
+                    [&](int j) { return BAD ? la_cols(lane, ks, LD, 16 * j, 16 * slice) : kf[j]; },
                     [&](int r, int j) { return meets(16 * t + 4 * g + r, j); });
             }
-            LaOut to;
-            if (a.wide) {
-                to.init(static_cast<float *>(a.d_q) + row0 * features, rows, a.heads * features, col, features);
-#pragma unroll
-                for (int u = 0; u < OT; ++u) to.store(S::tile(half, u), d[u], 0.0f);
-            } else {
-                to.init(static_cast<T *>(a.d_q) + row0 * features, rows, a.heads * features, col, features);
-#pragma unroll
-                for (int u = 0; u < OT; ++u) to.store(S::tile(half, u), d[u], T());
-            }
-            __builtin_amdgcn_sched_barrier(0);
+            store(a.d_q, d);
+            hold();
+            if constexpr (!SHARED) fetch_next();
             // dK, rows are steps j: w V E^T
             LaAcc c[OT] = {};
 #pragma unroll
@@ -1057,8 +1107,8 @@ __global__ __launch_bounds__((LaShape<T, D>::THREADS)) void la_back_kernel(const
                 if constexpr (SHARED) {
 #pragma unroll
                     for (int m = 0; m < S::ADDED; ++m) {
-                        e0[m] = la_rows<F>(es + m * D * LD, LD, 16 * slice, 16 * x);
-                        e1[m] = la_rows<F>(es + m * D * LD, LD, 16 * slice, 16 * x + 16);
+                        e0[m] = la_rows<F>(lane, es + m * D * LD, LD, 16 * slice, 16 * x);
+                        e1[m] = la_rows<F>(lane, es + m * D * LD, LD, 16 * slice, 16 * x + 16);
                     }
                 } else {
                     la_split(e[x], e0);
@@ -1067,10 +1117,11 @@ __global__ __launch_bounds__((LaShape<T, D>::THREADS)) void la_back_kernel(const
 #pragma unroll
                 for (int u = 0; u < OT; ++u) {
                     const int t = S::tile(half, u);
-                    const F v0 = la_rows<F>(vs, LD, 16 * t, 16 * x), v1 = la_rows<F>(vs, LD, 16 * t, 16 * x + 16);
+                    const F v0 = la_rows<F>(lane, vs, LD, 16 * t, 16 * x), v1 = la_rows<F>(lane, vs, LD, 16 * t, 16 * x + 16);
 #pragma unroll
                     for (int m = 0; m < S::ADDED; ++m) c[u] = la_mma(v0, v1, e0[m], e1[m], c[u]);
                 }
+                hold();
             }
 #pragma unroll
             for (int u = 0; u < OT; ++u) {
@@ -1082,20 +1133,12 @@ __global__ __launch_bounds__((LaShape<T, D>::THREADS)) void la_back_kernel(const
                 for (int r = 0; r < 4; ++r) at_end[r] = la_sum16(to_end[r] < 0.0f ? 0.0f : at_end[r]);
                 *reinterpret_cast<LaAcc *>(&sums.end[slice][j]) = at_end;
                 la_over_steps<BAD, S::INNER, TT, F>(
-                    c[u], S::pair_of(u), TT / 2 - 1, [&](int m, int i) { return la_rows<F>(ds + m * C * LDC, LDC, 16 * t, 16 * i); },
-                    [&](int i) { return BAD ? la_cols(qs, LD, 16 * i, 16 * slice) : qf[i]; },
+                    c[u], S::pair_of(u), TT / 2 - 1, [&](int m, int i) { return la_rows<F>(lane, ds + m * C * LDC, LDC, 16 * t, 16 * i); },
+                    [&](int i) { return BAD ? la_cols(lane, qs, LD, 16 * i, 16 * slice) : qf[i]; },
                     [&](int r, int i) { return meets(i, 16 * t + 4 * g + r); });
             }
-            if (a.wide) {
-                to.init(static_cast<float *>(a.d_k) + row0 * features, rows, a.heads * features, col, features);
-#pragma unroll
-                for (int u = 0; u < OT; ++u) to.store(S::tile(half, u), c[u], 0.0f);
-            } else {
-                to.init(static_cast<T *>(a.d_k) + row0 * features, rows, a.heads * features, col, features);
-#pragma unroll
-                for (int u = 0; u < OT; ++u) to.store(S::tile(half, u), c[u], T());
-            }
-            __builtin_amdgcn_sched_barrier(0);
+            store(a.d_k, c);
+            hold();
             // E in front of the chunk
 #pragma unroll
             for (int t = 0; t < OD; ++t) e[t] = la_times(e[t], decay);
@@ -1111,7 +1154,7 @@ __global__ __launch_bounds__((LaShape<T, D>::THREADS)) void la_back_kernel(const
 #pragma unroll
                 for (int x = 0; x < OD; ++x) {
                     const int at = 16 * (half * OD + x);
-                    F g0 = la_cols(gs, LD, 16 * t, at), g1 = la_cols(gs, LD, 16 * t + 16, at);
+                    F g0 = la_cols(lane, gs, LD, 16 * t, at), g1 = la_cols(lane, gs, LD, 16 * t + 16, at);
                     if constexpr (BAD) {
 #pragma unroll
                         for (int r = 0; r < 4; ++r) {
@@ -1122,6 +1165,7 @@ __global__ __launch_bounds__((LaShape<T, D>::THREADS)) void la_back_kernel(const
 #pragma unroll
                     for (int m = 0; m < S::ADDED; ++m) e[x] = la_mma(g0, g1, w[0][m], w[1][m], e[x]);
                 }
+                hold();
             }
         };
         if (__builtin_expect(bad, 0)) products(std::true_type());
