@@ -54,14 +54,16 @@ struct AttentionPlan {
 
 size_t rounded(size_t bytes) { return (bytes + 255) / 256 * 256; }
 
-// Sequences times heads are one workgroup each while they fill the 256 compute units; fewer are cut into segments.
+// Sequences times heads are one workgroup each, a compute unit's (registers and LDS hold no second one).  Fewer than half of the 256
+// are cut into as many segments as fill them, no more: 10 heads of 65537 steps in 26 segments leave four workgroups for
+// a second round and took twice the time of 25.
 AttentionPlan plan(const bf_linear_attention *p, bool back)
 {
     AttentionPlan r;
     const int64_t heads = p->batch * p->heads;
     r.chunks = r.segment_chunks = chunk_count(p);
-    if (heads < 192 && r.chunks > 4) {
-        const int64_t wanted = std::min<int64_t>((256 + heads - 1) / heads, (r.chunks + 1) / 2);
+    if (heads <= 128 && r.chunks > 4) {
+        const int64_t wanted = std::min<int64_t>(256 / heads, (r.chunks + 1) / 2);
         r.segment_chunks = (r.chunks + wanted - 1) / wanted;
         r.segments = (int)((r.chunks + r.segment_chunks - 1) / r.segment_chunks);
     }
