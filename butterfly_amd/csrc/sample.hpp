@@ -101,7 +101,6 @@ struct SampleWeight {
     // 2^44 exp((v - top) / temperature), rounded
     __device__ __forceinline__ unsigned long long operator()(float v) const
     {
-        if (!(below(v) <= range)) return 0;
         const double y = v == top ? 0.0 : ((double)v - (double)top) * per_nat, n = rint(y), x = (y - n) * 0.6931471805599453;
         // Taylor polynomial, |x| <= log(2) / 2: off by x^12 / 12! < 7e-15
         double p = 1.0 / 39916800.0;
@@ -116,7 +115,11 @@ struct SampleWeight {
         p = fma(p, x, 0.5);
         p = fma(p, x, 1.0);
         p = fma(p, x, 1.0);
-        return (unsigned long long)(ldexp(p, (int)n + kSampleBits) + 0.5);
+        // p in [0.7, 1.5): its 53 bits moved down to units of 2^-44, by 8 to 63 places
+        const uint64_t bits = __builtin_bit_cast(uint64_t, p);
+        const int down = min((int)(1023 - (bits >> 52)) - (int)n + 52 - kSampleBits, 63);
+        const uint64_t w = ((bits & 0xfffffffffffffull | 0x10000000000000ull) + (1ull << down >> 1)) >> down;
+        return below(v) <= range ? w : 0;
     }
 };
 
@@ -154,13 +157,16 @@ __device__ __forceinline__ unsigned long long sample_before(SampleLds &lds, unsi
     return before + inside - v;
 }
 
-// The bin in which the sum from the first bin on reaches the goal; lds.above: the sum in front of it.  -1: it is never reached.
-__device__ __forceinline__ int sample_crossing(SampleLds &lds, unsigned long long goal)
+// The bin in which the sum from the first bin on reaches goal(sum of all bins); lds.above: the sum in front of it.  -1: it is never
+// reached.
+template <typename G>
+__device__ __forceinline__ int sample_crossing(SampleLds &lds, G &&goal_of, unsigned long long &goal)
 {
     if (threadIdx.x == 0) lds.at = -1;
     const unsigned long long one = lds.bins[2 * threadIdx.x], two = lds.bins[2 * threadIdx.x + 1];
     unsigned long long total;
     const unsigned long long before = sample_before(lds, one + two, total);
+    goal = goal_of(total);
     if (before < goal && goal <= before + one + two) {
         const bool second = goal > before + one;
         lds.at = 2 * threadIdx.x + second;
@@ -192,31 +198,49 @@ struct SampleRow {
         }
     }
 
-    template <typename Fn>
+    // f(value, index) of every entry.  LONG: much is done for each, which is not to be laid out for all entries of a thread one behind
+    // the other: a dword at a time, in a loop.
+    template <bool LONG, typename Fn>
     __device__ __forceinline__ void each(Fn &&f) const
     {
         if constexpr (VECTORS > 0) {
 #pragma unroll
-            for (int n = 0; n < VECTORS; ++n)
-#pragma unroll
-                for (int i = 0; i < E; ++i) f(sample_element<T>(held[n], i), (int)piece(n) * E + i);
+            for (int n = 0; n < VECTORS; ++n) {
+                // (as something new to the compiler, which would otherwise keep what one pass has formed of every entry for the next)
+                uint4 v = held[n];
+                asm volatile("" : "+v"(v.x), "+v"(v.y), "+v"(v.z), "+v"(v.w));
+                piece_of<LONG>(v, (int)piece(n) * E, f);
+            }
         } else {
             for (int n = 0; n < span / 64; ++n) {
                 const int64_t at = piece(n);
                 if (at * E >= vocab) break;
-                const uint4 v = sample_load(row, at * E, vocab);
-#pragma unroll
-                for (int i = 0; i < E; ++i) f(sample_element<T>(v, i), (int)at * E + i);
+                piece_of<LONG>(sample_load(row, at * E, vocab), (int)at * E, f);
             }
+        }
+    }
+    template <bool LONG, typename Fn>
+    __device__ __forceinline__ void piece_of(uint4 v, int at, Fn &&f) const
+    {
+        if constexpr (LONG) {
+#pragma unroll 1
+            for (int k = 0; k < 4; ++k) {
+#pragma unroll
+                for (int i = 0; i < E / 4; ++i) f(sample_element<T>(v, i), at + k * (E / 4) + i);
+                v = make_uint4(v.y, v.z, v.w, v.x);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < E; ++i) f(sample_element<T>(v, i), at + i);
         }
     }
 };
 
-// The largest key t such that the weights of the logits from t up sum to the goal at least; lds.above: the sum of those above t.
-// False: all of them do not.
-template <typename T, typename Row, typename W>
-__device__ __forceinline__ bool sample_threshold(SampleLds &lds, const Row &row, const SampleWeight &weight, unsigned long long goal, W &&of,
-                                                 uint32_t &t)
+// The largest key t such that the weights of the logits from t up sum to goal(sum of all) at least; lds.above: the sum of those
+// above t.  False: all of them do not.  Weights are those of logits above key `floor`, and `ties` for all that are equal to it.
+template <typename T, bool LONG, typename Row, typename G, typename W>
+__device__ __forceinline__ bool sample_threshold(SampleLds &lds, const Row &row, const SampleWeight &weight, uint32_t floor,
+                                                 unsigned long long ties, G &&goal_of, W &&of, uint32_t &t)
 {
     auto clear = [&] {
         lds.bins[2 * threadIdx.x] = lds.bins[2 * threadIdx.x + 1] = 0;
@@ -225,32 +249,39 @@ __device__ __forceinline__ bool sample_threshold(SampleLds &lds, const Row &row,
     const float per = weight.range > 0.0f ? kSampleBins / weight.range : 0.0f;
     auto bin_of = [&](float v) { return min((int)(weight.below(v) * per), kSampleBins - 1); };
     clear();
-    row.each([&](float v, int) {
-        if (!(weight.below(v) <= weight.range)) return;
+    row.template each<LONG>([&](float v, int) {
+        if (!(weight.below(v) <= weight.range) | (sample_key<T>(v) <= floor)) return;
         const unsigned long long w = of(v);
         if (w) atomicAdd(&lds.bins[bin_of(v)], w);
     });
+    const float tie = sample_value<T>(floor);
+    if (threadIdx.x == 0 && ties) atomicAdd(&lds.bins[bin_of(tie)], ties);
     __syncthreads();
-    const int bin = sample_crossing(lds, goal);
+    unsigned long long goal;
+    const int bin = sample_crossing(lds, goal_of, goal);
     if (bin < 0) return false;
     unsigned long long above = lds.above;
     // (bins are off by rounding: a hundredth more on both sides)
     const float width = per > 0.0f ? 1.0f / per : 0.0f;
     uint32_t high = sample_key<T>(fminf(weight.top, weight.top - (bin - 0.01f) * width));
     uint32_t low = bin == kSampleBins - 1 ? sample_key<T>(weight.top - weight.range * 1.001f) : sample_key<T>(weight.top - (bin + 1.01f) * width);
+    low = max(low, floor);
     for (;;) {
         const uint32_t length = high - low;
         const int shift = length < (uint32_t)kSampleBins ? 0 : 32 - __clz((int)length) - 11;
         __syncthreads();
         clear();
-        row.each([&](float v, int) {
+        row.template each<false>([&](float v, int) {
             const uint32_t key = sample_key<T>(v);
-            if (key < low || key > high || !(weight.below(v) <= weight.range) || bin_of(v) != bin) return;
+            if ((key < low) | (key > high) | (key <= floor)) return;
+            if (!(weight.below(v) <= weight.range) || bin_of(v) != bin) return;
             const unsigned long long w = of(v);
             if (w) atomicAdd(&lds.bins[(high - key) >> shift], w);
         });
+        if (threadIdx.x == 0 && ties && floor >= low && floor <= high && bin_of(tie) == bin) atomicAdd(&lds.bins[(high - floor) >> shift], ties);
         __syncthreads();
-        const int at = sample_crossing(lds, goal - above);
+        unsigned long long rest;
+        const int at = sample_crossing(lds, [&](unsigned long long) { return goal - above; }, rest);
         if (at < 0) return false;   // (cannot be: the bin held it)
         above += lds.above;
         high -= (uint32_t)at << shift;
@@ -276,7 +307,7 @@ __global__ __launch_bounds__(kSampleThreads) void sample_kernel(const SampleArgs
     row.init(static_cast<const T *>(a.logits) + r * a.stride, a.vocab);
 
     float high = -INFINITY, low = INFINITY;
-    row.each([&](float v, int) {
+    row.template each<false>([&](float v, int) {
         high = fmaxf(high, v);
         low = fminf(low, v == -INFINITY ? INFINITY : v);
     });
@@ -304,7 +335,7 @@ __global__ __launch_bounds__(kSampleThreads) void sample_kernel(const SampleArgs
     if (!(temperature > 0.0)) {
         // the first of the largest
         int first = a.vocab;
-        row.each([&](float v, int at) { if (v == high) first = min(first, at); });
+        row.template each<false>([&](float v, int at) { if (v == high) first = min(first, at); });
 #pragma unroll
         for (int d = 1; d < 64; d *= 2) first = min(first, __shfl_xor(first, d, 64));
         if (lane == 0) lds.counts[wave] = (unsigned long long)first;
@@ -329,30 +360,17 @@ __global__ __launch_bounds__(kSampleThreads) void sample_kernel(const SampleArgs
     // kept: keys above t, and the first m of those equal to it
     uint32_t t = 0;
     unsigned long long m = 0;
-    auto kept_sums = [&](unsigned long long least, unsigned long long &sum, unsigned long long &ties) {
-        sum = ties = 0;
-        row.each([&](float v, int) {
-            const uint32_t key = sample_key<T>(v);
-            if (key > t) {
-                const unsigned long long w = weight(v);
-                sum += w >= least ? w : 0;
-            } else if (key == t) {
-                ++ties;
-            }
-        });
-    };
     if (top_k > 0 && top_k < a.vocab &&
-        sample_threshold<T>(lds, row, weight, (unsigned long long)top_k, [](float) { return 1ull; }, t))
+        sample_threshold<T, false>(lds, row, weight, 0, 0, [&](unsigned long long) { return (unsigned long long)top_k; }, [](float) { return 1ull; }, t))
         m = (unsigned long long)top_k - lds.above;
     if (top_p < 1.0) {
-        unsigned long long sum, ties, total;
-        kept_sums(1, sum, ties);
-        sample_before(lds, sum, total);
-        if (m > 0) total += m * weight(sample_value<T>(t));
-        const double share = ceil(fmax(top_p, 0.0) * (double)total);
-        const unsigned long long goal = max(1ull, min(total, (unsigned long long)share));
+        unsigned long long goal = 0;
+        auto goal_of = [&](unsigned long long total) {
+            goal = max(1ull, min(total, (unsigned long long)ceil(fmax(top_p, 0.0) * (double)total)));
+            return goal;
+        };
         uint32_t tp;
-        if (sample_threshold<T>(lds, row, weight, goal, [&](float v) { return weight(v); }, tp)) {
+        if (sample_threshold<T, true>(lds, row, weight, t, m > 0 ? m * weight(sample_value<T>(t)) : 0, goal_of, [&](float v) { return weight(v); }, tp)) {
             const unsigned long long w = weight(sample_value<T>(tp));
             t = tp;
             m = (goal - lds.above + w - 1) / w;
@@ -360,8 +378,15 @@ __global__ __launch_bounds__(kSampleThreads) void sample_kernel(const SampleArgs
     }
     const unsigned long long tie = m > 0 ? weight(sample_value<T>(t)) : 0;
     if (tie < weight.least) m = 0;
-    unsigned long long sum, ties;
-    kept_sums(weight.least, sum, ties);
+    unsigned long long sum = 0, ties = 0;
+    row.template each<true>([&](float v, int) {
+        const uint32_t key = sample_key<T>(v);
+        if (key > t) {
+            const unsigned long long w = weight(v);
+            sum += w >= weight.least ? w : 0;
+        }
+        ties += key == t;
+    });
     sum = sample_wave_sum(sum);
     ties = sample_wave_sum(ties);
     __syncthreads();
