@@ -7,9 +7,9 @@
 // over the values from the maximum down, then over the logits' bits within the bin where the sum crosses its goal.
 //
 // Weights are whole numbers, w in units of 2^-44: sums do not depend on their order (so the histograms may be filled by
-// atomics, and every call gives the same token), and are off by 2^-45 an entry, where borders between tokens are
-// decided as in 64 bits.  The exponential is a polynomial in double for the same reason: a float one moves each border by
-// some 1e-8 of the total, which with 50000 entries of similar weight is 1e-3 of the distance between two borders.
+// atomics, and every call gives the same token).  They are off by 2^-37 of themselves: a float exponential would move each border
+// between two tokens by some 1e-8 of the total, which with 50000 entries of similar weight is 1e-3 of the distance between two
+// borders; these move it by 1e-7 of that.
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -31,9 +31,10 @@ struct SampleArgs {
 };
 
 constexpr int kSampleThreads = 1024, kSampleWaves = kSampleThreads / 64, kSampleBins = 2 * kSampleThreads;
-constexpr int kSampleBits = 44;
+constexpr int kSampleBits = 44, kSampleFine = 4096;
 
 struct SampleLds {
+    unsigned long long powers[kSampleFine];   // 2^(k / 4096), in units of 2^-44
     unsigned long long bins[kSampleBins];
     unsigned long long sums[kSampleWaves];
     float low[kSampleWaves], high[kSampleWaves];
@@ -91,35 +92,29 @@ __device__ __forceinline__ float sample_element(const uint4 &v, int i)
 }
 
 struct SampleWeight {
+    const unsigned long long *powers = nullptr;
     float top = 0.0f;
-    double per_nat = 0.0;              // log2 e / temperature
+    float high = 0.0f, low = 0.0f;     // log2 e / temperature as two floats
     float range = 0.0f;                // farther below the maximum a weight is zero
     unsigned long long least = 1;      // smallest weight that min_p leaves
 
     __device__ __forceinline__ float below(float v) const { return v == top ? 0.0f : top - v; }
 
-    // 2^44 exp((v - top) / temperature), rounded
+    // 2^44 exp((v - top) / temperature), rounded: off by some 2^-37 of itself.  The exponent (of 2) as two floats, of which the next
+    // multiple of 1 / 4096 goes through the table and the rest, |x| < 2^-13, through 1 + s = 1 + x log 2 + (x log 2)^2 / 2.
+    // 26 operations; as a polynomial of 64-bit numbers the same took 50, of twice the time and more each.
     __device__ __forceinline__ unsigned long long operator()(float v) const
     {
-        const double y = v == top ? 0.0 : ((double)v - (double)top) * per_nat, n = rint(y), x = (y - n) * 0.6931471805599453;
-        // Taylor polynomial, |x| <= log(2) / 2: off by x^12 / 12! < 7e-15
-        double p = 1.0 / 39916800.0;
-        p = fma(p, x, 1.0 / 3628800.0);
-        p = fma(p, x, 1.0 / 362880.0);
-        p = fma(p, x, 1.0 / 40320.0);
-        p = fma(p, x, 1.0 / 5040.0);
-        p = fma(p, x, 1.0 / 720.0);
-        p = fma(p, x, 1.0 / 120.0);
-        p = fma(p, x, 1.0 / 24.0);
-        p = fma(p, x, 1.0 / 6.0);
-        p = fma(p, x, 0.5);
-        p = fma(p, x, 1.0);
-        p = fma(p, x, 1.0);
-        // p in [0.7, 1.5): its 53 bits moved down to units of 2^-44, by 8 to 63 places
-        const uint64_t bits = __builtin_bit_cast(uint64_t, p);
-        const int down = min((int)(1023 - (bits >> 52)) - (int)n + 52 - kSampleBits, 63);
-        const uint64_t w = ((bits & 0xfffffffffffffull | 0x10000000000000ull) + (1ull << down >> 1)) >> down;
-        return below(v) <= range ? w : 0;
+        const float d = below(v), back = d - top, rest = v == top ? 0.0f : (top - (d - back)) - (v + back);
+        const float y = d * high, y_rest = fmaf(d, high, -y) + fmaf(d, low, rest * high);
+        const float steps = rintf(y * kSampleFine), x = fmaf(steps, -1.0f / kSampleFine, y) + y_rest;
+        const float s = x * -0.6931472f, e = fmaf(s * s, 0.5f, s);
+        const int m = -(int)steps;
+        const uint64_t power = powers[m & (kSampleFine - 1)];
+        const float scaled = (float)(uint32_t)(power >> 13) * e;          // power * e / 2^13
+        const uint64_t w = power + 2 * (int64_t)(int)(scaled * 4096.0f);   // (power * e < 2^32)
+        const int down = min(-(m >> 12), 63);
+        return d <= range ? (w + (1ull << down >> 1)) >> down : 0;
     }
 };
 
@@ -347,9 +342,15 @@ __global__ __launch_bounds__(kSampleThreads) void sample_kernel(const SampleArgs
         }
         return;
     }
+    for (int k = threadIdx.x; k < kSampleFine; k += kSampleThreads)
+        lds.powers[k] = (unsigned long long)(exp2((double)k / kSampleFine) * (double)(1ull << kSampleBits) + 0.5);
+    __syncthreads();
     SampleWeight weight;
+    weight.powers = lds.powers;
     weight.top = high;
-    weight.per_nat = 1.4426950408889634 / temperature;
+    const double per_nat = 1.4426950408889634 / temperature;
+    weight.high = (float)per_nat;
+    weight.low = (float)(per_nat - (double)weight.high);
     weight.range = high == INFINITY ? 0.0f : fminf(high - low, (float)(temperature * ((kSampleBits + 2) * 0.6931471805599453)));
     const double min_p = a.min_p ? (double)a.min_p[r] : a.min_p_all;
     const double top_p = a.top_p ? (double)a.top_p[r] : a.top_p_all;
