@@ -91,30 +91,34 @@ __device__ __forceinline__ float sample_element(const uint4 &v, int i)
     else return __builtin_bit_cast(float, i % 2 ? words[i / 2] & 0xffff0000u : words[i / 2] << 16);
 }
 
+template <typename T>
 struct SampleWeight {
     const unsigned long long *powers = nullptr;
     float top = 0.0f;
-    float high = 0.0f, low = 0.0f;     // log2 e / temperature as two floats
+    float high = 0.0f, low = 0.0f;     // 4096 log2 e / temperature as two floats
     float range = 0.0f;                // farther below the maximum a weight is zero
-    unsigned long long least = 1;      // smallest weight that min_p leaves
 
-    __device__ __forceinline__ float below(float v) const { return v == top ? 0.0f : top - v; }
+    __device__ __forceinline__ bool reaches(float v) const { return top - v <= range; }
 
-    // 2^44 exp((v - top) / temperature), rounded: off by some 2^-37 of itself.  The exponent (of 2) as two floats, of which the next
-    // multiple of 1 / 4096 goes through the table and the rest, |x| < 2^-13, through 1 + s = 1 + x log 2 + (x log 2)^2 / 2.
-    // 26 operations; as a polynomial of 64-bit numbers the same took 50, of twice the time and more each.
+    // 2^44 exp((v - top) / temperature), rounded, of a v that it reaches: off by some 2^-37 of itself.  The exponent, of 2^(1 / 4096),
+    // as two floats: a whole number of steps goes through the table, the rest, |x| <= 1/2, through 1 + s = 1 + x l + (x l)^2 / 2 with
+    // l = log 2 / 4096 (e is 4096 s).  30 operations; a polynomial in 64-bit numbers took 50, many of them twice as long.
     __device__ __forceinline__ unsigned long long operator()(float v) const
     {
-        const float d = below(v), back = d - top, rest = v == top ? 0.0f : (top - (d - back)) - (v + back);
-        const float y = d * high, y_rest = fmaf(d, high, -y) + fmaf(d, low, rest * high);
-        const float steps = rintf(y * kSampleFine), x = fmaf(steps, -1.0f / kSampleFine, y) + y_rest;
-        const float s = x * -0.6931472f, e = fmaf(s * s, 0.5f, s);
+        const float d = top - v, z = d * high;
+        float rest = fmaf(d, low, fmaf(d, high, -z));
+        if constexpr (sizeof(T) == 4) {
+            // (bfloat16: the difference is exact, or that of a number so small that it is exact enough)
+            const float back = d - top;
+            rest = fmaf((top - (d - back)) - (v + back), high, rest);
+        }
+        const float steps = rintf(z), s = ((z - steps) + rest) * -0.6931472f, e = fmaf(s * s, 0.5f / kSampleFine, s);
         const int m = -(int)steps;
         const uint64_t power = powers[m & (kSampleFine - 1)];
-        const float scaled = (float)(uint32_t)(power >> 13) * e;          // power * e / 2^13
-        const uint64_t w = power + 2 * (int64_t)(int)(scaled * 4096.0f);   // (power * e < 2^32)
-        const int down = min(-(m >> 12), 63);
-        return d <= range ? (w + (1ull << down >> 1)) >> down : 0;
+        // (a step's power times 4096 s: less than 2^32 in units of 2^-43)
+        const uint64_t w = power + 2 * (int64_t)(int)((float)(uint32_t)(power >> 13) * e);
+        const int down = -(m >> 12);
+        return ((w << 1 >> down) + 1) >> 1;
     }
 };
 
@@ -192,7 +196,6 @@ struct SampleRow {
             for (int n = 0; n < VECTORS; ++n) held[n] = sample_load(row, piece(n) * E, vocab);
         }
     }
-
     // f(value, index) of every entry.  LONG: much is done for each, which is not to be laid out for all entries of a thread one behind
     // the other: a dword at a time, in a loop.
     template <bool LONG, typename Fn>
@@ -210,7 +213,7 @@ struct SampleRow {
             for (int n = 0; n < span / 64; ++n) {
                 const int64_t at = piece(n);
                 if (at * E >= vocab) break;
-                piece_of<LONG>(sample_load(row, at * E, vocab), (int)at * E, f);
+                piece_of<false>(sample_load(row, at * E, vocab), (int)at * E, f);
             }
         }
     }
@@ -231,26 +234,23 @@ struct SampleRow {
     }
 };
 
-// The largest key t such that the weights of the logits from t up sum to goal(sum of all) at least; lds.above: the sum of those
-// above t.  False: all of them do not.  Weights are those of logits above key `floor`, and `ties` for all that are equal to it.
+// The largest value t such that the weights of the logits from t up sum to goal(sum of all) at least; lds.above: the sum of those
+// above t.  False: all of them do not.  Weights are those of logits above `floor`, and `ties` for all that are equal to it.
 template <typename T, bool LONG, typename Row, typename G, typename W>
-__device__ __forceinline__ bool sample_threshold(SampleLds &lds, const Row &row, const SampleWeight &weight, uint32_t floor,
-                                                 unsigned long long ties, G &&goal_of, W &&of, uint32_t &t)
+__device__ __forceinline__ bool sample_threshold(SampleLds &lds, const Row &row, const SampleWeight<T> &weight, float floor,
+                                                 unsigned long long ties, G &&goal_of, W &&of, float &t)
 {
     auto clear = [&] {
         lds.bins[2 * threadIdx.x] = lds.bins[2 * threadIdx.x + 1] = 0;
         __syncthreads();
     };
     const float per = weight.range > 0.0f ? kSampleBins / weight.range : 0.0f;
-    auto bin_of = [&](float v) { return min((int)(weight.below(v) * per), kSampleBins - 1); };
+    auto bin_of = [&](float v) { return min((int)((weight.top - v) * per), kSampleBins - 1); };
     clear();
     row.template each<LONG>([&](float v, int) {
-        if (!(weight.below(v) <= weight.range) | (sample_key<T>(v) <= floor)) return;
-        const unsigned long long w = of(v);
-        if (w) atomicAdd(&lds.bins[bin_of(v)], w);
+        if (weight.reaches(v) & (v > floor)) atomicAdd(&lds.bins[bin_of(v)], of(v));
     });
-    const float tie = sample_value<T>(floor);
-    if (threadIdx.x == 0 && ties) atomicAdd(&lds.bins[bin_of(tie)], ties);
+    if (threadIdx.x == 0 && ties) atomicAdd(&lds.bins[bin_of(floor)], ties);
     __syncthreads();
     unsigned long long goal;
     const int bin = sample_crossing(lds, goal_of, goal);
@@ -260,20 +260,18 @@ __device__ __forceinline__ bool sample_threshold(SampleLds &lds, const Row &row,
     const float width = per > 0.0f ? 1.0f / per : 0.0f;
     uint32_t high = sample_key<T>(fminf(weight.top, weight.top - (bin - 0.01f) * width));
     uint32_t low = bin == kSampleBins - 1 ? sample_key<T>(weight.top - weight.range * 1.001f) : sample_key<T>(weight.top - (bin + 1.01f) * width);
-    low = max(low, floor);
     for (;;) {
         const uint32_t length = high - low;
         const int shift = length < (uint32_t)kSampleBins ? 0 : 32 - __clz((int)length) - 11;
+        const float least = sample_value<T>(low), most = sample_value<T>(high);
         __syncthreads();
         clear();
         row.template each<false>([&](float v, int) {
-            const uint32_t key = sample_key<T>(v);
-            if ((key < low) | (key > high) | (key <= floor)) return;
-            if (!(weight.below(v) <= weight.range) || bin_of(v) != bin) return;
-            const unsigned long long w = of(v);
-            if (w) atomicAdd(&lds.bins[(high - key) >> shift], w);
+            if ((v >= least) & (v <= most) & (v > floor))
+                if (weight.reaches(v) && bin_of(v) == bin) atomicAdd(&lds.bins[(high - sample_key<T>(v)) >> shift], of(v));
         });
-        if (threadIdx.x == 0 && ties && floor >= low && floor <= high && bin_of(tie) == bin) atomicAdd(&lds.bins[(high - floor) >> shift], ties);
+        if (threadIdx.x == 0 && ties && floor >= least && floor <= most && bin_of(floor) == bin)
+            atomicAdd(&lds.bins[(high - sample_key<T>(floor)) >> shift], ties);
         __syncthreads();
         unsigned long long rest;
         const int at = sample_crossing(lds, [&](unsigned long long) { return goal - above; }, rest);
@@ -284,11 +282,29 @@ __device__ __forceinline__ bool sample_threshold(SampleLds &lds, const Row &row,
         const uint32_t lowest = high - ((1u << shift) - 1);
         low = max(low, lowest > high ? 0u : lowest);
     }
-    t = high;
+    t = sample_value<T>(high);
     __syncthreads();
     if (threadIdx.x == 0) lds.above = above;
     __syncthreads();
     return true;
+}
+
+// The largest value whose weight is below `least` (of those that a weight reaches).
+template <typename T>
+__device__ __forceinline__ float sample_below(const SampleWeight<T> &weight, unsigned long long least)
+{
+    // keys low .. high - 1 are unknown, those from high on are not below; 1024 of them at a time
+    uint32_t low = sample_key<T>(weight.top - weight.range), high = sample_key<T>(weight.top);
+    while (low < high) {
+        const uint32_t step = (high - low) / kSampleThreads + 1, key = low + threadIdx.x * step;
+        const bool below = key < high && key >= low && weight(sample_value<T>(key)) < least;
+        const uint32_t count = (uint32_t)__syncthreads_count(below);
+        high = min(high, low + count * step);
+        low = count == 0 ? high : min(high, low + (count - 1) * step + 1);
+    }
+    // (there is no -0 among the entries, and it equals 0)
+    const uint32_t key = high - 1, zero = sample_key<T>(0.0f);
+    return sample_value<T>(key == zero - 1 ? key - 1 : key);
 }
 
 template <typename T, int VECTORS>
@@ -345,48 +361,57 @@ __global__ __launch_bounds__(kSampleThreads) void sample_kernel(const SampleArgs
     for (int k = threadIdx.x; k < kSampleFine; k += kSampleThreads)
         lds.powers[k] = (unsigned long long)(exp2((double)k / kSampleFine) * (double)(1ull << kSampleBits) + 0.5);
     __syncthreads();
-    SampleWeight weight;
+    const bool infinite = high == INFINITY;
+    SampleWeight<T> weight;
     weight.powers = lds.powers;
-    weight.top = high;
-    const double per_nat = 1.4426950408889634 / temperature;
+    weight.top = infinite ? 0.0f : high;
+    const double per_nat = kSampleFine * 1.4426950408889634 / temperature;
     weight.high = (float)per_nat;
     weight.low = (float)(per_nat - (double)weight.high);
-    weight.range = high == INFINITY ? 0.0f : fminf(high - low, (float)(temperature * ((kSampleBits + 2) * 0.6931471805599453)));
+    weight.range = infinite ? -1.0f : fminf(high - low, (float)(temperature * ((kSampleBits + 2) * 0.6931471805599453)));
     const double min_p = a.min_p ? (double)a.min_p[r] : a.min_p_all;
     const double top_p = a.top_p ? (double)a.top_p[r] : a.top_p_all;
     const int64_t top_k = a.top_k ? a.top_k[r] : a.top_k_all;
-    const unsigned long long one = 1ull << kSampleBits;
-    if (min_p > 0.0) weight.least = max(1ull, (unsigned long long)ceil(fmin(min_p, 1.0) * (double)one));
 
-    // kept: keys above t, and the first m of those equal to it
-    uint32_t t = 0;
+    // kept: values above t, and the first m of those equal to it
+    float t = -INFINITY;
     unsigned long long m = 0;
-    if (top_k > 0 && top_k < a.vocab &&
-        sample_threshold<T, false>(lds, row, weight, 0, 0, [&](unsigned long long) { return (unsigned long long)top_k; }, [](float) { return 1ull; }, t))
+    if (infinite) {
+        // those alone, all equally likely: the first ones
+        unsigned long long mine = 0, all;
+        row.template each<false>([&](float v, int) { mine += v == INFINITY; });
+        sample_before(lds, mine, all);
+        t = INFINITY;
+        m = top_k > 0 ? min((unsigned long long)top_k, all) : all;
+        if (top_p < 1.0) m = max(1ull, min(m, (unsigned long long)ceil(fmax(top_p, 0.0) * (double)m)));
+    } else if (top_k > 0 && top_k < a.vocab &&
+        sample_threshold<T, false>(lds, row, weight, t, 0, [&](unsigned long long) { return (unsigned long long)top_k; }, [](float) { return 1ull; }, t))
         m = (unsigned long long)top_k - lds.above;
-    if (top_p < 1.0) {
+    if (!infinite && top_p < 1.0) {
         unsigned long long goal = 0;
         auto goal_of = [&](unsigned long long total) {
             goal = max(1ull, min(total, (unsigned long long)ceil(fmax(top_p, 0.0) * (double)total)));
             return goal;
         };
-        uint32_t tp;
-        if (sample_threshold<T, true>(lds, row, weight, t, m > 0 ? m * weight(sample_value<T>(t)) : 0, goal_of, [&](float v) { return weight(v); }, tp)) {
-            const unsigned long long w = weight(sample_value<T>(tp));
+        float tp;
+        if (sample_threshold<T, true>(lds, row, weight, t, m > 0 ? m * weight(t) : 0, goal_of, [&](float v) { return weight(v); }, tp)) {
+            const unsigned long long w = weight(tp);
             t = tp;
             m = (goal - lds.above + w - 1) / w;
         }
     }
-    const unsigned long long tie = m > 0 ? weight(sample_value<T>(t)) : 0;
-    if (tie < weight.least) m = 0;
+    if (!infinite && min_p > 0.0) {
+        const float unlikely = sample_below<T>(weight, max(1ull, (unsigned long long)ceil(fmin(min_p, 1.0) * (double)(1ull << kSampleBits))));
+        if (unlikely >= t) {
+            t = unlikely;
+            m = 0;
+        }
+    }
+    const unsigned long long tie = infinite ? 1 : m > 0 ? weight(t) : 0;
     unsigned long long sum = 0, ties = 0;
     row.template each<true>([&](float v, int) {
-        const uint32_t key = sample_key<T>(v);
-        if (key > t) {
-            const unsigned long long w = weight(v);
-            sum += w >= weight.least ? w : 0;
-        }
-        ties += key == t;
+        if (weight.reaches(v) & (v > t)) sum += weight(v);
+        ties += v == t;
     });
     sum = sample_wave_sum(sum);
     ties = sample_wave_sum(ties);
@@ -423,12 +448,8 @@ __global__ __launch_bounds__(kSampleThreads) void sample_kernel(const SampleArgs
 #pragma unroll
             for (int i = 0; i < E; ++i) {
                 const float x = sample_element<T>(v, i);
-                const uint32_t key = sample_key<T>(x);
-                if (key > t) {
-                    const unsigned long long w = weight(x);
-                    mass += w >= weight.least ? w : 0;
-                }
-                equal += key == t;
+                if (weight.reaches(x) & (x > t)) mass += weight(x);
+                equal += x == t;
             }
         }
         unsigned long long all_equal, all;
@@ -440,12 +461,10 @@ __global__ __launch_bounds__(kSampleThreads) void sample_kernel(const SampleArgs
                 unsigned long long rest = target - before, used = 0;
                 for (int i = 0; i < E; ++i) {
                     const float x = sample_element<T>(v, i);
-                    const uint32_t key = sample_key<T>(x);
                     unsigned long long w = 0;
-                    if (key > t) {
-                        w = weight(x);
-                        if (w < weight.least) w = 0;
-                    } else if (key == t && used < allowed) {
+                    if (x > t) {
+                        if (weight.reaches(x)) w = weight(x);
+                    } else if (x == t && used < allowed) {
                         w = tie;
                         ++used;
                     }
