@@ -164,3 +164,24 @@ def test_c_abi_refuses_bad_descriptors():
         refused(code, lambda: L.bf_sample_tokens(ctypes.byref(d), one, one, null, null, null, null, one, null), text)
     refused(-1, lambda: L.bf_sample_tokens(ctypes.byref(s), one, null, null, null, null, null, one, null), b"NULL")
     assert L.bf_sample_tokens(ctypes.byref(changed(s, rows=0)), *[null] * 8) == 0
+
+
+def test_model_with_heads():
+    from butterfly_amd.sequence_model import ButterflyLM
+    torch.manual_seed(0)
+    m = ButterflyLM(50, 16, 2, heads=2, dropout=0.0)
+    tokens = torch.randint(0, 50, (2, 9))
+    loss = m.loss(tokens[:, :-1], tokens[:, 1:])
+    assert all(bool(torch.isfinite(g).all()) for g in torch.autograd.grad(loss, list(m.parameters())))
+    m.eval()
+    with torch.no_grad():
+        hidden, last = m.hidden(tokens)
+        states = m.empty_states(2)
+        for t in range(9):
+            logits = m.step(tokens[:, t], states)
+    want = hidden[:, -1] @ m.embedding.t()
+    # (float32 through some ten layers)
+    assert float((logits - want).detach().abs().max()) < 1e-4 * float(want.detach().abs().max())
+    assert m.generate(tokens, torch.rand(2, 4), 0.8, top_k=5).shape == (2, 4)
+    with pytest.raises(ValueError, match="multiple"):
+        ButterflyLM(50, 18, 1, heads=2)
