@@ -781,7 +781,9 @@ __global__ __launch_bounds__((LaShape<T, D>::THREADS)) void la_back_kernel(const
     T *const es = room, *const ps = room + (SHARED ? HELD : 0), *const ds = ps + S::INNER * C * LDC;
     __shared__ __align__(16) LaLevels<C> three_levels[3];   // of the chunk, the next one, and the last one's for its decays' gradients
     struct Sums {
-        float row[TT][C], col[TT][C], start[S::SLICES][C], end[S::SLICES][C], through[W];
+        // (of two chunks: the next one's are written while the decays' gradients of this one are formed)
+        float row[2][TT][C], col[2][TT][C];
+        float start[S::SLICES][C], end[S::SLICES][C], through[W];
     };
     __shared__ __align__(16) Sums sums;
     __shared__ int bad_chunk[2];
@@ -848,8 +850,8 @@ __global__ __launch_bounds__((LaShape<T, D>::THREADS)) void la_back_kernel(const
         float later = 0.0f, earlier = 0.0f;
 #pragma unroll
         for (int x = 0; x < TT; ++x) {
-            later += x <= ((t >> 4) | 1) ? sums.row[x][t] : 0.0f;
-            later -= x >= ((t >> 4) & ~1) ? sums.col[x][t] : 0.0f;
+            later += x <= ((t >> 4) | 1) ? sums.row[n & 1][x][t] : 0.0f;
+            later -= x >= ((t >> 4) & ~1) ? sums.col[n & 1][x][t] : 0.0f;
         }
 #pragma unroll
         for (int x = 0; x < S::SLICES; ++x) {
@@ -998,11 +1000,11 @@ __global__ __launch_bounds__((LaShape<T, D>::THREADS)) void la_back_kernel(const
             float column = (gg[u][0] + gg[u][1]) + (gg[u][2] + gg[u][3]);
             column += __shfl_xor(column, 16, 64);
             column += __shfl_xor(column, 32, 64);
-            sums.col[ti][j] = column;   // (the same from four lanes)
+            sums.col[n & 1][ti][j] = column;   // (the same from four lanes)
             LaAcc row;
 #pragma unroll
             for (int r = 0; r < 4; ++r) row[r] = la_sum16(gg[u][r]);
-            *reinterpret_cast<LaAcc *>(&sums.row[tj][i]) = row;   // (from sixteen)
+            *reinterpret_cast<LaAcc *>(&sums.row[n & 1][tj][i]) = row;   // (from sixteen)
         }
         __syncthreads();
         if constexpr (!SHARED) fetch_state();

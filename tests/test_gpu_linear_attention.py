@@ -292,6 +292,28 @@ def test_same_bits_at_every_call_and_on_other_streams():
             assert torch.equal(got[k], want[k]), k
 
 
+@pytest.mark.parametrize("dtype, size", [(torch.float32, 64), (torch.bfloat16, 64), (torch.float32, 128), (torch.bfloat16, 100)])
+def test_a_full_chip(dtype, size):
+    """256 workgroups of some twenty chunks, wavefronts at their own pace: the same bits at every call, and some heads
+    against the definition."""
+    v = make(16, 700, 16, 16, size, size, dtype)
+    c = {k: t.cuda() for k, t in v.items()}
+    leaves = [c[k].requires_grad_() for k in NAMES]
+    first = None
+    for _ in range(4):
+        o, last = tb.linear_attention(*leaves, scale=0.2)
+        got = [o.detach(), last.detach(), *torch.autograd.grad([o, last], leaves, [c["grad"], c["grad_last"]])]
+        if first is None:
+            first = got
+        for a, b in zip(got, first):
+            assert torch.equal(a, b)
+    for b, h in ((0, 0), (5, 7), (15, 15)):
+        one = {k: (t[b:b + 1, h:h + 1] if k in ("state", "grad_last") else t[b:b + 1, :, h:h + 1]) for k, t in v.items()}
+        part = dict(zip(("o", "last", "d_q", "d_k", "d_v", "d_log_decay", "d_state"), first))
+        part = {k: (t[b:b + 1, h:h + 1] if k in ("last", "d_state") else t[b:b + 1, :, h:h + 1]) for k, t in part.items()}
+        compare(part, reference(one, 0.2), dtype, wide=size > 64)
+
+
 def test_captured_calls():
     v = {k: t.cuda() for k, t in make(2, 400, 3, 1, 40, 64, torch.float32).items()}
     leaves = [v[k].requires_grad_() for k in NAMES]
