@@ -53,7 +53,7 @@ extern "C" int bf_rotary_apply(const bf_rotary *p, const void *x, const int64_t 
     a.back = back != 0;
     // some four items a thread where there are enough for 1024 workgroups, fewer otherwise
     const int pairs = a.rotated / 2, rest = a.features - a.rotated;
-    const int64_t items = (p->interleaved ? (a.rotated + 7) / 8 : (pairs + 7) / 8) + (rest + 7) / 8;
+    const int64_t items = p->interleaved ? (a.features + 7) / 8 : (pairs + 7) / 8 + (rest + 7) / 8;
     const int64_t each = std::max<int64_t>(256, std::min<int64_t>(1024, a.tokens * a.heads * items / 1024));
     a.heads_each = (int)std::max<int64_t>(1, std::min<int64_t>(a.heads, each / items));
     a.head_parts = (a.heads + a.heads_each - 1) / a.heads_each;

@@ -46,8 +46,8 @@ __global__ __launch_bounds__(256) void rotary_kernel(const RotaryArgs a)
         table[at] = make_float2(a.magnitude * cosine, a.back ? -a.magnitude * sine : a.magnitude * sine);
     }
     __syncthreads();
-    // eight pairs at a time (four neighbouring ones), then eight of the features that are copied
-    const int turned = NEIGHBOURS ? (a.rotated + 7) / 8 : (pairs + 7) / 8, items = turned + (rest + 7) / 8;
+    // Eight pairs at a time, then eight of the features that are copied; or eight neighbours of all of them.
+    const int turned = NEIGHBOURS ? (a.features + 7) / 8 : (pairs + 7) / 8, items = NEIGHBOURS ? turned : turned + (rest + 7) / 8;
     for (int at = threadIdx.x; at < tokens * heads * items; at += 256) {
         const int item = at % items, n = at / items, head = head0 + n % heads, t = n / heads;
         const int64_t token = first + t;
@@ -55,19 +55,21 @@ __global__ __launch_bounds__(256) void rotary_kernel(const RotaryArgs a)
         T *y = static_cast<T *>(a.y) + (token * a.heads + head) * a.features;
         const float2 *turn = table + t * pairs;
         float u[8], v[8];
-        if (item >= turned) {
+        if (!NEIGHBOURS && item >= turned) {
             const int col = (item - turned) * 8;
             load8(x + a.rotated, col, rest, 0.0f, u);
             store8(y + a.rotated, col, rest, u);
         } else if (NEIGHBOURS) {
-            load8(x, item * 8, a.rotated, 0.0f, u);
+            load8(x, item * 8, a.features, 0.0f, u);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const float2 z = turn[min(item * 4 + i, pairs - 1)];
-                v[2 * i] = u[2 * i] * z.x - u[2 * i + 1] * z.y;
-                v[2 * i + 1] = u[2 * i] * z.y + u[2 * i + 1] * z.x;
+                const bool turns = item * 4 + i < pairs;
+                const float2 z = turn[turns ? item * 4 + i : 0];
+                const float one = u[2 * i] * z.x - u[2 * i + 1] * z.y, two = u[2 * i] * z.y + u[2 * i + 1] * z.x;
+                v[2 * i] = turns ? one : u[2 * i];
+                v[2 * i + 1] = turns ? two : u[2 * i + 1];
             }
-            store8(y, item * 8, a.rotated, v);
+            store8(y, item * 8, a.features, v);
         } else {
             load8(x, item * 8, pairs, 0.0f, u);
             load8(x + pairs, item * 8, pairs, 0.0f, v);
