@@ -32,6 +32,7 @@ struct SampleArgs {
 
 constexpr int kSampleThreads = 1024, kSampleWaves = kSampleThreads / 64, kSampleBins = 2 * kSampleThreads;
 constexpr int kSampleBits = 44, kSampleFine = 4096;
+constexpr int kSampleFew = 512;   // entries of a bin that are compared with each other
 
 struct SampleLds {
     unsigned long long powers[kSampleFine];   // 2^(k / 4096), in units of 2^-44
@@ -40,7 +41,8 @@ struct SampleLds {
     float low[kSampleWaves], high[kSampleWaves];
     unsigned long long counts[kSampleWaves];
     unsigned long long above;
-    int at;
+    float few[kSampleFew], threshold;
+    int at, number;
 };
 
 // Order of floats as an order of whole numbers (of bfloat16: 16 bits).
@@ -256,6 +258,43 @@ __device__ __forceinline__ bool sample_threshold(SampleLds &lds, const Row &row,
     const int bin = sample_crossing(lds, goal_of, goal);
     if (bin < 0) return false;
     unsigned long long above = lds.above;
+    // Few entries in the bin (a vocabulary of 2^17 makes some 64): each sums up those above it.  (The order in which they come
+    // does not show in sums of whole numbers.)  bfloat16: a bin holds few distinct values, which the next round tells apart.
+    if constexpr (sizeof(T) == 4) {
+        if (threadIdx.x == 0) lds.number = 0;
+        __syncthreads();
+        row.template each<false>([&](float v, int) {
+            if (weight.reaches(v) & (v > floor))
+                if (bin_of(v) == bin) {
+                    const int at = atomicAdd(&lds.number, 1);
+                    if (at < kSampleFew) lds.few[at] = v;
+                }
+        });
+        __syncthreads();
+        const int number = lds.number;
+        if (number <= kSampleFew) {
+            if (threadIdx.x < number) lds.bins[threadIdx.x] = of(lds.few[threadIdx.x]);
+            __syncthreads();
+            const bool tied = ties && bin_of(floor) == bin;
+            if (threadIdx.x < number + tied) {
+                const float v = threadIdx.x < number ? lds.few[threadIdx.x] : floor;
+                unsigned long long greater = above, equal = threadIdx.x < number ? 0 : ties;
+                for (int j = 0; j < number; ++j) {
+                    const float x = lds.few[j];
+                    const unsigned long long w = lds.bins[j];
+                    greater += x > v ? w : 0;
+                    equal += x == v ? w : 0;
+                }
+                if (greater < goal && goal <= greater + equal) {
+                    lds.threshold = v;
+                    lds.above = greater;
+                }
+            }
+            __syncthreads();
+            t = lds.threshold;
+            return true;
+        }
+    }
     // (bins are off by rounding: a hundredth more on both sides)
     const float width = per > 0.0f ? 1.0f / per : 0.0f;
     uint32_t high = sample_key<T>(fminf(weight.top, weight.top - (bin - 0.01f) * width));
@@ -317,6 +356,17 @@ __global__ __launch_bounds__(kSampleThreads) void sample_kernel(const SampleArgs
     SampleRow<T, VECTORS> row;
     row.init(static_cast<const T *>(a.logits) + r * a.stride, a.vocab);
 
+    // the table, while the row is on its way: 2^(i / 64) 2^(j / 4096)
+    if (threadIdx.x < 128) {
+        const int i = threadIdx.x & 63;
+        lds.bins[threadIdx.x] = __builtin_bit_cast(unsigned long long, exp2(threadIdx.x < 64 ? i / 64.0 : i / 4096.0));
+    }
+    __syncthreads();
+    for (int k = threadIdx.x; k < kSampleFine; k += kSampleThreads) {
+        const double coarse = __builtin_bit_cast(double, lds.bins[k >> 6]), fine = __builtin_bit_cast(double, lds.bins[64 + (k & 63)]);
+        lds.powers[k] = (unsigned long long)(coarse * fine * (double)(1ull << kSampleBits) + 0.5);
+    }
+
     float high = -INFINITY, low = INFINITY;
     row.template each<false>([&](float v, int) {
         high = fmaxf(high, v);
@@ -358,9 +408,6 @@ __global__ __launch_bounds__(kSampleThreads) void sample_kernel(const SampleArgs
         }
         return;
     }
-    for (int k = threadIdx.x; k < kSampleFine; k += kSampleThreads)
-        lds.powers[k] = (unsigned long long)(exp2((double)k / kSampleFine) * (double)(1ull << kSampleBits) + 0.5);
-    __syncthreads();
     const bool infinite = high == INFINITY;
     SampleWeight<T> weight;
     weight.powers = lds.powers;
