@@ -356,17 +356,6 @@ __global__ __launch_bounds__(kSampleThreads) void sample_kernel(const SampleArgs
     SampleRow<T, VECTORS> row;
     row.init(static_cast<const T *>(a.logits) + r * a.stride, a.vocab);
 
-    // the table, while the row is on its way: 2^(i / 64) 2^(j / 4096)
-    if (threadIdx.x < 128) {
-        const int i = threadIdx.x & 63;
-        lds.bins[threadIdx.x] = __builtin_bit_cast(unsigned long long, exp2(threadIdx.x < 64 ? i / 64.0 : i / 4096.0));
-    }
-    __syncthreads();
-    for (int k = threadIdx.x; k < kSampleFine; k += kSampleThreads) {
-        const double coarse = __builtin_bit_cast(double, lds.bins[k >> 6]), fine = __builtin_bit_cast(double, lds.bins[64 + (k & 63)]);
-        lds.powers[k] = (unsigned long long)(coarse * fine * (double)(1ull << kSampleBits) + 0.5);
-    }
-
     float high = -INFINITY, low = INFINITY;
     row.template each<false>([&](float v, int) {
         high = fmaxf(high, v);
@@ -408,6 +397,17 @@ __global__ __launch_bounds__(kSampleThreads) void sample_kernel(const SampleArgs
         }
         return;
     }
+    // the table: 2^(i / 64) 2^(j / 4096)
+    if (threadIdx.x < 128) {
+        const int i = threadIdx.x & 63;
+        lds.bins[threadIdx.x] = __builtin_bit_cast(unsigned long long, exp2(threadIdx.x < 64 ? i / 64.0 : i / 4096.0));
+    }
+    __syncthreads();
+    for (int k = threadIdx.x; k < kSampleFine; k += kSampleThreads) {
+        const double coarse = __builtin_bit_cast(double, lds.bins[k >> 6]), fine = __builtin_bit_cast(double, lds.bins[64 + (k & 63)]);
+        lds.powers[k] = (unsigned long long)(coarse * fine * (double)(1ull << kSampleBits) + 0.5);
+    }
+    __syncthreads();
     const bool infinite = high == INFINITY;
     SampleWeight<T> weight;
     weight.powers = lds.powers;
@@ -441,7 +441,7 @@ __global__ __launch_bounds__(kSampleThreads) void sample_kernel(const SampleArgs
             return goal;
         };
         float tp;
-        if (sample_threshold<T, true>(lds, row, weight, t, m > 0 ? m * weight(t) : 0, goal_of, [&](float v) { return weight(v); }, tp)) {
+        if (sample_threshold<T, (VECTORS > 8)>(lds, row, weight, t, m > 0 ? m * weight(t) : 0, goal_of, [&](float v) { return weight(v); }, tp)) {
             const unsigned long long w = weight(tp);
             t = tp;
             m = (goal - lds.above + w - 1) / w;
@@ -456,7 +456,7 @@ __global__ __launch_bounds__(kSampleThreads) void sample_kernel(const SampleArgs
     }
     const unsigned long long tie = infinite ? 1 : m > 0 ? weight(t) : 0;
     unsigned long long sum = 0, ties = 0;
-    row.template each<true>([&](float v, int) {
+    row.template each<(VECTORS > 8)>([&](float v, int) {
         if (weight.reaches(v) & (v > t)) sum += weight(v);
         ties += v == t;
     });
