@@ -100,6 +100,9 @@ __device__ __forceinline__ LaAcc la_mma(LaAcc a0, LaAcc a1, LaAcc b0, LaAcc b1, 
     return c;
 }
 
+template <typename P>
+__device__ __forceinline__ LaAcc la_mma(P a, P b, LaAcc c) { return la_mma(a.a, a.b, b.a, b.b, c); }
+
 // The lane's number, of TIGHT kernels as something that the compiler knows nothing of: what is computed from it is computed where
 // it is needed.  (Left to itself it forms every address of a chunk in front of the loop and keeps them all, in scratch memory
 // where registers end.)
@@ -131,6 +134,38 @@ __device__ __forceinline__ LaAcc la_cols(int lane, const float *lds, int stride,
 {
     const float *p = lds + (row0 + 4 * (lane >> 4)) * stride + col0 + (lane & 15);
     return LaAcc{p[0], p[stride], p[2 * stride], p[3 * stride]};
+}
+
+// An operand of 32 steps or features, in two pieces.  bfloat16: eight neighbours 8 g .. 8 g + 7 in a lane, so that rows are read 16
+// bytes at a time (LDS moves 128 bytes a cycle then, 64 in pieces of 8, and was busy for two thirds of the time); float: 4 g ..
+// 4 g + 3 of both halves, whose rows start in different banks.
+template <typename F>
+struct LaPair {
+    F a, b;
+};
+template <typename T>
+constexpr int la_first(int g) { return sizeof(T) == 2 ? 8 * g : 4 * g; }            // where a lane's first piece starts
+template <typename T>
+constexpr int la_second(int g) { return sizeof(T) == 2 ? 8 * g + 4 : 16 + 4 * g; }  // and its second
+
+__device__ __forceinline__ LaPair<LaHalf4> la_rows2(int lane, const bf16 *lds, int stride, int row0, int col0)
+{
+    const LaHalf8 v = *reinterpret_cast<const LaHalf8 *>(lds + (row0 + (lane & 15)) * stride + col0 + 8 * (lane >> 4));
+    return {__builtin_shufflevector(v, v, 0, 1, 2, 3), __builtin_shufflevector(v, v, 4, 5, 6, 7)};
+}
+__device__ __forceinline__ LaPair<LaAcc> la_rows2(int lane, const float *lds, int stride, int row0, int col0)
+{
+    return {la_rows<LaAcc>(lane, lds, stride, row0, col0), la_rows<LaAcc>(lane, lds, stride, row0, col0 + 16)};
+}
+__device__ __forceinline__ LaPair<LaHalf4> la_cols2(int lane, const bf16 *lds, int stride, int row0, int col0)
+{
+    // (rows 8 g instead of 4 g)
+    const int more = row0 + 4 * (lane >> 4);
+    return {la_cols(lane, lds, stride, more, col0), la_cols(lane, lds, stride, more + 4, col0)};
+}
+__device__ __forceinline__ LaPair<LaAcc> la_cols2(int lane, const float *lds, int stride, int row0, int col0)
+{
+    return {la_cols(lane, lds, stride, row0, col0), la_cols(lane, lds, stride, row0 + 16, col0)};
 }
 
 // x as N numbers of the operands' type, each the rounded rest of those before it.
@@ -418,18 +453,18 @@ __device__ __forceinline__ F la_only(F f, int t)
     return f;
 }
 
-// Sum over the steps of the pairs of tiles first .. last of a(part, tile) x b(tile), onto c (rows: steps of the chunk).
-// BAD: something in the chunk is not finite.  Then step by step, and only onto the rows that `meets(row, step)`: what a factor of
+// Sum over the steps of the pairs of tiles first .. last of a2(part, pair) x b2(pair), onto c (rows: steps of the chunk).
+// BAD: something in the chunk is not finite.  Then step by step (a, b: of a tile), and only onto the rows that `meets(row, step)`: what a factor of
 // zero stands for must not turn into NaN.
-template <bool BAD, int N, int TT, typename F, typename A, typename B, typename M>
-__device__ __forceinline__ void la_over_steps(LaAcc &c, int first, int last, A &&a, B &&b, M &&meets)
+template <bool BAD, int N, int TT, typename F, typename A2, typename B2, typename A, typename B, typename M>
+__device__ __forceinline__ void la_over_steps(LaAcc &c, int first, int last, A2 &&a2, B2 &&b2, A &&a, B &&b, M &&meets)
 {
     if constexpr (!BAD) {
 #pragma unroll
         for (int p = 0; p < TT / 2; ++p)
             if (p >= first && p <= last) {
 #pragma unroll
-                for (int n = 0; n < N; ++n) c = la_mma(a(n, 2 * p), a(n, 2 * p + 1), b(2 * p), b(2 * p + 1), c);
+                for (int n = 0; n < N; ++n) c = la_mma(a2(n, p), b2(p), c);
             }
     } else {
         const F zero = {};
@@ -621,8 +656,7 @@ __global__ __launch_bounds__((LaShape<T, D>::THREADS)) void la_walk_kernel(const
                     LaAcc c = {};
 #pragma unroll
                     for (int x = 0; x < D; x += 32)
-                        c = la_mma(la_rows<F>(lane, ks, LD, 16 * tj, x), la_rows<F>(lane, ks, LD, 16 * tj, x + 16), la_rows<F>(lane, qs, LD, 16 * ti, x),
-                                   la_rows<F>(lane, qs, LD, 16 * ti, x + 16), c);
+                        c = la_mma(la_rows2(lane, ks, LD, 16 * tj, x), la_rows2(lane, qs, LD, 16 * ti, x), c);
                     const int i = 16 * ti + i16, j = 16 * tj + 4 * g, part = levels.part[i];
                     const LaAcc f_ij = levels.between(levels.quad(levels.hi, j), levels.quad(levels.lo, j), levels.hi[i], levels.lo[i], -1.0f);
                     const LaParts parts = *reinterpret_cast<const LaParts *>(levels.part + j);
@@ -637,9 +671,9 @@ __global__ __launch_bounds__((LaShape<T, D>::THREADS)) void la_walk_kernel(const
                     for (int m = 0; m < S::INNER; ++m) *reinterpret_cast<F *>(ps + (m * C + i) * LDC + j) = f[m];
                 }
             }
-            F vf[TT];
+            LaPair<F> vf[TT / 2];
 #pragma unroll
-            for (int t = 0; t < TT; ++t) vf[t] = la_cols(lane, vs, LD, 16 * t, 16 * slice);
+            for (int p = 0; p < TT / 2; ++p) vf[p] = la_cols2(lane, vs, LD, 32 * p, 16 * slice);
             if constexpr (OUT) {
                 if (a.kept) {
                     const LaOut<float> to(a.kept + (bh * a.chunks + chunk) * features * la_line(values), features, la_line(values), g, col, la_line(values));
@@ -648,24 +682,27 @@ __global__ __launch_bounds__((LaShape<T, D>::THREADS)) void la_walk_kernel(const
                 }
                 LaAcc o[OT] = {};
 #pragma unroll
-                for (int x = 0; x < DT; x += 2) {
-                    F s0[S::INNER], s1[S::INNER];
+                for (int x = 0; x < D; x += 32) {
+                    // (a state from its sums has their order: 4 g .. 4 g + 3 of two tiles)
+                    LaPair<F> sx[S::INNER];
                     if constexpr (SHARED) {
 #pragma unroll
-                        for (int m = 0; m < S::INNER; ++m) {
-                            s0[m] = la_rows<F>(lane, ss + m * D * LD, LD, 16 * slice, 16 * x);
-                            s1[m] = la_rows<F>(lane, ss + m * D * LD, LD, 16 * slice, 16 * x + 16);
-                        }
+                        for (int m = 0; m < S::INNER; ++m) sx[m] = la_rows2(lane, ss + m * D * LD, LD, 16 * slice, x);
                     } else {
-                        la_split(s[x], s0);
-                        la_split(s[x + 1], s1);
+                        F s0[S::INNER], s1[S::INNER];
+                        la_split(s[x / 16], s0);
+                        la_split(s[x / 16 + 1], s1);
+#pragma unroll
+                        for (int m = 0; m < S::INNER; ++m) sx[m] = {s0[m], s1[m]};
                     }
 #pragma unroll
                     for (int u = 0; u < OT; ++u) {
                         const int t = S::tile(half, u);
-                        const F q0 = la_rows<F>(lane, qs, LD, 16 * t, 16 * x), q1 = la_rows<F>(lane, qs, LD, 16 * t, 16 * x + 16);
+                        LaPair<F> qx;
+                        if constexpr (SHARED) qx = la_rows2(lane, qs, LD, 16 * t, x);
+                        else qx = {la_rows<F>(lane, qs, LD, 16 * t, x), la_rows<F>(lane, qs, LD, 16 * t, x + 16)};
 #pragma unroll
-                        for (int m = 0; m < S::INNER; ++m) o[u] = la_mma(q0, q1, s0[m], s1[m], o[u]);
+                        for (int m = 0; m < S::INNER; ++m) o[u] = la_mma(qx, sx[m], o[u]);
                     }
                 }
                 __syncthreads();
@@ -675,8 +712,9 @@ __global__ __launch_bounds__((LaShape<T, D>::THREADS)) void la_walk_kernel(const
                     const int t = S::tile(half, u);
                     o[u] = la_times(o[u], levels.quad(levels.start, 16 * t + 4 * g));
                     la_over_steps<BAD, S::INNER, TT, F>(
-                        o[u], 0, S::pair_of(u), [&](int m, int j) { return la_rows<F>(lane, ps + m * C * LDC, LDC, 16 * t, 16 * j); },
-                        [&](int j) { return BAD ? la_cols(lane, vs, LD, 16 * j, 16 * slice) : vf[j]; },
+                        o[u], 0, S::pair_of(u), [&](int m, int p) { return la_rows2(lane, ps + m * C * LDC, LDC, 16 * t, 32 * p); },
+                        [&](int p) { return vf[p]; }, [&](int m, int j) { return la_rows<F>(lane, ps + m * C * LDC, LDC, 16 * t, 16 * j); },
+                        [&](int j) { return la_cols(lane, vs, LD, 16 * j, 16 * slice); },
                         [&](int r, int j) { const int i = 16 * t + 4 * g + r; return j <= i && levels.part[j] == levels.part[i]; });
                 }
 #pragma unroll
@@ -687,27 +725,24 @@ __global__ __launch_bounds__((LaShape<T, D>::THREADS)) void la_walk_kernel(const
 #pragma unroll
             for (int t = 0; t < OD; ++t) s[t] = la_times(s[t], decay);
 #pragma unroll
-            for (int t = 0; t < TT; t += 2) {
-                F w[2][S::ADDED];
-                LaAcc factor[2];
-#pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    factor[u] = levels.quad(BACK ? levels.start : levels.end, 16 * (t + u) + 4 * g);
-                    la_split(la_times(la_float(vf[t + u]), factor[u]), w[u]);
-                }
+            for (int p = 0; p < TT / 2; ++p) {
+                const LaAcc one = levels.quad(BACK ? levels.start : levels.end, 32 * p + la_first<T>(g));
+                const LaAcc two = levels.quad(BACK ? levels.start : levels.end, 32 * p + la_second<T>(g));
+                F w1[S::ADDED], w2[S::ADDED];
+                la_split(la_times(la_float(vf[p].a), one), w1);
+                la_split(la_times(la_float(vf[p].b), two), w2);
 #pragma unroll
                 for (int x = 0; x < OD; ++x) {
-                    const int at = 16 * (half * OD + x);
-                    F k0 = la_cols(lane, ks, LD, 16 * t, at), k1 = la_cols(lane, ks, LD, 16 * t + 16, at);
+                    LaPair<F> kx = la_cols2(lane, ks, LD, 32 * p, 16 * (half * OD + x));
                     if constexpr (BAD) {
 #pragma unroll
                         for (int r = 0; r < 4; ++r) {
-                            if (factor[0][r] < 0.0f) k0[r] = 0.0f;
-                            if (factor[1][r] < 0.0f) k1[r] = 0.0f;
+                            if (one[r] < 0.0f) kx.a[r] = 0.0f;
+                            if (two[r] < 0.0f) kx.b[r] = 0.0f;
                         }
                     }
 #pragma unroll
-                    for (int m = 0; m < S::ADDED; ++m) s[x] = la_mma(k0, k1, w[0][m], w[1][m], s[x]);
+                    for (int m = 0; m < S::ADDED; ++m) s[x] = la_mma(kx, LaPair<F>{w1[m], w2[m]}, s[x]);
                 }
             }
         };
@@ -783,7 +818,7 @@ __global__ __launch_bounds__((LaShape<T, D>::THREADS)) void la_back_kernel(const
     struct Sums {
         // (of two chunks: the next one's are written while the decays' gradients of this one are formed)
         float row[2][TT][C], col[2][TT][C];
-        float start[S::SLICES][C], end[S::SLICES][C], through[W];
+        float start[S::SLICES][C], end[S::SLICES][C], through[S::SLICES];
     };
     __shared__ __align__(16) Sums sums;
     __shared__ int bad_chunk[2];
@@ -866,7 +901,7 @@ __global__ __launch_bounds__((LaShape<T, D>::THREADS)) void la_back_kernel(const
         float crossing = 0.0f;
         if (parts == 0) {
 #pragma unroll
-            for (int x = 0; x < W; ++x) crossing += sums.through[x];
+            for (int x = 0; x < S::SLICES; ++x) crossing += sums.through[x];
             crossing *= levels.decay;
         }
         // (the decay of a reset step meets nothing)
@@ -912,11 +947,13 @@ __global__ __launch_bounds__((LaShape<T, D>::THREADS)) void la_back_kernel(const
         const bool bad = bad_chunk[n & 1] != 0;
         if (threadIdx.x == 0) bad_chunk[(n + 1) & 1] = 0;
         // the state in front of the chunk (what lies outside of it: some address inside, zero when it is used)
+        // before[t]: values value_of(t) .. + 3, in the order of the operands that it meets: those in LDS, or E's sums
         LaAcc before[DT] = {};
+        auto value_of = [](int t, int g) { return SHARED ? 32 * (t / 2) + (t % 2 ? la_second<T>(g) : la_first<T>(g)) : 16 * t + 4 * g; };
         auto fetch_state = [&] {
             const float *from = a.kept + (bh * a.chunks + chunk) * features * line + (col < features ? col * line : 0);
 #pragma unroll
-            for (int t = 0; t < DT; ++t) before[t] = *reinterpret_cast<const LaAcc *>(from + (16 * t + 4 * g < line ? 16 * t + 4 * g : 0));
+            for (int t = 0; t < DT; ++t) before[t] = *reinterpret_cast<const LaAcc *>(from + (value_of(t, g) < line ? value_of(t, g) : 0));
         };
         // (behind the last chunk: that one once more)
         auto fetch_next = [&] {
@@ -935,18 +972,14 @@ __global__ __launch_bounds__((LaShape<T, D>::THREADS)) void la_back_kernel(const
         LaAcc dv[OT] = {};
 #pragma unroll
         for (int x = 0; x < D; x += 32) {
-            F e0[S::INNER], e1[S::INNER];
+            LaPair<F> ex[S::INNER];
 #pragma unroll
-            for (int m = 0; m < S::INNER; ++m) {
-                e0[m] = la_cols(lane, es + m * D * LD, LD, x, 16 * slice);
-                e1[m] = la_cols(lane, es + m * D * LD, LD, x + 16, 16 * slice);
-            }
+            for (int m = 0; m < S::INNER; ++m) ex[m] = la_cols2(lane, es + m * D * LD, LD, x, 16 * slice);
 #pragma unroll
             for (int u = 0; u < OT; ++u) {
-                const int t = S::tile(half, u);
-                const F k0 = la_rows<F>(lane, ks, LD, 16 * t, x), k1 = la_rows<F>(lane, ks, LD, 16 * t, x + 16);
+                const LaPair<F> kx = la_rows2(lane, ks, LD, 16 * S::tile(half, u), x);
 #pragma unroll
-                for (int m = 0; m < S::INNER; ++m) dv[u] = la_mma(k0, k1, e0[m], e1[m], dv[u]);
+                for (int m = 0; m < S::INNER; ++m) dv[u] = la_mma(kx, ex[m], dv[u]);
             }
             hold();
         }
@@ -962,10 +995,8 @@ __global__ __launch_bounds__((LaShape<T, D>::THREADS)) void la_back_kernel(const
             LaAcc c = {}, d = {};
 #pragma unroll
             for (int x = 0; x < D; x += 32) {
-                c = la_mma(la_rows<F>(lane, qs, LD, 16 * ti, x), la_rows<F>(lane, qs, LD, 16 * ti, x + 16), la_rows<F>(lane, ks, LD, 16 * tj, x),
-                           la_rows<F>(lane, ks, LD, 16 * tj, x + 16), c);
-                d = la_mma(la_rows<F>(lane, gs, LD, 16 * ti, x), la_rows<F>(lane, gs, LD, 16 * ti, x + 16), la_rows<F>(lane, vs, LD, 16 * tj, x),
-                           la_rows<F>(lane, vs, LD, 16 * tj, x + 16), d);
+                c = la_mma(la_rows2(lane, qs, LD, 16 * ti, x), la_rows2(lane, ks, LD, 16 * tj, x), c);
+                d = la_mma(la_rows2(lane, gs, LD, 16 * ti, x), la_rows2(lane, vs, LD, 16 * tj, x), d);
                 hold();
             }
             const int j = 16 * tj + i16, i = 16 * ti + 4 * g, part = levels.part[j];
@@ -1030,7 +1061,9 @@ __global__ __launch_bounds__((LaShape<T, D>::THREADS)) void la_back_kernel(const
                 const int t = S::tile(half, u);
                 dv[u] = la_times(dv[u], levels.quad(levels.end, 16 * t + 4 * g));
                 la_over_steps<BAD, S::INNER, TT, F>(
-                    dv[u], S::pair_of(u), TT / 2 - 1, [&](int m, int i) { return la_rows<F>(lane, ps + m * C * LDC, LDC, 16 * t, 16 * i); },
+                    dv[u], S::pair_of(u), TT / 2 - 1, [&](int m, int p) { return la_rows2(lane, ps + m * C * LDC, LDC, 16 * t, 32 * p); },
+                    [&](int p) { return la_cols2(lane, gs, LD, 32 * p, 16 * slice); },
+                    [&](int m, int i) { return la_rows<F>(lane, ps + m * C * LDC, LDC, 16 * t, 16 * i); },
                     [&](int i) { return la_cols(lane, gs, LD, 16 * i, 16 * slice); },
                     [&](int r, int i) { return meets(i, 16 * t + 4 * g + r); });
             }
@@ -1044,7 +1077,7 @@ __global__ __launch_bounds__((LaShape<T, D>::THREADS)) void la_back_kernel(const
             LaAcc d[OT] = {};
 #pragma unroll
             for (int x = 0; x < DT; ++x) {
-                const bool there = (col < features) & (16 * x + 4 * g < line);
+                const bool there = (col < features) & (value_of(x, g) < line);
 #pragma unroll
                 for (int r = 0; r < 4; ++r) before[x][r] = there ? before[x][r] : 0.0f;
             }
@@ -1056,46 +1089,42 @@ __global__ __launch_bounds__((LaShape<T, D>::THREADS)) void la_back_kernel(const
 #pragma unroll
                 for (int u = 0; u < OT; ++u) {
                     const int t = S::tile(half, u);
-                    const F g0 = la_rows<F>(lane, gs, LD, 16 * t, 16 * x), g1 = la_rows<F>(lane, gs, LD, 16 * t, 16 * x + 16);
+                    LaPair<F> gx;
+                    if constexpr (SHARED) gx = la_rows2(lane, gs, LD, 16 * t, 16 * x);
+                    else gx = {la_rows<F>(lane, gs, LD, 16 * t, 16 * x), la_rows<F>(lane, gs, LD, 16 * t, 16 * x + 16)};
 #pragma unroll
-                    for (int m = 0; m < S::ADDED; ++m) d[u] = la_mma(g0, g1, s0[m], s1[m], d[u]);
+                    for (int m = 0; m < S::ADDED; ++m) d[u] = la_mma(gx, LaPair<F>{s0[m], s1[m]}, d[u]);
                 }
                 hold();
             }
-            F qf[TT], kf[TT];
+            LaPair<F> qf[TT / 2], kf[TT / 2];
 #pragma unroll
-            for (int t = 0; t < TT; ++t) {
-                qf[t] = la_cols(lane, qs, LD, 16 * t, 16 * slice);
-                kf[t] = la_cols(lane, ks, LD, 16 * t, 16 * slice);
+            for (int p = 0; p < TT / 2; ++p) {
+                qf[p] = la_cols2(lane, qs, LD, 32 * p, 16 * slice);
+                kf[p] = la_cols2(lane, ks, LD, 32 * p, 16 * slice);
             }
-            // <E, S>
+            // <E, S>, where E is in registers
             float sum = 0.0f;
+            if constexpr (!SHARED) {
 #pragma unroll
-            for (int t = 0; t < OD; ++t)
+                for (int t = 0; t < DT; ++t)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) sum += e[t][r] * (S::HALVES == 1 || half == 0 ? before[t][r] : before[(DT - OD) + t][r]);
-            sum = la_sum16(sum);
-            sum += __shfl_xor(sum, 16, 64);
-            sum += __shfl_xor(sum, 32, 64);
-            sums.through[wave] = sum;
-            // (of the wavefront's tile u; the operands are those of all tiles)
-            auto mine = [&](const F (&f)[TT], int u) {
-                if constexpr (S::HALVES == 1) return la_float(f[u]);
-                else return la_float(u == 0 ? (half == 0 ? f[0] : f[1]) : (half == 0 ? f[3] : f[2]));
-            };
+                    for (int r = 0; r < 4; ++r) sum += e[t][r] * before[t][r];
+            }
 #pragma unroll
             for (int u = 0; u < OT; ++u) {
                 const int t = S::tile(half, u), i = 16 * t + 4 * g;
                 const LaAcc to_start = levels.quad(levels.start, i);
                 d[u] = la_times(d[u], to_start);
                 // (a step that a reset parts from the state: zero times what may not be finite)
-                LaAcc at_start = d[u] * mine(qf, u);
+                LaAcc at_start = d[u] * la_float(la_cols(lane, qs, LD, 16 * t, 16 * slice));
 #pragma unroll
                 for (int r = 0; r < 4; ++r) at_start[r] = la_sum16(to_start[r] < 0.0f ? 0.0f : at_start[r]);
                 *reinterpret_cast<LaAcc *>(&sums.start[slice][i]) = at_start;
                 la_over_steps<BAD, S::INNER, TT, F>(
-                    d[u], 0, S::pair_of(u), [&](int m, int j) { return la_cols(lane, ds + m * C * LDC, LDC, 16 * j, 16 * t); },
-                    [&](int j) { return BAD ? la_cols(lane, ks, LD, 16 * j, 16 * slice) : kf[j]; },
+                    d[u], 0, S::pair_of(u), [&](int m, int p) { return la_cols2(lane, ds + m * C * LDC, LDC, 32 * p, 16 * t); },
+                    [&](int p) { return kf[p]; }, [&](int m, int j) { return la_cols(lane, ds + m * C * LDC, LDC, 16 * j, 16 * t); },
+                    [&](int j) { return la_cols(lane, ks, LD, 16 * j, 16 * slice); },
                     [&](int r, int j) { return meets(16 * t + 4 * g + r, j); });
             }
             store(a.d_q, d);
@@ -1105,23 +1134,34 @@ __global__ __launch_bounds__((LaShape<T, D>::THREADS)) void la_back_kernel(const
             LaAcc c[OT] = {};
 #pragma unroll
             for (int x = 0; x < DT; x += 2) {
-                F e0[S::ADDED], e1[S::ADDED];
+                LaPair<F> ex[S::ADDED];
                 if constexpr (SHARED) {
+                    LaAcc one = {}, two = {};
 #pragma unroll
                     for (int m = 0; m < S::ADDED; ++m) {
-                        e0[m] = la_rows<F>(lane, es + m * D * LD, LD, 16 * slice, 16 * x);
-                        e1[m] = la_rows<F>(lane, es + m * D * LD, LD, 16 * slice, 16 * x + 16);
+                        ex[m] = la_rows2(lane, es + m * D * LD, LD, 16 * slice, 16 * x);
+                        one += la_float(ex[m].a);
+                        two += la_float(ex[m].b);
                     }
+                    // (both halves read all of it: <E, S> of the first one)
+                    one *= before[x];
+                    two *= before[x + 1];
+                    sum += ((one[0] + one[1]) + (one[2] + one[3])) + ((two[0] + two[1]) + (two[2] + two[3]));
                 } else {
+                    F e0[S::ADDED], e1[S::ADDED];
                     la_split(e[x], e0);
                     la_split(e[x + 1], e1);
+#pragma unroll
+                    for (int m = 0; m < S::ADDED; ++m) ex[m] = {e0[m], e1[m]};
                 }
 #pragma unroll
                 for (int u = 0; u < OT; ++u) {
                     const int t = S::tile(half, u);
-                    const F v0 = la_rows<F>(lane, vs, LD, 16 * t, 16 * x), v1 = la_rows<F>(lane, vs, LD, 16 * t, 16 * x + 16);
+                    LaPair<F> vx;
+                    if constexpr (SHARED) vx = la_rows2(lane, vs, LD, 16 * t, 16 * x);
+                    else vx = {la_rows<F>(lane, vs, LD, 16 * t, 16 * x), la_rows<F>(lane, vs, LD, 16 * t, 16 * x + 16)};
 #pragma unroll
-                    for (int m = 0; m < S::ADDED; ++m) c[u] = la_mma(v0, v1, e0[m], e1[m], c[u]);
+                    for (int m = 0; m < S::ADDED; ++m) c[u] = la_mma(vx, ex[m], c[u]);
                 }
                 hold();
             }
@@ -1130,42 +1170,43 @@ __global__ __launch_bounds__((LaShape<T, D>::THREADS)) void la_back_kernel(const
                 const int t = S::tile(half, u), j = 16 * t + 4 * g;
                 const LaAcc to_end = levels.quad(levels.end, j);
                 c[u] = la_times(c[u], to_end);
-                LaAcc at_end = c[u] * mine(kf, u);
+                LaAcc at_end = c[u] * la_float(la_cols(lane, ks, LD, 16 * t, 16 * slice));
 #pragma unroll
                 for (int r = 0; r < 4; ++r) at_end[r] = la_sum16(to_end[r] < 0.0f ? 0.0f : at_end[r]);
                 *reinterpret_cast<LaAcc *>(&sums.end[slice][j]) = at_end;
                 la_over_steps<BAD, S::INNER, TT, F>(
-                    c[u], S::pair_of(u), TT / 2 - 1, [&](int m, int i) { return la_rows<F>(lane, ds + m * C * LDC, LDC, 16 * t, 16 * i); },
-                    [&](int i) { return BAD ? la_cols(lane, qs, LD, 16 * i, 16 * slice) : qf[i]; },
+                    c[u], S::pair_of(u), TT / 2 - 1, [&](int m, int p) { return la_rows2(lane, ds + m * C * LDC, LDC, 16 * t, 32 * p); },
+                    [&](int p) { return qf[p]; }, [&](int m, int i) { return la_rows<F>(lane, ds + m * C * LDC, LDC, 16 * t, 16 * i); },
+                    [&](int i) { return la_cols(lane, qs, LD, 16 * i, 16 * slice); },
                     [&](int r, int i) { return meets(i, 16 * t + 4 * g + r); });
             }
             store(a.d_k, c);
+            sum = la_sum16(sum);
+            sum += __shfl_xor(sum, 16, 64);
+            sum += __shfl_xor(sum, 32, 64);
+            if (half == 0) sums.through[slice] = sum;
             hold();
             // E in front of the chunk
 #pragma unroll
             for (int t = 0; t < OD; ++t) e[t] = la_times(e[t], decay);
 #pragma unroll
-            for (int t = 0; t < TT; t += 2) {
-                F w[2][S::ADDED];
-                LaAcc factor[2];
-#pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    factor[u] = levels.quad(levels.start, 16 * (t + u) + 4 * g);
-                    la_split(la_times(la_float(qf[t + u]), factor[u]), w[u]);
-                }
+            for (int p = 0; p < TT / 2; ++p) {
+                const LaAcc one = levels.quad(levels.start, 32 * p + la_first<T>(g)), two = levels.quad(levels.start, 32 * p + la_second<T>(g));
+                F w1[S::ADDED], w2[S::ADDED];
+                la_split(la_times(la_float(qf[p].a), one), w1);
+                la_split(la_times(la_float(qf[p].b), two), w2);
 #pragma unroll
                 for (int x = 0; x < OD; ++x) {
-                    const int at = 16 * (half * OD + x);
-                    F g0 = la_cols(lane, gs, LD, 16 * t, at), g1 = la_cols(lane, gs, LD, 16 * t + 16, at);
+                    LaPair<F> gx = la_cols2(lane, gs, LD, 32 * p, 16 * (half * OD + x));
                     if constexpr (BAD) {
 #pragma unroll
                         for (int r = 0; r < 4; ++r) {
-                            if (factor[0][r] < 0.0f) g0[r] = 0.0f;
-                            if (factor[1][r] < 0.0f) g1[r] = 0.0f;
+                            if (one[r] < 0.0f) gx.a[r] = 0.0f;
+                            if (two[r] < 0.0f) gx.b[r] = 0.0f;
                         }
                     }
 #pragma unroll
-                    for (int m = 0; m < S::ADDED; ++m) e[x] = la_mma(g0, g1, w[0][m], w[1][m], e[x]);
+                    for (int m = 0; m < S::ADDED; ++m) e[x] = la_mma(gx, LaPair<F>{w1[m], w2[m]}, e[x]);
                 }
                 hold();
             }
