@@ -780,13 +780,25 @@ __global__ __launch_bounds__(256) void la_enter_kernel(const LaArgs a)
     for (int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x; at < count; at += (int64_t)gridDim.x * 256) {
         const int64_t bh = at / square;
         float s = from ? from[at] : 0.0f;
-        for (int n = 0; n < a.segments; ++n) {
-            const int64_t segment = BACK ? a.segments - 1 - n : n;
-            float *p = a.segment_state + segment * count + at;
-            const float added = *p, decay = a.segment_decay[segment * heads + bh];
-            const bool cut = a.segment_cut[segment * heads + bh] != 0;
-            *p = s;
-            s = cut ? added : decay * s + added;
+        // (eight segments on their way at once: none waits for the state of the one in front)
+        for (int n = 0; n < a.segments; n += 8) {
+            float added[8] = {}, decay[8] = {};
+            int cut[8] = {};
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                if (n + i >= a.segments) break;
+                const int64_t segment = BACK ? a.segments - 1 - (n + i) : n + i;
+                added[i] = a.segment_state[segment * count + at];
+                decay[i] = a.segment_decay[segment * heads + bh];
+                cut[i] = a.segment_cut[segment * heads + bh];
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                if (n + i >= a.segments) break;
+                const int64_t segment = BACK ? a.segments - 1 - (n + i) : n + i;
+                a.segment_state[segment * count + at] = s;
+                s = cut[i] != 0 ? added[i] : decay[i] * s + added[i];
+            }
         }
     }
 }
