@@ -27,6 +27,9 @@ int check_attention(const bf_linear_attention *p)
     if (p->batch > ((int64_t)1 << 22) || p->heads > ((int64_t)1 << 22) || p->batch * p->heads > ((int64_t)1 << 22))
         return fail(BF_ERR_UNSUPPORTED, "more than 2^22 sequences and heads are not supported");
     if (p->steps > ((int64_t)1 << 31)) return fail(BF_ERR_UNSUPPORTED, "more than 2^31 steps are not supported");
+    // (a chunk's rows of a result lie within 2^31 bytes of each other)
+    if (p->heads * std::max(p->features, p->values) > ((int64_t)1 << 22))
+        return fail(BF_ERR_UNSUPPORTED, "steps of more than 2^22 features or values are not supported");
     for (int i = 0; i < 3; ++i)
         if (p->q_stride[i] < 0 || p->k_stride[i] < 0 || p->v_stride[i] < 0 || p->grad_stride[i] < 0 || p->decay_stride[i] < 0)
             return fail(BF_ERR_INVALID, "strides must be non-negative");

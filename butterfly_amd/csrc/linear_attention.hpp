@@ -299,13 +299,16 @@ struct LaPiece {
 
 // What the products take from a chunk's decays.  Sums of log decays, to the base 2, as two floats of together 48 bits: their
 // differences keep the bits of the decays between two steps, whatever the steps in front have summed up to.  part: resets
-// so far.  start, end: what steps meet of the states in front of and behind the chunk (scale exp(L_i), exp(L_C - L_j)), -1 where a
-// reset lies between.
+// so far.  start, end: what steps meet of the states in front of and behind the chunk (scale exp(L_i), exp(L_C - L_j)),
+// kNothing where a reset lies between.
+constexpr float kNothing = -0.0f;
+__device__ __forceinline__ bool la_nothing(float factor) { return __builtin_bit_cast(int, factor) == INT32_MIN; }
+
 template <int C>
 struct LaLevels {
     float hi[C], lo[C], start[C], end[C];
     int part[C];
-    float decay;   // over the whole chunk; -1: a reset lies within
+    float decay;   // over the whole chunk; kNothing: a reset lies within
 
     __device__ __forceinline__ LaAcc quad(const float (&v)[C], int at) const { return *reinterpret_cast<const LaAcc *>(v + at); }
     // scale exp(L_i - L_j) for four neighbouring steps i or j and one other one
@@ -318,11 +321,11 @@ struct LaLevels {
     }
 };
 
-// (-1: nothing, whatever x is)
+// (kNothing: zero, whatever x is)
 __device__ __forceinline__ LaAcc la_times(LaAcc x, LaAcc factor)
 {
 #pragma unroll
-    for (int r = 0; r < 4; ++r) x[r] = factor[r] < 0.0f ? 0.0f : x[r] * factor[r];
+    for (int r = 0; r < 4; ++r) x[r] = la_nothing(factor[r]) ? 0.0f : x[r] * factor[r];
     return x;
 }
 __device__ __forceinline__ LaAcc la_times(LaAcc x, float factor) { return la_times(x, LaAcc{factor, factor, factor, factor}); }
@@ -394,10 +397,10 @@ __device__ __forceinline__ void la_levels(LaLevels<C> &out, float log_decay, boo
     if (lane < C) {
         out.hi[lane] = hi;
         out.lo[lane] = (float)(level - (double)hi);
-        out.start[lane] = part == 0 ? scale * from_start : -1.0f;
-        out.end[lane] = part == parts ? to_end : -1.0f;
+        out.start[lane] = part == 0 ? scale * from_start : kNothing;
+        out.end[lane] = part == parts ? to_end : kNothing;
         out.part[lane] = part;
-        if (lane == C - 1) out.decay = part == 0 ? from_start : -1.0f;
+        if (lane == C - 1) out.decay = part == 0 ? from_start : kNothing;
     }
 }
 
@@ -737,8 +740,8 @@ __global__ __launch_bounds__((LaShape<T, D>::THREADS)) void la_walk_kernel(const
                     if constexpr (BAD) {
 #pragma unroll
                         for (int r = 0; r < 4; ++r) {
-                            if (one[r] < 0.0f) kx.a[r] = 0.0f;
-                            if (two[r] < 0.0f) kx.b[r] = 0.0f;
+                            if (la_nothing(one[r])) kx.a[r] = 0.0f;
+                            if (la_nothing(two[r])) kx.b[r] = 0.0f;
                         }
                     }
 #pragma unroll
@@ -1131,7 +1134,7 @@ __global__ __launch_bounds__((LaShape<T, D>::THREADS)) void la_back_kernel(const
                 // (a step that a reset parts from the state: zero times what may not be finite)
                 LaAcc at_start = d[u] * la_float(la_cols(lane, qs, LD, 16 * t, 16 * slice));
 #pragma unroll
-                for (int r = 0; r < 4; ++r) at_start[r] = la_sum16(to_start[r] < 0.0f ? 0.0f : at_start[r]);
+                for (int r = 0; r < 4; ++r) at_start[r] = la_sum16(la_nothing(to_start[r]) ? 0.0f : at_start[r]);
                 *reinterpret_cast<LaAcc *>(&sums.start[slice][i]) = at_start;
                 la_over_steps<BAD, S::INNER, TT, F>(
                     d[u], 0, S::pair_of(u), [&](int m, int p) { return la_cols2(lane, ds + m * C * LDC, LDC, 32 * p, 16 * t); },
@@ -1184,7 +1187,7 @@ __global__ __launch_bounds__((LaShape<T, D>::THREADS)) void la_back_kernel(const
                 c[u] = la_times(c[u], to_end);
                 LaAcc at_end = c[u] * la_float(la_cols(lane, ks, LD, 16 * t, 16 * slice));
 #pragma unroll
-                for (int r = 0; r < 4; ++r) at_end[r] = la_sum16(to_end[r] < 0.0f ? 0.0f : at_end[r]);
+                for (int r = 0; r < 4; ++r) at_end[r] = la_sum16(la_nothing(to_end[r]) ? 0.0f : at_end[r]);
                 *reinterpret_cast<LaAcc *>(&sums.end[slice][j]) = at_end;
                 la_over_steps<BAD, S::INNER, TT, F>(
                     c[u], S::pair_of(u), TT / 2 - 1, [&](int m, int p) { return la_rows2(lane, ds + m * C * LDC, LDC, 16 * t, 32 * p); },
@@ -1213,8 +1216,8 @@ __global__ __launch_bounds__((LaShape<T, D>::THREADS)) void la_back_kernel(const
                     if constexpr (BAD) {
 #pragma unroll
                         for (int r = 0; r < 4; ++r) {
-                            if (one[r] < 0.0f) gx.a[r] = 0.0f;
-                            if (two[r] < 0.0f) gx.b[r] = 0.0f;
+                            if (la_nothing(one[r])) gx.a[r] = 0.0f;
+                            if (la_nothing(two[r])) gx.b[r] = 0.0f;
                         }
                     }
 #pragma unroll

@@ -426,7 +426,7 @@ int bf_linear_xent_bw(const bf_linear_xent *p, const void *weight, const float *
  * heads / groups neighbouring heads share queries and keys.  The last dimension is adjacent (log_decay: the strides
  * say it all), the others have the given strides; o and every gradient are dense, states dense (batch, heads,
  * features, values).  reset (bytes, (batch, steps), may be NULL): where set, S_{t-1} counts as zero whatever it is
- * (a packed document starts).  features and values: 1 to 128.                                    */
+ * (a packed document starts).  features and values: 1 to 128; heads times either: up to 2^22.     */
 typedef struct bf_linear_attention {
     int32_t dtype; /* BF_F32 or BF_BF16: q, k, v, o and their gradients */
     int64_t batch, steps, heads, groups, features, values;
@@ -477,7 +477,7 @@ int bf_rotary_apply(const bf_rotary *p, const void *x, const int64_t *positions,
  * w_i = exp((z_i - max z) / temperature): of the top_k largest logits (<= 0: all; ties: lowest indexes first) the likeliest
  * ones until their sum reaches top_p of all of theirs (>= 1: all; at least one), of those the ones with w_i >= min_p (<= 0: all;
  * at most 1); the token is the first index whose cumulated w, in the order of indexes, exceeds uniform * total (uniform in [0, 1)).
- * temperature <= 0: the first of the largest logits.  NaN counts as -inf, which is never drawn; a row of nothing else gives
+ * temperature <= 0: the first of the largest logits; others count as between 2^-100 and 2^100.  NaN settings: none.  NaN counts as -inf, which is never drawn; a row of nothing else gives
  * -1; with +inf among the logits only those are drawn.  w is rounded to whole multiples of 2^-44: the same token at every call.
  * Up to 2^19 entries. */
 typedef struct bf_sample {

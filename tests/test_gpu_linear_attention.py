@@ -376,3 +376,25 @@ def test_refusals():
     g, = torch.autograd.grad(o.sum(), args[0], create_graph=True)
     with pytest.raises(RuntimeError, match="no second derivative"):
         torch.autograd.grad(g.sum(), args[0])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("scale", [-0.4, 0.0])
+def test_scales_of_any_sign(scale, dtype):
+    v = make(2, 150, 2, 1, 40, 24, dtype)
+    reset = torch.zeros(2, 150, dtype=torch.bool)
+    reset[1, 70] = True
+    compare(device(v, scale, reset), reference(v, scale, reset), dtype)
+
+
+def test_states_at_any_address():
+    """One step of a state that does not start at 16 bytes, and of one that does."""
+    v = make(3, 1, 2, 2, 8, 12, torch.float32)
+    args = [v[k].cuda()[:, 0] for k in NAMES[:4]]
+    room = torch.empty(3 * 2 * 8 * 12 + 1, device="cuda")
+    want = reference(v, 0.5)
+    for start in (0, 1):
+        state = room[start:start + 3 * 2 * 8 * 12].view(3, 2, 8, 12).copy_(v["state"])
+        o = tb.linear_attention_step(*args, state, 0.5)
+        assert (o.cpu() - want["o"][:, 0]).abs().max() <= 1e-5 * want["o"].abs().max()
+        assert (state.cpu() - want["last"]).abs().max() <= 1e-5 * want["last"].abs().max()
