@@ -380,9 +380,8 @@ __global__ __launch_bounds__(kSampleThreads) void sample_kernel(const SampleArgs
         if (threadIdx.x == 0) a.token[r] = -1;
         return;
     }
-    // (beyond 2^100 the differences of all finite logits are nearly nothing, and below what a float range holds)
-    const double temperature = fmin(a.temperature ? (double)a.temperature[r] : a.temperature_all, 0x1p100);
-    if (!(temperature > 0.0)) {
+    const double asked = a.temperature ? (double)a.temperature[r] : a.temperature_all;
+    if (!(asked > 0.0)) {
         // the first of the largest
         int first = a.vocab;
         row.template each<false>([&](float v, int at) { if (v == high) first = min(first, at); });
@@ -412,6 +411,8 @@ __global__ __launch_bounds__(kSampleThreads) void sample_kernel(const SampleArgs
     SampleWeight<T> weight;
     weight.powers = lds.powers;
     weight.top = infinite ? 0.0f : high;
+    // (between 2^-100 and 2^100: what is formed of it stays within the range of floats)
+    const double temperature = fmin(fmax(asked, 0x1p-100), 0x1p100);
     const double per_nat = kSampleFine * 1.4426950408889634 / temperature;
     weight.high = (float)per_nat;
     weight.low = (float)(per_nat - (double)weight.high);

@@ -14,7 +14,8 @@ def sample(logits, uniform, temperature=None, top_k=None, top_p=None, min_p=None
     likeliest ones until their sum reaches ``top_p`` of it (at least one), of those the ones with ``w >= min_p`` (at most 1); the
     token is the first index whose cumulated ``w``, in the order of indexes, exceeds ``uniform * total``.  Settings are
     a number for all rows or a tensor (*) (float32, ``top_k`` int64); ``None``, ``top_k <= 0``, ``top_p >= 1`` and
-    ``min_p <= 0`` leave a filter out.  ``temperature <= 0``: the first of the largest logits.
+    ``min_p <= 0`` leave a filter out.  ``temperature <= 0``: the first of the largest logits; others count as between 2^-100 and 2^100.
+    A setting that is NaN is none (a temperature: 0).
 
     NaN counts as -inf, and -inf is never drawn; a row of nothing else gives -1.  Where +inf is among the logits, only those
     are drawn.  On the device weights are whole multiples of 2^-44 (the same token at every call), and up to
@@ -39,7 +40,7 @@ def _host_sample(logits, uniform, settings):
         for s, kind in zip(settings, (torch.float64, torch.int64, torch.float64, torch.float64)))
     ordered, order = torch.sort(x, dim=1, descending=True, stable=True)
     greedy = ~(temperature > 0)
-    w = torch.exp((ordered - ordered[:, :1]) / torch.where(greedy, 1.0, temperature))
+    w = torch.exp((ordered - ordered[:, :1]) / torch.where(greedy, 1.0, temperature).clamp(2.0 ** -100, 2.0 ** 100))
     w = torch.where(ordered == ordered[:, :1], 1.0, torch.where(ordered == -torch.inf, 0.0, w))
     w = torch.where(ordered[:, :1] == -torch.inf, 0.0, w)
     keep = (torch.arange(entries) < torch.where(top_k > 0, top_k, entries)) & (w > 0)
@@ -48,7 +49,7 @@ def _host_sample(logits, uniform, settings):
     before[:, 0] = 0.0
     keep &= (before < top_p.clamp(min=0.0) * total) | ~(top_p < 1.0)
     keep[:, 0] |= w[:, 0] > 0
-    keep &= w >= min_p.clamp(max=1.0)
+    keep &= ~(w < min_p.clamp(max=1.0))
     kept = torch.zeros_like(w).scatter_(1, order, torch.where(keep, w, 0.0))
     running = kept.cumsum(1)
     u = torch.nan_to_num(uniform.reshape(-1, 1).to(torch.float64)).clamp(0.0, 1.0)

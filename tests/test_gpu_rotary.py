@@ -113,3 +113,14 @@ def test_captured_with_positions_that_move():
         graph.replay()
         torch.cuda.synchronize()
         check(y, reference(x, positions, frequencies, False, 1.0), torch.float32)
+
+
+@pytest.mark.parametrize("lead", [(), (5,), (2, 3, 4), (0, 3)])
+def test_any_number_of_dimensions_in_front(lead):
+    gen = torch.Generator().manual_seed(1)
+    x, positions = torch.randn(*lead, 3, 10, generator=gen), torch.randint(0, 1000, lead, generator=gen)
+    frequencies, _ = tb.rotary_frequencies(8)
+    got, want = tb.rotary(x.cuda(), positions.cuda(), frequencies.cuda()), tb.rotary(x.double(), positions, frequencies)
+    assert got.shape == x.shape
+    # (a sum of two products whose factors and whose sum are off by 2^-24 each, the angle by 2^-24 of a half turn)
+    assert x.numel() == 0 or float((got.cpu() - want).abs().max()) <= 8 * 2.0 ** -24 * float(x.abs().max())

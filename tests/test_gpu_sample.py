@@ -175,3 +175,19 @@ def test_refusals():
                        ("shape", lambda: tb.sample(x[:, :0], u)), ("2\\^19", lambda: tb.sample(torch.zeros(1, (1 << 19) + 1, device="cuda"), u[:1]))):
         with pytest.raises(RuntimeError, match=text):
             call()
+
+
+def test_settings_at_their_ends():
+    logits = torch.tensor([[0.0, 1.0, 3.0, 2.0]] * 4)
+    u = torch.tensor([0.01, 0.3, 0.6, 0.99])
+    for filters in ({"min_p": math.nan}, {"top_p": math.nan}, {"temperature": math.nan}, {"temperature": 1e-300}, {"temperature": 1e-38},
+                    {"temperature": math.inf}, {"temperature": 1e30, "top_p": 0.6}, {"temperature": 1e-40, "top_p": 0.5, "min_p": 0.1},
+                    {"temperature": -math.inf}, {"top_k": 1 << 62}, {"top_k": -(1 << 62)}, {"top_p": -1.0}, {"min_p": math.inf}):
+        assert tb.sample(logits.cuda(), u.cuda(), **filters).tolist() == tb.sample(logits, u, **filters).tolist(), filters
+
+
+def test_a_row_without_more():
+    """Logits of one dimension, a random number of none."""
+    logits = torch.randn(77, generator=torch.Generator().manual_seed(3))
+    token = tb.sample(logits.cuda(), torch.tensor(0.7, device="cuda"), top_k=torch.tensor(9, device="cuda"))
+    assert token.shape == () and int(token) == int(tb.sample(logits, torch.tensor(0.7), top_k=9))

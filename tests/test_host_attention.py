@@ -185,3 +185,23 @@ def test_model_with_heads():
     assert m.generate(tokens, torch.rand(2, 4), 0.8, top_k=5).shape == (2, 4)
     with pytest.raises(ValueError, match="multiple"):
         ButterflyLM(50, 18, 1, heads=2)
+
+
+def test_c_abi_refuses_steps_that_are_too_wide():
+    from butterfly_amd import _capi
+    L, null, one = _capi.lib(), ctypes.c_void_p(0), ctypes.c_void_p(256)   # (never dereferenced: every call is refused on the host)
+    for sizes in (dict(features=128, values=1), dict(features=1, values=128)):
+        a = _capi.LinearAttention(dtype=2, batch=1, steps=10, heads=(1 << 15) + 2, groups=2, scale=1.0, **sizes)
+        assert L.bf_linear_attention_kept_bytes(ctypes.byref(a)) == _capi.SIZE_INVALID
+        assert L.bf_linear_attention_fw(ctypes.byref(a), one, one, one, one, null, null, one, null, null, 0, one, 1 << 40, null) == -2
+        assert b"2^22" in L.bf_last_error()
+        a.heads = 1 << 15
+        # (rows of the states are whole quads of values)
+        assert L.bf_linear_attention_kept_bytes(ctypes.byref(a)) == (1 << 15) * sizes["features"] * max(4, sizes["values"]) * 4
+
+
+def test_sample_settings_at_their_ends():
+    logits, u = torch.tensor([[0.0, 1.0, 3.0, 2.0]]), torch.tensor([0.01])
+    assert int(tb.sample(logits, u, min_p=math.nan)) == int(tb.sample(logits, u, top_p=math.nan)) == int(tb.sample(logits, u)) == 0
+    assert int(tb.sample(logits, u, temperature=math.nan)) == int(tb.sample(logits, u, temperature=1e-300)) == 2
+    assert int(tb.sample(logits, torch.tensor([0.3]), temperature=math.inf)) == 1
