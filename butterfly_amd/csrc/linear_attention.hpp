@@ -1163,9 +1163,12 @@ __global__ __launch_bounds__((LaShape<T, D>::THREADS)) void la_back_kernel(const
                     two *= before[x + 1];
                     sum += ((one[0] + one[1]) + (one[2] + one[3])) + ((two[0] + two[1]) + (two[2] + two[3]));
                 } else {
+                    // (as something new: the numbers split off for dV would be kept for this in registers that there are not)
+                    LaAcc here = e[x], next = e[x + 1];
+                    asm volatile("" : "+v"(here), "+v"(next));
                     F e0[S::ADDED], e1[S::ADDED];
-                    la_split(e[x], e0);
-                    la_split(e[x + 1], e1);
+                    la_split(here, e0);
+                    la_split(next, e1);
 #pragma unroll
                     for (int m = 0; m < S::ADDED; ++m) ex[m] = {e0[m], e1[m]};
                 }
