@@ -471,11 +471,13 @@ __device__ __forceinline__ void la_over_steps(LaAcc &c, int first, int last, A2 
             }
     } else {
         const F zero = {};
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll 1
         for (int t = 32 * first; t < 32 * last + 32; ++t) {
+            const int lane = la_lane<true>();
             LaAcc d = {};
 #pragma unroll 1
-            for (int n = 0; n < N; ++n) d = la_mma(la_only(a(n, t >> 4), t), zero, la_only(b(t >> 4), t), zero, d);
+            for (int n = 0; n < N; ++n) d = la_mma(la_only(a(lane, n, t >> 4), t), zero, la_only(b(lane, t >> 4), t), zero, d);
 #pragma unroll
             for (int r = 0; r < 4; ++r)
                 if (meets(r, t)) c[r] += d[r];
@@ -716,8 +718,8 @@ __global__ __launch_bounds__((LaShape<T, D>::THREADS)) void la_walk_kernel(const
                     o[u] = la_times(o[u], levels.quad(levels.start, 16 * t + 4 * g));
                     la_over_steps<BAD, S::INNER, TT, F>(
                         o[u], 0, S::pair_of(u), [&](int m, int p) { return la_rows2(lane, ps + m * C * LDC, LDC, 16 * t, 32 * p); },
-                        [&](int p) { return vf[p]; }, [&](int m, int j) { return la_rows<F>(lane, ps + m * C * LDC, LDC, 16 * t, 16 * j); },
-                        [&](int j) { return la_cols(lane, vs, LD, 16 * j, 16 * slice); },
+                        [&](int p) { return vf[p]; }, [&](int lane, int m, int j) { return la_rows<F>(lane, ps + m * C * LDC, LDC, 16 * t, 16 * j); },
+                        [&](int lane, int j) { return la_cols(lane, vs, LD, 16 * j, 16 * slice); },
                         [&](int r, int j) { const int i = 16 * t + 4 * g + r; return j <= i && levels.part[j] == levels.part[i]; });
                 }
 #pragma unroll
@@ -1078,8 +1080,8 @@ __global__ __launch_bounds__((LaShape<T, D>::THREADS)) void la_back_kernel(const
                 la_over_steps<BAD, S::INNER, TT, F>(
                     dv[u], S::pair_of(u), TT / 2 - 1, [&](int m, int p) { return la_rows2(lane, ps + m * C * LDC, LDC, 16 * t, 32 * p); },
                     [&](int p) { return la_cols2(lane, gs, LD, 32 * p, 16 * slice); },
-                    [&](int m, int i) { return la_rows<F>(lane, ps + m * C * LDC, LDC, 16 * t, 16 * i); },
-                    [&](int i) { return la_cols(lane, gs, LD, 16 * i, 16 * slice); },
+                    [&](int lane, int m, int i) { return la_rows<F>(lane, ps + m * C * LDC, LDC, 16 * t, 16 * i); },
+                    [&](int lane, int i) { return la_cols(lane, gs, LD, 16 * i, 16 * slice); },
                     [&](int r, int i) { return meets(i, 16 * t + 4 * g + r); });
             }
             {
@@ -1138,8 +1140,8 @@ __global__ __launch_bounds__((LaShape<T, D>::THREADS)) void la_back_kernel(const
                 *reinterpret_cast<LaAcc *>(&sums.start[slice][i]) = at_start;
                 la_over_steps<BAD, S::INNER, TT, F>(
                     d[u], 0, S::pair_of(u), [&](int m, int p) { return la_cols2(lane, ds + m * C * LDC, LDC, 32 * p, 16 * t); },
-                    [&](int p) { return kf[p]; }, [&](int m, int j) { return la_cols(lane, ds + m * C * LDC, LDC, 16 * j, 16 * t); },
-                    [&](int j) { return la_cols(lane, ks, LD, 16 * j, 16 * slice); },
+                    [&](int p) { return kf[p]; }, [&](int lane, int m, int j) { return la_cols(lane, ds + m * C * LDC, LDC, 16 * j, 16 * t); },
+                    [&](int lane, int j) { return la_cols(lane, ks, LD, 16 * j, 16 * slice); },
                     [&](int r, int j) { return meets(16 * t + 4 * g + r, j); });
             }
             store(a.d_q, d);
@@ -1194,8 +1196,8 @@ __global__ __launch_bounds__((LaShape<T, D>::THREADS)) void la_back_kernel(const
                 *reinterpret_cast<LaAcc *>(&sums.end[slice][j]) = at_end;
                 la_over_steps<BAD, S::INNER, TT, F>(
                     c[u], S::pair_of(u), TT / 2 - 1, [&](int m, int p) { return la_rows2(lane, ds + m * C * LDC, LDC, 16 * t, 32 * p); },
-                    [&](int p) { return qf[p]; }, [&](int m, int i) { return la_rows<F>(lane, ds + m * C * LDC, LDC, 16 * t, 16 * i); },
-                    [&](int i) { return la_cols(lane, qs, LD, 16 * i, 16 * slice); },
+                    [&](int p) { return qf[p]; }, [&](int lane, int m, int i) { return la_rows<F>(lane, ds + m * C * LDC, LDC, 16 * t, 16 * i); },
+                    [&](int lane, int i) { return la_cols(lane, qs, LD, 16 * i, 16 * slice); },
                     [&](int r, int i) { return meets(i, 16 * t + 4 * g + r); });
             }
             store(a.d_k, c);
