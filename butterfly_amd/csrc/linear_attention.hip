@@ -59,13 +59,14 @@ size_t rounded(size_t bytes) { return (bytes + 255) / 256 * 256; }
 
 // Sequences times heads are one workgroup each, a compute unit's (registers and LDS hold no second one).  Fewer than half of the 256
 // are cut into as many segments as fill them, no more: 10 heads of 65537 steps in 26 segments leave four workgroups for
-// a second round and took twice the time of 25.
+// a second round and took twice the time of 25.  Segments of two chunks at least: 16 heads of 256 steps forward and backward 73 us in two
+// segments, 86 in one (float; bfloat16 57 and 58); of 1024 steps 80 in eight, 303 in one.
 AttentionPlan plan(const bf_linear_attention *p, bool back)
 {
     AttentionPlan r;
     const int64_t heads = p->batch * p->heads;
     r.chunks = r.segment_chunks = chunk_count(p);
-    if (heads <= 128 && r.chunks > 4) {
+    if (heads <= 128 && r.chunks > 2) {
         const int64_t wanted = std::min<int64_t>(256 / heads, (r.chunks + 1) / 2);
         r.segment_chunks = (r.chunks + wanted - 1) / wanted;
         r.segments = (int)((r.chunks + r.segment_chunks - 1) / r.segment_chunks);

@@ -51,10 +51,12 @@ extern "C" int bf_rotary_apply(const bf_rotary *p, const void *x, const int64_t 
     a.rotated = (int)p->rotated;
     a.magnitude = (float)p->magnitude;
     a.back = back != 0;
-    // some four items a thread where there are enough for 1024 workgroups, fewer otherwise
+    // Two items a thread where there are enough for 1024 workgroups, one otherwise.  The two large cases of rotary.hpp: 23.8 and 107 us;
+    // with four 29.2 and 126, with one 24.2 and 130 (a token of 130 items leaves half of the threads idle); 64 tokens x 32 heads
+    // with one 3.5, with four 6.0.
     const int pairs = a.rotated / 2, rest = a.features - a.rotated;
     const int64_t items = p->interleaved ? (a.features + 7) / 8 : (pairs + 7) / 8 + (rest + 7) / 8;
-    const int64_t each = std::max<int64_t>(256, std::min<int64_t>(1024, a.tokens * a.heads * items / 1024));
+    const int64_t each = std::max<int64_t>(256, std::min<int64_t>(512, a.tokens * a.heads * items / 1024));
     a.heads_each = (int)std::max<int64_t>(1, std::min<int64_t>(a.heads, each / items));
     a.head_parts = (a.heads + a.heads_each - 1) / a.heads_each;
     a.tokens_each = (int)std::max<int64_t>(1, std::min<int64_t>(each / (items * a.heads_each), pairs > 0 ? kRotaryTable / pairs : each));

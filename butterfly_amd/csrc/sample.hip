@@ -30,6 +30,8 @@ void launch(const SampleArgs &a, int64_t rows, hipStream_t s)
 {
     const dim3 grid((unsigned)rows), threads(kSampleThreads);
     const int64_t held = (int64_t)kSampleThreads * (16 / sizeof(T));   // entries that one piece a thread holds
+    // The fewest pieces that hold the row: a pass goes through all of them, whether the row fills them or not (64 rows of 30001 floats in
+    // 8 pieces 34.6 us, in 16 of them 45.7).
     if (a.vocab <= held) sample_kernel<T, 1><<<grid, threads, 0, s>>>(a);
     else if (a.vocab <= 2 * held) sample_kernel<T, 2><<<grid, threads, 0, s>>>(a);
     else if (a.vocab <= 4 * held) sample_kernel<T, 4><<<grid, threads, 0, s>>>(a);
