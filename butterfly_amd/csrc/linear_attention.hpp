@@ -20,15 +20,15 @@
 // inputs as they are; float factors as several bfloat16 numbers that add up to them: three (24 bits) for what is added
 // to a state, two (16 bits) for states and for the products' inner factors Q K^T . D, dO V^T . D (the results are rounded to
 // 8 bits; one number would leave errors of the size of that rounding).  The decays' gradients are floats: what they are summed
-// from, b dO S^T and w V E^T, takes S and E as three numbers as well (two: 287 instead of 302 us and 735 instead of 753 for the
+// from, b dO S^T and w V E^T, takes S and E as three numbers as well (two: 287 instead of 300 us and 735 instead of 765 for the
 // backward kernels below, and decays' gradients off by 2e-6 instead of 3e-7).  An operand of a product over 32 steps or features is two
 // pieces of 4 elements in a lane (LaPair); a state that is taken from sums keeps their order, 4 g .. 4 g + 3 (g: lane / 16)
 // of two neighbouring tiles, and so does what it meets, so that sums become operands without leaving their lane.
 //
 // Measured, one workgroup a compute unit, 64 x 64 states and 128 x 128 ones:
-//   16 x 2048 steps, 16 heads, bfloat16       forward 132 us                          backward 302
+//   16 x 2048 steps, 16 heads, bfloat16       forward 132 us                          backward 300
 //    8 x 1001 steps, 16 heads, float          forward 27 + 5 + 60                     backward 27 + 5 + 123
-//    1 x 65537 steps, 10 heads of 100         forward 135 + 8 + 385                   backward 139 + 9 + 780
+//    1 x 65537 steps, 10 heads of 100         forward 140 + 8 + 390                   backward 140 + 9 + 765
 // (sums of a segment, states between segments, outputs).  The first one moves 403 MB forward, 3.1 TB/s, and 604 MB backward, 2.0: it
 // is bound by the chunk's own chain of products (LDS moves data for 59% and 55% of the cycles, the vector unit issues for 46%
 // and 50%, the matrix unit for 11%; three or four barriers a chunk between them), with two wavefronts a SIMD to hide each other.
