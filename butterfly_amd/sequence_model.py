@@ -137,7 +137,7 @@ class ButterflyLM(nn.Module):
             if t > 0:
                 logits = self.step(tokens[-1], states)
             tokens.append(sample(logits, uniform[:, t], temperature, top_k, top_p, min_p))
-        return torch.stack(tokens, 1)
+        return torch.stack(tokens, 1) if tokens else prompt[:, :0]
 
     def empty_states(self, batch):
         return [mixer.empty_state(batch, self.embedding.device) for mixer in self.mixers]

@@ -205,3 +205,8 @@ def test_sample_settings_at_their_ends():
     assert int(tb.sample(logits, u, min_p=math.nan)) == int(tb.sample(logits, u, top_p=math.nan)) == int(tb.sample(logits, u)) == 0
     assert int(tb.sample(logits, u, temperature=math.nan)) == int(tb.sample(logits, u, temperature=1e-300)) == 2
     assert int(tb.sample(logits, torch.tensor([0.3]), temperature=math.inf)) == 1
+
+
+def test_nothing_to_generate():
+    model = tb.sequence_model.ButterflyLM(20, 16, 1, heads=2).eval()
+    assert model.generate(torch.tensor([[1, 2, 3]]), torch.zeros(1, 0)).shape == (1, 0)
