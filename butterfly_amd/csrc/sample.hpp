@@ -48,6 +48,7 @@ struct SampleLds {
     unsigned long long counts[kSampleWaves];
     unsigned long long above;
     float few[kSampleFew], threshold;
+    float lowest;   // no entry below it has a weight
     int at, number;
 };
 
@@ -324,12 +325,12 @@ __device__ __forceinline__ bool sample_threshold(SampleLds &lds, const Row &row,
     return true;
 }
 
-// The largest value whose weight is below `least` (of those that a weight reaches).
+// The largest value whose weight is below `least`, of those from lds.lowest on; the value in front of that one where none is.
 template <typename T>
-__device__ __forceinline__ float sample_below(const SampleWeight<T> &weight, unsigned long long least)
+__device__ __forceinline__ float sample_below(const SampleLds &lds, const SampleWeight<T> &weight, unsigned long long least)
 {
     // keys low .. high - 1 are unknown, those from high on are not below; 1024 of them at a time
-    uint32_t low = sample_key<T>(weight.top - weight.range), high = sample_key<T>(weight.top);
+    uint32_t low = sample_key<T>(lds.lowest), high = sample_key<T>(weight.top);
     while (low < high) {
         const uint32_t step = (high - low) / kSampleThreads + 1, key = low + threadIdx.x * step;
         const bool below = key < high && key >= low && weight(sample_value<T>(key)) < least;
@@ -392,6 +393,11 @@ __global__ __launch_bounds__(kSampleThreads) void sample_kernel(const SampleArgs
         }
         return;
     }
+    // (between 2^-100 and 2^100: what is formed of it stays within the range of floats)
+    const double temperature = fmin(fmax(asked, 0x1p-100), 0x1p100);
+    const float far = (float)(temperature * ((kSampleBits + 2) * 0.6931471805599453));
+    // (the lowest entry itself, where it is not too far: high - low is rounded, and high less that may lie above it)
+    if (threadIdx.x == 0) lds.lowest = high - low <= far ? low : high - far;
     // the table: 2^(i / 64) 2^(j / 4096)
     if (threadIdx.x < 128) {
         const int i = threadIdx.x & 63;
@@ -407,12 +413,10 @@ __global__ __launch_bounds__(kSampleThreads) void sample_kernel(const SampleArgs
     SampleWeight<T> weight;
     weight.powers = lds.powers;
     weight.top = infinite ? 0.0f : high;
-    // (between 2^-100 and 2^100: what is formed of it stays within the range of floats)
-    const double temperature = fmin(fmax(asked, 0x1p-100), 0x1p100);
     const double per_nat = kSampleFine * 1.4426950408889634 / temperature;
     weight.high = (float)per_nat;
     weight.low = (float)(per_nat - (double)weight.high);
-    weight.range = infinite ? -1.0f : fminf(high - low, (float)(temperature * ((kSampleBits + 2) * 0.6931471805599453)));
+    weight.range = infinite ? -1.0f : fminf(high - low, far);
     const double min_p = a.min_p ? (double)a.min_p[r] : a.min_p_all;
     const double top_p = a.top_p ? (double)a.top_p[r] : a.top_p_all;
     const int64_t top_k = a.top_k ? a.top_k[r] : a.top_k_all;
@@ -445,7 +449,7 @@ __global__ __launch_bounds__(kSampleThreads) void sample_kernel(const SampleArgs
         }
     }
     if (!infinite && min_p > 0.0) {
-        const float unlikely = sample_below<T>(weight, max(1ull, (unsigned long long)ceil(fmin(min_p, 1.0) * (double)(1ull << kSampleBits))));
+        const float unlikely = sample_below<T>(lds, weight, max(1ull, (unsigned long long)ceil(fmin(min_p, 1.0) * (double)(1ull << kSampleBits))));
         if (unlikely >= t) {
             t = unlikely;
             m = 0;
