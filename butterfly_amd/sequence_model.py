@@ -130,13 +130,16 @@ class ButterflyLM(nn.Module):
     @torch.no_grad()
     def generate(self, prompt, uniform, temperature=None, top_k=None, top_p=None, min_p=None):
         """(batch, prompt) tokens -> the (batch, steps) tokens that follow, drawn (as ``sample`` does) with ``uniform`` (batch,
-        steps), random numbers in [0, 1).  Settings are numbers or one of each sequence.  (Call ``eval()`` first: dropout.)"""
+        steps), random numbers in [0, 1).  Settings are numbers or one of each sequence.  Where nothing can be drawn (logits that are
+        NaN or -inf, all of them) the token and those behind it are -1.  (Call ``eval()`` first: dropout.)"""
         hidden, states = self.hidden(prompt)
         logits, tokens = F.linear(hidden[:, -1], self.embedding), []
         for t in range(uniform.shape[1]):
             if t > 0:
-                logits = self.step(tokens[-1], states)
-            tokens.append(sample(logits, uniform[:, t], temperature, top_k, top_p, min_p))
+                # (-1 is no row of the embedding: any row in its place, what comes of it is not looked at)
+                logits = self.step(tokens[-1].clamp(min=0), states)
+            token = sample(logits, uniform[:, t], temperature, top_k, top_p, min_p)
+            tokens.append(torch.where(tokens[-1] < 0, tokens[-1], token) if tokens else token)
         return torch.stack(tokens, 1) if tokens else prompt[:, :0]
 
     def empty_states(self, batch):
