@@ -54,6 +54,15 @@ class AttentionMixer(nn.Module):
         self.decay = nn.Parameter(torch.log(torch.logspace(1, 3, heads) - 1))
         self.register_buffer("frequencies", rotary_frequencies(features // heads)[0], persistent=False)
 
+    def _apply(self, fn, recurse=True):
+        # (the parameters' type is not the angles': a frequency of fewer than 64 bits loses them at far positions)
+        frequencies = self.frequencies
+        super()._apply(fn, recurse)
+        if frequencies.is_meta:
+            frequencies = rotary_frequencies(self.out.in_size // self.heads)[0]
+        self.frequencies = frequencies.to(self.frequencies.device)
+        return self
+
     def _parts(self, x, positions):
         """Queries and keys (turned), values, decays of x (*, features) at positions (*)."""
         features = self.out.in_size
