@@ -24,7 +24,7 @@ int check_attention(const bf_linear_attention *p)
         return fail(BF_ERR_UNSUPPORTED, "heads of more than %d features or values are not supported", kWidest);
     if (p->features == 0 || p->values == 0) return fail(BF_ERR_INVALID, "features and values must be positive");
     // (one workgroup of up to 512 threads each: a grid has less than 2^32 of them)
-    if (p->batch > ((int64_t)1 << 22) || p->heads > ((int64_t)1 << 22) || p->batch * p->heads > ((int64_t)1 << 22))
+    if (p->batch > ((int64_t)1 << 22) || p->heads > ((int64_t)1 << 22) || p->groups > ((int64_t)1 << 22) || p->batch * p->heads > ((int64_t)1 << 22))
         return fail(BF_ERR_UNSUPPORTED, "more than 2^22 sequences and heads are not supported");
     if (p->steps > ((int64_t)1 << 31)) return fail(BF_ERR_UNSUPPORTED, "more than 2^31 steps are not supported");
     // (a chunk's rows of a result lie within 2^31 bytes of each other)
@@ -139,6 +139,16 @@ dim3 walk_grid(const LaArgs &a) { return dim3((unsigned)((a.batch * a.heads * a.
 
 dim3 enter_grid(const LaArgs &a) { return dim3((unsigned)std::min<int64_t>((a.batch * a.heads * a.features * a.values + 255) / 256, 1 << 16)); }
 
+// d_q or d_k from the gradients of each head, or of no heads: zeros (from: not read).
+template <typename T>
+void add_shared(const bf_linear_attention *p, const void *from, void *to, hipStream_t s)
+{
+    const int64_t rows = p->batch * p->steps, count = rows * p->groups * p->features;
+    const dim3 grid((unsigned)std::min<int64_t>((count + 255) / 256, 1 << 16));
+    la_shared_kernel<T><<<grid, dim3(256), 0, s>>>(static_cast<const float *>(from), static_cast<T *>(to), rows, (int)p->groups,
+                                                   (int)(p->heads / p->groups), (int)p->features);
+}
+
 int copy_state(const bf_linear_attention *p, const float *from, float *to, hipStream_t s)
 {
     if (!to) return BF_OK;
@@ -212,8 +222,15 @@ int bf_linear_attention_bw(const bf_linear_attention *p, const void *q, const vo
 {
     int rc = check_attention(p);
     if (rc) return rc;
-    if (nothing(p)) return BF_OK;
     hipStream_t s = static_cast<hipStream_t>(stream);
+    if (nothing(p)) {
+        // (queries and keys of groups without heads)
+        if (p->batch == 0 || p->steps == 0 || p->groups == 0) return BF_OK;
+        if (!d_q || !d_k) return fail(BF_ERR_INVALID, "d_q or d_k is NULL");
+        for (void *to : {d_q, d_k}) p->dtype == BF_F32 ? add_shared<float>(p, nullptr, to, s) : add_shared<bf16>(p, nullptr, to, s);
+        BF_HIP_CHECK(hipGetLastError());
+        return BF_OK;
+    }
     if (p->steps == 0) return copy_state(p, grad_last, d_state, s);
     if (!q || !k || !v || !log_decay) return fail(BF_ERR_INVALID, "q, k, v or log_decay is NULL");
     if (!d_q || !d_k || !d_v || !d_log_decay) return fail(BF_ERR_INVALID, "d_q, d_k, d_v or d_log_decay is NULL");
@@ -245,11 +262,8 @@ int bf_linear_attention_bw(const bf_linear_attention *p, const void *q, const vo
         }
         la_back_kernel<T, D><<<walk_grid(a), dim3(LaShape<T, D>::THREADS), 0, s>>>(a);
         if (a.wide) {
-            const int64_t rows = p->batch * p->steps, count = rows * p->groups * p->features;
-            const dim3 grid((unsigned)std::min<int64_t>((count + 255) / 256, 1 << 16));
-            for (const auto &x : {std::make_pair(a.d_q, d_q), std::make_pair(a.d_k, d_k)})
-                la_shared_kernel<T><<<grid, dim3(256), 0, s>>>(static_cast<const float *>(x.first), static_cast<T *>(x.second), rows,
-                                                               (int)p->groups, a.shared, a.features);
+            add_shared<T>(p, a.d_q, d_q, s);
+            add_shared<T>(p, a.d_k, d_k, s);
         }
     });
     BF_HIP_CHECK(hipGetLastError());

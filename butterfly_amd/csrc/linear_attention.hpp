@@ -1261,7 +1261,7 @@ __global__ __launch_bounds__((LaShape<T, D>::THREADS)) void la_back_kernel(const
     }
 }
 
-// Gradients of queries or keys that heads share: the sum over those heads, in order.
+// Gradients of queries or keys that heads share: the sum over those heads, in order (zero over none).
 template <typename T>
 __global__ __launch_bounds__(256) void la_shared_kernel(const float *from, T *to, int64_t rows, int groups, int shared, int features)
 {
@@ -1269,7 +1269,7 @@ __global__ __launch_bounds__(256) void la_shared_kernel(const float *from, T *to
     for (int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x; at < count; at += (int64_t)gridDim.x * 256) {
         const int64_t row = at / features;
         const float *p = from + row * shared * features + at % features;
-        float sum = p[0];
+        float sum = shared > 0 ? p[0] : 0.0f;
         for (int n = 1; n < shared; ++n) sum += p[(int64_t)n * features];
         to[at] = (T)sum;
     }
