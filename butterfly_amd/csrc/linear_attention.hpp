@@ -310,15 +310,24 @@ struct LaPiece {
 // What the products take from a chunk's decays.  Sums of log decays, to the base 2, as two floats of together 48 bits: their
 // differences keep the bits of the decays between two steps, whatever the steps in front have summed up to.  part: resets
 // so far.  start, end: what steps meet of the states in front of and behind the chunk (scale exp(L_i), exp(L_C - L_j)),
-// kNothing where a reset lies between.
+// kNothing where a reset lies between.  group: decays so far that are infinite (less than 256), and 256 times those that are NaN.  They
+// are left out of the sums, which start behind them as behind a reset, so that steps on one side keep their factors, and
+// steps that are parted by one get it.
 constexpr float kNothing = -0.0f;
 __device__ __forceinline__ bool la_nothing(float factor) { return __builtin_bit_cast(int, factor) == INT32_MIN; }
+
+// The factor f between steps of two groups.
+__device__ __forceinline__ float la_crossed(float f, int one, int other)
+{
+    return one == other ? f : (one ^ other) >> 8 ? NAN : INFINITY;
+}
 
 template <int C>
 struct LaLevels {
     float hi[C], lo[C], start[C], end[C];
-    int part[C];
+    int part[C], group[C];
     float decay;   // over the whole chunk; kNothing: a reset lies within
+    bool broken;   // not all groups are 0
 
     __device__ __forceinline__ LaAcc quad(const float (&v)[C], int at) const { return *reinterpret_cast<const LaAcc *>(v + at); }
     // scale exp(L_i - L_j) for four neighbouring steps i or j and one other one
@@ -327,6 +336,14 @@ struct LaLevels {
         LaAcc f;
 #pragma unroll
         for (int r = 0; r < 4; ++r) f[r] = __builtin_amdgcn_exp2f(sign * ((hi0[r] - hi1) + (lo0[r] - lo1)));
+        return f;
+    }
+    // the same of a broken chunk
+    __device__ __forceinline__ LaAcc crossed(LaAcc f, int at, int other) const
+    {
+        const LaParts groups = *reinterpret_cast<const LaParts *>(group + at);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) f[r] = la_crossed(f[r], groups[r], other);
         return f;
     }
 };
@@ -390,27 +407,38 @@ __device__ __forceinline__ void la_scan(V &sum)
     sum += la_up<32>((V)0, sum);
 }
 
-// One step a lane.  A decay below 2^-160 is zero beside anything in 32 bits and counts as that.
+// One step a lane.  A decay below 2^-160 is zero beside anything in 32 bits and counts as that, one of 2^128 or more as infinite.
 template <int C>
 __device__ __forceinline__ void la_levels(LaLevels<C> &out, float log_decay, bool reset, float scale)
 {
     const int lane = threadIdx.x & 63;
     const double x = (double)log_decay * 1.4426950408889634;
-    double level = reset ? 0.0 : x < -160.0 ? -160.0 : x;
-    const uint64_t resets = __ballot(reset), below = ((uint64_t)2 << lane) - 1;
+    const bool infinite = !reset && x >= 128.0, nan = !reset && x != x;
+    double level = reset | infinite | nan ? 0.0 : x < -160.0 ? -160.0 : x;
+    const uint64_t resets = __ballot(reset), infinities = __ballot(infinite), nans = __ballot(nan), below = ((uint64_t)2 << lane) - 1;
     const int part = __popcll(resets & below), parts = __popcll(resets);
-    if (resets == 0) la_scan(level);
-    else la_scan(level, part);
+    const bool broken = (infinities | nans) != 0;
+    int group = 0, groups = 0;
+    if (broken) {
+        group = __popcll(infinities & below) + 256 * __popcll(nans & below);
+        groups = __popcll(infinities) + 256 * __popcll(nans);
+    }
+    if ((resets | infinities | nans) == 0) la_scan(level);
+    else la_scan(level, part + __popcll((infinities | nans) & below));
     const float hi = (float)level, from_start = __builtin_amdgcn_exp2f(hi);
     const double last = __shfl(level, C - 1, 64);
     const float to_end = __builtin_amdgcn_exp2f((float)(last - level));
     if (lane < C) {
         out.hi[lane] = hi;
         out.lo[lane] = (float)(level - (double)hi);
-        out.start[lane] = part == 0 ? scale * from_start : kNothing;
-        out.end[lane] = part == parts ? to_end : kNothing;
+        out.start[lane] = part == 0 ? scale * la_crossed(from_start, group, 0) : kNothing;
+        out.end[lane] = part == parts ? la_crossed(to_end, group, groups) : kNothing;
         out.part[lane] = part;
-        if (lane == C - 1) out.decay = part == 0 ? from_start : kNothing;
+        out.group[lane] = group;
+        if (lane == C - 1) {
+            out.decay = part == 0 ? la_crossed(from_start, group, 0) : kNothing;
+            out.broken = broken;
+        }
     }
 }
 
@@ -467,7 +495,7 @@ __device__ __forceinline__ F la_only(F f, int t)
 }
 
 // Sum over the steps of the pairs of tiles first .. last of a2(part, pair) x b2(pair), onto c (rows: steps of the chunk).
-// BAD: something in the chunk is not finite.  Then step by step (a, b: of a tile), and only onto the rows that `meets(row, step)`: what a factor of
+// BAD: something in the chunk, or one of its decays, is not finite.  Then step by step (a, b: of a tile), and only onto the rows that `meets(row, step)`: what a factor of
 // zero stands for must not turn into NaN.
 template <bool BAD, int N, int TT, typename F, typename A2, typename B2, typename A, typename B, typename M>
 __device__ __forceinline__ void la_over_steps(LaAcc &c, int first, int last, A2 &&a2, B2 &&b2, A &&a, B &&b, M &&meets)
@@ -650,7 +678,7 @@ __global__ __launch_bounds__((LaShape<T, D>::THREADS)) void la_walk_kernel(const
         }
         if (la_not_finite<T>(magnitude)) bad_chunk[n & 1] = 1;
         __syncthreads();
-        const bool bad = bad_chunk[n & 1] != 0;
+        const bool bad = (bad_chunk[n & 1] != 0) | levels.broken;
         if (threadIdx.x == 0) bad_chunk[(n + 1) & 1] = 0;
         if (wave == W - 1) {
             if (n + 1 < count) nd.levels(both_levels[(n + 1) & 1], a.scale);
@@ -674,7 +702,8 @@ __global__ __launch_bounds__((LaShape<T, D>::THREADS)) void la_walk_kernel(const
                     for (int x = 0; x < D; x += 32)
                         c = la_mma(la_rows2(lane, ks, LD, 16 * tj, x), la_rows2(lane, qs, LD, 16 * ti, x), c);
                     const int i = 16 * ti + i16, j = 16 * tj + 4 * g, part = levels.part[i];
-                    const LaAcc f_ij = levels.between(levels.quad(levels.hi, j), levels.quad(levels.lo, j), levels.hi[i], levels.lo[i], -1.0f);
+                    LaAcc f_ij = levels.between(levels.quad(levels.hi, j), levels.quad(levels.lo, j), levels.hi[i], levels.lo[i], -1.0f);
+                    if constexpr (BAD) f_ij = levels.crossed(f_ij, j, levels.group[i]);
                     const LaParts parts = *reinterpret_cast<const LaParts *>(levels.part + j);
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
@@ -765,7 +794,7 @@ __global__ __launch_bounds__((LaShape<T, D>::THREADS)) void la_walk_kernel(const
         if (__builtin_expect(bad, 0)) products(std::true_type());
         else products(std::false_type());
         if constexpr (!OUT) {
-            total += (double)levels.hi[C - 1] + (double)levels.lo[C - 1];
+            total += levels.broken ? (double)levels.decay : (double)levels.hi[C - 1] + (double)levels.lo[C - 1];
             cuts |= levels.part[C - 1];
         }
         __syncthreads();
@@ -974,7 +1003,7 @@ __global__ __launch_bounds__((LaShape<T, D>::THREADS)) void la_back_kernel(const
             for (int m = 0; m < EP; ++m) *reinterpret_cast<F *>(es + (m * D + col) * LD + 16 * half * OD + 4 * g + 16 * t) = f[m];
         }
         __syncthreads();
-        const bool bad = bad_chunk[n & 1] != 0;
+        const bool bad = (bad_chunk[n & 1] != 0) | levels.broken;
         if (threadIdx.x == 0) bad_chunk[(n + 1) & 1] = 0;
         // the state in front of the chunk (what lies outside of it: some address inside, zero when it is used)
         // before[t]: values value_of(t) .. + 3, in the order of the operands that it meets: those in LDS, or E's sums
@@ -1030,7 +1059,8 @@ __global__ __launch_bounds__((LaShape<T, D>::THREADS)) void la_back_kernel(const
                 hold();
             }
             const int j = 16 * tj + i16, i = 16 * ti + 4 * g, part = levels.part[j];
-            const LaAcc f_ij = levels.between(levels.quad(levels.hi, i), levels.quad(levels.lo, i), levels.hi[j], levels.lo[j], 1.0f);
+            LaAcc f_ij = levels.between(levels.quad(levels.hi, i), levels.quad(levels.lo, i), levels.hi[j], levels.lo[j], 1.0f);
+            if (__builtin_expect(bad, 0)) f_ij = levels.crossed(f_ij, i, levels.group[j]);
             const LaParts parts = *reinterpret_cast<const LaParts *>(levels.part + i);
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
