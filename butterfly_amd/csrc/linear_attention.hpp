@@ -322,8 +322,9 @@ __device__ __forceinline__ float la_crossed(float f, int one, int other)
     return one == other ? f : (one ^ other) >> 8 ? NAN : INFINITY;
 }
 
+// (a multiple of 16 bytes: several lie one behind the other, and four neighbouring steps are read at once)
 template <int C>
-struct LaLevels {
+struct __align__(16) LaLevels {
     float hi[C], lo[C], start[C], end[C];
     int part[C], group[C];
     float decay;   // over the whole chunk; kNothing: a reset lies within
@@ -347,6 +348,8 @@ struct LaLevels {
         return f;
     }
 };
+
+static_assert(sizeof(LaLevels<32>) % 16 == 0 && sizeof(LaLevels<64>) % 16 == 0);
 
 // (kNothing: zero, whatever x is)
 __device__ __forceinline__ LaAcc la_times(LaAcc x, LaAcc factor)
