@@ -21,6 +21,9 @@ int check_rotary(const bf_rotary *p)
     if (p->rotated > 2 * kRotaryTable) return fail(BF_ERR_UNSUPPORTED, "more than %d rotated features are not supported", 2 * kRotaryTable);
     if (p->features > ((int64_t)1 << 20) || p->heads > ((int64_t)1 << 20) || p->batch > ((int64_t)1 << 40) || p->steps > ((int64_t)1 << 40))
         return fail(BF_ERR_UNSUPPORTED, "too many tokens, heads or features");
+    // (their product counts items and workgroups)
+    if ((double)p->batch * (double)p->steps * (double)p->heads * (double)p->features > 0x1p48)
+        return fail(BF_ERR_UNSUPPORTED, "too many tokens, heads or features");
     for (int i = 0; i < 3; ++i)
         if (p->x_stride[i] < 0) return fail(BF_ERR_INVALID, "strides must be non-negative");
     if (p->position_stride[0] < 0 || p->position_stride[1] < 0) return fail(BF_ERR_INVALID, "strides must be non-negative");
