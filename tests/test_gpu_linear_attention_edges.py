@@ -1,4 +1,4 @@
-"""Linear attention: decays that are not finite.  References are the definition in 64 bits, step by step, with
+"""Linear attention: decays that are not finite, bits that results keep.  References are the definition in 64 bits, step by step, with
 gradients by automatic differentiation; tolerances as for any other call (float32 1e-5 of the largest; bfloat16 results
 rounded once, what they are summed from has 16 bits: 2^-8 + 2^-12)."""
 import math
@@ -81,3 +81,15 @@ def test_decays_that_are_not_finite(at, resets, dtype, size, bad):
     # decays' gradients: not finite where they are not, and all of that document's in the chunk
     assert not bool((torch.isfinite(got["d_log_decay"]) & ~torch.isfinite(want["d_log_decay"])).any())
     assert bool(torch.isfinite(got["d_log_decay"][..., 1]).all())
+
+
+@pytest.mark.parametrize("shape", [(2, 200, 4, 2, 64, 64), (2, 97, 2, 1, 128, 128), (1, 300, 6, 2, 100, 100), (1, 700, 2, 1, 128, 72), (1, 1000, 2, 2, 64, 64), (1, 129, 3, 3, 17, 33)])
+def test_bfloat16_keeps_the_bits_that_it_says(shape):
+    """Decays' gradients are floats and so is all that they are summed from: sums of products of bfloat16 numbers, which are exact,
+    states and their gradients as three numbers (24 bits), decays; 1e-5 as with float32 inputs.  Results are rounded once (2^-8);
+    inner factors, states and their gradients are read with 16 bits, wide heads' too: 2^-8 + 2^-12."""
+    v = make(*shape, torch.bfloat16)
+    want, got = definition(v, shape[4] ** -0.5), device(v, shape[4] ** -0.5)
+    for name in RESULTS:
+        err = float((got[name] - want[name]).abs().max() / want[name].abs().max())
+        assert err <= (1e-5 if name in ("last", "d_state", "d_log_decay") else 2.0 ** -8 + 2.0 ** -12), (name, err)
