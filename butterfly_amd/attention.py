@@ -18,10 +18,11 @@ def linear_attention(q, k, v, log_decay, state=None, reset=None, scale=None):
     zero (a packed document starts).  ``scale``: ``features ** -0.5`` by default.
 
     On the device sums and states are float32 (bfloat16: inner products that are factors again are rounded to 16 bits,
-    results once to 8).  Decays below 2^-160 count as that, of 2^128 and more as infinite.  What is not finite stays in its own document, and does not reach
-    outputs and gradients of steps that do not meet it, except that gradients of ``log_decay`` are NaN for its whole
-    document in the chunk of 64 (32) steps that holds it.  Training keeps a state for every chunk.  There is no second derivative:
-    following a gradient's history raises."""
+    results once to 8).  Decays below 2^-160 count as that, of 2^128 and more as infinite.  What is not finite (a decay, too) stays
+    in its own document, and does not reach outputs and gradients of steps that do not meet it, except that gradients of
+    ``log_decay`` are not finite for its whole document in the chunk of 64 (32) steps that holds it.  Decays above one that
+    multiply up to 2^128 within a chunk are infinite there, and what they meet is infinite or NaN, zeros as well.  Training keeps
+    a state for every chunk.  There is no second derivative: following a gradient's history raises."""
     if scale is None:
         scale = q.shape[-1] ** -0.5
     if v.is_cuda:

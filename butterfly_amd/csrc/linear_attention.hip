@@ -57,7 +57,8 @@ struct AttentionPlan {
 
 size_t rounded(size_t bytes) { return (bytes + 255) / 256 * 256; }
 
-// Sequences times heads are one workgroup each, a compute unit's (registers and LDS hold no second one).  Fewer than half of the 256
+// Sequences times heads are one workgroup each, a compute unit's: the registers of the launches with outputs or gradients (160 to 256 a
+// lane, eight wavefronts) hold no second one.  (Those of the sums alone, 112 a lane for 64-wide heads, would; they share the cut.)  Fewer than half of the 256
 // are cut into as many segments as fill them, no more: 10 heads of 65537 steps in 26 segments leave four workgroups for
 // a second round and took twice the time of 25.  Segments of two chunks at least: 16 heads of 256 steps forward and backward 73 us in two
 // segments, 86 in one (float; bfloat16 57 and 58); of 1024 steps 80 in eight, 303 in one.

@@ -20,18 +20,19 @@
 // inputs as they are; float factors as several bfloat16 numbers that add up to them: three (24 bits) for what is added
 // to a state, two (16 bits) for states and for the products' inner factors Q K^T . D, dO V^T . D (the results are rounded to
 // 8 bits; one number would leave errors of the size of that rounding).  The decays' gradients are floats: what they are summed
-// from, b dO S^T and w V E^T, takes S and E as three numbers as well (two: 287 instead of 300 us and 735 instead of 765 for the
-// backward kernels below, and decays' gradients off by 2e-6 instead of 3e-7).  An operand of a product over 32 steps or features is two
+// from, b dO S^T and w V E^T, takes S and E as three numbers as well (two: 4% off the backward kernels' time, and decays'
+// gradients off by 2e-6 instead of 3e-7).  An operand of a product over 32 steps or features is two
 // pieces of 4 elements in a lane (LaPair); a state that is taken from sums keeps their order, 4 g .. 4 g + 3 (g: lane / 16)
 // of two neighbouring tiles, and so does what it meets, so that sums become operands without leaving their lane.
 //
 // Measured, one workgroup a compute unit, 64 x 64 states and 128 x 128 ones:
-//   16 x 2048 steps, 16 heads, bfloat16       forward 132 us                          backward 300
-//    8 x 1001 steps, 16 heads, float          forward 27 + 5 + 60                     backward 27 + 5 + 123
-//    1 x 65537 steps, 10 heads of 100         forward 140 + 8 + 390                   backward 140 + 9 + 765
-// (sums of a segment, states between segments, outputs).  The first one moves 403 MB forward, 3.1 TB/s, and 604 MB backward, 2.0: it
-// is bound by the chunk's own chain of products (LDS moves data for 59% and 55% of the cycles, the vector unit issues for 46%
-// and 50%, the matrix unit for 11%; three or four barriers a chunk between them), with two wavefronts a SIMD to hide each other.
+//   16 x 2048 steps, 16 heads, bfloat16       forward 116 us                          backward 244
+//    8 x 1001 steps, 16 heads, float          forward 26 + 6 + 56                     backward 26 + 5 + 110
+//    1 x 65537 steps, 10 heads of 100         forward 132 + 7 + 350                   backward 134 + 8 + 656
+// (sums of a segment, states between segments, outputs).  The first one moves 403 MB forward, 3.5 TB/s, and 604 MB backward, 2.5: it
+// is bound by the chunk's own chain of products (LDS moves data for 37% of the cycles both ways, the vector unit issues for 50%
+// and 57%, the matrix unit for 12% and 13%; three or four barriers a chunk between them), with two wavefronts a SIMD to hide each
+// other.  The backward kernel of 128-wide bfloat16 heads has 38 registers and 156 bytes a lane in scratch memory.
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -77,7 +78,8 @@ struct LaShape {
     static constexpr int C = sizeof(T) == 4 && D == 128 ? 32 : 64;
     static constexpr int SLICES = D / 16;            // of 16 columns of a state or a result
     // wavefronts of a slice: two of 64 columns share the steps and the rows of the state (two wavefronts on each SIMD), the
-    // state's operands then go through LDS, where there is no room for those of 128
+    // state's operands then go through LDS.  Those of 128 columns stay in the sums: the backward kernel has no room for them (152 of
+    // 160 KB without), the forward one of bfloat16 would (74 and 70)
     static constexpr int HALVES = D == 64 ? 2 : 1;
     static constexpr int W = SLICES * HALVES, THREADS = 64 * W;
     static constexpr int TT = C / 16, DT = D / 16;   // tiles of a chunk, of a state
@@ -859,7 +861,7 @@ __global__ __launch_bounds__(256) void la_copy_kernel(const float *from, float *
 }
 
 // The gradients, chunk by chunk from a segment's end, with the states that the forward call kept (formed again they would cost the
-// walk once more, 132 us of the first case above; kept, 268 MB to write and read, 56 us).
+// walk once more, 116 us of the first case above; kept, 268 MB to write and read, 56 us).
 template <typename T, int D>
 __global__ __launch_bounds__((LaShape<T, D>::THREADS)) void la_back_kernel(const LaArgs a)
 {
@@ -1309,7 +1311,7 @@ __global__ __launch_bounds__(256) void la_shared_kernel(const float *from, T *to
 }
 
 // One step of every head: the state is read and written once, which is all that this costs.  LANES lanes take V neighbouring
-// values of a feature's row each, the others of 256 its further features.  64 x 16 heads of 64 x 64: 33.5 MB in 7.6 us, 4.4 TB/s; one sequence: 4.1 us, a launch.
+// values of a feature's row each, the others of 256 its further features.  64 x 16 heads of 64 x 64: 33.5 MB in 7.4 us, 4.5 TB/s; one sequence: 4.1 us, a launch.
 template <typename T, int V>
 __global__ __launch_bounds__(256) void la_step_kernel(const LaArgs a, float *state, T *o, int lanes_log)
 {

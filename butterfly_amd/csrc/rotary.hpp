@@ -6,8 +6,8 @@
 // is formed in double and reduced to a turn there (a float would have lost it at a position of a few thousand); what is left
 // of it, at most half a turn, goes through the float functions.
 //
-// Bound by memory: 16 x 2048 x 16 x 64 bfloat16 in 23.8 us, 134 MB at 5.6 TB/s; 65537 x 10 x 100 floats, neighbours, 50 of them
-// turned, in 106 us, 524 MB at 4.9 TB/s; 64 tokens x 32 heads in 3.5 us, a launch.
+// Bound by memory: 16 x 2048 x 16 x 64 bfloat16 in 23.2 us, 134 MB at 5.8 TB/s; 65537 x 10 x 100 floats, neighbours, 50 of them
+// turned, in 107 us, 524 MB at 4.9 TB/s; 64 tokens x 32 heads in 3.4 us, a launch.
 #pragma once
 
 #include <hip/hip_runtime.h>

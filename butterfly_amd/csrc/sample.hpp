@@ -2,7 +2,8 @@
 // largest logits (ties: the lowest indexes) the likeliest ones until their sum reaches top_p of it, of those the ones with
 // w_i >= min_p; the token is the first index whose cumulated w, in the order of indexes, exceeds uniform * total.
 //
-// A workgroup takes a row and keeps it in registers (up to 256 KiB; longer ones are read again, out of the caches).  There is no
+// A workgroup takes a row and keeps it in registers (up to 256 KiB, of the largest 56 to 128 bytes a lane in scratch memory; longer
+// rows are read again, out of the caches).  There is no
 // sort: what is kept is "logit above t, and the first m of those equal to t", and t is found by histograms of 2048 bins, first
 // over the values from the maximum down, then, within the bin where the sum crosses its goal: float by comparing its few entries with
 // each other (some 64 of 2^17: one pass less), bfloat16, or many, over the logits' bits.
@@ -12,10 +13,10 @@
 // between two tokens by some 1e-8 of the total, which with 50000 entries of similar weight is 1e-3 of the distance between two
 // borders; these move it by 1e-7 of that.
 //
-// Measured: 256 rows of 2^17 bfloat16 with top_p 101 us (67 MB: 14 us at a copy's rate), 64 rows of 30001 floats with top_p 33,
-// one row of 32768 floats with top_k, top_p and min_p 30.  The large one is bound by the vector unit, busy for 91% of the cycles:
-// some 30 operations for each weight, formed twice (histogram, sum), which no filter allows to leave out; the small ones by the
-// chain of passes, barriers and scans within a workgroup.
+// Measured: 256 rows of 2^17 bfloat16 with top_p 102 us (67 MB: 14 us at a copy's rate), 64 rows of 30001 floats with top_p 34,
+// one row of 32768 floats with top_k, top_p and min_p 30.  The large one is bound by the vector unit, busy for 87% of the cycles:
+// some 30 operations for each weight, formed for each entry and twice (histogram, sum); the small ones by the chain of
+// passes, barriers and scans within a workgroup.
 #pragma once
 
 #include <hip/hip_runtime.h>

@@ -15,7 +15,7 @@ def rotary(x, positions, frequencies, interleaved=False, magnitude=1.0):
     features stay as they are.
 
     ``x`` float32 or bfloat16 with any strides, ``positions`` (*) int64, ``frequencies`` float64 (``rotary_frequencies``
-    makes them).  Angles are formed in 64 bits, whatever the position.  All derivatives exist."""
+    makes them).  Angles are formed in 64 bits, whatever the position.  Gradients of any order exist (no forward mode)."""
     if x.is_cuda:
         return ops.rotary(x, positions, frequencies, interleaved, magnitude)
     pairs = frequencies.shape[0]

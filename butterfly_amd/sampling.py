@@ -17,7 +17,7 @@ def sample(logits, uniform, temperature=None, top_k=None, top_p=None, min_p=None
     ``min_p <= 0`` leave a filter out.  ``temperature <= 0``: the first of the largest logits; others count as between 2^-100 and 2^100.
     A setting that is NaN is none (a temperature: 0).
 
-    NaN counts as -inf, and -inf is never drawn; a row of nothing else gives -1.  Where +inf is among the logits, only those
+    NaN counts as -inf, and -inf is never drawn; a row of nothing else gives -1 (no index of anything).  Where +inf is among the logits, only those
     are drawn.  On the device weights are whole multiples of 2^-44 (the same token at every call), and up to
     2^19 entries are supported.  There is no gradient."""
     settings = [(temperature, 1.0, float), (top_k, 0, int), (top_p, 1.0, float), (min_p, 0.0, float)]

@@ -34,7 +34,6 @@ class RecurrentMixer(nn.Module):
         gate, value = self.into(x).chunk(2, -1)
         return self.out(gated_recurrence_step(gate, value, state))
 
-
     def empty_state(self, batch, device):
         return torch.zeros(batch, self.out.in_size, device=device)
 
@@ -66,10 +65,10 @@ class AttentionMixer(nn.Module):
     def _parts(self, x, positions):
         """Queries and keys (turned), values, decays of x (*, features) at positions (*)."""
         features = self.out.in_size
-        parts, gate = self.into(x).split((3 * features, self.heads), -1)
+        parts, decay = self.into(x).split((3 * features, self.heads), -1)
         parts = parts.reshape(*x.shape[:-1], 3 * self.heads, features // self.heads)
         q, k = rotary(parts[..., :2 * self.heads, :], positions, self.frequencies).split(self.heads, -2)
-        return q, k, parts[..., 2 * self.heads:, :], F.logsigmoid(gate + self.decay)
+        return q, k, parts[..., 2 * self.heads:, :], F.logsigmoid(decay + self.decay)
 
     def forward(self, x, state=None, reset=None):
         """(batch, steps, features) -> the same, and the state behind the last step."""

@@ -425,7 +425,8 @@ int bf_linear_xent_bw(const bf_linear_xent *p, const void *weight, const float *
  * features), v (batch, steps, heads, values), log_decay (batch, steps, heads) floats; heads is a multiple of groups, and
  * heads / groups neighbouring heads share queries and keys.  The last dimension is adjacent (log_decay: the strides
  * say it all), the others have the given strides; o and every gradient are dense, states dense (batch, heads,
- * features, values).  reset (bytes, (batch, steps), may be NULL): where set, S_{t-1} counts as zero whatever it is
+ * features, values).  A decay of 2^128 or more, or NaN, parts the steps on both sides of it: only what meets both is not finite.
+ * reset (bytes, (batch, steps), may be NULL): where set, S_{t-1} counts as zero whatever it is
  * (a packed document starts).  features and values: 1 to 128; heads times either: up to 2^22.     */
 typedef struct bf_linear_attention {
     int32_t dtype; /* BF_F32 or BF_BF16: q, k, v, o and their gradients */
